@@ -65,6 +65,38 @@ cudaError_t rt_gemm_skinny_bf16(const void* X, long ldx, const void* W, const vo
 cudaError_t rt_gemm_swiglu_bf16(const void* A, long lda, const void* Bg, const void* Bu, long ldb, void* C, long ldc,
                                 int M, int N, int K, int choice, int* status, cudaStream_t stream);
 
+// Losses of the vocabulary head (csrc/head/): hidden [rows, width] and weight [vocab, width] bf16 with row strides
+// ld_*; index [rows, K] held vocabulary entries per row, log_probs [rows, K] their teacher log-probabilities (null: the
+// cross entropy's targets, K = 1). Entries without a token are `ignore` (targets) or negative (records). reduction
+// 0 none, 1 sum, 2 mean over rows with an entry (loss [1]); row_loss [rows] always. row_grad [rows]: the upstream
+// gradient of each row's loss (null: 1, or 1 / rows with a loss for the mean). dhidden [rows, width] and
+// dweight [vocab, width] bf16, contiguous, written when not null.
+#define RT_HEAD_MAX_RECORD 1024
+struct RtHeadLoss {
+  const void* hidden;
+  long ld_hidden;
+  const void* weight;
+  long ld_weight;
+  const long* index;
+  const float* log_probs;
+  long rows, vocab;
+  int width, K;
+  long ignore;
+  float scale;  // 1 / temperature
+  int tail;     // the vocabulary outside the record is one more class
+  int reduction;
+  const float* row_grad;
+  float* row_loss;
+  float* loss;
+  void* dhidden;
+  void* dweight;
+};
+long rt_head_loss_workspace_floats(long rows, long vocab, int width, int K, int grad_h, int grad_w);
+cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream_t stream);
+cudaError_t rt_scale_bf16(void* x, const float* factor, long n, cudaStream_t stream);
+cudaError_t rt_top_log_probs(int dtype, const void* logits, long rows, long V, long ld, int k, float scale,
+                             float* logp, long* index, cudaStream_t stream);
+
 // Teacher-block kernels (bf16 activations, fp32 parameters).
 cudaError_t rt_rmsnorm_1p(const void* x, const void* h, const float* w, void* sum_out, void* out, long rows, int C,
                           float eps, cudaStream_t stream);

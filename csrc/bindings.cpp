@@ -477,6 +477,92 @@ at::Tensor kl_rows(at::Tensor student, at::Tensor teacher) {
   return out;
 }
 
+// Vocabulary-head loss from hidden states (see RtHeadLoss): returns {loss, dhidden, dweight}; the gradients that are
+// not asked for are empty. log_probs none: cross entropy of index [rows, 1].
+std::vector<at::Tensor> head_loss(at::Tensor hidden, at::Tensor weight, at::Tensor index,
+                                  c10::optional<at::Tensor> log_probs, int64_t ignore, double scale, bool tail,
+                                  int64_t reduction, c10::optional<at::Tensor> row_grad, bool grad_h, bool grad_w) {
+  const auto h = operand(hidden, "hidden"), w = operand(weight, "weight");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(h.ptr) % 16 == 0 && reinterpret_cast<uintptr_t>(w.ptr) % 16 == 0,
+              "head_loss: hidden and weight need 16-byte alignment");
+  c10::cuda::CUDAGuard guard(hidden.device());
+  const long rows = hidden.size(0), V = weight.size(0), C = hidden.size(1);
+  TORCH_CHECK(weight.size(1) == C && C >= 1, "head_loss: hidden width ", C, " and weight width ", weight.size(1));
+  TORCH_CHECK(V >= 1 && rows <= (1 << 24) && C <= (1 << 20), "head_loss: size out of range");
+  TORCH_CHECK(C % 8 == 0, "head_loss: the width must be a multiple of 8");
+  TORCH_CHECK(weight.device() == hidden.device() && index.device() == hidden.device(),
+              "head_loss: operands on different devices");
+  TORCH_CHECK(index.dim() == 2 && index.size(0) == rows && index.scalar_type() == at::kLong && index.is_contiguous(),
+              "head_loss: index must be contiguous int64 [rows, K]");
+  const long K = index.size(1);
+  TORCH_CHECK(K >= 1 && K <= RT_HEAD_MAX_RECORD, "head_loss: 1 to ", RT_HEAD_MAX_RECORD, " entries per row, got ", K);
+  TORCH_CHECK(log_probs.has_value() || K == 1, "head_loss: one target per row");
+  TORCH_CHECK(!log_probs.has_value() ||
+                  (log_probs->device() == hidden.device() && log_probs->scalar_type() == at::kFloat &&
+                   log_probs->is_contiguous() && log_probs->sizes() == index.sizes()),
+              "head_loss: log_probs must be contiguous fp32 like index");
+  TORCH_CHECK(!row_grad.has_value() || (row_grad->device() == hidden.device() && row_grad->is_contiguous() &&
+                                        row_grad->scalar_type() == at::kFloat && row_grad->numel() == rows),
+              "head_loss: row_grad must be contiguous fp32 [rows]");
+  TORCH_CHECK(reduction >= 0 && reduction <= 2, "head_loss: reduction 0 (none), 1 (sum) or 2 (mean)");
+  const auto f32 = hidden.options().dtype(at::kFloat);
+  auto row_loss = at::empty({rows}, f32);
+  auto loss = reduction ? at::empty({}, f32) : row_loss;
+  auto dh = grad_h ? at::empty({rows, C}, hidden.options()) : at::empty({0}, hidden.options());
+  auto dw = grad_w ? at::empty({V, C}, weight.options()) : at::empty({0}, weight.options());
+  auto work = at::empty({std::max(4L, rt_head_loss_workspace_floats(rows, V, C, K, grad_h, grad_w))}, f32);
+  RtHeadLoss p;
+  p.hidden = h.ptr;
+  p.ld_hidden = h.ld;
+  p.weight = w.ptr;
+  p.ld_weight = w.ld;
+  p.index = reinterpret_cast<const long*>(index.data_ptr<int64_t>());
+  p.log_probs = log_probs.has_value() ? log_probs->data_ptr<float>() : nullptr;
+  p.rows = rows;
+  p.vocab = V;
+  p.width = (int)C;
+  p.K = (int)K;
+  p.ignore = ignore;
+  p.scale = (float)scale;
+  p.tail = tail;
+  p.reduction = (int)reduction;
+  p.row_grad = row_grad.has_value() ? row_grad->data_ptr<float>() : nullptr;
+  p.row_loss = row_loss.data_ptr<float>();
+  p.loss = reduction ? loss.data_ptr<float>() : nullptr;
+  p.dhidden = grad_h ? dh.data_ptr() : nullptr;
+  p.dweight = grad_w ? dw.data_ptr() : nullptr;
+  check_cuda(rt_head_loss(&p, work.data_ptr<float>(), stream_of(hidden)), "head_loss");
+  return {loss, dh, dw};
+}
+
+// x *= factor (device fp32 scalar) for a contiguous bf16 tensor; no pass over x when the factor is one.
+void scale_bf16_(at::Tensor x, at::Tensor factor) {
+  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && x.scalar_type() == at::kBFloat16 && factor.device() == x.device() &&
+                  factor.scalar_type() == at::kFloat && factor.numel() == 1,
+              "scale_bf16_: contiguous CUDA bf16 tensor and an fp32 scalar on its device");
+  c10::cuda::CUDAGuard guard(x.device());
+  check_cuda(rt_scale_bf16(x.data_ptr(), factor.data_ptr<float>(), x.numel(), stream_of(x)), "scale_bf16_");
+}
+
+// The k largest log-probabilities of softmax(scale * logits) per row and their indices, largest first, equal logits by
+// the lowest index.
+std::vector<at::Tensor> top_log_probs(at::Tensor logits, int64_t k, double scale) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1,
+              "top_log_probs: CUDA [rows, V] logits with unit inner stride");
+  c10::cuda::CUDAGuard guard(logits.device());
+  const int dtype = dtype_code(logits);
+  const long rows = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(k >= 1 && k <= V && k <= RT_HEAD_MAX_RECORD, "top_log_probs: k must be in 1..min(V, ",
+              RT_HEAD_MAX_RECORD, "), got ", k);
+  auto logp = at::empty({rows, k}, logits.options().dtype(at::kFloat));
+  auto index = at::empty({rows, k}, logits.options().dtype(at::kLong));
+  check_cuda(rt_top_log_probs(dtype, logits.data_ptr(), rows, V, logits.stride(0), (int)k, (float)scale,
+                              logp.data_ptr<float>(), reinterpret_cast<long*>(index.data_ptr<int64_t>()),
+                              stream_of(logits)),
+             "top_log_probs");
+  return {logp, index};
+}
+
 // Student output projection fused with the distillation loss: returns dpred [M, N] bf16; stats += [sum nmse,
 // sum cos, rows] (x [M, K] bf16, w [N, K] bf16, target [M, N] bf16; p = x w^T is never stored).
 at::Tensor gemm_nmse(at::Tensor x, at::Tensor w, at::Tensor target, at::Tensor stats, double eps) {
@@ -807,6 +893,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "1 if a GEMM gave up a bounded wait since the last call (then cleared); synchronizes the device");
   m.def("kl_rows", &kl_rows, "per-row KL(teacher || student) over the vocabulary in one pass", py::arg("student"),
         py::arg("teacher"));
+  m.def("head_loss", &head_loss, "vocabulary-head loss from hidden states: (loss, dhidden, dweight)",
+        py::arg("hidden"), py::arg("weight"), py::arg("index"), py::arg("log_probs"), py::arg("ignore"),
+        py::arg("scale"), py::arg("tail"), py::arg("reduction"), py::arg("row_grad"), py::arg("grad_h"),
+        py::arg("grad_w"));
+  m.def("scale_bf16_", &scale_bf16_, "x *= device scalar, without a pass when it is one");
+  m.def("top_log_probs", &top_log_probs, "k largest log-probabilities per row and their indices", py::arg("logits"),
+        py::arg("k"), py::arg("scale"));
   m.def("gemm_nmse", &gemm_nmse, "output GEMM with the NMSE/cosine loss in the epilogue: returns d loss / d p",
         py::arg("x"), py::arg("w"), py::arg("target"), py::arg("stats"), py::arg("eps"));
   m.def("gemm_swiglu", &gemm_swiglu, "silu(A . Bg^T) * (A . Bu^T) in one tcgen05 GEMM", py::arg("A"), py::arg("Bg"),

@@ -1,10 +1,14 @@
-"""Distillation statistics (reference ``theseus/losses.py:5-30``).
+"""Distillation statistics (reference ``theseus/losses.py:5-30``) and losses of the vocabulary head.
 
 ``statistics`` returns the differentiable sums ``[sum NMSE, sum cosine, count]``
 over tokens, with per-token NMSE = mean((x-y)^2) / max(mean(y^2), eps). On CUDA
 the fused loss kernel computes the same three sums in one pass (and the NMSE
 gradient in the same kernel, see ``ops.loss``); this module is the
 device-agnostic definition used on CPU and as the test oracle.
+
+``linear_cross_entropy``, ``linear_topk_kl`` and ``top_log_probs`` score and train through the vocabulary head: the
+first two take hidden states and the head's weight and never keep the logits, the third makes the teacher's record
+that the second learns from.
 """
 import math
 
@@ -52,3 +56,93 @@ def kl_sum(student_logits, teacher_logits):
     teacher = F.log_softmax(teacher_logits.float(), dim=-1)
     student = F.log_softmax(student_logits.float(), dim=-1)
     return (teacher.exp() * (teacher - student)).sum()
+
+
+def _check_head(hidden, weight, reduction):
+    if reduction not in ("none", "sum", "mean"):
+        raise ValueError(f"Unknown reduction: {reduction}")
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"expected hidden [..., C] and weight [V, C], got {tuple(hidden.shape)} and "
+                         f"{tuple(weight.shape)}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError("empty vocabulary or width")
+    if weight.device != hidden.device:
+        raise ValueError("hidden and weight are on different devices")
+    if hidden.is_cuda and (hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16):
+        raise TypeError("the CUDA head losses take bf16 hidden states and weight")
+    if hidden.is_cuda and (weight.stride(1) != 1 or weight.stride(0) % 8 or weight.shape[1] % 8 or
+                           weight.data_ptr() % 16):
+        raise ValueError("the CUDA head losses need a width and weight row stride that are multiples of 8, unit inner "
+                         "stride and 16-byte alignment")
+
+
+def _check_index(index, shape, name, device):
+    if index.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name} must be int32 or int64, got {index.dtype}")
+    if index.shape[:len(shape)] != shape or index.device != device:
+        raise ValueError(f"{name} {tuple(index.shape)} on {index.device} does not match hidden {tuple(shape)} on "
+                         f"{device}")
+
+
+def _head_loss(hidden, *args):
+    if hidden.is_cuda:
+        from .ops.head import head_loss
+    else:
+        from .ops.reference import head_loss
+    return head_loss(hidden, *args)
+
+
+def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of ``hidden @ weight.T`` (hidden [..., C], weight [V, C]) with ``targets`` [...], without
+    keeping the logits; differentiable in ``hidden`` and ``weight``.
+
+    Tokens whose target is ``ignore_index`` have loss 0 and gradient 0 whatever their hidden state holds, and are not
+    counted by the mean (which is 0 when none is left). fp32 result: [...] for reduction "none", else a scalar. On
+    CUDA a target outside the vocabulary makes its token's loss NaN and its gradient 0; on CPU it raises."""
+    _check_head(hidden, weight, reduction)
+    _check_index(targets, hidden.shape[:-1], "targets", hidden.device)
+    if targets.dim() != hidden.dim() - 1:
+        raise ValueError("one target per token")
+    return _head_loss(hidden, weight, targets.unsqueeze(-1).long(), None, int(ignore_index), 1.0, False, reduction)
+
+
+def linear_topk_kl(hidden, weight, indices, log_probs, temperature=1.0, tail=True, reduction="mean"):
+    """KL from a teacher's recorded top log-probabilities to the student ``softmax(hidden @ weight.T / temperature)``,
+    without keeping the logits; differentiable in ``hidden`` and ``weight``.
+
+    ``indices``, ``log_probs`` [..., K] are a record as ``top_log_probs`` makes it at the same temperature, K <= 1024;
+    the indices of a token are distinct, negative ones are padding, and a token without any has loss 0 and gradient 0
+    and is not counted by the mean. With ``tail`` the vocabulary outside a token's record is one more class, which
+    holds the teacher's remaining mass; without it the sum runs over the recorded entries alone. ``log_probs`` get no
+    gradient. fp32 result: [...] for reduction "none", else a scalar. On CUDA an index beyond the vocabulary makes its
+    token's loss NaN and its gradient 0; on CPU it raises."""
+    _check_head(hidden, weight, reduction)
+    _check_index(indices, hidden.shape[:-1], "indices", hidden.device)
+    if indices.dim() != hidden.dim() or log_probs.shape != indices.shape or log_probs.device != indices.device:
+        raise ValueError("indices and log_probs must both be [..., K]")
+    if not 1 <= indices.shape[-1] <= 1024:
+        raise ValueError(f"a record holds 1 to 1024 entries per token, got {indices.shape[-1]}")
+    if not log_probs.is_floating_point():
+        raise TypeError("log_probs must be floating point")
+    if not temperature > 0:
+        raise ValueError("temperature must be positive")
+    return _head_loss(hidden, weight, indices.long(), log_probs.detach(), -1, 1.0 / float(temperature), bool(tail),
+                      reduction)
+
+
+@torch.no_grad()
+def top_log_probs(logits, k, temperature=1.0):
+    """(log_probs fp32, indices int64), both [..., k]: the k largest log-probabilities of
+    ``softmax(logits / temperature)`` over the last axis, largest first, equal logits by the lowest index. CUDA logits
+    are bf16 or fp32 and k is at most 1024."""
+    if logits.dim() < 1 or not 1 <= k <= min(logits.shape[-1], 1024):
+        raise ValueError(f"k must be in 1..min(V, 1024), got {k} for logits {tuple(logits.shape)}")
+    if not temperature > 0:
+        raise ValueError("temperature must be positive")
+    if logits.is_cuda:
+        if logits.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError("top_log_probs takes bf16 or fp32 logits on CUDA")
+        from .ops.head import top_log_probs as run
+    else:
+        from .ops.reference import top_log_probs as run
+    return run(logits, int(k), 1.0 / float(temperature))

@@ -104,3 +104,38 @@ def attention(q, k_all, v_all, offset):
     mask = cols <= rows
     out = F.scaled_dot_product_attention(qh, kh, vh, attn_mask=mask, scale=D ** -0.5)
     return out.transpose(1, 2)
+
+
+def head_loss(hidden, weight, index, log_probs, ignore, scale, tail, reduction):
+    """Vocabulary-head loss against a record (see ``ops.head``), in fp32 (fp64 for fp64 operands)."""
+    wide = torch.float64 if hidden.dtype == torch.float64 else torch.float32
+    z = (hidden.to(wide) @ weight.to(wide).t()) * scale
+    log_q = z - z.logsumexp(-1, keepdim=True)
+    held = (index != ignore) if log_probs is None else (index >= 0)
+    if bool((held & ((index < 0) | (index >= weight.shape[0]))).any()):
+        raise IndexError(f"vocabulary index outside 0..{weight.shape[0] - 1}")
+    valid = held.any(-1)
+    logp = torch.zeros(index.shape, dtype=wide, device=z.device) if log_probs is None else log_probs.to(wide)
+    logp = logp.masked_fill(~held, float("-inf"))
+    p = logp.exp()
+    index = index.masked_fill(~held, 0)
+    # p log p is 0 at p = 0 (padding, and recorded log-probabilities of -inf)
+    terms = p * (logp.masked_fill(p == 0, 0.0) - log_q.gather(-1, index))
+    loss = terms.masked_fill(p == 0, 0.0).sum(-1)
+    if tail:
+        inside = torch.zeros(z.shape, dtype=torch.int32, device=z.device).scatter_add_(-1, index, held.int()) > 0
+        rest = (1.0 - p.sum(-1)).clamp_min(0.0)
+        counted = (rest > 0) & ~inside.all(-1) & valid
+        log_rest = log_q.masked_fill(inside & counted[..., None], float("-inf")).logsumexp(-1)
+        loss = loss + (rest * (rest.masked_fill(~counted, 1.0).log() - log_rest)).masked_fill(~counted, 0.0)
+    loss = loss.masked_fill(~valid, 0.0)
+    if reduction == "none":
+        return loss
+    return loss.sum() if reduction == "sum" else loss.sum() / valid.sum().clamp_min(1)
+
+
+def top_log_probs(logits, k, scale):
+    """k largest log-probabilities of softmax(scale * logits) and their indices, equal logits by the lowest index."""
+    z = logits.float() if logits.dtype != torch.float64 else logits
+    index = torch.sort(z, dim=-1, descending=True, stable=True)[1][..., :k]
+    return torch.log_softmax(z * scale, -1).gather(-1, index), index
