@@ -1,6 +1,5 @@
 // Losses of the vocabulary head from hidden states: next-token cross entropy and the KL from a teacher's recorded top
-// log-probabilities, with the gradients of the hidden states and of the head's weight. The logits are formed in pieces
-// of the vocabulary and never kept.
+// log-probabilities, with the gradients of the hidden states and of the head's weight.
 //
 // With z_tv = scale x_t . W_v, a row's record is a set S of held entries (v, log p_v); the cross entropy's record is
 // its target with p = 1. With P = sum_S p, r = max(0, 1 - P) (the rest as one more class, or 0 without it), w = P + r,
@@ -10,41 +9,113 @@
 //          = exp(z_v) / Z (w - r Z / Z_rest)            (v not in S)
 // Z_rest is summed without the held entries instead of as Z minus them, so a row that is sure of its target keeps the
 // relative precision of 1 - q. All sums and row statistics are fp32 (the few held terms of a row: double).
+//
+// Launches of one call: the rows that have a loss are counted and packed (gather_kernel: their hidden states, sorted
+// records and held logits), z = X W^T leaves per row and 256-column tile its maximum and sum of exponentials
+// (head_gemm.cuh), merge_kernel forms the losses. With gradients the same product also leaves the exponentials in bf16,
+// relative to their tile's maximum; gradient_kernel turns them into dz in place, and dX = dz W, dW = dz^T X follow.
+// That is 6 T V C operations, against 8 T V C where the logits are formed a second time, for T V bf16 values of
+// workspace; CHUNK_VALUES bounds it, and more rows run in chunks whose dW adds up in fp32. Rows without a loss cost
+// nothing but their packing, and what they hold never meets the other rows.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include "../api.h"
 #include "../common/common.cuh"
+#include "head_gemm.cuh"
 
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 
-// ---------------------------------------------------------------- records
-// One block per row: held entries sorted by vocabulary index (entries outside the record last, as INT_MAX), their
-// log-probabilities in the same order, and the row's kind: 0 no entry (no loss), 1 valid, 2 an index outside the
-// vocabulary (its loss is NaN and its gradient zero). K is padded to a power of two in shared memory.
-__global__ void records_kernel(const long* __restrict__ idx, const float* __restrict__ logp, int K, int Kp, long V,
-                               long ignore, int* __restrict__ sidx, float* __restrict__ slogp,
-                               int* __restrict__ kind) {
+// ---------------------------------------------------------------- rows with a loss
+// Kind of each row: 0 no entry (no loss), 1 valid, 2 an index outside the vocabulary (loss NaN, gradient zero).
+__device__ __forceinline__ int entry_kind(long id, bool record, long ignore, long V) {
+  if (record ? id < 0 : id == ignore) return 0;
+  return id < 0 || id >= V ? 2 : 1;
+}
+
+// One warp per row: kind[row] of a record of K entries.
+__global__ void kinds_kernel(const long* __restrict__ idx, long rows, int K, long V, int* __restrict__ kind) {
+  const long row = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  if (row >= rows) return;
+  int any = 0;
+  for (int k = threadIdx.x & 31; k < K; k += 32) any |= entry_kind(idx[row * K + k], true, 0, V);
+  any = __reduce_or_sync(~0u, any);
+  if ((threadIdx.x & 31) == 0) kind[row] = any & 2 ? 2 : any;
+}
+
+// One block: slot[row] = place of a valid row among the valid ones, or -1 (no loss), -2 (outside the vocabulary);
+// row_of[place] its row; counts = {valid rows, rows with a loss, status}. The kinds come from `kind`, or from targets.
+__global__ void __launch_bounds__(1024) pack_kernel(const int* __restrict__ kind, const long* __restrict__ targets,
+                                                    long ignore, long V, long rows, int* __restrict__ slot,
+                                                    int* __restrict__ row_of, int* __restrict__ counts) {
+  __shared__ int warps[2][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int valid = 0, bad = 0;
+  for (long base = 0; base < rows; base += 1024) {
+    const long t = base + threadIdx.x;
+    const int k = t >= rows ? 0 : kind ? kind[t] : entry_kind(targets[t], false, ignore, V);
+    const unsigned good = __ballot_sync(~0u, k == 1), outside = __ballot_sync(~0u, k == 2);
+    if (lane == 0) {
+      warps[0][warp] = __popc(good);
+      warps[1][warp] = __popc(outside);
+    }
+    __syncthreads();
+    int at = valid + __popc(good & ((1u << lane) - 1));
+    const int g = warps[0][lane], b = warps[1][lane];
+    at += __reduce_add_sync(~0u, lane < warp ? g : 0);
+    valid += __reduce_add_sync(~0u, g);
+    bad += __reduce_add_sync(~0u, b);
+    if (t < rows) slot[t] = k == 1 ? at : -k - (k == 0);
+    if (t < rows && k == 1) row_of[at] = (int)t;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    counts[0] = valid;
+    counts[1] = valid + bad;
+    counts[2] = 0;
+  }
+}
+
+// One block per row, and 64 more for the zero rows that fill the packed rows' last block of 64. A valid row's hidden
+// state goes to its place in `x`; its entries are sorted by vocabulary index (INT_MAX behind the last) with their
+// log-probabilities, and their logits in units of log2 are summed here: they enter the loss with a weight of about one,
+// where all others enter it through the sum of exponentials, so they come from fp32 fused multiply-adds, which round,
+// instead of from the tensor cores, which truncate (see mma_gain). Rows without a gradient get their zeros here.
+__global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ idx, const float* __restrict__ logp,
+                                                     int K, int Kp, long rows, const __nv_bfloat16* __restrict__ hidden,
+                                                     long ldh, const __nv_bfloat16* __restrict__ w, long ldw, int C,
+                                                     float scale2, const int* __restrict__ slot,
+                                                     const int* __restrict__ counts, uint4* __restrict__ x,
+                                                     int* __restrict__ sidx, float* __restrict__ slogp,
+                                                     float* __restrict__ hit, float* __restrict__ row_loss,
+                                                     uint4* __restrict__ dhidden) {
   extern __shared__ unsigned long long keys[];
   const long row = blockIdx.x;
-  __shared__ int bad, held;
-  if (threadIdx.x == 0) bad = held = 0;
-  __syncthreads();
+  const int C8 = C / 8;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  if (row >= rows) {
+    const long n = counts[0], fill = n + (row - rows);
+    if (fill < max((n + 63) / 64 * 64, 64L))
+      for (int c = threadIdx.x; c < C8; c += blockDim.x) x[fill * C8 + c] = zero;
+    return;
+  }
+  const long place = slot[row];
+  if (place < 0) {
+    if (threadIdx.x == 0) row_loss[row] = place == -1 ? 0.f : NAN;
+    if (dhidden)
+      for (int c = threadIdx.x; c < C8; c += blockDim.x) dhidden[row * C8 + c] = zero;
+    return;
+  }
+  const uint4* src = reinterpret_cast<const uint4*>(hidden + row * ldh);
+  for (int c = threadIdx.x; c < C8; c += blockDim.x) x[place * C8 + c] = __ldg(src + c);
   for (int k = threadIdx.x; k < Kp; k += blockDim.x) {
     int v = INT_MAX;
     float lp = 0.f;
-    if (k < K) {
-      const long id = idx[row * K + k];
-      const bool none = logp ? id < 0 : id == ignore;
-      if (!none) {
-        if (id < 0 || id >= V) atomicOr(&bad, 1);
-        else {
-          v = (int)id;
-          lp = logp ? logp[row * K + k] : 0.f;
-          atomicOr(&held, 1);
-        }
-      }
+    if (k < K && idx[row * K + k] >= 0) {
+      v = (int)idx[row * K + k];
+      lp = logp ? logp[row * K + k] : 0.f;
     }
     keys[k] = ((unsigned long long)v << 32) | __float_as_uint(lp);
   }
@@ -53,235 +124,227 @@ __global__ void records_kernel(const long* __restrict__ idx, const float* __rest
     for (int step = size >> 1; step > 0; step >>= 1) {
       for (int i = threadIdx.x; i < Kp / 2; i += blockDim.x) {
         const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-        const bool up = (lo & size) == 0;
         const unsigned long long a = keys[lo], b = keys[hi];
-        if ((a > b) == up) {
+        if ((a > b) == ((lo & size) == 0)) {
           keys[lo] = b;
           keys[hi] = a;
         }
       }
       __syncthreads();
     }
-  for (int k = threadIdx.x; k < K; k += blockDim.x) {
-    sidx[row * K + k] = (int)(keys[k] >> 32);
-    slogp[row * K + k] = __uint_as_float((unsigned)keys[k]);
-  }
-  if (threadIdx.x == 0) kind[row] = bad ? 2 : held;
-}
-
-// count[0] = rows with a loss (valid or NaN).
-__global__ void count_kernel(const int* __restrict__ kind, long rows, int* __restrict__ count) {
-  __shared__ float scratch[32];
-  int n = 0;
-  for (long t = threadIdx.x; t < rows; t += blockDim.x) n += kind[t] != 0;
-  const float total = rt::block_sum((float)n, scratch);
-  if (threadIdx.x == 0) count[0] = (int)total;
-}
-
-// ---------------------------------------------------------------- logits of the held entries
-// hit[row, k] = scale2 x_row . W_sidx (units of log2), one warp per entry. These logits enter the loss with a weight
-// of about one, where all others enter it through the sum of exponentials, so they are summed by fp32 fused
-// multiply-adds, which round, instead of on the tensor cores, which truncate (see mma_gain).
-__global__ void __launch_bounds__(256) held_logits_kernel(const __nv_bfloat16* __restrict__ x, long ldx,
-                                                          const __nv_bfloat16* __restrict__ w, long ldw, int C,
-                                                          long entries, int K, const int* __restrict__ sidx,
-                                                          float scale2, float* __restrict__ hit) {
-  const long e = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
-  if (e >= entries) return;
-  const int v = sidx[e];
-  if (v == INT_MAX) return;
-  const uint4* xr = reinterpret_cast<const uint4*>(x + e / K * ldx);
-  const uint4* wr = reinterpret_cast<const uint4*>(w + (long)v * ldw);
-  float sum = 0.f;
-  for (int c = lane; c < C / 8; c += 32) {
-    float a[8], b[8];
-    rt::unpack8(__ldg(xr + c), a);
-    rt::unpack8(__ldg(wr + c), b);
+  for (int k = threadIdx.x >> 5; k < K; k += blockDim.x >> 5) {
+    const int v = (int)(keys[k] >> 32);
+    float sum = 0.f;
+    if (v != INT_MAX) {
+      const uint4* wr = reinterpret_cast<const uint4*>(w + (long)v * ldw);
+      for (int c = lane; c < C8; c += 32) {
+        float a[8], b[8];
+        rt::unpack8(__ldg(src + c), a);
+        rt::unpack8(__ldg(wr + c), b);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum = fmaf(a[j], b[j], sum);
-  }
-  sum = rt::warp_sum(sum);
-  if (lane == 0) hit[e] = sum * scale2;
-}
-
-// ---------------------------------------------------------------- statistics of one vocabulary piece
-// Block per row over z [rows, width] (columns [first, first + width) of the vocabulary): part[row] = (max, sum of
-// exp2 relative to it) of the row's logits outside the record, in units of log2.
-__global__ void __launch_bounds__(256) piece_stats_kernel(const float* __restrict__ z, int width, int first, int K,
-                                                          const int* __restrict__ sidx, float scale2,
-                                                          float2* __restrict__ part) {
-  extern __shared__ unsigned mask[];  // one bit per column: held
-  __shared__ float2 warps[8];
-  const long row = blockIdx.x;
-  const float* zr = z + row * (long)width;
-  for (int i = threadIdx.x; i < (width + 31) / 32; i += blockDim.x) mask[i] = 0;
-  __syncthreads();
-  for (int k = threadIdx.x; k < K; k += blockDim.x) {
-    const int c = sidx[row * K + k] - first;
-    if (c >= 0 && c < width) atomicOr(&mask[c >> 5], 1u << (c & 31));
-  }
-  __syncthreads();
-  float m = -INFINITY, s = 0.f;
-  for (int c = threadIdx.x; c < width; c += blockDim.x) {
-    if (mask[c >> 5] >> (c & 31) & 1) continue;
-    const float v = zr[c] * scale2;
-    if (v > m) {
-      s *= exp2f(m - v);
-      m = v;
+        for (int j = 0; j < 8; ++j) sum = fmaf(a[j], b[j], sum);
+      }
+      sum = rt::warp_sum(sum);
     }
-    s += v == -INFINITY ? 0.f : exp2f(v - m);
-  }
-  auto merge = [](float2 a, float2 b) {
-    const float m = fmaxf(a.x, b.x);
-    const float fa = a.x == -INFINITY ? 1.f : exp2f(a.x - m), fb = b.x == -INFINITY ? 1.f : exp2f(b.x - m);
-    return make_float2(m, a.y * fa + b.y * fb);
-  };
-  float2 o = make_float2(m, s);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1)
-    o = merge(o, make_float2(__shfl_xor_sync(~0u, o.x, off), __shfl_xor_sync(~0u, o.y, off)));
-  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = o;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < (int)blockDim.x / 32; ++w) o = merge(o, warps[w]);
-    part[row] = o;
-  }
-}
-
-// ---------------------------------------------------------------- rows
-// Warp per row: merges the pieces' statistics in a fixed order, forms the loss and the row's gradient coefficients:
-// d/dz_v = tail[row] exp2(z_v - lse[row]) outside the record, coef[k] for its held entries, both times scale and the
-// row's upstream gradient (given per row, or 1, or 1 / rows with a loss).
-__global__ void rows_kernel(const float2* __restrict__ part, int pieces, long rows, int K, int tail_class,
-                            const int* __restrict__ kind, const int* __restrict__ sidx,
-                            const float* __restrict__ slogp, const float* __restrict__ hit, float scale,
-                            const float* __restrict__ grad, int mean, const int* __restrict__ count,
-                            float* __restrict__ loss, float* __restrict__ lse2, float* __restrict__ tail,
-                            float* __restrict__ coef) {
-  const long row = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (row >= rows) return;
-  if (kind[row] != 1) {
     if (lane == 0) {
-      loss[row] = kind[row] ? NAN : 0.f;
-      lse2[row] = 0.f;
-      tail[row] = 0.f;
+      sidx[place * K + k] = v;
+      slogp[place * K + k] = __uint_as_float((unsigned)keys[k]);
+      hit[place * K + k] = sum * scale2;
     }
-    for (int k = lane; k < K; k += 32) coef[row * K + k] = 0.f;
-    return;
-  }
-  float m = -INFINITY, top = -INFINITY;
-  for (int i = lane; i < pieces; i += 32) m = fmaxf(m, part[i * rows + row].x);
-  for (int k = lane; k < K; k += 32)
-    if (sidx[row * K + k] != INT_MAX) top = fmaxf(top, hit[row * K + k]);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    m = fmaxf(m, __shfl_xor_sync(~0u, m, off));
-    top = fmaxf(top, __shfl_xor_sync(~0u, top, off));
-  }
-  const float peak = fmaxf(m, top);
-  float rest = 0.f, heldz = 0.f;
-  for (int i = lane; i < pieces; i += 32) {
-    const float2 p = part[i * rows + row];
-    rest += p.x == -INFINITY ? p.y : p.y * exp2f(p.x - m);
-  }
-  double P = 0., L = 0.;
-  for (int k = lane; k < K; k += 32) {
-    if (sidx[row * K + k] == INT_MAX) continue;
-    const float z2 = hit[row * K + k], lp = slogp[row * K + k];
-    heldz += exp2f(z2 - peak);
-    const double p = exp((double)lp);
-    P += p;
-    if (!(p <= 0.)) L += p * ((double)lp - (double)z2 * 0.6931471805599453);
-  }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    rest += __shfl_xor_sync(~0u, rest, off);
-    heldz += __shfl_xor_sync(~0u, heldz, off);
-    P += __shfl_xor_sync(~0u, P, off);
-    L += __shfl_xor_sync(~0u, L, off);
-  }
-  // rest is relative to m, heldz to peak
-  const float Z = heldz + (m == -INFINITY ? rest : rest * exp2f(m - peak));
-  const double l2 = (double)peak + log2((double)Z);
-  const double lse = l2 * 0.6931471805599453;
-  const double r = tail_class && P < 1. ? 1. - P : 0.;
-  const bool has_rest = !(rest <= 0.f);  // an empty rest of the vocabulary has no class
-  double w = P, a = P;
-  double value = L + P * lse;
-  if (tail_class) {
-    w = P + r;
-    a = w;
-    if (r > 0. && has_rest) {
-      const double lr = ((double)m + log2((double)rest)) * 0.6931471805599453 - lse;  // log of the student's rest
-      value += r * (log(r) - lr);
-      a = w - r * exp(-lr);
-    }
-  }
-  const float g = scale * (grad ? grad[row] : (mean ? 1.f / (float)max(count[0], 1) : 1.f));
-  if (lane == 0) {
-    loss[row] = (float)value;
-    lse2[row] = (float)l2;
-    tail[row] = g * (float)a;
-  }
-  for (int k = lane; k < K; k += 32) {
-    float c = 0.f;
-    if (sidx[row * K + k] != INT_MAX) {
-      // for one held entry with p = 1 (cross entropy) q - 1 = -Z_rest / Z without cancellation
-      const double p = exp((double)slogp[row * K + k]);
-      const double q = exp2((double)hit[row * K + k] - l2);
-      c = K == 1 && p == 1. ? -g * (m == -INFINITY ? rest : rest * exp2f((float)((double)m - l2))) : g * (float)(w * q - p);
-    }
-    coef[row * K + k] = c;
   }
 }
 
-// out[0] = sum (or mean over rows with a loss) of loss, in a fixed order.
-__global__ void total_kernel(const float* __restrict__ loss, long rows, int mean, const int* __restrict__ count,
-                             float* __restrict__ out) {
+// ---------------------------------------------------------------- losses of the valid rows of a chunk
+// Eight warps per 32 rows: lanes are rows while the tiles' statistics are merged (in a fixed order), then each warp
+// takes four rows and forms their losses and gradient coefficients: d/dz_v = tail exp2(z_v - lse2) outside the record,
+// coef[k] for its held entries, both times scale and the row's upstream gradient (given per row, or 1, or 1 / rows
+// with a loss).
+struct MergeArgs {
+  const float2* part;
+  long part_ld;
+  int tiles, row0, rows, K, tail_class, mean;
+  const int* counts;
+  const int* row_of;
+  const int* sidx;
+  const float* slogp;
+  const float* hit;
+  float scale;
+  const float* grad;
+  float* row_loss;
+  float* lse2;
+  float* tail;
+  float* coef;
+};
+
+__global__ void __launch_bounds__(256) merge_kernel(const MergeArgs p) {
+  __shared__ float2 merged[8][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = min(max(p.counts[0] - p.row0, 0), p.rows);
+  const int first = blockIdx.x * 32;
+  if (first >= n) return;
+  {
+    const int r = first + lane;
+    float m = -INFINITY, s = 0.f;
+    if (r < n)
+      for (int i = warp; i < p.tiles; i += 8) {
+        const float2 t = p.part[i * p.part_ld + r];
+        if (t.x > m) {
+          s = s * exp2f(m - t.x) + t.y;
+          m = t.x;
+        } else {
+          s += t.x == -INFINITY ? t.y : t.y * exp2f(t.x - m);
+        }
+      }
+    merged[warp][lane] = make_float2(m, s);
+  }
+  __syncthreads();
+  for (int j = warp; j < 32 && first + j < n; j += 8) {
+    const int r = first + j;
+    const long place = p.row0 + r, row = p.row_of[place];
+    const int* sidx = p.sidx + place * p.K;
+    const float* slogp = p.slogp + place * p.K;
+    const float* hit = p.hit + place * p.K;
+    float m = -INFINITY, top = -INFINITY;
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, merged[w][j].x);
+    float rest = 0.f;
+    for (int w = 0; w < 8; ++w) {
+      const float2 t = merged[w][j];
+      rest += t.x == -INFINITY ? t.y : t.y * exp2f(t.x - m);
+    }
+    for (int k = lane; k < p.K; k += 32)
+      if (sidx[k] != INT_MAX) top = fmaxf(top, hit[k]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, off));
+    const float peak = fmaxf(m, top);
+    float heldz = 0.f;
+    double P = 0., L = 0.;
+    for (int k = lane; k < p.K; k += 32) {
+      if (sidx[k] == INT_MAX) continue;
+      const float z2 = hit[k], lp = slogp[k];
+      heldz += exp2f(z2 - peak);
+      const double q = exp((double)lp);
+      P += q;
+      if (!(q <= 0.)) L += q * ((double)lp - (double)z2 * 0.6931471805599453);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      heldz += __shfl_xor_sync(~0u, heldz, off);
+      P += __shfl_xor_sync(~0u, P, off);
+      L += __shfl_xor_sync(~0u, L, off);
+    }
+    // rest is relative to m, heldz to peak
+    const float Z = heldz + (m == -INFINITY ? rest : rest * exp2f(m - peak));
+    const double l2 = (double)peak + log2((double)Z);
+    const double lse = l2 * 0.6931471805599453;
+    const double r1 = p.tail_class && P < 1. ? 1. - P : 0.;
+    const double weight = P + r1;
+    double a = weight, value = L + P * lse;
+    if (r1 > 0. && !(rest <= 0.f)) {  // an empty rest of the vocabulary has no class
+      const double lr = ((double)m + log2((double)rest)) * 0.6931471805599453 - lse;  // log of the student's rest
+      value += r1 * (log(r1) - lr);
+      a -= r1 * exp(-lr);
+    }
+    const float g = p.scale * (p.grad ? p.grad[row] : (p.mean ? 1.f / (float)max(p.counts[1], 1) : 1.f));
+    if (lane == 0) {
+      p.row_loss[row] = (float)value;
+      p.lse2[place] = (float)l2;
+      p.tail[place] = g * (float)a;
+    }
+    if (!p.coef) continue;
+    for (int k = lane; k < p.K; k += 32) {
+      float c = 0.f;
+      if (sidx[k] != INT_MAX) {
+        // for one held entry with p = 1 (cross entropy) q - 1 = -Z_rest / Z without cancellation
+        const double q = exp((double)slogp[k]);
+        c = p.K == 1 && q == 1. ? -g * (m == -INFINITY ? rest : rest * exp2f((float)((double)m - l2)))
+                                : g * (float)(weight * exp2((double)hit[k] - l2) - q);
+      }
+      p.coef[place * p.K + k] = c;
+    }
+  }
+}
+
+// Last launch of a call: out[0] = sum (or mean over rows with a loss) of the rows' losses, in a fixed order. A wait that
+// gave up in one of the products makes every loss NaN.
+__global__ void __launch_bounds__(1024) total_kernel(float* __restrict__ loss, long rows, int mean,
+                                                     const int* __restrict__ counts, float* __restrict__ out) {
   __shared__ double part[32];
+  const bool failed = counts[2] != 0;
   double s = 0.;
-  for (long t = threadIdx.x; t < rows; t += blockDim.x) s += (double)loss[t];
+  for (long t = threadIdx.x; t < rows; t += blockDim.x) {
+    if (failed) loss[t] = NAN;
+    else s += (double)loss[t];
+  }
+  if (!out) return;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(~0u, s, off);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < (int)blockDim.x / 32; ++w) s += part[w];
-    out[0] = (float)(mean ? s / (double)max(count[0], 1) : s);
+    out[0] = failed ? NAN : (float)(mean ? s / (double)max(counts[1], 1) : s);
   }
 }
 
-// ---------------------------------------------------------------- gradient of one vocabulary piece
-// dz [rows, ld] bf16 from z [rows, width] fp32; rows without a gradient are zero whatever their logits hold.
-__global__ void __launch_bounds__(256) piece_grad_kernel(const float* __restrict__ z, int width, int first, int ld,
-                                                         int K, const int* __restrict__ sidx, float scale2,
-                                                         const float* __restrict__ lse2,
-                                                         const float* __restrict__ tail,
-                                                         const float* __restrict__ coef, const int* __restrict__ kind,
-                                                         __nv_bfloat16* __restrict__ dz) {
-  const long row = blockIdx.x;
-  const float* zr = z + row * (long)width;
-  __nv_bfloat16* out = dz + row * (long)ld;
-  const float l = lse2[row], a = tail[row];
-  const bool live = kind[row] == 1;
-  for (int c = threadIdx.x; c < ld; c += blockDim.x)
-    out[c] = __float2bfloat16_rn(live && c < width ? a * exp2f(zr[c] * scale2 - l) : 0.f);
-  __syncthreads();
-  for (int k = threadIdx.x; k < K; k += blockDim.x) {
-    const int c = sidx[row * K + k] - first;
-    if (c >= 0 && c < width && live) out[c] = __float2bfloat16_rn(coef[row * K + k]);
+// ---------------------------------------------------------------- gradient of the logits
+// In place: exponentials of a chunk's rows (relative to their tile's maximum) -> dz, one warp per row and tile; rows
+// that fill the last block of 64 become zero. The held entries' places hold zeros until held_gradient_kernel.
+__global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict__ e, long ld, int V, int tiles,
+                                                       int row0, int rows, const int* __restrict__ counts,
+                                                       const float2* __restrict__ part, long part_ld,
+                                                       const float* __restrict__ lse2, const float* __restrict__ tail) {
+  const int n = min(max(counts[0] - row0, 0), rows), r = blockIdx.y;
+  if (r >= max((n + 63) / 64 * 64, 64)) return;
+  const int lane = threadIdx.x & 31;
+  const bool live = r < n;
+  const float l = live ? lse2[row0 + r] : 0.f, a = live ? tail[row0 + r] : 0.f;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int t = (blockIdx.x * 4 + u) * 8 + (threadIdx.x >> 5), c = t * 256 + lane * 8;
+    if (t >= tiles || c >= ld) continue;
+    uint4* at = reinterpret_cast<uint4*>(e + r * ld + c);
+    if (!live) {
+      *at = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    float v[8];
+    rt::unpack8(*at, v);
+    const float m = part[t * part_ld + r].x, f = m == -INFINITY ? 0.f : a * exp2f(m - l);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= f;
+    *at = rt::pack8(v);
   }
 }
 
-// out = x with the rows that have no gradient zero (they may hold anything: 0 times NaN would reach every weight row).
-__global__ void live_rows_kernel(const __nv_bfloat16* __restrict__ x, long ld, int C, const int* __restrict__ kind,
-                                 __nv_bfloat16* __restrict__ out) {
-  const long row = blockIdx.x;
-  const bool live = kind[row] == 1;
-  for (int c = threadIdx.x; c < C; c += blockDim.x)
-    out[row * (long)C + c] = live ? x[row * ld + c] : __float2bfloat16_rn(0.f);
+__global__ void held_gradient_kernel(__nv_bfloat16* __restrict__ dz, long ld, int K, int row0, int rows,
+                                     const int* __restrict__ counts, const int* __restrict__ sidx,
+                                     const float* __restrict__ coef) {
+  const int n = min(max(counts[0] - row0, 0), rows);
+  const long e = (long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (e >= (long)n * K) return;
+  const long at = (long)row0 * K + e;
+  const int v = sidx[at];
+  if (v != INT_MAX) dz[e / K * ld + v] = __float2bfloat16_rn(coef[at]);
+}
+
+// dhidden[row_of[place]] = bf16 of the row's partial sums, added in order.
+__global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ partial, int splits, long split_rows,
+                                                      int C, int row0, int rows, const int* __restrict__ counts,
+                                                      const int* __restrict__ row_of, __nv_bfloat16* __restrict__ out) {
+  const int n = min(max(counts[0] - row0, 0), rows), r = blockIdx.x;
+  if (r >= n) return;
+  uint4* dst = reinterpret_cast<uint4*>(out + (long)row_of[row0 + r] * C);
+  for (int c = threadIdx.x; c < C / 8; c += blockDim.x) {
+    float v[8] = {};
+    for (int s = 0; s < splits; ++s) {
+      const float4* src = reinterpret_cast<const float4*>(partial + ((long)s * split_rows + r) * C) + 2 * c;
+      const float4 x = __ldg(src), y = __ldg(src + 1);
+      v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+      v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    }
+    dst[c] = rt::pack8(v);
+  }
 }
 
 // x *= *factor, nothing at all for a factor of one (the usual upstream gradient of a training loss).
@@ -307,42 +370,101 @@ __global__ void scale_kernel(__nv_bfloat16* __restrict__ x, const float* __restr
 // Undoing it takes the error of log Z from 9.6e-6 to 2e-7 at width 5120.
 float mma_gain(int C) { return 1.f + (float)(C / 16) * 0x1p-26f; }
 
-long up(long n, long to) { return (n + to - 1) / to * to; }
+constexpr long up(long n, long to) { return (n + to - 1) / to * to; }
 
-// Columns of a vocabulary piece: a multiple of 64 whose fp32 logits take about 64 MB, at most 8192.
-int piece_columns(long rows, long V) {
-  const long fit = (16L << 20) / std::max(rows, 1L) / 64 * 64;
-  return (int)std::min(up(V, 64), std::max(256L, std::min(8192L, fit)));
+// Rows of a chunk: with gradients their exponentials take up to 2 GiB of bf16, without their statistics take 8 bytes per
+// row and tile.
+constexpr long CHUNK_VALUES = 1L << 30, CHUNK_ROWS = 32768;
+constexpr long SCORE_ROWS = 16384;
+
+int pairs() {
+  static const int n = [] {
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return std::max(1, sms / 2);
+  }();
+  return n;
+}
+
+// Parts of K = V for dX. A wave of tiles takes kblocks / S blocks of 512 cycles and fills `pairs` pairs, or part of them
+// in the last wave; each part adds a write and a read of rows x C fp32 partial sums (16 bytes per value at about 5
+// TB/s = 2800 bytes a cycle).
+int dx_splits(long rows, long V, int C) {
+  const long tiles = up(rows, 256) / 256 * (up(C, 256) / 256), kblocks = up(V, 64) / 64;
+  int best = 1;
+  double least = 1e300;
+  for (int S = 1; S <= 64 && S <= std::max(1L, kblocks / 16); ++S) {
+    const long waves = (tiles * S + pairs() - 1) / pairs();
+    const double cycles = waves * ((double)kblocks / S * 512 + 3000) + (double)S * rows * C * 16 / 2800;
+    if (cycles < least * 0.995) {
+      least = cycles;
+      best = S;
+    }
+  }
+  return best;
 }
 
 struct Layout {  // offsets in floats, each 16-byte aligned
-  long sidx, slogp, hit, coef, kind, count, lse2, tail, part, z, dz, dx, x, total;
+  long rows, ld_e, tiles, splits, split_rows;  // rows of a chunk, row stride of the exponentials, tiles of the vocabulary
+  bool dw32;
+  long kind, slot, row_of, counts, x, sidx, slogp, hit, coef, lse2, tail, part, e, dx, dw, total;
 };
-Layout layout(long rows, long V, int C, int K, bool grad_h, bool grad_w) {
+Layout layout(long T, long V, int C, int K, bool grad_h, bool grad_w) {
   Layout l;
   long at = 0;
-  auto take = [&](long n) {
+  auto take = [&](long floats) {
     const long o = at;
-    at += up(n, 4);
+    at += up(floats, 4);
     return o;
   };
-  const int cols = piece_columns(rows, V);
-  const long pieces = (V + cols - 1) / cols;
-  l.sidx = take(rows * K);
-  l.slogp = take(rows * K);
-  l.hit = take(rows * K);
-  l.coef = take(rows * K);
-  l.kind = take(rows);
-  l.count = take(4);
-  l.lse2 = take(rows);
-  l.tail = take(rows);
-  l.part = take(2 * rows * pieces);
-  l.z = take(rows * cols);
-  l.dz = take(grad_h || grad_w ? rows * cols / 2 + 4 : 0);
-  l.dx = take(grad_h ? rows * C : 0);
-  l.x = take(grad_w ? rows * C / 2 + 4 : 0);
+  const bool grad = grad_h || grad_w;
+  l.ld_e = up(V, 64);
+  l.tiles = up(V, 256) / 256;
+  l.rows = std::min(up(T, 64),
+                    grad ? std::min(CHUNK_ROWS, std::max(256L, CHUNK_VALUES / l.ld_e / 256 * 256)) : SCORE_ROWS);
+  l.dw32 = grad_w && l.rows < T;
+  l.splits = grad_h ? dx_splits(l.rows, V, C) : 0;
+  l.split_rows = up(l.rows, 256);
+  l.kind = take(T);
+  l.slot = take(T);
+  l.row_of = take(T);
+  l.counts = take(4);
+  l.x = take(up(T, 64) * C / 2);
+  l.sidx = take(T * K);
+  l.slogp = take(T * K);
+  l.hit = take(T * K);
+  l.coef = take(grad ? T * K : 0);
+  l.lse2 = take(T);
+  l.tail = take(T);
+  l.part = take(2 * l.tiles * l.rows);
+  l.e = take(grad ? l.rows * l.ld_e / 2 : 0);
+  l.dx = take(l.splits * l.split_rows * C);
+  l.dw = take(l.dw32 ? V * C : 0);
   l.total = at;
   return l;
+}
+
+bool map2d(CUtensorMap* map, bool f32, const void* base, long inner, long outer, long row_bytes, int box_rows) {
+  const uint64_t dims[2] = {(uint64_t)inner, (uint64_t)outer}, strides[1] = {(uint64_t)row_bytes};
+  const uint32_t box[2] = {f32 ? 32u : 64u, (uint32_t)box_rows};
+  return tmap::encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims,
+                      strides, box);
+}
+
+template <int MODE>
+cudaError_t launch(const head::Maps& maps, const head::Args& args, long units, cudaStream_t s) {
+  static std::atomic<uint64_t> set{0};  // per device: the shared-memory size has been raised
+  int dev = 0;
+  RT_CUDA_CHECK(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!bit || !(set.load(std::memory_order_acquire) & bit)) {
+    RT_CUDA_CHECK(cudaFuncSetAttribute(head::pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       head::SMEM_BYTES));
+    set.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  const unsigned grid = 2 * (unsigned)std::min<long>(units, pairs());
+  head::pair_kernel<MODE><<<grid, head::THREADS, head::SMEM_BYTES, s>>>(maps, args);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -355,71 +477,95 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   if (!p || !work) return cudaErrorInvalidValue;
   const long T = p->rows, V = p->vocab;
   const int C = p->width, K = p->K;
-  if (T < 0 || V < 1 || V > INT_MAX - 1 || T > (1 << 24) || C < 1 || C % 8 || K < 1 || K > RT_HEAD_MAX_RECORD ||
-      (reinterpret_cast<uintptr_t>(work) & 15))
+  if (T < 0 || V < 1 || V > INT_MAX - 512 || T > (1 << 24) || C < 1 || C % 8 || K < 1 || K > RT_HEAD_MAX_RECORD ||
+      (!p->log_probs && K != 1) || p->ld_hidden % 8 || p->ld_weight % 8 || (T && !p->hidden) || !p->weight ||
+      ((reinterpret_cast<uintptr_t>(work) | reinterpret_cast<uintptr_t>(p->hidden) |
+        reinterpret_cast<uintptr_t>(p->weight) | reinterpret_cast<uintptr_t>(p->dhidden) |
+        reinterpret_cast<uintptr_t>(p->dweight)) & 15))
     return cudaErrorInvalidValue;
   if (T == 0) {
     if (p->reduction) RT_CUDA_CHECK(cudaMemsetAsync(p->loss, 0, sizeof(float), s));
     if (p->dweight) RT_CUDA_CHECK(cudaMemsetAsync(p->dweight, 0, (size_t)V * C * 2, s));
     return cudaSuccess;
   }
+  const bool grad = p->dhidden || p->dweight;
   const Layout l = layout(T, V, C, K, p->dhidden != nullptr, p->dweight != nullptr);
-  int* sidx = reinterpret_cast<int*>(work + l.sidx);
-  float* slogp = work + l.slogp;
-  float* hit = work + l.hit;
-  float* coef = work + l.coef;
-  int* kind = reinterpret_cast<int*>(work + l.kind);
-  int* count = reinterpret_cast<int*>(work + l.count);
+  auto ints = [&](long at) { return reinterpret_cast<int*>(work + at); };
+  int* counts = ints(l.counts);
+  __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(work + l.x);
+  __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(work + l.e);
   float2* part = reinterpret_cast<float2*>(work + l.part);
-  float* z = work + l.z;
-  __nv_bfloat16* dz = reinterpret_cast<__nv_bfloat16*>(work + l.dz);
   const float scale2 = p->scale * LOG2E;
-  const float scale2_mma = scale2 * mma_gain(C);
+  if (p->log_probs) kinds_kernel<<<(unsigned)((T * 32 + 255) / 256), 256, 0, s>>>(p->index, T, K, V, ints(l.kind));
+  pack_kernel<<<1, 1024, 0, s>>>(p->log_probs ? ints(l.kind) : nullptr, p->index, p->ignore, V, T, ints(l.slot),
+                                 ints(l.row_of), counts);
   int Kp = 1;
   while (Kp < K) Kp <<= 1;
-  const int threads = std::min(256, std::max(32, Kp / 2));
-  records_kernel<<<(unsigned)T, threads, Kp * 8, s>>>(p->index, p->log_probs, K, Kp, V, p->ignore, sidx, slogp, kind);
-  count_kernel<<<1, 1024, 0, s>>>(kind, T, count);
-  const int cols = piece_columns(T, V);
-  const int pieces = (int)((V + cols - 1) / cols);
-  const __nv_bfloat16* W = reinterpret_cast<const __nv_bfloat16*>(p->weight);
-  held_logits_kernel<<<(unsigned)((T * K * 32 + 255) / 256), 256, 0, s>>>(
-      reinterpret_cast<const __nv_bfloat16*>(p->hidden), p->ld_hidden, W, p->ld_weight, C, T * K, K, sidx, scale2, hit);
-  for (int i = 0; i < pieces; ++i) {
-    const int first = i * cols, width = (int)std::min<long>(cols, V - first);
-    RT_CUDA_CHECK(rt_gemm_bf16(p->hidden, p->ld_hidden, 0, W + (long)first * p->ld_weight, p->ld_weight, 0, z, width,
-                               (int)T, width, C, 1, 1.f, nullptr, s));
-    piece_stats_kernel<<<(unsigned)T, 256, (width + 31) / 32 * 4, s>>>(z, width, first, K, sidx, scale2_mma,
-                                                                       part + (long)i * T);
-  }
-  rows_kernel<<<(unsigned)((T * 32 + 127) / 128), 128, 0, s>>>(part, pieces, T, K, p->tail, kind, sidx, slogp, hit,
-                                                               p->scale, p->row_grad, p->reduction == 2, count,
-                                                               p->row_loss, work + l.lse2, work + l.tail, coef);
-  if (p->reduction) total_kernel<<<1, 1024, 0, s>>>(p->row_loss, T, p->reduction == 2, count, p->loss);
+  gather_kernel<<<(unsigned)(T + 64), 256, Kp * 8, s>>>(
+      p->index, p->log_probs, K, Kp, T, reinterpret_cast<const __nv_bfloat16*>(p->hidden), p->ld_hidden,
+      reinterpret_cast<const __nv_bfloat16*>(p->weight), p->ld_weight, C, scale2, ints(l.slot), counts,
+      reinterpret_cast<uint4*>(x), ints(l.sidx), work + l.slogp, work + l.hit, p->row_loss,
+      reinterpret_cast<uint4*>(p->dhidden));
   RT_CUDA_CHECK(cudaGetLastError());
-  if (!p->dhidden && !p->dweight) return cudaSuccess;
-  float* dx = work + l.dx;
-  if (p->dhidden) RT_CUDA_CHECK(rt_zero_f32(dx, T * C, s));
-  __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(work + l.x);
-  if (p->dweight)
-    live_rows_kernel<<<(unsigned)T, 256, 0, s>>>(reinterpret_cast<const __nv_bfloat16*>(p->hidden), p->ld_hidden, C,
-                                                 kind, x);
-  for (int i = 0; i < pieces; ++i) {
-    const int first = i * cols, width = (int)std::min<long>(cols, V - first);
-    const int ld = (int)up(width, 8);
-    RT_CUDA_CHECK(rt_gemm_bf16(p->hidden, p->ld_hidden, 0, W + (long)first * p->ld_weight, p->ld_weight, 0, z, width,
-                               (int)T, width, C, 1, 1.f, nullptr, s));
-    piece_grad_kernel<<<(unsigned)T, 256, 0, s>>>(z, width, first, ld, K, sidx, scale2_mma, work + l.lse2, work + l.tail,
-                                                  coef, kind, dz);
-    if (p->dhidden)
-      RT_CUDA_CHECK(rt_gemm_bf16(dz, ld, 0, W + (long)first * p->ld_weight, p->ld_weight, 1, dx, C, (int)T, C, width,
-                                 2, 1.f, nullptr, s));
-    if (p->dweight)
-      RT_CUDA_CHECK(rt_gemm_bf16(dz, ld, 1, x, C, 1,
-                                 reinterpret_cast<__nv_bfloat16*>(p->dweight) + (long)first * C, C, width, C, (int)T,
-                                 0, 1.f, nullptr, s));
+
+  head::Maps logits, dx, dw;
+  head::Args args{};
+  args.live = counts;
+  args.V = (int)V;
+  args.C = C;
+  args.K = K;
+  args.scale2 = scale2 * mma_gain(C);
+  args.part = part;
+  args.part_ld = l.rows;
+  args.store_e = grad;
+  args.splits = (int)std::max(1L, l.splits);
+  args.split_rows = (int)l.split_rows;
+  args.status = counts + 2;
+  for (long row0 = 0; row0 < T; row0 += l.rows) {
+    const long rows = std::min(l.rows, up(T - row0, 64));  // packed rows of x are filled up to a block of 64
+    __nv_bfloat16* xc = x + row0 * C;
+    args.row0 = (int)row0;
+    args.rows = (int)l.rows;
+    args.sidx = ints(l.sidx) + row0 * K;
+    args.add = row0 > 0;
+    if (!map2d(&logits.a, false, xc, C, rows, 2L * C, 128) ||
+        !map2d(&logits.b, false, p->weight, C, V, 2 * p->ld_weight, 128) ||
+        !map2d(&logits.out, false, grad ? (void*)e : (void*)xc, grad ? V : C, rows, 2 * (grad ? l.ld_e : C), 32))
+      return cudaErrorInvalidValue;
+    const long tiles_m = up(rows, 256) / 256, tiles_c = up(C, 256) / 256;
+    RT_CUDA_CHECK(launch<head::LOGITS>(logits, args, tiles_m * l.tiles, s));
+    MergeArgs m{part, l.rows, (int)l.tiles, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, counts,
+                ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->scale, p->row_grad, p->row_loss,
+                work + l.lse2, work + l.tail, grad ? work + l.coef : nullptr};
+    merge_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, s>>>(m);
+    if (grad) {
+      gradient_kernel<<<dim3((unsigned)((l.tiles + 31) / 32), (unsigned)rows), 256, 0, s>>>(
+          e, l.ld_e, (int)V, (int)l.tiles, (int)row0, (int)l.rows, counts, part, l.rows, work + l.lse2, work + l.tail);
+      held_gradient_kernel<<<(unsigned)((rows * K + 255) / 256), 256, 0, s>>>(e, l.ld_e, K, (int)row0, (int)l.rows,
+                                                                              counts, ints(l.sidx), work + l.coef);
+    }
+    RT_CUDA_CHECK(cudaGetLastError());
+    if (p->dhidden) {
+      if (!map2d(&dx.a, false, e, V, rows, 2 * l.ld_e, 128) ||
+          !map2d(&dx.b, false, p->weight, C, V, 2 * p->ld_weight, 64) ||
+          !map2d(&dx.out, true, work + l.dx, C, l.splits * l.split_rows, 4L * C, 32))
+        return cudaErrorInvalidValue;
+      RT_CUDA_CHECK(launch<head::DX>(dx, args, tiles_m * tiles_c * l.splits, s));
+      dhidden_kernel<<<(unsigned)rows, 256, 0, s>>>(work + l.dx, (int)l.splits, l.split_rows, C, (int)row0,
+                                                    (int)l.rows, counts, ints(l.row_of),
+                                                    reinterpret_cast<__nv_bfloat16*>(p->dhidden));
+    }
+    if (p->dweight) {
+      void* out = l.dw32 ? (void*)(work + l.dw) : p->dweight;
+      if (!map2d(&dw.a, false, e, V, rows, 2 * l.ld_e, 64) || !map2d(&dw.b, false, xc, C, rows, 2L * C, 64) ||
+          !map2d(&dw.out, l.dw32, out, C, V, (l.dw32 ? 4L : 2L) * C, 32))
+        return cudaErrorInvalidValue;
+      const long units = l.tiles * tiles_c;
+      RT_CUDA_CHECK(l.dw32 ? launch<head::DW32>(dw, args, units, s) : launch<head::DW>(dw, args, units, s));
+    }
   }
-  if (p->dhidden) RT_CUDA_CHECK(rt_to_bf16(dx, p->dhidden, T * C, s));
+  if (l.dw32) RT_CUDA_CHECK(rt_to_bf16(work + l.dw, p->dweight, V * C, s));
+  total_kernel<<<1, 1024, 0, s>>>(p->row_loss, T, p->reduction == 2, counts, p->reduction ? p->loss : nullptr);
   return cudaGetLastError();
 }
 

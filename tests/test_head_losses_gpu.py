@@ -356,3 +356,15 @@ def test_gpu_refusals():
         linear_cross_entropy(hidden, weight.cpu(), targets)
     with pytest.raises(TypeError, match="bf16 or fp32"):
         top_log_probs(hidden.half(), 3)
+
+
+@cuda
+@pytest.mark.parametrize("ignored", [0, 500, 32900])
+def test_more_rows_than_a_chunk(ignored):
+    """32768 rows at a time with gradients, 16384 without; the weight's gradient adds up over the chunks."""
+    hidden, weight, targets, g = _inputs(33000, 300, 64)
+    targets[torch.randperm(33000, device="cuda", generator=g)[:ignored]] = -100
+    _check(hidden, weight, targets[:, None], None, 1.0, False, "sum")
+    loss = linear_cross_entropy(hidden, weight, targets, reduction="none")
+    expected, _, _ = _oracle(hidden, weight, targets[:, None], None, -100, 1.0, 0)
+    torch.testing.assert_close(loss.double(), expected, rtol=1e-5, atol=1e-4)
