@@ -95,7 +95,8 @@ long rt_head_loss_workspace_floats(long rows, long vocab, int width, int K, int 
 cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream_t stream);
 cudaError_t rt_scale_bf16(void* x, const float* factor, long n, cudaStream_t stream);
 cudaError_t rt_top_log_probs(int dtype, const void* logits, long rows, long V, long ld, int k, float scale,
-                             float* logp, long* index, cudaStream_t stream);
+                             float* logp, long* index, void* work, cudaStream_t stream);
+long rt_top_workspace_bytes(int dtype, long rows, long V, int k);
 
 // Teacher-block kernels (bf16 activations, fp32 parameters).
 cudaError_t rt_rmsnorm_1p(const void* x, const void* h, const float* w, void* sum_out, void* out, long rows, int C,

@@ -556,9 +556,13 @@ std::vector<at::Tensor> top_log_probs(at::Tensor logits, int64_t k, double scale
               RT_HEAD_MAX_RECORD, "), got ", k);
   auto logp = at::empty({rows, k}, logits.options().dtype(at::kFloat));
   auto index = at::empty({rows, k}, logits.options().dtype(at::kLong));
+  const long bytes = rt_top_workspace_bytes(dtype, rows, V, (int)k);
+  TORCH_CHECK(bytes >= 0, "top_log_probs: ", V, " logits are too many for k = ", k);
+  at::Tensor work;
+  if (bytes) work = at::empty({bytes}, logits.options().dtype(at::kByte));
   check_cuda(rt_top_log_probs(dtype, logits.data_ptr(), rows, V, logits.stride(0), (int)k, (float)scale,
                               logp.data_ptr<float>(), reinterpret_cast<long*>(index.data_ptr<int64_t>()),
-                              stream_of(logits)),
+                              bytes ? work.data_ptr() : nullptr, stream_of(logits)),
              "top_log_probs");
   return {logp, index};
 }

@@ -1,49 +1,120 @@
 // The k largest log-probabilities of each row of logits, largest first, equal logits by the lowest index.
+//
+// One read of the logits. A row is streamed in groups of 8 or 32 values, whose maxima stay in shared memory, while the
+// softmax's denominator is summed. A value t that k of the maxima reach is reached by k logits at least, so the result
+// lies in the groups whose maximum reaches t: t is searched by bisection of the maxima's order-preserving keys until k
+// to `cap` of them reach it, those groups (about k) are read again, and their values from t up (about k) are sorted as
+// unique 64-bit keys (value above, lower index first below). Rows whose equal values or special values defeat the
+// bounds (thousands of equal maxima, infinities, NaN) take a radix descent over the whole row instead.
+//
+// Bound by memory: per value one packed maximum's half, unpacking, multiply-add, ex2 and add (about 5 issue slots of the
+// 11 that the bandwidth leaves). Several blocks per SM, so that one streams while another selects. Few rows are cut
+// into segments over as many blocks, whose k candidates a second kernel merges.
+#include <algorithm>
 #include <climits>
 #include "../api.h"
 #include "../common/common.cuh"
 
 namespace {
 
-// Order-preserving 32-bit key of a logit: -0 equals +0, and NaN is above every number.
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int MAX_KEYS = 8192;     // group maxima of a segment
+constexpr int BATCH = 4;           // vectors of 16 bytes in flight per thread
+constexpr float LOG2E = 1.4426950408889634f;
+
+// Order-preserving 32-bit key of a logit: -0 equals +0, NaN is above every number; 0 is below all of them.
 __device__ __forceinline__ unsigned order_key(float v) {
   if (v != v) return 0xffffffffu;
   const unsigned b = __float_as_uint(v + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float key_value(unsigned key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+__device__ __forceinline__ unsigned long long entry(unsigned key, int index) {
+  return (unsigned long long)key << 32 | (unsigned)~index;
+}
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
+// Group maxima in shared memory: a bf16's key fits the upper half of its 32-bit key.
+template <typename T> struct Key { using type = unsigned; };
+template <> struct Key<__nv_bfloat16> { using type = unsigned short; };
+template <typename T> __device__ __forceinline__ typename Key<T>::type pack_key(unsigned key) {
+  return (typename Key<T>::type)(sizeof(T) == 2 ? key >> 16 : key);
+}
 
-// Block per row: the k-th largest key by a radix descent over its four bytes, then the entries above it and the first
-// ones equal to it, sorted. The first sweep also sums the softmax's denominator.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// (max of logits, sum of exp2(c (logit - max))).
+__device__ __forceinline__ float2 merge(float2 a, float2 b, float c) {
+  const float m = fmaxf(a.x, b.x);
+  const float fa = a.x == m ? 1.f : exp2f((a.x - m) * c), fb = b.x == m ? 1.f : exp2f((b.x - m) * c);
+  return make_float2(m, a.y * fa + b.y * fb);
+}
+
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) { rt::unpack8(u, f); }
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[4]) {
+  f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ float vec_max(const uint4& u, const __nv_bfloat16*) {
+  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&u);
+  const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float vec_max(const uint4& u, const float*) {
+  float f[4];
+  unpack(u, f);
+  return fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+}
+
+// Sum over the block of a per-thread count (every thread gets it). `slot` cycles over three counters.
+__device__ __forceinline__ int block_count(int n, int* counters, int& slot) {
+  n = __reduce_add_sync(~0u, n);
+  if ((threadIdx.x & 31) == 0 && n) atomicAdd(&counters[slot], n);
+  if (threadIdx.x == 0) counters[slot == 2 ? 0 : slot + 1] = 0;
+  __syncthreads();
+  const int total = counters[slot];
+  slot = slot == 2 ? 0 : slot + 1;
+  return total;
+}
+
+// list[0, n) sorted downwards; its capacity is a power of two of at least n. Entries are unique but for zeros.
+__device__ void sort_down(unsigned long long* list, int n) {
+  int np = 1;
+  while (np < n) np <<= 1;
+  for (int i = n + threadIdx.x; i < np; i += blockDim.x) list[i] = 0;
+  __syncthreads();
+  for (int size = 2; size <= np; size <<= 1)
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      for (int i = threadIdx.x; i < np / 2; i += blockDim.x) {
+        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+        const unsigned long long a = list[lo], b = list[hi];
+        if ((a < b) == ((lo & size) == 0)) {
+          list[lo] = b;
+          list[hi] = a;
+        }
+      }
+      __syncthreads();
+    }
+}
+
+// The k largest entries of z[0, n) into list, unsorted, by a radix descent over the keys' bytes: five reads of the row.
 template <typename T>
-__global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logits, long ld, int V, int k, int kp,
-                                                      float scale, float* __restrict__ logp, long* __restrict__ index) {
-  extern __shared__ unsigned long long pick[];  // kp entries: key above, ~index below
+__device__ __noinline__ void descend(const T* z, int n, int k, unsigned long long* list) {
   __shared__ int hist[256];
   __shared__ int found, need, digit, wsum[WARPS];
-  __shared__ float2 warps[WARPS];
-  __shared__ float lse;
-  const T* z = logits + blockIdx.x * ld;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned prefix = 0, seen = 0;
   int left = k;
-  float m = -INFINITY, s = 0.f;
   for (int shift = 24; shift >= 0; shift -= 8) {
     for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
     __syncthreads();
-    for (int v = tid; v < V; v += THREADS) {
-      const float x = rt::to_f<T>(z[v]);
-      const unsigned key = order_key(x);
+    for (int v = tid; v < n; v += THREADS) {
+      const unsigned key = order_key(rt::to_f<T>(z[v]));
       if ((key & seen) == prefix) atomicAdd(&hist[key >> shift & 255], 1);
-      if (shift == 24) {
-        const float y = x * scale;
-        if (y > m) {
-          s *= expf(m - y);
-          m = y;
-        }
-        s += y == -INFINITY && m == -INFINITY ? 0.f : expf(y - m);
-      }
     }
     __syncthreads();
     if (tid == 0) {
@@ -58,31 +129,14 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
     left = need;
     __syncthreads();
   }
-  auto merge = [](float2 a, float2 b) {
-    const float m = fmaxf(a.x, b.x);
-    const float fa = a.x == -INFINITY ? 1.f : expf(a.x - m), fb = b.x == -INFINITY ? 1.f : expf(b.x - m);
-    return make_float2(m, a.y * fa + b.y * fb);
-  };
-  float2 o = make_float2(m, s);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1)
-    o = merge(o, make_float2(__shfl_xor_sync(~0u, o.x, off), __shfl_xor_sync(~0u, o.y, off)));
-  if (lane == 0) warps[warp] = o;
-  for (int i = tid; i < kp; i += THREADS) pick[i] = 0;
   if (tid == 0) found = 0;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < WARPS; ++w) o = merge(o, warps[w]);
-    lse = o.x + logf(o.y);
-  }
-  // entries above the threshold in any order, the first `left` equal ones in index order
-  int equal = 0;
-  for (int base = 0; base < V; base += THREADS) {
+  int equal = 0;  // entries above the threshold in any order, the first `left` equal ones in index order
+  for (int base = 0; base < n; base += THREADS) {
     const int v = base + tid;
-    const unsigned key = v < V ? order_key(rt::to_f<T>(z[v])) : 0u;
-    const unsigned long long entry = (unsigned long long)key << 32 | (unsigned)~v;
-    if (v < V && key > prefix) pick[atomicAdd(&found, 1)] = entry;
-    const bool same = v < V && key == prefix;
+    const unsigned key = v < n ? order_key(rt::to_f<T>(z[v])) : 0u;
+    if (v < n && key > prefix) list[atomicAdd(&found, 1)] = entry(key, v);
+    const bool same = v < n && key == prefix;
     const unsigned ballot = __ballot_sync(~0u, same);
     if (lane == 0) wsum[warp] = __popc(ballot);
     __syncthreads();
@@ -91,45 +145,345 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
       before += w < warp ? wsum[w] : 0;
       all += wsum[w];
     }
-    if (same && before < left) pick[k - left + before] = entry;
+    if (same && before < left) list[k - left + before] = entry(key, v);
     equal += all;
     __syncthreads();
   }
-  for (int size = 2; size <= kp; size <<= 1)
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      for (int i = tid; i < kp / 2; i += THREADS) {
-        const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-        const bool down = (lo & size) == 0;
-        const unsigned long long a = pick[lo], b = pick[hi];
-        if ((a < b) == down) {
-          pick[lo] = b;
-          pick[hi] = a;
+}
+
+struct TopArgs {
+  long ld;
+  int V, k, segments, capacity;  // capacity of the list, a power of two of at least 2 k
+  float scale;
+  float* logp;                   // [rows, k]
+  long* index;
+  unsigned long long* entries;   // segments > 1: [rows, segments, k], zeros behind a short segment's values
+  float2* sums;                  // [rows, segments]
+};
+
+// list[0, n), n >= min(k, available): the row's result from its candidates and denominator.
+__device__ void write_row(const TopArgs& a, long row, unsigned long long* list, int n, float2 ms) {
+  const float lse = ms.x * a.scale + logf(ms.y);
+  auto put = [&](int rank, unsigned long long e) {
+    a.index[row * a.k + rank] = (long)(int)~(unsigned)e;
+    a.logp[row * a.k + rank] = key_value((unsigned)(e >> 32)) * a.scale - lse;
+  };
+  if (n <= 512) {  // place = number of larger entries
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const unsigned long long e = list[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += list[j] > e;
+      if (rank < a.k) put(rank, e);
+    }
+    return;
+  }
+  sort_down(list, n);
+  for (int i = threadIdx.x; i < a.k; i += blockDim.x) put(i, list[i]);
+}
+
+// Block (segment, row). U = vectors of a group: 1, or BATCH for long segments.
+template <typename T, int U>
+__global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logits, const TopArgs a) {
+  constexpr int VEC = 16 / sizeof(T);
+  using K = typename Key<T>::type;
+  extern __shared__ __align__(16) uint8_t smem[];
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(smem);
+  K* keys = reinterpret_cast<K*>(list + a.capacity);
+  __shared__ int counters[3], picked, found;
+  __shared__ float2 warps[WARPS];
+  __shared__ unsigned short groups[2048];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const long row = blockIdx.y;
+  const int lo = (int)((long)a.V * blockIdx.x / a.segments), n = (int)((long)a.V * (blockIdx.x + 1) / a.segments) - lo;
+  const T* z = logits + row * a.ld + lo;
+  const float c = a.scale * LOG2E;
+  // aligned vectors, and the few values before and behind them, one per thread
+  const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int)sizeof(T));
+  const int nvec = (n - head) / VEC, tail = n - head - nvec * VEC;
+  const uint4* zv = reinterpret_cast<const uint4*>(z + head);
+  int single = -1;
+  if (tid < head) single = tid;
+  else if (tid >= 16 && tid < 16 + tail) single = n - tail + (tid - 16);
+  if (tid == 0) counters[0] = counters[1] = counters[2] = picked = found = 0;
+
+  float m = -INFINITY, s = 0.f;
+  bool special = false;  // NaN or +inf: left to the descent
+  unsigned single_key = 0;
+  if (single >= 0) {
+    const float v = rt::to_f<T>(z[single]);
+    single_key = order_key(v);
+    special = !(v < INFINITY);
+    if (v > -INFINITY) {
+      m = v;
+      s = 1.f;
+    }
+    if (special) s = NAN;
+  }
+  const int steps = (nvec + BATCH * THREADS - 1) / (BATCH * THREADS);
+  for (int it = 0; it < steps; ++it) {
+    uint4 u[BATCH];
+    float g[BATCH];
+    const int v0 = it * BATCH * THREADS + tid;
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;  // -inf
+      u[b] = v0 + b * THREADS < nvec ? __ldg(zv + v0 + b * THREADS) : make_uint4(none, none, none, none);
+    }
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) g[b] = vec_max(u[b], (const T*)nullptr);
+    const float top = fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3]));
+    if (U == 1) {
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b)
+        keys[(it * BATCH + b) * THREADS + tid] = v0 + b * THREADS < nvec ? pack_key<T>(order_key(g[b])) : (K)0;
+    } else {
+      keys[it * THREADS + tid] = v0 < nvec ? pack_key<T>(order_key(top)) : (K)0;
+    }
+    if (top > m) {
+      s *= m == -INFINITY ? 0.f : ex2((m - top) * c);
+      m = top;
+    }
+    const float mc = m == -INFINITY ? 0.f : m * c;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      float f[VEC];
+      unpack(u[b], f);
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) {
+        s0 += ex2(fmaf(f[j], c, -mc));
+        s1 += ex2(fmaf(f[j + 1], c, -mc));
+      }
+    }
+    s += s0 + s1;
+  }
+  float2 o = make_float2(m, s);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+    o = merge(o, make_float2(__shfl_xor_sync(~0u, o.x, off), __shfl_xor_sync(~0u, o.y, off)), c);
+  if (lane == 0) warps[tid >> 5] = o;
+  __syncthreads();
+  o = warps[0];
+  for (int w = 1; w < WARPS; ++w) o = merge(o, warps[w], c);
+
+  // ---- threshold
+  const int slots = steps * THREADS * (U == 1 ? BATCH : 1);
+  const int cap = min(2048, max(2 * a.k, 128));
+  int slot = 0;
+  unsigned threshold = 0;
+  // NaN and +inf make the sum NaN; a row of -inf has nothing above it
+  bool ok = !special && o.y == o.y && o.x > -INFINITY;
+  ok = !__syncthreads_or(!ok);
+  auto reaching = [&](unsigned t) {
+    int count = single_key >= t && single >= 0;
+    const K tk = pack_key<T>(t);
+#pragma unroll 4
+    for (int i = tid; i < slots; i += THREADS) count += keys[i] >= tk;
+    return block_count(count, counters, slot);
+  };
+  if (ok && slots + 2 * VEC > cap) {
+    // keys compare in steps of the kept bits
+    const int shift = sizeof(T) == 2 ? 16 : 0;
+    unsigned below = 0, above = (order_key(o.x) >> shift) + 1;  // too many (or all) reach `below`, under k `above`
+    ok = false;
+    int low = slots + 2 * VEC;
+    while (above - below > 1) {
+      const unsigned mid = below + (above - below) / 2;
+      const int count = reaching(mid << shift);
+      if (count < a.k) {
+        above = mid;
+      } else {
+        below = mid;
+        low = count;
+        if (count <= cap) break;
+      }
+    }
+    ok = low <= cap;
+    threshold = below << shift;
+    if (!ok && below == 0) {  // fewer than k groups in all: every value is a candidate
+      threshold = 0;
+      ok = reaching(1u << shift) < a.k;
+    }
+  }
+  // ---- candidates
+  if (ok) {
+    const K tk = pack_key<T>(threshold);
+    for (int i = tid; i < slots; i += THREADS) {
+      const K key = keys[i];
+      if (key && key >= tk) {
+        const int at = atomicAdd(&picked, 1);
+        if (at < 2048) groups[at] = (unsigned short)i;
+      }
+    }
+    if (single >= 0 && single_key >= threshold) {
+      const int at = atomicAdd(&found, 1);
+      if (at < a.capacity) list[at] = entry(single_key, lo + single);
+    }
+    __syncthreads();
+    ok = picked <= 2048;
+    for (int i = tid; ok && i < picked * U; i += THREADS) {
+      const int g = groups[i / U];
+      const int v = U == 1 ? g : (g / THREADS) * BATCH * THREADS + (i % U) * THREADS + g % THREADS;
+      if (v >= nvec) continue;
+      float f[VEC];
+      unpack(__ldg(zv + v), f);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const unsigned key = order_key(f[j]);
+        if (key >= threshold) {
+          const int at = atomicAdd(&found, 1);
+          if (at < a.capacity) list[at] = entry(key, lo + head + v * VEC + j);
         }
       }
-      __syncthreads();
     }
-  for (int i = tid; i < k; i += THREADS) {
-    const int v = (int)~(unsigned)pick[i];
-    index[(long)blockIdx.x * k + i] = v;
-    logp[(long)blockIdx.x * k + i] = rt::to_f<T>(z[v]) * scale - lse;
+    __syncthreads();
+    ok = ok && found <= a.capacity;
   }
+  int have = found;
+  if (!ok) {
+    have = min(n, a.k);
+    __syncthreads();
+    descend<T>(z, n, have, list);
+    __syncthreads();
+    for (int i = tid; i < have; i += THREADS) list[i] -= (unsigned)lo;  // ~(index + lo) = ~index - lo
+    __syncthreads();
+  }
+  if (a.segments == 1) {
+    write_row(a, row, list, have, o);
+    return;
+  }
+  const long at = row * a.segments + blockIdx.x;
+  if (tid == 0) a.sums[at] = o;
+  if (have > a.k) sort_down(list, have);
+  for (int i = tid; i < a.k; i += THREADS) a.entries[at * a.k + i] = i < have ? list[i] : 0ull;
+}
+
+constexpr int MERGE_THREADS = 512, MERGE_EACH = 16;
+
+// Block per row: the segments' candidates, at most MERGE_THREADS x MERGE_EACH, are unique, so bisection of the keys
+// always ends at a threshold that k to `capacity` of them reach.
+__global__ void __launch_bounds__(MERGE_THREADS) top_merge_kernel(const TopArgs a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(smem);
+  __shared__ int counters[3], found;
+  __shared__ unsigned long long peak;
+  const long row = blockIdx.x;
+  const int tid = threadIdx.x, total = a.segments * a.k;
+  const unsigned long long* in = a.entries + row * total;
+  unsigned long long e[MERGE_EACH], top = 0;
+#pragma unroll
+  for (int j = 0; j < MERGE_EACH; ++j) {
+    e[j] = j * MERGE_THREADS + tid < total ? in[j * MERGE_THREADS + tid] : 0ull;
+    top = e[j] > top ? e[j] : top;
+  }
+  if (tid == 0) {
+    counters[0] = counters[1] = counters[2] = found = 0;
+    peak = 0;
+  }
+  __syncthreads();
+  atomicMax(&peak, top);
+  __syncthreads();
+  int slot = 0;
+  unsigned long long below = 1, above = peak + 1;
+  if (total > a.capacity)
+    while (above - below > 1) {
+      const unsigned long long mid = below + (above - below) / 2;
+      int count = 0;
+#pragma unroll
+      for (int j = 0; j < MERGE_EACH; ++j) count += e[j] >= mid;
+      count = block_count(count, counters, slot);
+      if (count < a.k) {
+        above = mid;
+      } else {
+        below = mid;
+        if (count <= a.capacity) break;
+      }
+    }
+#pragma unroll
+  for (int j = 0; j < MERGE_EACH; ++j)
+    if (e[j] >= below) list[atomicAdd(&found, 1)] = e[j];
+  const float c = a.scale * LOG2E;
+  float2 ms = a.sums[row * a.segments];
+  for (int i = 1; i < a.segments; ++i) ms = merge(ms, a.sums[row * a.segments + i], c);
+  __syncthreads();
+  write_row(a, row, list, found, ms);
+}
+
+int capacity_for(int k) {
+  int c = 1024;
+  while (c < 4 * k) c <<= 1;
+  return c;
+}
+
+// Segments of a row: enough blocks for two per SM while a segment keeps 4096 values and the merge's candidates fit,
+// and no more vectors per segment than its maxima have room (past a million values, a long record may not fit: 0).
+int segments_for(int dtype, long rows, long V, int k) {
+  const int vec = dtype == 1 ? 8 : 4;
+  const long least = (V / vec + (long)MAX_KEYS * BATCH - 1) / ((long)MAX_KEYS * BATCH);
+  const long spread = std::min({(2L * 148 + rows - 1) / std::max(rows, 1L), V / 4096,
+                                (long)MERGE_THREADS * MERGE_EACH / k});
+  const long segments = std::max({1L, least, spread});
+  return segments == 1 || segments * k <= MERGE_THREADS * MERGE_EACH ? (int)segments : 0;
+}
+
+template <typename T, int U>
+cudaError_t launch(const T* logits, long rows, const TopArgs& a, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
+  const long longest = (a.V + a.segments - 1) / a.segments;
+  const long steps = (longest / VEC + BATCH * THREADS - 1) / (BATCH * THREADS);
+  const size_t smem = (size_t)a.capacity * 8 + (size_t)steps * THREADS * (U == 1 ? BATCH : 1) *
+                                                   sizeof(typename Key<T>::type);
+  if (smem > 40 * 1024)  // 48 KB without asking, static arrays included
+    RT_CUDA_CHECK(cudaFuncSetAttribute(top_kernel<T, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  for (long r = 0; r < rows; r += 65535) {
+    const long some = std::min(rows - r, 65535L);
+    TopArgs b = a;
+    b.logp += r * a.k;
+    b.index += r * a.k;
+    b.entries += r * a.segments * a.k;
+    b.sums += r * a.segments;
+    top_kernel<T, U><<<dim3((unsigned)a.segments, (unsigned)some), THREADS, smem, s>>>(logits + r * a.ld, b);
+  }
+  return cudaGetLastError();
 }
 
 }  // namespace
 
-// dtype 1 = bf16, 0 = fp32; logits [rows, V] with row stride ld; logp, index [rows, k].
+extern "C" long rt_top_workspace_bytes(int dtype, long rows, long V, int k) {
+  const int s = segments_for(dtype, rows, V, k);
+  return s > 1 ? rows * s * (8L * k + 8) : s - 1;  // -1: too many logits for a record of this length
+}
+
+// dtype 1 = bf16, 0 = fp32; logits [rows, V] with row stride ld; logp, index [rows, k]; work: rt_top_workspace_bytes,
+// 16-byte aligned.
 extern "C" cudaError_t rt_top_log_probs(int dtype, const void* logits, long rows, long V, long ld, int k, float scale,
-                                        float* logp, long* index, cudaStream_t s) {
-  if (rows < 0 || rows > INT_MAX || V < 1 || V > INT_MAX - THREADS || k < 1 || k > V || k > RT_HEAD_MAX_RECORD)
+                                        float* logp, long* index, void* work, cudaStream_t s) {
+  if (rows < 0 || rows > INT_MAX || V < 1 || V > INT_MAX / 2 || k < 1 || k > V || k > RT_HEAD_MAX_RECORD)
     return cudaErrorInvalidValue;
   if (rows == 0) return cudaSuccess;
-  int kp = 1;
-  while (kp < k) kp <<= 1;
-  if (dtype == 1)
-    top_kernel<__nv_bfloat16><<<(unsigned)rows, THREADS, kp * 8, s>>>((const __nv_bfloat16*)logits, ld, (int)V, k, kp,
-                                                                     scale, logp, index);
-  else
-    top_kernel<float><<<(unsigned)rows, THREADS, kp * 8, s>>>((const float*)logits, ld, (int)V, k, kp, scale, logp,
-                                                             index);
+  TopArgs a{};
+  a.ld = ld;
+  a.V = (int)V;
+  a.k = k;
+  a.segments = segments_for(dtype, rows, V, k);
+  a.capacity = capacity_for(k);
+  a.scale = scale;
+  a.logp = logp;
+  a.index = index;
+  if (a.segments == 0 || (a.segments > 1 && !work)) return cudaErrorInvalidValue;
+  if (a.segments > 1) {
+    a.entries = static_cast<unsigned long long*>(work);
+    a.sums = reinterpret_cast<float2*>(a.entries + rows * a.segments * k);
+  }
+  const long values = (V + a.segments - 1) / a.segments;
+  if (dtype == 1) {
+    const auto* z = static_cast<const __nv_bfloat16*>(logits);
+    RT_CUDA_CHECK((values / 8 <= MAX_KEYS ? launch<__nv_bfloat16, 1>(z, rows, a, s)
+                                          : launch<__nv_bfloat16, BATCH>(z, rows, a, s)));
+  } else {
+    const auto* z = static_cast<const float*>(logits);
+    RT_CUDA_CHECK((values / 4 <= MAX_KEYS ? launch<float, 1>(z, rows, a, s) : launch<float, BATCH>(z, rows, a, s)));
+  }
+  if (a.segments > 1) top_merge_kernel<<<(unsigned)rows, MERGE_THREADS, a.capacity * 8, s>>>(a);
   return cudaGetLastError();
 }
