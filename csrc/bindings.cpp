@@ -6,6 +6,7 @@
 
 #include <map>
 #include <string>
+#include <tuple>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <vector>
@@ -544,23 +545,27 @@ void scale_bf16_(at::Tensor x, at::Tensor factor) {
   check_cuda(rt_scale_bf16(x.data_ptr(), factor.data_ptr<float>(), x.numel(), stream_of(x)), "scale_bf16_");
 }
 
-// The k largest log-probabilities of softmax(scale * logits) per row and their indices, largest first, equal logits by
-// the lowest index.
-std::vector<at::Tensor> top_log_probs(at::Tensor logits, int64_t k, double scale) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1,
-              "top_log_probs: CUDA [rows, V] logits with unit inner stride");
+// The k largest log-probabilities of softmax(scale * logits) over the last axis and their indices, largest first, equal
+// logits by the lowest index.
+std::tuple<at::Tensor, at::Tensor> top_log_probs(const at::Tensor& logits, int64_t k, double scale) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() >= 1, "top_log_probs: CUDA logits [..., V]");
   c10::cuda::CUDAGuard guard(logits.device());
   const int dtype = dtype_code(logits);
-  const long rows = logits.size(0), V = logits.size(1);
+  const long V = logits.size(-1);
   TORCH_CHECK(k >= 1 && k <= V && k <= RT_HEAD_MAX_RECORD, "top_log_probs: k must be in 1..min(V, ",
               RT_HEAD_MAX_RECORD, "), got ", k);
-  auto logp = at::empty({rows, k}, logits.options().dtype(at::kFloat));
-  auto index = at::empty({rows, k}, logits.options().dtype(at::kLong));
+  at::Tensor z = logits.dim() == 2 ? logits : logits.reshape({-1, V});
+  if (z.stride(1) != 1) z = z.contiguous();
+  const long rows = z.size(0);
+  auto shape = logits.sizes().vec();
+  shape.back() = k;
+  auto logp = at::empty(shape, logits.options().dtype(at::kFloat));
+  auto index = at::empty(shape, logits.options().dtype(at::kLong));
   const long bytes = rt_top_workspace_bytes(dtype, rows, V, (int)k);
   TORCH_CHECK(bytes >= 0, "top_log_probs: ", V, " logits are too many for k = ", k);
   at::Tensor work;
   if (bytes) work = at::empty({bytes}, logits.options().dtype(at::kByte));
-  check_cuda(rt_top_log_probs(dtype, logits.data_ptr(), rows, V, logits.stride(0), (int)k, (float)scale,
+  check_cuda(rt_top_log_probs(dtype, z.data_ptr(), rows, V, z.stride(0), (int)k, (float)scale,
                               logp.data_ptr<float>(), reinterpret_cast<long*>(index.data_ptr<int64_t>()),
                               bytes ? work.data_ptr() : nullptr, stream_of(logits)),
              "top_log_probs");

@@ -2,10 +2,11 @@
 //
 // One read of the logits. A row is streamed in groups of 8 or 32 values, whose maxima stay in shared memory, while the
 // softmax's denominator is summed. A value t that k of the maxima reach is reached by k logits at least, so the result
-// lies in the groups whose maximum reaches t: t is searched by bisection of the maxima's order-preserving keys until k
-// to `cap` of them reach it, those groups (about k) are read again, and their values from t up (about k) are sorted as
-// unique 64-bit keys (value above, lower index first below). Rows whose equal values or special values defeat the
-// bounds (thousands of equal maxima, infinities, NaN) take a radix descent over the whole row instead.
+// lies in the groups whose maximum reaches t. t is the k-th largest of 2 k to 4 k maxima over several groups each, found
+// by one warp's bisection of their order-preserving keys; the groups that reach it (about 1.2 k) are read again, and
+// their values from t up are sorted as unique 64-bit keys (value above, lower index first below). Rows whose equal or
+// special values defeat the bounds (thousands of equal maxima, infinities, NaN) take a radix descent over the whole
+// row instead.
 //
 // Bound by memory: per value one packed maximum's half, unpacking, multiply-add, ex2 and add (about 5 issue slots of the
 // 11 that the bandwidth leaves). Several blocks per SM, so that one streams while another selects. Few rows are cut
@@ -19,6 +20,7 @@ namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int MAX_KEYS = 8192;     // group maxima of a segment
+constexpr int MAX_GROUPS = 2048;   // groups read again
 constexpr int BATCH = 4;           // vectors of 16 bytes in flight per thread
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -79,6 +81,29 @@ __device__ __forceinline__ int block_count(int n, int* counters, int& slot) {
   const int total = counters[slot];
   slot = slot == 2 ? 0 : slot + 1;
   return total;
+}
+
+// By one warp: the largest t found that at least k of maxima[0, 32 each) reach and, as far as they differ, few more (0
+// where fewer than k are above 0). `top` is their largest; each is a multiple of 8.
+template <typename K>
+__device__ __forceinline__ unsigned reached_by(const K* maxima, int each, int k, unsigned top) {
+  unsigned below = 0, above = top + 1;
+  while (above - below > 1) {
+    const unsigned mid = below + (above - below) / 2;
+    int count = 0;
+    for (int j = 0; j < each; j += 8) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) count += (unsigned)maxima[(j + q) * 32 + (threadIdx.x & 31)] >= mid;
+    }
+    count = __reduce_add_sync(~0u, count);
+    if (count < k) {
+      above = mid;
+    } else {
+      below = mid;
+      if (count <= k + k / 16) break;
+    }
+  }
+  return below;
 }
 
 // list[0, n) sorted downwards; its capacity is a power of two of at least n. Entries are unique but for zeros.
@@ -189,9 +214,11 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
   extern __shared__ __align__(16) uint8_t smem[];
   unsigned long long* list = reinterpret_cast<unsigned long long*>(smem);
   K* keys = reinterpret_cast<K*>(list + a.capacity);
-  __shared__ int counters[3], picked, found;
+  K* maxima = reinterpret_cast<K*>(list);  // until candidates are listed
+  __shared__ int picked, found;
+  __shared__ unsigned bound;
   __shared__ float2 warps[WARPS];
-  __shared__ unsigned short groups[2048];
+  __shared__ unsigned short groups[MAX_GROUPS];
   const int tid = threadIdx.x, lane = tid & 31;
   const long row = blockIdx.y;
   const int lo = (int)((long)a.V * blockIdx.x / a.segments), n = (int)((long)a.V * (blockIdx.x + 1) / a.segments) - lo;
@@ -204,7 +231,7 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
   int single = -1;
   if (tid < head) single = tid;
   else if (tid >= 16 && tid < 16 + tail) single = n - tail + (tid - 16);
-  if (tid == 0) counters[0] = counters[1] = counters[2] = picked = found = 0;
+  if (tid == 0) picked = found = 0;
 
   float m = -INFINITY, s = 0.f;
   bool special = false;  // NaN or +inf: left to the descent
@@ -266,44 +293,28 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
   o = warps[0];
   for (int w = 1; w < WARPS; ++w) o = merge(o, warps[w], c);
 
-  // ---- threshold
+  // ---- threshold: THREADS x parts maxima, each of one thread's every parts-th group; the k-th largest of them
   const int slots = steps * THREADS * (U == 1 ? BATCH : 1);
-  const int cap = min(2048, max(2 * a.k, 128));
-  int slot = 0;
-  unsigned threshold = 0;
+  unsigned threshold = 0;  // every value, where there are few groups
   // NaN and +inf make the sum NaN; a row of -inf has nothing above it
   bool ok = !special && o.y == o.y && o.x > -INFINITY;
   ok = !__syncthreads_or(!ok);
-  auto reaching = [&](unsigned t) {
-    int count = single_key >= t && single >= 0;
-    const K tk = pack_key<T>(t);
-#pragma unroll 4
-    for (int i = tid; i < slots; i += THREADS) count += keys[i] >= tk;
-    return block_count(count, counters, slot);
-  };
-  if (ok && slots + 2 * VEC > cap) {
-    // keys compare in steps of the kept bits
-    const int shift = sizeof(T) == 2 ? 16 : 0;
-    unsigned below = 0, above = (order_key(o.x) >> shift) + 1;  // too many (or all) reach `below`, under k `above`
-    ok = false;
-    int low = slots + 2 * VEC;
-    while (above - below > 1) {
-      const unsigned mid = below + (above - below) / 2;
-      const int count = reaching(mid << shift);
-      if (count < a.k) {
-        above = mid;
-      } else {
-        below = mid;
-        low = count;
-        if (count <= cap) break;
-      }
+  if (ok && slots > max(2 * a.k, 128)) {
+    int parts = 1;
+    while (parts < 8 && parts * (THREADS / 2) < a.k) parts <<= 1;
+    for (int p = 0; p < parts; ++p) {
+      unsigned best = 0;
+      for (int i = tid + p * THREADS; i < slots; i += parts * THREADS) best = max(best, (unsigned)keys[i]);
+      maxima[p * THREADS + tid] = (K)best;
     }
-    ok = low <= cap;
-    threshold = below << shift;
-    if (!ok && below == 0) {  // fewer than k groups in all: every value is a candidate
-      threshold = 0;
-      ok = reaching(1u << shift) < a.k;
+    __syncthreads();
+    if (tid < 32) {
+      const int shift = sizeof(T) == 2 ? 16 : 0;
+      const unsigned t = reached_by(maxima, 8 * parts, a.k, order_key(o.x) >> shift) << shift;
+      if (lane == 0) bound = t;
     }
+    __syncthreads();
+    threshold = bound;
   }
   // ---- candidates
   if (ok) {
@@ -312,7 +323,7 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
       const K key = keys[i];
       if (key && key >= tk) {
         const int at = atomicAdd(&picked, 1);
-        if (at < 2048) groups[at] = (unsigned short)i;
+        if (at < MAX_GROUPS) groups[at] = (unsigned short)i;
       }
     }
     if (single >= 0 && single_key >= threshold) {
@@ -320,7 +331,7 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
       if (at < a.capacity) list[at] = entry(single_key, lo + single);
     }
     __syncthreads();
-    ok = picked <= 2048;
+    ok = picked <= MAX_GROUPS;
     for (int i = tid; ok && i < picked * U; i += THREADS) {
       const int g = groups[i / U];
       const int v = U == 1 ? g : (g / THREADS) * BATCH * THREADS + (i % U) * THREADS + g % THREADS;
@@ -360,35 +371,63 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
 
 constexpr int MERGE_THREADS = 512, MERGE_EACH = 16;
 
-// Block per row: the segments' candidates, at most MERGE_THREADS x MERGE_EACH, are unique, so bisection of the keys
-// always ends at a threshold that k to `capacity` of them reach.
+// Block per row: the segments' candidates, at most MERGE_THREADS x MERGE_EACH. The threshold is found as above, from
+// the maxima of one or a few candidates each; where too many are equal to it, by bisection of the unique 64-bit keys.
 __global__ void __launch_bounds__(MERGE_THREADS) top_merge_kernel(const TopArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   unsigned long long* list = reinterpret_cast<unsigned long long*>(smem);
+  unsigned* maxima = reinterpret_cast<unsigned*>(smem);  // until candidates are listed
   __shared__ int counters[3], found;
-  __shared__ unsigned long long peak;
+  __shared__ unsigned peak, bound;
+  __shared__ float2 sums[MERGE_THREADS / 32];
   const long row = blockIdx.x;
-  const int tid = threadIdx.x, total = a.segments * a.k;
+  const int tid = threadIdx.x, total = a.segments * a.k, parts = a.k <= MERGE_THREADS / 2 ? 1 : 4;
   const unsigned long long* in = a.entries + row * total;
-  unsigned long long e[MERGE_EACH], top = 0;
+  unsigned long long e[MERGE_EACH];
+  unsigned top = 0, part_top = 0;
 #pragma unroll
   for (int j = 0; j < MERGE_EACH; ++j) {
     e[j] = j * MERGE_THREADS + tid < total ? in[j * MERGE_THREADS + tid] : 0ull;
-    top = e[j] > top ? e[j] : top;
+    part_top = max(part_top, (unsigned)(e[j] >> 32));
+    if (parts == 1 ? j == MERGE_EACH - 1 : j % 4 == 3) {
+      maxima[(parts == 1 ? 0 : j / 4) * MERGE_THREADS + tid] = part_top;
+      top = max(top, part_top);
+      part_top = 0;
+    }
   }
-  if (tid == 0) {
-    counters[0] = counters[1] = counters[2] = found = 0;
-    peak = 0;
+  const float c = a.scale * LOG2E;
+  float2 ms = make_float2(-INFINITY, 0.f);
+  for (int i = tid; i < a.segments; i += MERGE_THREADS) ms = merge(ms, a.sums[row * a.segments + i], c);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+    ms = merge(ms, make_float2(__shfl_xor_sync(~0u, ms.x, off), __shfl_xor_sync(~0u, ms.y, off)), c);
+  top = __reduce_max_sync(~0u, top);
+  if (tid == 0) counters[0] = counters[1] = counters[2] = found = peak = 0;
+  __syncthreads();
+  if ((tid & 31) == 0) {
+    atomicMax(&peak, top);
+    sums[tid >> 5] = ms;
   }
   __syncthreads();
-  atomicMax(&peak, top);
+  ms = sums[0];
+#pragma unroll
+  for (int w = 1; w < MERGE_THREADS / 32; ++w) ms = merge(ms, sums[w], c);
+  if (tid < 32) {
+    // a NaN's key is the largest there is: one less, as its successor has to exist
+    const unsigned t = reached_by(maxima, parts * MERGE_THREADS / 32, a.k, min(peak, 0xfffffffeu));
+    if (tid == 0) bound = t;
+  }
   __syncthreads();
-  int slot = 0;
-  unsigned long long below = 1, above = peak + 1;
-  if (total > a.capacity)
+  unsigned long long below = max(1ull, (unsigned long long)bound << 32);
+  int count = 0, slot = 0;
+#pragma unroll
+  for (int j = 0; j < MERGE_EACH; ++j) count += e[j] >= below;
+  count = block_count(count, counters, slot);
+  if (count > a.capacity) {
+    unsigned long long above = ~0ull;  // no entry: its index would be 0 and its key a NaN's, and it alone reaches it
     while (above - below > 1) {
       const unsigned long long mid = below + (above - below) / 2;
-      int count = 0;
+      count = 0;
 #pragma unroll
       for (int j = 0; j < MERGE_EACH; ++j) count += e[j] >= mid;
       count = block_count(count, counters, slot);
@@ -399,12 +438,10 @@ __global__ void __launch_bounds__(MERGE_THREADS) top_merge_kernel(const TopArgs 
         if (count <= a.capacity) break;
       }
     }
+  }
 #pragma unroll
   for (int j = 0; j < MERGE_EACH; ++j)
     if (e[j] >= below) list[atomicAdd(&found, 1)] = e[j];
-  const float c = a.scale * LOG2E;
-  float2 ms = a.sums[row * a.segments];
-  for (int i = 1; i < a.segments; ++i) ms = merge(ms, a.sums[row * a.segments + i], c);
   __syncthreads();
   write_row(a, row, list, found, ms);
 }

@@ -15,6 +15,8 @@ import math
 import torch
 from torch.nn import functional as F
 
+from .ops import native, reference
+
 
 def statistics(prediction, target, epsilon=1e-6, mask=None):
     x, y = prediction.float(), target.float()
@@ -46,7 +48,6 @@ def kl_sum(student_logits, teacher_logits):
     CUDA tensors take the one-pass kernel (``csrc/fused/kl.cu``: online max / sums per row, per-row results
     summed here in a fixed order); otherwise two log_softmax passes (reference ``theseus/losses.py:27-30``)."""
     if student_logits.is_cuda:
-        from .ops import native
         V = student_logits.shape[-1]
         s = student_logits.reshape(-1, V)
         t = teacher_logits.reshape(-1, V)
@@ -130,7 +131,6 @@ def linear_topk_kl(hidden, weight, indices, log_probs, temperature=1.0, tail=Tru
                       reduction)
 
 
-@torch.no_grad()
 def top_log_probs(logits, k, temperature=1.0):
     """(log_probs fp32, indices int64), both [..., k]: the k largest log-probabilities of
     ``softmax(logits / temperature)`` over the last axis, largest first, equal logits by the lowest index. CUDA logits
@@ -142,7 +142,6 @@ def top_log_probs(logits, k, temperature=1.0):
     if logits.is_cuda:
         if logits.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("top_log_probs takes bf16 or fp32 logits on CUDA")
-        from .ops.head import top_log_probs as run
-    else:
-        from .ops.reference import top_log_probs as run
-    return run(logits, int(k), 1.0 / float(temperature))
+        return native().top_log_probs(logits, k, 1.0 / temperature)
+    with torch.no_grad():
+        return reference.top_log_probs(logits, k, 1.0 / temperature)

@@ -1,4 +1,4 @@
-"""Operators of the vocabulary head on CUDA: losses from hidden states without logits, and top log-probabilities.
+"""Losses of the vocabulary head on CUDA, from hidden states without logits.
 
 ``head_loss`` covers the cross entropy (``log_probs`` None, ``index`` [rows, 1] targets) and the KL from a recorded
 top-k (``index``, ``log_probs`` [rows, K]); the mathematics stands in ``csrc/head/head_loss.cu``. A reduced loss forms
@@ -58,10 +58,3 @@ def head_loss(hidden, weight, index, log_probs, ignore, scale, tail, reduction):
     out = _HeadLoss.apply(rows, weight, index, log_probs, ignore, scale, tail, REDUCTIONS[reduction])
     return out.view(lead) if reduction == "none" else out
 
-
-def top_log_probs(logits, k, scale):
-    rows = logits.reshape(-1, logits.shape[-1])
-    if rows.stride(-1) != 1:
-        rows = rows.contiguous()
-    log_probs, index = native().top_log_probs(rows, k, scale)
-    return log_probs.view(*logits.shape[:-1], k), index.view(*logits.shape[:-1], k)
