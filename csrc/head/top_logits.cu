@@ -2,8 +2,8 @@
 //
 // One read of the logits. A row is streamed in groups of 8 or 32 values, whose maxima stay in shared memory, while the
 // softmax's denominator is summed. A value t that k of the maxima reach is reached by k logits at least, so the result
-// lies in the groups whose maximum reaches t. t is the k-th largest of 2 k to 4 k maxima over several groups each, found
-// by one warp's bisection of their order-preserving keys; the groups that reach it (about 1.2 k) are read again, and
+// lies in the groups whose maximum reaches t. t is the k-th largest of 1.5 k maxima or more over several groups each, found
+// by one warp's bisection of their order-preserving keys; the groups that reach it (about 1.4 k at most) are read again, and
 // their values from t up are sorted as unique 64-bit keys (value above, lower index first below). Rows whose equal or
 // special values defeat the bounds (thousands of equal maxima, infinities, NaN) take a radix descent over the whole
 // row instead.
@@ -18,7 +18,7 @@
 
 namespace {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int THREADS = 384, WARPS = THREADS / 32;
 constexpr int MAX_KEYS = 8192;     // group maxima of a segment
 constexpr int MAX_GROUPS = 2048;   // groups read again
 constexpr int BATCH = 4;           // vectors of 16 bytes in flight per thread
@@ -29,6 +29,11 @@ __device__ __forceinline__ unsigned order_key(float v) {
   if (v != v) return 0xffffffffu;
   const unsigned b = __float_as_uint(v + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+// Of a maximum, which is no NaN.
+__device__ __forceinline__ unsigned max_key(float v) {
+  const int b = __float_as_int(v + 0.f);
+  return (unsigned)b ^ ((unsigned)(b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(unsigned key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
@@ -48,6 +53,26 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
 // (max of logits, sum of exp2(c (logit - max))).
@@ -84,27 +109,56 @@ __device__ __forceinline__ int block_count(int n, int* counters, int& slot) {
 }
 
 // By one warp: the largest t found that at least k of maxima[0, 32 each) reach and, as far as they differ, few more (0
-// where fewer than k are above 0). `top` is their largest; each is a multiple of 8.
+// where fewer than k are above 0). `top` is their largest.
 template <typename K>
 __device__ __forceinline__ unsigned reached_by(const K* maxima, int each, int k, unsigned top) {
-  unsigned below = 0, above = top + 1;
+  constexpr int HELD = 16;  // per lane in registers, which serves records of up to 256
+  const int lane = threadIdx.x & 31;
+  unsigned r[HELD], least = top;
+#pragma unroll
+  for (int j = 0; j < HELD; ++j) {
+    r[j] = j < each ? (unsigned)maxima[j * 32 + lane] : 0u;
+    if (j < each) least = min(least, r[j]);
+  }
+  for (int j = HELD; j < each; ++j) least = min(least, (unsigned)maxima[j * 32 + lane]);
+  unsigned below = __reduce_min_sync(~0u, least), above = top + 1;  // all of them reach `below`
   while (above - below > 1) {
     const unsigned mid = below + (above - below) / 2;
     int count = 0;
-    for (int j = 0; j < each; j += 8) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) count += (unsigned)maxima[(j + q) * 32 + (threadIdx.x & 31)] >= mid;
-    }
+    for (int j = 0; j < HELD; ++j) count += r[j] >= mid;
+    for (int j = HELD; j < each; ++j) count += (unsigned)maxima[j * 32 + lane] >= mid;
     count = __reduce_add_sync(~0u, count);
     if (count < k) {
       above = mid;
     } else {
       below = mid;
-      if (count <= k + k / 16) break;
+      if (count <= k + k / 8) break;
     }
   }
   return below;
 }
+
+// Keys of 16 bytes at once: their maximum, and the j-th.
+template <typename K> struct KeyVec;
+template <> struct KeyVec<unsigned short> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ unsigned max(const uint4& u) {
+    const unsigned m = __vmaxu2(__vmaxu2(u.x, u.y), __vmaxu2(u.z, u.w));
+    return ::max(m & 0xffffu, m >> 16);
+  }
+  static __device__ __forceinline__ unsigned at(const uint4& u, int j) {
+    const unsigned w = j < 4 ? (j < 2 ? u.x : u.y) : (j < 6 ? u.z : u.w);
+    return j & 1 ? w >> 16 : w & 0xffffu;
+  }
+};
+template <> struct KeyVec<unsigned> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ unsigned max(const uint4& u) { return ::max(::max(u.x, u.y), ::max(u.z, u.w)); }
+  static __device__ __forceinline__ unsigned at(const uint4& u, int j) {
+    return j < 2 ? (j < 1 ? u.x : u.y) : (j < 3 ? u.z : u.w);
+  }
+};
 
 // list[0, n) sorted downwards; its capacity is a power of two of at least n. Entries are unique but for zeros.
 __device__ void sort_down(unsigned long long* list, int n) {
@@ -197,7 +251,10 @@ __device__ void write_row(const TopArgs& a, long row, unsigned long long* list, 
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
       const unsigned long long e = list[i];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += list[j] > e;
+      const ulonglong2* two = reinterpret_cast<const ulonglong2*>(list);
+#pragma unroll 8
+      for (int j = 0; j < n / 2; ++j) rank += (two[j].x > e) + (two[j].y > e);
+      if (n & 1) rank += list[n - 1] > e;
       if (rank < a.k) put(rank, e);
     }
     return;
@@ -208,7 +265,7 @@ __device__ void write_row(const TopArgs& a, long row, unsigned long long* list, 
 
 // Block (segment, row). U = vectors of a group: 1, or BATCH for long segments.
 template <typename T, int U>
-__global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logits, const TopArgs a) {
+__global__ void __launch_bounds__(THREADS, 4) top_kernel(const T* __restrict__ logits, const TopArgs a) {
   constexpr int VEC = 16 / sizeof(T);
   using K = typename Key<T>::type;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -247,14 +304,15 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
     if (special) s = NAN;
   }
   const int steps = (nvec + BATCH * THREADS - 1) / (BATCH * THREADS);
-  for (int it = 0; it < steps; ++it) {
+  auto step = [&](int it, bool whole) {
     uint4 u[BATCH];
     float g[BATCH];
     const int v0 = it * BATCH * THREADS + tid;
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
       const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;  // -inf
-      u[b] = v0 + b * THREADS < nvec ? __ldg(zv + v0 + b * THREADS) : make_uint4(none, none, none, none);
+      if (whole || v0 + b * THREADS < nvec) u[b] = __ldg(zv + v0 + b * THREADS);
+      else u[b] = make_uint4(none, none, none, none);
     }
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) g[b] = vec_max(u[b], (const T*)nullptr);
@@ -262,28 +320,33 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
     if (U == 1) {
 #pragma unroll
       for (int b = 0; b < BATCH; ++b)
-        keys[(it * BATCH + b) * THREADS + tid] = v0 + b * THREADS < nvec ? pack_key<T>(order_key(g[b])) : (K)0;
+        keys[(it * BATCH + b) * THREADS + tid] =
+            whole || v0 + b * THREADS < nvec ? pack_key<T>(max_key(g[b])) : (K)0;
     } else {
-      keys[it * THREADS + tid] = v0 < nvec ? pack_key<T>(order_key(top)) : (K)0;
+      keys[it * THREADS + tid] = whole || v0 < nvec ? pack_key<T>(max_key(top)) : (K)0;
     }
     if (top > m) {
       s *= m == -INFINITY ? 0.f : ex2((m - top) * c);
       m = top;
     }
-    const float mc = m == -INFINITY ? 0.f : m * c;
-    float s0 = 0.f, s1 = 0.f;
+    const float mc = m == -INFINITY ? 0.f : -m * c;
+    float2 sum = make_float2(0.f, 0.f);
+    const float2 c2 = make_float2(c, c), mc2 = make_float2(mc, mc);
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
       float f[VEC];
       unpack(u[b], f);
 #pragma unroll
       for (int j = 0; j < VEC; j += 2) {
-        s0 += ex2(fmaf(f[j], c, -mc));
-        s1 += ex2(fmaf(f[j + 1], c, -mc));
+        const float2 y = fma2(make_float2(f[j], f[j + 1]), c2, mc2);
+        sum = add2(sum, make_float2(ex2(y.x), ex2(y.y)));
       }
     }
-    s += s0 + s1;
-  }
+    s += sum.x + sum.y;
+  };
+  const int whole = nvec / (BATCH * THREADS);
+  for (int it = 0; it < whole; ++it) step(it, true);
+  if (whole < steps) step(whole, false);
   float2 o = make_float2(m, s);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1)
@@ -294,23 +357,31 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
   for (int w = 1; w < WARPS; ++w) o = merge(o, warps[w], c);
 
   // ---- threshold: THREADS x parts maxima, each of one thread's every parts-th group; the k-th largest of them
-  const int slots = steps * THREADS * (U == 1 ? BATCH : 1);
+  const int slots = steps * THREADS * (U == 1 ? BATCH : 1), vecs = slots / KeyVec<K>::N;
+  const uint4* kv = reinterpret_cast<const uint4*>(keys);
   unsigned threshold = 0;  // every value, where there are few groups
   // NaN and +inf make the sum NaN; a row of -inf has nothing above it
   bool ok = !special && o.y == o.y && o.x > -INFINITY;
   ok = !__syncthreads_or(!ok);
   if (ok && slots > max(2 * a.k, 128)) {
+    // (by 16 bytes of keys, or by single keys where the row is too short for that many)
+    const bool wide = nvec / (U * KeyVec<K>::N) >= 2 * a.k;
     int parts = 1;
-    while (parts < 8 && parts * (THREADS / 2) < a.k) parts <<= 1;
+    while (parts < 8 && parts * THREADS * 2 < 3 * a.k) parts <<= 1;
     for (int p = 0; p < parts; ++p) {
       unsigned best = 0;
-      for (int i = tid + p * THREADS; i < slots; i += parts * THREADS) best = max(best, (unsigned)keys[i]);
+      if (wide) {
+#pragma unroll 2
+        for (int i = tid + p * THREADS; i < vecs; i += parts * THREADS) best = max(best, KeyVec<K>::max(kv[i]));
+      } else {
+        for (int i = tid + p * THREADS; i < slots; i += parts * THREADS) best = max(best, (unsigned)keys[i]);
+      }
       maxima[p * THREADS + tid] = (K)best;
     }
     __syncthreads();
     if (tid < 32) {
       const int shift = sizeof(T) == 2 ? 16 : 0;
-      const unsigned t = reached_by(maxima, 8 * parts, a.k, order_key(o.x) >> shift) << shift;
+      const unsigned t = reached_by(maxima, WARPS * parts, a.k, order_key(o.x) >> shift) << shift;
       if (lane == 0) bound = t;
     }
     __syncthreads();
@@ -318,13 +389,17 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
   }
   // ---- candidates
   if (ok) {
-    const K tk = pack_key<T>(threshold);
-    for (int i = tid; i < slots; i += THREADS) {
-      const K key = keys[i];
-      if (key && key >= tk) {
-        const int at = atomicAdd(&picked, 1);
-        if (at < MAX_GROUPS) groups[at] = (unsigned short)i;
-      }
+    const unsigned tk = max((unsigned)pack_key<T>(threshold), 1u);
+#pragma unroll 2
+    for (int i = tid; i < vecs; i += THREADS) {
+      const uint4 u = kv[i];
+      if (KeyVec<K>::max(u) < tk) continue;
+#pragma unroll
+      for (int j = 0; j < KeyVec<K>::N; ++j)
+        if (KeyVec<K>::at(u, j) >= tk) {
+          const int at = atomicAdd(&picked, 1);
+          if (at < MAX_GROUPS) groups[at] = (unsigned short)(i * KeyVec<K>::N + j);
+        }
     }
     if (single >= 0 && single_key >= threshold) {
       const int at = atomicAdd(&found, 1);
@@ -332,18 +407,29 @@ __global__ void __launch_bounds__(THREADS) top_kernel(const T* __restrict__ logi
     }
     __syncthreads();
     ok = picked <= MAX_GROUPS;
-    for (int i = tid; ok && i < picked * U; i += THREADS) {
-      const int g = groups[i / U];
-      const int v = U == 1 ? g : (g / THREADS) * BATCH * THREADS + (i % U) * THREADS + g % THREADS;
-      if (v >= nvec) continue;
-      float f[VEC];
-      unpack(__ldg(zv + v), f);
+    const int lines = ok ? picked * U : 0;
+    for (int i = tid; i < lines; i += 2 * THREADS) {
+      int v[2];
+      uint4 u[2];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const unsigned key = order_key(f[j]);
-        if (key >= threshold) {
-          const int at = atomicAdd(&found, 1);
-          if (at < a.capacity) list[at] = entry(key, lo + head + v * VEC + j);
+      for (int h = 0; h < 2; ++h) {
+        const int at = i + h * THREADS, g = at < lines ? groups[at / U] : 0;
+        v[h] = U == 1 ? g : (g / THREADS) * BATCH * THREADS + (at % U) * THREADS + g % THREADS;
+        if (at >= lines || v[h] >= nvec) v[h] = -1;
+        if (v[h] >= 0) u[h] = __ldg(zv + v[h]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (v[h] < 0) continue;
+        float f[VEC];
+        unpack(u[h], f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const unsigned key = order_key(f[j]);
+          if (key >= threshold) {
+            const int at = atomicAdd(&found, 1);
+            if (at < a.capacity) list[at] = entry(key, lo + head + v[h] * VEC + j);
+          }
         }
       }
     }
