@@ -93,7 +93,7 @@ struct RtHeadLoss {
 };
 long rt_head_loss_workspace_floats(long rows, long vocab, int width, int K, int grad_h, int grad_w);
 cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream_t stream);
-cudaError_t rt_scale_bf16(void* x, const float* factor, long n, cudaStream_t stream);
+cudaError_t rt_scale_bf16(void* const x[2], const long n[2], const float* factor, cudaStream_t stream);
 cudaError_t rt_top_log_probs(int dtype, const void* logits, long rows, long V, long ld, int k, float scale,
                              float* logp, long* index, void* work, cudaStream_t stream);
 long rt_top_workspace_bytes(int dtype, long rows, long V, int k);

@@ -478,71 +478,145 @@ at::Tensor kl_rows(at::Tensor student, at::Tensor teacher) {
   return out;
 }
 
-// Vocabulary-head loss from hidden states (see RtHeadLoss): returns {loss, dhidden, dweight}; the gradients that are
-// not asked for are empty. log_probs none: cross entropy of index [rows, 1].
-std::vector<at::Tensor> head_loss(at::Tensor hidden, at::Tensor weight, at::Tensor index,
-                                  c10::optional<at::Tensor> log_probs, int64_t ignore, double scale, bool tail,
-                                  int64_t reduction, c10::optional<at::Tensor> row_grad, bool grad_h, bool grad_w) {
-  const auto h = operand(hidden, "hidden"), w = operand(weight, "weight");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(h.ptr) % 16 == 0 && reinterpret_cast<uintptr_t>(w.ptr) % 16 == 0,
-              "head_loss: hidden and weight need 16-byte alignment");
+// ---- vocabulary-head losses (see RtHeadLoss). index [..., K] with log_probs like it, or targets [...] without.
+struct HeadLossCall {
+  int64_t ignore;
+  double scale;
+  bool tail;
+  int64_t reduction;  // 0 none, 1 sum, 2 mean
+};
+
+struct HeadLossResult {
+  at::Tensor loss, dhidden, dweight;
+};
+
+HeadLossResult run_head_loss(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& index,
+                             const c10::optional<at::Tensor>& log_probs, const HeadLossCall& call,
+                             const at::Tensor& row_grad, bool grad_h, bool grad_w) {
+  TORCH_CHECK(hidden.is_cuda() && hidden.dim() >= 1 && hidden.scalar_type() == at::kBFloat16,
+              "head_loss: hidden must be CUDA bf16 [..., C]");
   c10::cuda::CUDAGuard guard(hidden.device());
-  const long rows = hidden.size(0), V = weight.size(0), C = hidden.size(1);
-  TORCH_CHECK(weight.size(1) == C && C >= 1, "head_loss: hidden width ", C, " and weight width ", weight.size(1));
+  const long C = hidden.size(-1), V = weight.size(0), rows = hidden.numel() / std::max(C, 1L);
+  at::Tensor flat = hidden.dim() == 2 ? hidden : hidden.reshape({rows, C});
+  if (flat.stride(1) != 1 || flat.stride(0) < C || flat.stride(0) % 8 ||
+      reinterpret_cast<uintptr_t>(flat.data_ptr()) % 16)
+    flat = flat.clone(at::MemoryFormat::Contiguous);
+  const auto w = operand(weight, "weight");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(w.ptr) % 16 == 0, "head_loss: weight needs 16-byte alignment");
+  TORCH_CHECK(weight.size(1) == C && C >= 8 && C % 8 == 0, "head_loss: hidden and weight need one width, a multiple of 8");
   TORCH_CHECK(V >= 1 && rows <= (1 << 24) && C <= (1 << 20), "head_loss: size out of range");
-  TORCH_CHECK(C % 8 == 0, "head_loss: the width must be a multiple of 8");
-  TORCH_CHECK(weight.device() == hidden.device() && index.device() == hidden.device(),
+  const long K = log_probs.has_value() ? index.size(-1) : 1;
+  TORCH_CHECK(K >= 1 && K <= RT_HEAD_MAX_RECORD && index.numel() == rows * K, "head_loss: index does not match hidden");
+  const at::Tensor ids = index.to(at::kLong).contiguous();
+  at::Tensor logp;
+  if (log_probs.has_value()) {
+    TORCH_CHECK(log_probs->numel() == rows * K, "head_loss: log_probs does not match index");
+    logp = log_probs->to(at::kFloat).contiguous();
+  }
+  TORCH_CHECK(weight.device() == hidden.device() && ids.device() == hidden.device() &&
+                  (!logp.defined() || logp.device() == hidden.device()),
               "head_loss: operands on different devices");
-  TORCH_CHECK(index.dim() == 2 && index.size(0) == rows && index.scalar_type() == at::kLong && index.is_contiguous(),
-              "head_loss: index must be contiguous int64 [rows, K]");
-  const long K = index.size(1);
-  TORCH_CHECK(K >= 1 && K <= RT_HEAD_MAX_RECORD, "head_loss: 1 to ", RT_HEAD_MAX_RECORD, " entries per row, got ", K);
-  TORCH_CHECK(log_probs.has_value() || K == 1, "head_loss: one target per row");
-  TORCH_CHECK(!log_probs.has_value() ||
-                  (log_probs->device() == hidden.device() && log_probs->scalar_type() == at::kFloat &&
-                   log_probs->is_contiguous() && log_probs->sizes() == index.sizes()),
-              "head_loss: log_probs must be contiguous fp32 like index");
-  TORCH_CHECK(!row_grad.has_value() || (row_grad->device() == hidden.device() && row_grad->is_contiguous() &&
-                                        row_grad->scalar_type() == at::kFloat && row_grad->numel() == rows),
-              "head_loss: row_grad must be contiguous fp32 [rows]");
-  TORCH_CHECK(reduction >= 0 && reduction <= 2, "head_loss: reduction 0 (none), 1 (sum) or 2 (mean)");
+  TORCH_CHECK(call.reduction >= 0 && call.reduction <= 2, "head_loss: reduction 0 (none), 1 (sum) or 2 (mean)");
+  TORCH_CHECK(!row_grad.defined() || row_grad.numel() == rows, "head_loss: one upstream gradient per row");
   const auto f32 = hidden.options().dtype(at::kFloat);
-  auto row_loss = at::empty({rows}, f32);
-  auto loss = reduction ? at::empty({}, f32) : row_loss;
-  auto dh = grad_h ? at::empty({rows, C}, hidden.options()) : at::empty({0}, hidden.options());
-  auto dw = grad_w ? at::empty({V, C}, weight.options()) : at::empty({0}, weight.options());
-  auto work = at::empty({std::max(4L, rt_head_loss_workspace_floats(rows, V, C, K, grad_h, grad_w))}, f32);
-  RtHeadLoss p;
-  p.hidden = h.ptr;
-  p.ld_hidden = h.ld;
+  HeadLossResult r;
+  r.loss = call.reduction ? at::empty({}, f32) : at::empty(hidden.sizes().slice(0, hidden.dim() - 1), f32);
+  if (grad_h) r.dhidden = at::empty(hidden.sizes(), hidden.options());
+  if (grad_w) r.dweight = at::empty({V, C}, weight.options());
+  const long row_floats = call.reduction ? (rows + 3) / 4 * 4 : 0;  // the rows' losses, where only their sum is returned
+  auto work = at::empty({row_floats + std::max(4L, rt_head_loss_workspace_floats(rows, V, C, K, grad_h, grad_w))}, f32);
+  RtHeadLoss p{};
+  p.hidden = flat.data_ptr();
+  p.ld_hidden = rows ? flat.stride(0) : C;
   p.weight = w.ptr;
   p.ld_weight = w.ld;
-  p.index = reinterpret_cast<const long*>(index.data_ptr<int64_t>());
-  p.log_probs = log_probs.has_value() ? log_probs->data_ptr<float>() : nullptr;
+  p.index = reinterpret_cast<const long*>(ids.data_ptr<int64_t>());
+  p.log_probs = logp.defined() ? logp.data_ptr<float>() : nullptr;
   p.rows = rows;
   p.vocab = V;
   p.width = (int)C;
   p.K = (int)K;
-  p.ignore = ignore;
-  p.scale = (float)scale;
-  p.tail = tail;
-  p.reduction = (int)reduction;
-  p.row_grad = row_grad.has_value() ? row_grad->data_ptr<float>() : nullptr;
-  p.row_loss = row_loss.data_ptr<float>();
-  p.loss = reduction ? loss.data_ptr<float>() : nullptr;
-  p.dhidden = grad_h ? dh.data_ptr() : nullptr;
-  p.dweight = grad_w ? dw.data_ptr() : nullptr;
-  check_cuda(rt_head_loss(&p, work.data_ptr<float>(), stream_of(hidden)), "head_loss");
-  return {loss, dh, dw};
+  p.ignore = call.ignore;
+  p.scale = (float)call.scale;
+  p.tail = call.tail;
+  p.reduction = (int)call.reduction;
+  p.row_grad = row_grad.defined() ? row_grad.data_ptr<float>() : nullptr;
+  p.row_loss = call.reduction ? work.data_ptr<float>() : r.loss.data_ptr<float>();
+  p.loss = call.reduction ? r.loss.data_ptr<float>() : nullptr;
+  p.dhidden = grad_h ? r.dhidden.data_ptr() : nullptr;
+  p.dweight = grad_w ? r.dweight.data_ptr() : nullptr;
+  check_cuda(rt_head_loss(&p, work.data_ptr<float>() + row_floats, stream_of(hidden)), "head_loss");
+  return r;
 }
 
-// x *= factor (device fp32 scalar) for a contiguous bf16 tensor; no pass over x when the factor is one.
-void scale_bf16_(at::Tensor x, at::Tensor factor) {
-  TORCH_CHECK(x.is_cuda() && x.is_contiguous() && x.scalar_type() == at::kBFloat16 && factor.device() == x.device() &&
-                  factor.scalar_type() == at::kFloat && factor.numel() == 1,
-              "scale_bf16_: contiguous CUDA bf16 tensor and an fp32 scalar on its device");
-  c10::cuda::CUDAGuard guard(x.device());
-  check_cuda(rt_scale_bf16(x.data_ptr(), factor.data_ptr<float>(), x.numel(), stream_of(x)), "scale_bf16_");
+// A reduced loss forms its gradients in the forward call, from the same pass over the vocabulary as the loss; backward
+// multiplies them by the upstream scalar (no pass over them when it is one). An unreduced loss forms them in backward,
+// from the upstream gradient of each row. A second backward of a kept graph computes them again.
+struct HeadLossFunction : public torch::autograd::Function<HeadLossFunction> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden, const at::Tensor& weight,
+                            const at::Tensor& index, const c10::optional<at::Tensor>& log_probs, int64_t ignore,
+                            double scale, bool tail, int64_t reduction, bool grad_h, bool grad_w) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const HeadLossCall call{ignore, scale, tail, reduction};
+    auto r = run_head_loss(hidden, weight, index, log_probs, call, at::Tensor(), reduction && grad_h,
+                           reduction && grad_w);
+    ctx->save_for_backward({hidden, weight, index, log_probs.has_value() ? *log_probs : at::Tensor()});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["tail"] = tail;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["grad_h"] = grad_h;
+    ctx->saved_data["grad_w"] = grad_w;
+    ctx->saved_data["ready"] = reduction != 0;
+    if (r.dhidden.defined()) ctx->saved_data["dhidden"] = r.dhidden;
+    if (r.dweight.defined()) ctx->saved_data["dweight"] = r.dweight;
+    return r.loss;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list upstreams) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the head losses have no second derivative (create_graph)");
+    auto& data = ctx->saved_data;
+    const HeadLossCall call{data["ignore"].toInt(), data["scale"].toDouble(), data["tail"].toBool(),
+                            data["reduction"].toInt()};
+    const bool grad_h = data["grad_h"].toBool(), grad_w = data["grad_w"].toBool();
+    const at::Tensor upstream = upstreams[0].to(at::kFloat).contiguous();
+    at::Tensor dh, dw;
+    if (data["ready"].toBool()) {
+      if (grad_h) dh = data["dhidden"].toTensor();
+      if (grad_w) dw = data["dweight"].toTensor();
+      data["ready"] = false;
+      data.erase("dhidden");
+      data.erase("dweight");
+    } else {
+      const auto saved = ctx->get_saved_variables();
+      c10::optional<at::Tensor> log_probs;
+      if (saved[3].defined()) log_probs = saved[3];
+      auto r = run_head_loss(saved[0], saved[1], saved[2], log_probs, call, call.reduction ? at::Tensor() : upstream,
+                             grad_h, grad_w);
+      dh = r.dhidden;
+      dw = r.dweight;
+    }
+    if (call.reduction) {
+      c10::cuda::CUDAGuard guard(upstream.device());
+      void* grads[2] = {dh.defined() ? dh.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr};
+      const long sizes[2] = {dh.defined() ? (long)dh.numel() : 0, dw.defined() ? (long)dw.numel() : 0};
+      check_cuda(rt_scale_bf16(grads, sizes, upstream.data_ptr<float>(), stream_of(upstream)), "head_loss backward");
+    }
+    return {dh, dw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor()};
+  }
+};
+
+at::Tensor head_loss(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& index,
+                     const c10::optional<at::Tensor>& log_probs, int64_t ignore, double scale, bool tail,
+                     int64_t reduction) {
+  const bool on = at::GradMode::is_enabled(), grad_h = on && hidden.requires_grad(),
+             grad_w = on && weight.requires_grad();
+  if (!grad_h && !grad_w)
+    return run_head_loss(hidden, weight, index, log_probs, {ignore, scale, tail, reduction}, at::Tensor(), false, false)
+        .loss;
+  return HeadLossFunction::apply(hidden, weight, index, log_probs, ignore, scale, tail, reduction, grad_h, grad_w);
 }
 
 // The k largest log-probabilities of softmax(scale * logits) over the last axis and their indices, largest first, equal
@@ -902,11 +976,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "1 if a GEMM gave up a bounded wait since the last call (then cleared); synchronizes the device");
   m.def("kl_rows", &kl_rows, "per-row KL(teacher || student) over the vocabulary in one pass", py::arg("student"),
         py::arg("teacher"));
-  m.def("head_loss", &head_loss, "vocabulary-head loss from hidden states: (loss, dhidden, dweight)",
+  m.def("head_loss", &head_loss, "vocabulary-head loss from hidden states, differentiable in hidden and weight",
         py::arg("hidden"), py::arg("weight"), py::arg("index"), py::arg("log_probs"), py::arg("ignore"),
-        py::arg("scale"), py::arg("tail"), py::arg("reduction"), py::arg("row_grad"), py::arg("grad_h"),
-        py::arg("grad_w"));
-  m.def("scale_bf16_", &scale_bf16_, "x *= device scalar, without a pass when it is one");
+        py::arg("scale"), py::arg("tail"), py::arg("reduction"));
   m.def("top_log_probs", &top_log_probs, "k largest log-probabilities per row and their indices", py::arg("logits"),
         py::arg("k"), py::arg("scale"));
   m.def("gemm_nmse", &gemm_nmse, "output GEMM with the NMSE/cosine loss in the epilogue: returns d loss / d p",

@@ -156,10 +156,11 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
 }
 
 // ---------------------------------------------------------------- losses of the valid rows of a chunk
-// Eight warps per 32 rows: lanes are rows while the tiles' statistics are merged (in a fixed order), then each warp
-// takes four rows and forms their losses and gradient coefficients: d/dz_v = tail exp2(z_v - lse2) outside the record,
-// coef[k] for its held entries, both times scale and the row's upstream gradient (given per row, or 1, or 1 / rows
-// with a loss).
+// Block of MERGE_ROWS rows: its threads merge the tiles' statistics (in a fixed order: each row's tiles go round-robin
+// to MERGE_GROUPS threads), then one warp per row forms the loss and the gradient's coefficients: d/dz_v = tail
+// exp2(z_v - lse2) outside the record, coef[k] for its held entries, both times scale and the row's upstream gradient
+// (given per row, or 1, or 1 / rows with a loss).
+constexpr int MERGE_ROWS = 4, MERGE_GROUPS = 64;
 struct MergeArgs {
   const float2* part;
   long part_ld;
@@ -177,41 +178,46 @@ struct MergeArgs {
   float* coef;
 };
 
-__global__ void __launch_bounds__(256) merge_kernel(const MergeArgs p) {
-  __shared__ float2 merged[8][33];
+// (max, sum of exponentials relative to it) of two sets.
+__device__ __forceinline__ float2 merge2(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x);
+  return make_float2(m, (a.x == m ? a.y : a.y * exp2f(a.x - m)) + (b.x == m ? b.y : b.y * exp2f(b.x - m)));
+}
+
+__global__ void __launch_bounds__(MERGE_ROWS * MERGE_GROUPS) merge_kernel(const MergeArgs p) {
+  __shared__ float2 merged[MERGE_GROUPS][MERGE_ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = min(max(p.counts[0] - p.row0, 0), p.rows);
-  const int first = blockIdx.x * 32;
+  const int first = blockIdx.x * MERGE_ROWS;
   if (first >= n) return;
   {
-    const int r = first + lane;
-    float m = -INFINITY, s = 0.f;
-    if (r < n)
-      for (int i = warp; i < p.tiles; i += 8) {
-        const float2 t = p.part[i * p.part_ld + r];
-        if (t.x > m) {
-          s = s * exp2f(m - t.x) + t.y;
-          m = t.x;
-        } else {
-          s += t.x == -INFINITY ? t.y : t.y * exp2f(t.x - m);
-        }
-      }
-    merged[warp][lane] = make_float2(m, s);
+    const int j = threadIdx.x % MERGE_ROWS, group = threadIdx.x / MERGE_ROWS;
+    const float2* part = p.part + min(first + j, n - 1);
+    float2 sum = make_float2(-INFINITY, 0.f);
+    for (int i = group; i < p.tiles; i += 4 * MERGE_GROUPS) {
+      float2 t[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        t[u] = i + u * MERGE_GROUPS < p.tiles ? part[(i + u * MERGE_GROUPS) * p.part_ld] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) sum = merge2(sum, t[u]);
+    }
+    merged[group][j] = sum;
   }
   __syncthreads();
-  for (int j = warp; j < 32 && first + j < n; j += 8) {
+  const int j = warp;
+  if (j < MERGE_ROWS && first + j < n) {
     const int r = first + j;
     const long place = p.row0 + r, row = p.row_of[place];
     const int* sidx = p.sidx + place * p.K;
     const float* slogp = p.slogp + place * p.K;
     const float* hit = p.hit + place * p.K;
-    float m = -INFINITY, top = -INFINITY;
-    for (int w = 0; w < 8; ++w) m = fmaxf(m, merged[w][j].x);
-    float rest = 0.f;
-    for (int w = 0; w < 8; ++w) {
-      const float2 t = merged[w][j];
-      rest += t.x == -INFINITY ? t.y : t.y * exp2f(t.x - m);
-    }
+    float2 all = merge2(merged[lane][j], merged[lane + 32][j]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+      all = merge2(all, make_float2(__shfl_xor_sync(~0u, all.x, off), __shfl_xor_sync(~0u, all.y, off)));
+    const float m = all.x, rest = all.y;
+    float top = -INFINITY;
     for (int k = lane; k < p.K; k += 32)
       if (sidx[k] != INT_MAX) top = fmaxf(top, hit[k]);
 #pragma unroll
@@ -251,7 +257,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const MergeArgs p) {
       p.lse2[place] = (float)l2;
       p.tail[place] = g * (float)a;
     }
-    if (!p.coef) continue;
+    if (!p.coef) return;
     for (int k = lane; k < p.K; k += 32) {
       float c = 0.f;
       if (sidx[k] != INT_MAX) {
@@ -347,21 +353,28 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ 
   }
 }
 
-// x *= *factor, nothing at all for a factor of one (the usual upstream gradient of a training loss).
-__global__ void scale_kernel(__nv_bfloat16* __restrict__ x, const float* __restrict__ factor, long n) {
+// x *= *factor for up to two tensors, nothing at all for a factor of one (the usual upstream gradient of a loss).
+struct ScaleArgs {
+  __nv_bfloat16* x[2];
+  long n[2];
+};
+__global__ void scale_kernel(const ScaleArgs p, const float* __restrict__ factor) {
   const float f = *factor;
   if (f == 1.f) return;
-  const long step = (long)gridDim.x * blockDim.x, n8 = n / 8;
-  uint4* x8 = reinterpret_cast<uint4*>(x);
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += step) {
-    float v[8];
-    rt::unpack8(x8[i], v);
+  const long step = (long)gridDim.x * blockDim.x, at = (long)blockIdx.x * blockDim.x + threadIdx.x;
+  for (int t = 0; t < 2; ++t) {
+    const long n8 = p.n[t] / 8;
+    uint4* x8 = reinterpret_cast<uint4*>(p.x[t]);
+    for (long i = at; i < n8; i += step) {
+      float v[8];
+      rt::unpack8(x8[i], v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= f;
-    x8[i] = rt::pack8(v);
+      for (int j = 0; j < 8; ++j) v[j] *= f;
+      x8[i] = rt::pack8(v);
+    }
+    for (long i = 8 * n8 + at; i < p.n[t]; i += step)
+      p.x[t][i] = __float2bfloat16_rn(__bfloat162float(p.x[t][i]) * f);
   }
-  for (long i = 8 * n8 + (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step)
-    x[i] = __float2bfloat16_rn(__bfloat162float(x[i]) * f);
 }
 
 // The tensor cores round each of the C / 16 partial sums of a logit towards zero. Given the sum z, the partial sums are
@@ -537,7 +550,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
     MergeArgs m{part, l.rows, (int)l.tiles, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, counts,
                 ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->scale, p->row_grad, p->row_loss,
                 work + l.lse2, work + l.tail, grad ? work + l.coef : nullptr};
-    merge_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, s>>>(m);
+    merge_kernel<<<(unsigned)((rows + MERGE_ROWS - 1) / MERGE_ROWS), MERGE_ROWS * MERGE_GROUPS, 0, s>>>(m);
     if (grad) {
       gradient_kernel<<<dim3((unsigned)((l.tiles + 31) / 32), (unsigned)rows), 256, 0, s>>>(
           e, l.ld_e, (int)V, (int)l.tiles, (int)row0, (int)l.rows, counts, part, l.rows, work + l.lse2, work + l.tail);
@@ -569,11 +582,16 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   return cudaGetLastError();
 }
 
-// x [n] bf16 *= *factor (device scalar).
-extern "C" cudaError_t rt_scale_bf16(void* x, const float* factor, long n, cudaStream_t s) {
-  if (n <= 0) return cudaSuccess;
-  if (reinterpret_cast<uintptr_t>(x) & 15) return cudaErrorInvalidValue;
-  const long blocks = std::min((n / 8 + 255) / 256 + 1, 148L * 8);
-  scale_kernel<<<(unsigned)blocks, 256, 0, s>>>(reinterpret_cast<__nv_bfloat16*>(x), factor, n);
+// x[t] [n[t]] bf16 *= *factor (device scalar), t = 0, 1 (n = 0: none).
+extern "C" cudaError_t rt_scale_bf16(void* const x[2], const long n[2], const float* factor, cudaStream_t s) {
+  const long most = std::max(n[0], n[1]);
+  if (most <= 0) return cudaSuccess;
+  ScaleArgs p;
+  for (int t = 0; t < 2; ++t) {
+    if (reinterpret_cast<uintptr_t>(x[t]) & 15) return cudaErrorInvalidValue;
+    p.x[t] = reinterpret_cast<__nv_bfloat16*>(x[t]);
+    p.n[t] = n[t];
+  }
+  scale_kernel<<<(unsigned)std::min((most / 8 + 255) / 256 + 1, 148L * 8), 256, 0, s>>>(p, factor);
   return cudaGetLastError();
 }

@@ -59,38 +59,32 @@ def kl_sum(student_logits, teacher_logits):
     return (teacher.exp() * (teacher - student)).sum()
 
 
-def _check_head(hidden, weight, reduction):
-    if reduction not in ("none", "sum", "mean"):
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def _head_loss(hidden, weight, index, log_probs, ignore, scale, tail, reduction):
+    """Checks what both head losses share and runs the CUDA kernels or the plain definition."""
+    if reduction not in _REDUCTIONS:
         raise ValueError(f"Unknown reduction: {reduction}")
-    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or weight.numel() == 0:
         raise ValueError(f"expected hidden [..., C] and weight [V, C], got {tuple(hidden.shape)} and "
                          f"{tuple(weight.shape)}")
-    if weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError("empty vocabulary or width")
-    if weight.device != hidden.device:
-        raise ValueError("hidden and weight are on different devices")
-    if hidden.is_cuda and (hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16):
+    if index.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"vocabulary indices must be int32 or int64, got {index.dtype}")
+    if weight.device != hidden.device or index.device != hidden.device:
+        raise ValueError("hidden states, weight and indices are on different devices")
+    if index.shape != hidden.shape[:-1] + (() if log_probs is None else index.shape[-1:]):
+        raise ValueError(f"indices {tuple(index.shape)} do not match hidden {tuple(hidden.shape)}")
+    if not hidden.is_cuda:
+        if log_probs is None:
+            index = index.unsqueeze(-1)
+        return reference.head_loss(hidden, weight, index.long(), log_probs, ignore, scale, tail, reduction)
+    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
         raise TypeError("the CUDA head losses take bf16 hidden states and weight")
-    if hidden.is_cuda and (weight.stride(1) != 1 or weight.stride(0) % 8 or weight.shape[1] % 8 or
-                           weight.data_ptr() % 16):
+    if weight.stride(1) != 1 or weight.stride(0) % 8 or weight.shape[1] % 8 or weight.data_ptr() % 16:
         raise ValueError("the CUDA head losses need a width and weight row stride that are multiples of 8, unit inner "
                          "stride and 16-byte alignment")
-
-
-def _check_index(index, shape, name, device):
-    if index.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"{name} must be int32 or int64, got {index.dtype}")
-    if index.shape[:len(shape)] != shape or index.device != device:
-        raise ValueError(f"{name} {tuple(index.shape)} on {index.device} does not match hidden {tuple(shape)} on "
-                         f"{device}")
-
-
-def _head_loss(hidden, *args):
-    if hidden.is_cuda:
-        from .ops.head import head_loss
-    else:
-        from .ops.reference import head_loss
-    return head_loss(hidden, *args)
+    return native().head_loss(hidden, weight, index, log_probs, ignore, scale, tail, _REDUCTIONS[reduction])
 
 
 def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="mean"):
@@ -100,11 +94,7 @@ def linear_cross_entropy(hidden, weight, targets, ignore_index=-100, reduction="
     Tokens whose target is ``ignore_index`` have loss 0 and gradient 0 whatever their hidden state holds, and are not
     counted by the mean (which is 0 when none is left). fp32 result: [...] for reduction "none", else a scalar. On
     CUDA a target outside the vocabulary makes its token's loss NaN and its gradient 0; on CPU it raises."""
-    _check_head(hidden, weight, reduction)
-    _check_index(targets, hidden.shape[:-1], "targets", hidden.device)
-    if targets.dim() != hidden.dim() - 1:
-        raise ValueError("one target per token")
-    return _head_loss(hidden, weight, targets.unsqueeze(-1).long(), None, int(ignore_index), 1.0, False, reduction)
+    return _head_loss(hidden, weight, targets, None, ignore_index, 1.0, False, reduction)
 
 
 def linear_topk_kl(hidden, weight, indices, log_probs, temperature=1.0, tail=True, reduction="mean"):
@@ -117,18 +107,15 @@ def linear_topk_kl(hidden, weight, indices, log_probs, temperature=1.0, tail=Tru
     holds the teacher's remaining mass; without it the sum runs over the recorded entries alone. ``log_probs`` get no
     gradient. fp32 result: [...] for reduction "none", else a scalar. On CUDA an index beyond the vocabulary makes its
     token's loss NaN and its gradient 0; on CPU it raises."""
-    _check_head(hidden, weight, reduction)
-    _check_index(indices, hidden.shape[:-1], "indices", hidden.device)
-    if indices.dim() != hidden.dim() or log_probs.shape != indices.shape or log_probs.device != indices.device:
-        raise ValueError("indices and log_probs must both be [..., K]")
-    if not 1 <= indices.shape[-1] <= 1024:
-        raise ValueError(f"a record holds 1 to 1024 entries per token, got {indices.shape[-1]}")
+    if log_probs.shape != indices.shape or log_probs.device != indices.device:
+        raise ValueError(f"indices {tuple(indices.shape)} and log_probs {tuple(log_probs.shape)} must match")
+    if indices.dim() < 1 or not 1 <= indices.shape[-1] <= 1024:
+        raise ValueError(f"a record holds 1 to 1024 entries per token, got {tuple(indices.shape)}")
     if not log_probs.is_floating_point():
         raise TypeError("log_probs must be floating point")
     if not temperature > 0:
         raise ValueError("temperature must be positive")
-    return _head_loss(hidden, weight, indices.long(), log_probs.detach(), -1, 1.0 / float(temperature), bool(tail),
-                      reduction)
+    return _head_loss(hidden, weight, indices, log_probs.detach(), -1, 1.0 / temperature, tail, reduction)
 
 
 def top_log_probs(logits, k, temperature=1.0):

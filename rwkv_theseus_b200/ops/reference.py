@@ -107,7 +107,7 @@ def attention(q, k_all, v_all, offset):
 
 
 def head_loss(hidden, weight, index, log_probs, ignore, scale, tail, reduction):
-    """Vocabulary-head loss against a record (see ``ops.head``), in fp32 (fp64 for fp64 operands)."""
+    """Vocabulary-head loss against a record (see ``losses.linear_topk_kl``), in fp32 (fp64 for fp64 operands)."""
     wide = torch.float64 if hidden.dtype == torch.float64 else torch.float32
     z = (hidden.to(wide) @ weight.to(wide).t()) * scale
     log_q = z - z.logsumexp(-1, keepdim=True)

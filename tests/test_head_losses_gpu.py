@@ -350,8 +350,10 @@ def test_gpu_refusals():
         linear_cross_entropy(hidden[:, :60], weight[:, :60], targets)
     with pytest.raises(ValueError, match="multiples of 8"):
         linear_cross_entropy(hidden, weight.t().contiguous().t(), targets)
-    with pytest.raises(ValueError, match="does not match"):
+    with pytest.raises(ValueError, match="devices"):
         linear_cross_entropy(hidden, weight, targets.cpu())
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(linear_cross_entropy(hidden.requires_grad_(), weight, targets), hidden, create_graph=True)
     with pytest.raises(ValueError, match="devices"):
         linear_cross_entropy(hidden, weight.cpu(), targets)
     with pytest.raises(TypeError, match="bf16 or fp32"):
