@@ -523,7 +523,7 @@ HeadLossResult run_head_loss(const at::Tensor& hidden, const at::Tensor& weight,
   r.loss = call.reduction ? at::empty({}, f32) : at::empty(hidden.sizes().slice(0, hidden.dim() - 1), f32);
   if (grad_h) r.dhidden = at::empty(hidden.sizes(), hidden.options());
   if (grad_w) r.dweight = at::empty({V, C}, weight.options());
-  const long row_floats = call.reduction ? (rows + 3) / 4 * 4 : 0;  // the rows' losses, where only their sum is returned
+  const long row_floats = call.reduction ? (rows + 255) / 256 * 256 : 0;  // the rows' losses, where only their sum is returned
   auto work = at::empty({row_floats + std::max(4L, rt_head_loss_workspace_floats(rows, V, C, K, grad_h, grad_w))}, f32);
   RtHeadLoss p{};
   p.hidden = flat.data_ptr();

@@ -417,7 +417,9 @@ int dx_splits(long rows, long V, int C) {
   return best;
 }
 
-struct Layout {  // offsets in floats, each 16-byte aligned
+// Offsets in floats. Each is a multiple of 1 KB: a TMA box row of 128 bytes that straddles two lines costs twice the L2
+// accesses (dW of 1024 tokens: 2.8 ms from a 16-byte aligned dz, 1.8 ms from an aligned one).
+struct Layout {
   long rows, ld_e, tiles, splits, split_rows;  // rows of a chunk, row stride of the exponentials, tiles of the vocabulary
   bool dw32;
   long kind, slot, row_of, counts, x, sidx, slogp, hit, coef, lse2, tail, part, e, dx, dw, total;
@@ -427,7 +429,7 @@ Layout layout(long T, long V, int C, int K, bool grad_h, bool grad_w) {
   long at = 0;
   auto take = [&](long floats) {
     const long o = at;
-    at += up(floats, 4);
+    at += up(floats, 256);
     return o;
   };
   const bool grad = grad_h || grad_w;
