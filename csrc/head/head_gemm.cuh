@@ -45,6 +45,7 @@ struct Args {
   int store_e;
   int add;          // DW32: add to what is there
   int* status;
+  uint4* poison;    // DW: the gradient's first 16 bytes, NaN if a wait gave up
 };
 
 struct Maps {
@@ -385,7 +386,10 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
     sm100::tc_fence_after();
     sm100::tmem_dealloc_pair(tmem_base, 512);
   }
-  if (threadIdx.x == 0 && *abort) atomicExch(args.status, 1);
+  if (threadIdx.x == 0 && *abort) {
+    atomicExch(args.status, 1);
+    if (MODE == DW) *args.poison = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+  }
 }
 
 }  // namespace head

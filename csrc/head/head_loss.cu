@@ -16,7 +16,8 @@
 // relative to their tile's maximum; gradient_kernel turns them into dz in place, and dX = dz W, dW = dz^T X follow.
 // That is 6 T V C operations, against 8 T V C where the logits are formed a second time, for T V bf16 values of
 // workspace; CHUNK_VALUES bounds it, and more rows run in chunks whose dW adds up in fp32. Rows without a loss cost
-// nothing but their packing, and what they hold never meets the other rows.
+// nothing but their packing, and what they hold never meets the other rows. A product that gave up a bounded wait leaves
+// NaN in the losses, or in the gradient it was forming.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -34,6 +35,7 @@ __device__ __forceinline__ int entry_kind(long id, bool record, long ignore, lon
   if (record ? id < 0 : id == ignore) return 0;
   return id < 0 || id >= V ? 2 : 1;
 }
+__device__ __forceinline__ int row_kind(int entries) { return entries & 2 ? 2 : entries; }  // of the entries' kinds or'd
 
 // One warp per row: kind[row] of a record of K entries.
 __global__ void kinds_kernel(const long* __restrict__ idx, long rows, int K, long V, int* __restrict__ kind) {
@@ -42,14 +44,20 @@ __global__ void kinds_kernel(const long* __restrict__ idx, long rows, int K, lon
   int any = 0;
   for (int k = threadIdx.x & 31; k < K; k += 32) any |= entry_kind(idx[row * K + k], true, 0, V);
   any = __reduce_or_sync(~0u, any);
-  if ((threadIdx.x & 31) == 0) kind[row] = any & 2 ? 2 : any;
+  if ((threadIdx.x & 31) == 0) kind[row] = row_kind(any);
 }
 
-// One block: slot[row] = place of a valid row among the valid ones, or -1 (no loss), -2 (outside the vocabulary);
-// row_of[place] its row; counts = {valid rows, rows with a loss, status}. The kinds come from `kind`, or from targets.
+// What the rows' losses and gradients are taken over: valid rows, rows with a loss, a product that gave up a wait, and
+// blocks of merge_kernel that are done.
+struct Counts {
+  int valid, counted, failed, done;
+};
+
+// One block: slot[row] = place of a valid row among the valid ones, or -1 (no loss), -2 (outside the vocabulary). The
+// kinds come from `kind`, or from targets.
 __global__ void __launch_bounds__(1024) pack_kernel(const int* __restrict__ kind, const long* __restrict__ targets,
                                                     long ignore, long V, long rows, int* __restrict__ slot,
-                                                    int* __restrict__ row_of, int* __restrict__ counts) {
+                                                    Counts* __restrict__ counts) {
   __shared__ int warps[2][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int valid = 0, bad = 0;
@@ -68,14 +76,42 @@ __global__ void __launch_bounds__(1024) pack_kernel(const int* __restrict__ kind
     valid += __reduce_add_sync(~0u, g);
     bad += __reduce_add_sync(~0u, b);
     if (t < rows) slot[t] = k == 1 ? at : -k - (k == 0);
-    if (t < rows && k == 1) row_of[at] = (int)t;
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    counts[0] = valid;
-    counts[1] = valid + bad;
-    counts[2] = 0;
+  if (threadIdx.x == 0) *counts = Counts{valid, valid + bad, 0, 0};
+}
+
+// The same for the block of one row of a short call (at most SHORT_ENTRIES in all its records), which counts the rows
+// before its own itself: the place or -1 / -2, and the number of valid rows. Saves one or two launches.
+constexpr int SHORT_ENTRIES = 4096;
+__device__ __forceinline__ int place_in_short(const long* idx, bool record, int K, long rows, long row, long ignore,
+                                              long V, Counts* counts, int* scratch, int& valid) {
+  int before = 0, all = 0, bad = 0;
+  for (long t = threadIdx.x; t < rows; t += blockDim.x) {
+    int any = 0;
+    for (int k = 0; k < K; ++k) any |= entry_kind(idx[t * K + k], record, ignore, V);
+    const int kind = row_kind(any);
+    before += t < row && kind == 1;
+    all += kind == 1;
+    bad += kind == 2;
+    if (t == row) scratch[3] = kind;
   }
+  if (threadIdx.x < 3) scratch[threadIdx.x] = 0;
+  __syncthreads();
+  before = __reduce_add_sync(~0u, before);
+  all = __reduce_add_sync(~0u, all);
+  bad = __reduce_add_sync(~0u, bad);
+  if ((threadIdx.x & 31) == 0) {
+    atomicAdd(&scratch[0], before);
+    atomicAdd(&scratch[1], all);
+    atomicAdd(&scratch[2], bad);
+  }
+  __syncthreads();
+  valid = scratch[1];
+  if (row == 0 && threadIdx.x == 0) *counts = Counts{valid, valid + scratch[2], 0, 0};
+  if (row >= rows) return 0;
+  const int kind = scratch[3];
+  return kind == 1 ? scratch[0] : -kind - (kind == 0);
 }
 
 // One block per row, and 64 more for the zero rows that fill the packed rows' last block of 64. A valid row's hidden
@@ -86,8 +122,9 @@ __global__ void __launch_bounds__(1024) pack_kernel(const int* __restrict__ kind
 __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ idx, const float* __restrict__ logp,
                                                      int K, int Kp, long rows, const __nv_bfloat16* __restrict__ hidden,
                                                      long ldh, const __nv_bfloat16* __restrict__ w, long ldw, int C,
-                                                     float scale2, const int* __restrict__ slot,
-                                                     const int* __restrict__ counts, uint4* __restrict__ x,
+                                                     float scale2, long V, long ignore, bool brief,
+                                                     const int* __restrict__ slot, Counts* __restrict__ counts,
+                                                     int* __restrict__ row_of, uint4* __restrict__ x,
                                                      int* __restrict__ sidx, float* __restrict__ slogp,
                                                      float* __restrict__ hit, float* __restrict__ row_loss,
                                                      uint4* __restrict__ dhidden) {
@@ -95,19 +132,28 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
   const long row = blockIdx.x;
   const int C8 = C / 8;
   const uint4 zero = make_uint4(0, 0, 0, 0);
+  __shared__ int scratch[4];
+  int valid;
+  long place;
+  if (brief) {
+    place = place_in_short(idx, logp != nullptr, K, rows, row, ignore, V, counts, scratch, valid);
+  } else {
+    valid = counts->valid;
+    place = row < rows ? slot[row] : 0;
+  }
   if (row >= rows) {
-    const long n = counts[0], fill = n + (row - rows);
+    const long n = valid, fill = n + (row - rows);
     if (fill < max((n + 63) / 64 * 64, 64L))
       for (int c = threadIdx.x; c < C8; c += blockDim.x) x[fill * C8 + c] = zero;
     return;
   }
-  const long place = slot[row];
   if (place < 0) {
     if (threadIdx.x == 0) row_loss[row] = place == -1 ? 0.f : NAN;
     if (dhidden)
       for (int c = threadIdx.x; c < C8; c += blockDim.x) dhidden[row * C8 + c] = zero;
     return;
   }
+  if (threadIdx.x == 0) row_of[place] = (int)row;
   const uint4* src = reinterpret_cast<const uint4*>(hidden + row * ldh);
   for (int c = threadIdx.x; c < C8; c += blockDim.x) x[place * C8 + c] = __ldg(src + c);
   for (int k = threadIdx.x; k < Kp; k += blockDim.x) {
@@ -165,7 +211,9 @@ struct MergeArgs {
   const float2* part;
   long part_ld;
   int tiles, row0, rows, K, tail_class, mean;
-  const int* counts;
+  int blocks;  // of all chunks
+  long all_rows;
+  Counts* counts;
   const int* row_of;
   const int* sidx;
   const float* slogp;
@@ -173,6 +221,7 @@ struct MergeArgs {
   float scale;
   const float* grad;
   float* row_loss;
+  float* loss;  // null: the rows' losses are the result
   float* lse2;
   float* tail;
   float* coef;
@@ -184,13 +233,12 @@ __device__ __forceinline__ float2 merge2(float2 a, float2 b) {
   return make_float2(m, (a.x == m ? a.y : a.y * exp2f(a.x - m)) + (b.x == m ? b.y : b.y * exp2f(b.x - m)));
 }
 
-__global__ void __launch_bounds__(MERGE_ROWS * MERGE_GROUPS) merge_kernel(const MergeArgs p) {
+__device__ __forceinline__ void merge_rows(const MergeArgs& p) {
   __shared__ float2 merged[MERGE_GROUPS][MERGE_ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = min(max(p.counts[0] - p.row0, 0), p.rows);
+  const int n = min(max(p.counts->valid - p.row0, 0), p.rows);
   const int first = blockIdx.x * MERGE_ROWS;
-  if (first >= n) return;
-  {
+  if (first < n) {
     const int j = threadIdx.x % MERGE_ROWS, group = threadIdx.x / MERGE_ROWS;
     const float2* part = p.part + min(first + j, n - 1);
     float2 sum = make_float2(-INFINITY, 0.f);
@@ -251,9 +299,9 @@ __global__ void __launch_bounds__(MERGE_ROWS * MERGE_GROUPS) merge_kernel(const 
       value += r1 * (log(r1) - lr);
       a -= r1 * exp(-lr);
     }
-    const float g = p.scale * (p.grad ? p.grad[row] : (p.mean ? 1.f / (float)max(p.counts[1], 1) : 1.f));
+    const float g = p.scale * (p.grad ? p.grad[row] : (p.mean ? 1.f / (float)max(p.counts->counted, 1) : 1.f));
     if (lane == 0) {
-      p.row_loss[row] = (float)value;
+      p.row_loss[row] = p.counts->failed ? NAN : (float)value;
       p.lse2[place] = (float)l2;
       p.tail[place] = g * (float)a;
     }
@@ -271,78 +319,85 @@ __global__ void __launch_bounds__(MERGE_ROWS * MERGE_GROUPS) merge_kernel(const 
   }
 }
 
-// Last launch of a call: out[0] = sum (or mean over rows with a loss) of the rows' losses, in a fixed order. A wait that
-// gave up in one of the products makes every loss NaN.
-__global__ void __launch_bounds__(1024) total_kernel(float* __restrict__ loss, long rows, int mean,
-                                                     const int* __restrict__ counts, float* __restrict__ out) {
-  __shared__ double part[32];
-  const bool failed = counts[2] != 0;
+// The last block to finish also adds up the rows' losses, in a fixed order (mean: over rows with a loss).
+__global__ void __launch_bounds__(MERGE_ROWS * MERGE_GROUPS) merge_kernel(const MergeArgs p) {
+  __shared__ double part[MERGE_ROWS * MERGE_GROUPS / 32];
+  __shared__ bool last;
+  merge_rows(p);
+  if (!p.loss) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(&p.counts->done, 1) == p.blocks - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
   double s = 0.;
-  for (long t = threadIdx.x; t < rows; t += blockDim.x) {
-    if (failed) loss[t] = NAN;
-    else s += (double)loss[t];
-  }
-  if (!out) return;
+  for (long t = threadIdx.x; t < p.all_rows; t += blockDim.x) s += (double)__ldcg(p.row_loss + t);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(~0u, s, off);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < (int)blockDim.x / 32; ++w) s += part[w];
-    out[0] = failed ? NAN : (float)(mean ? s / (double)max(counts[1], 1) : s);
+    *p.loss = (float)(p.mean ? s / (double)max(p.counts->counted, 1) : s);
   }
 }
 
 // ---------------------------------------------------------------- gradient of the logits
-// In place: exponentials of a chunk's rows (relative to their tile's maximum) -> dz, one warp per row and tile; rows
-// that fill the last block of 64 become zero. The held entries' places hold zeros until held_gradient_kernel.
+// In place: exponentials of a chunk's rows (relative to their tile's maximum) -> dz, one warp per row and tile, which
+// also puts the tile's held entries in their places; rows that fill the last block of 64 become zero. A read and a write
+// of every value: 0.18 ms for 1024 x 248077 (5.7 TB/s), where forming the logits again would cost 1.8 ms.
 __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict__ e, long ld, int V, int tiles,
-                                                       int row0, int rows, const int* __restrict__ counts,
+                                                       int row0, int rows, const Counts* __restrict__ counts,
                                                        const float2* __restrict__ part, long part_ld,
-                                                       const float* __restrict__ lse2, const float* __restrict__ tail) {
-  const int n = min(max(counts[0] - row0, 0), rows), r = blockIdx.y;
+                                                       const float* __restrict__ lse2, const float* __restrict__ tail,
+                                                       int K, const int* __restrict__ sidx,
+                                                       const float* __restrict__ coef) {
+  const int n = min(max(counts->valid - row0, 0), rows), r = blockIdx.y;
   if (r >= max((n + 63) / 64 * 64, 64)) return;
   const int lane = threadIdx.x & 31;
   const bool live = r < n;
   const float l = live ? lse2[row0 + r] : 0.f, a = live ? tail[row0 + r] : 0.f;
+  sidx += (long)(row0 + r) * K;
+  coef += (long)(row0 + r) * K;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int t = (blockIdx.x * 4 + u) * 8 + (threadIdx.x >> 5), c = t * 256 + lane * 8;
-    if (t >= tiles || c >= ld) continue;
-    uint4* at = reinterpret_cast<uint4*>(e + r * ld + c);
-    if (!live) {
-      *at = make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    float v[8];
-    rt::unpack8(*at, v);
-    const float m = part[t * part_ld + r].x, f = m == -INFINITY ? 0.f : a * exp2f(m - l);
+    if (t >= tiles) continue;
+    __nv_bfloat16* out = e + r * ld;
+    if (c < ld) {
+      uint4* at = reinterpret_cast<uint4*>(out + c);
+      float v[8] = {};
+      if (live) {
+        rt::unpack8(*at, v);
+        const float m = part[t * part_ld + r].x, f = m == -INFINITY ? 0.f : a * exp2f(m - l);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= f;
-    *at = rt::pack8(v);
+        for (int j = 0; j < 8; ++j) v[j] *= f;
+      }
+      *at = rt::pack8(v);
+    }
+    if (!live) continue;
+    __syncwarp();
+    for (int k = 0; k < K; k += 32) {  // ascending indices
+      const int s = k + lane < K ? sidx[k + lane] : INT_MAX;
+      if (s >= t * 256 && s < t * 256 + 256 && s < V) out[s] = __float2bfloat16_rn(coef[k + lane]);
+      if (__any_sync(~0u, s >= t * 256 + 256)) break;
+    }
   }
-}
-
-__global__ void held_gradient_kernel(__nv_bfloat16* __restrict__ dz, long ld, int K, int row0, int rows,
-                                     const int* __restrict__ counts, const int* __restrict__ sidx,
-                                     const float* __restrict__ coef) {
-  const int n = min(max(counts[0] - row0, 0), rows);
-  const long e = (long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (e >= (long)n * K) return;
-  const long at = (long)row0 * K + e;
-  const int v = sidx[at];
-  if (v != INT_MAX) dz[e / K * ld + v] = __float2bfloat16_rn(coef[at]);
 }
 
 // dhidden[row_of[place]] = bf16 of the row's partial sums, added in order.
 __global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ partial, int splits, long split_rows,
-                                                      int C, int row0, int rows, const int* __restrict__ counts,
+                                                      int C, int row0, int rows, const Counts* __restrict__ counts,
                                                       const int* __restrict__ row_of, __nv_bfloat16* __restrict__ out) {
-  const int n = min(max(counts[0] - row0, 0), rows), r = blockIdx.x;
+  const int n = min(max(counts->valid - row0, 0), rows), r = blockIdx.x;
   if (r >= n) return;
+  const float failed = counts->failed ? NAN : 0.f;  // a product gave up a wait
   uint4* dst = reinterpret_cast<uint4*>(out + (long)row_of[row0 + r] * C);
   for (int c = threadIdx.x; c < C / 8; c += blockDim.x) {
-    float v[8] = {};
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = failed;
     for (int s = 0; s < splits; ++s) {
       const float4* src = reinterpret_cast<const float4*>(partial + ((long)s * split_rows + r) * C) + 2 * c;
       const float4 x = __ldg(src), y = __ldg(src + 1);
@@ -351,6 +406,11 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ 
     }
     dst[c] = rt::pack8(v);
   }
+}
+
+// The weight's gradient of a product that gave up a wait (the one-chunk kernel leaves its NaN itself).
+__global__ void failed_kernel(const Counts* __restrict__ counts, __nv_bfloat16* __restrict__ dweight) {
+  if (counts->failed && threadIdx.x < 8) dweight[threadIdx.x] = __float2bfloat16_rn(NAN);
 }
 
 // x *= *factor for up to two tensors, nothing at all for a factor of one (the usual upstream gradient of a loss).
@@ -506,26 +566,29 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   const bool grad = p->dhidden || p->dweight;
   const Layout l = layout(T, V, C, K, p->dhidden != nullptr, p->dweight != nullptr);
   auto ints = [&](long at) { return reinterpret_cast<int*>(work + at); };
-  int* counts = ints(l.counts);
+  Counts* counts = reinterpret_cast<Counts*>(work + l.counts);
   __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(work + l.x);
   __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(work + l.e);
   float2* part = reinterpret_cast<float2*>(work + l.part);
   const float scale2 = p->scale * LOG2E;
-  if (p->log_probs) kinds_kernel<<<(unsigned)((T * 32 + 255) / 256), 256, 0, s>>>(p->index, T, K, V, ints(l.kind));
-  pack_kernel<<<1, 1024, 0, s>>>(p->log_probs ? ints(l.kind) : nullptr, p->index, p->ignore, V, T, ints(l.slot),
-                                 ints(l.row_of), counts);
+  const bool brief = T * K <= SHORT_ENTRIES;
+  if (!brief) {
+    if (p->log_probs) kinds_kernel<<<(unsigned)((T * 32 + 255) / 256), 256, 0, s>>>(p->index, T, K, V, ints(l.kind));
+    pack_kernel<<<1, 1024, 0, s>>>(p->log_probs ? ints(l.kind) : nullptr, p->index, p->ignore, V, T, ints(l.slot),
+                                   counts);
+  }
   int Kp = 1;
   while (Kp < K) Kp <<= 1;
   gather_kernel<<<(unsigned)(T + 64), 256, Kp * 8, s>>>(
       p->index, p->log_probs, K, Kp, T, reinterpret_cast<const __nv_bfloat16*>(p->hidden), p->ld_hidden,
-      reinterpret_cast<const __nv_bfloat16*>(p->weight), p->ld_weight, C, scale2, ints(l.slot), counts,
-      reinterpret_cast<uint4*>(x), ints(l.sidx), work + l.slogp, work + l.hit, p->row_loss,
+      reinterpret_cast<const __nv_bfloat16*>(p->weight), p->ld_weight, C, scale2, V, p->ignore, brief,
+      ints(l.slot), counts, ints(l.row_of), reinterpret_cast<uint4*>(x), ints(l.sidx), work + l.slogp, work + l.hit, p->row_loss,
       reinterpret_cast<uint4*>(p->dhidden));
   RT_CUDA_CHECK(cudaGetLastError());
 
   head::Maps logits, dx, dw;
   head::Args args{};
-  args.live = counts;
+  args.live = &counts->valid;
   args.V = (int)V;
   args.C = C;
   args.K = K;
@@ -535,7 +598,10 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   args.store_e = grad;
   args.splits = (int)std::max(1L, l.splits);
   args.split_rows = (int)l.split_rows;
-  args.status = counts + 2;
+  args.status = &counts->failed;
+  int merge_blocks = 0;
+  for (long row0 = 0; row0 < T; row0 += l.rows)
+    merge_blocks += (int)((std::min(l.rows, up(T - row0, 64)) + MERGE_ROWS - 1) / MERGE_ROWS);
   for (long row0 = 0; row0 < T; row0 += l.rows) {
     const long rows = std::min(l.rows, up(T - row0, 64));  // packed rows of x are filled up to a block of 64
     __nv_bfloat16* xc = x + row0 * C;
@@ -549,16 +615,14 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
       return cudaErrorInvalidValue;
     const long tiles_m = up(rows, 256) / 256, tiles_c = up(C, 256) / 256;
     RT_CUDA_CHECK(launch<head::LOGITS>(logits, args, tiles_m * l.tiles, s));
-    MergeArgs m{part, l.rows, (int)l.tiles, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, counts,
-                ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->scale, p->row_grad, p->row_loss,
-                work + l.lse2, work + l.tail, grad ? work + l.coef : nullptr};
+    MergeArgs m{part, l.rows, (int)l.tiles, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, merge_blocks, T,
+                counts, ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->scale, p->row_grad, p->row_loss,
+                p->reduction ? p->loss : nullptr, work + l.lse2, work + l.tail, grad ? work + l.coef : nullptr};
     merge_kernel<<<(unsigned)((rows + MERGE_ROWS - 1) / MERGE_ROWS), MERGE_ROWS * MERGE_GROUPS, 0, s>>>(m);
-    if (grad) {
+    if (grad)
       gradient_kernel<<<dim3((unsigned)((l.tiles + 31) / 32), (unsigned)rows), 256, 0, s>>>(
-          e, l.ld_e, (int)V, (int)l.tiles, (int)row0, (int)l.rows, counts, part, l.rows, work + l.lse2, work + l.tail);
-      held_gradient_kernel<<<(unsigned)((rows * K + 255) / 256), 256, 0, s>>>(e, l.ld_e, K, (int)row0, (int)l.rows,
-                                                                              counts, ints(l.sidx), work + l.coef);
-    }
+          e, l.ld_e, (int)V, (int)l.tiles, (int)row0, (int)l.rows, counts, part, l.rows, work + l.lse2, work + l.tail, K,
+          ints(l.sidx), work + l.coef);
     RT_CUDA_CHECK(cudaGetLastError());
     if (p->dhidden) {
       if (!map2d(&dx.a, false, e, V, rows, 2 * l.ld_e, 128) ||
@@ -576,11 +640,14 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
           !map2d(&dw.out, l.dw32, out, C, V, (l.dw32 ? 4L : 2L) * C, 32))
         return cudaErrorInvalidValue;
       const long units = l.tiles * tiles_c;
+      args.poison = static_cast<uint4*>(p->dweight);
       RT_CUDA_CHECK(l.dw32 ? launch<head::DW32>(dw, args, units, s) : launch<head::DW>(dw, args, units, s));
     }
   }
-  if (l.dw32) RT_CUDA_CHECK(rt_to_bf16(work + l.dw, p->dweight, V * C, s));
-  total_kernel<<<1, 1024, 0, s>>>(p->row_loss, T, p->reduction == 2, counts, p->reduction ? p->loss : nullptr);
+  if (l.dw32) {
+    RT_CUDA_CHECK(rt_to_bf16(work + l.dw, p->dweight, V * C, s));
+    failed_kernel<<<1, 32, 0, s>>>(counts, reinterpret_cast<__nv_bfloat16*>(p->dweight));
+  }
   return cudaGetLastError();
 }
 
