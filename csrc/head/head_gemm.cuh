@@ -164,7 +164,6 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = (int)sm100::cluster_rank();
-  const int n = min(max(*args.live - args.row0, 0), args.rows);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -191,6 +190,8 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
   sm100::cluster_sync();
   sm100::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  rt::grid_wait();  // all above runs beside the end of the kernel before
+  const int n = min(max(*args.live - args.row0, 0), args.rows);
   Work<MODE> work(args, n);
   int tm, tn, split, k0, k1;
 
