@@ -1,10 +1,15 @@
-// The three matrix products of the vocabulary-head losses on CTA pairs: 256 x 256 tiles, fp32 accumulators in TMEM,
-// one persistent kernel each.
+// The three matrix products of the vocabulary-head losses on CTA pairs: tiles of 256 x 256 (256 x NT for few rows), fp32
+// accumulators in TMEM, one persistent kernel each.
 //
 //   LOGITS  z = X . W^T              X [n, C] live rows, W [V, C]; z stays on chip: per row and tile the epilogue
 //                                    leaves (max, sum of exponentials) and, for gradients, the exponentials in bf16
 //   DX      dX = dz . W              dz [n, V]; K = V is cut into `splits` parts, each an fp32 partial sum
 //   DW      dW = dz^T . X            bf16, or fp32 added up over chunks of rows
+//   LOGITS_N, DX_N                   the first two for up to NT = 32 or 128 rows, as z^T = W . X^T and dX^T = W^T . dz^T:
+//                                    the rows are the tile's columns, so the tensor cores do 1/8 or 1/2 of the work of
+//                                    a 256-row tile that is mostly padding. These calls are bound by reading W; with
+//                                    padded tiles the 1 kW power cap halved the clock and with it the bandwidth (one
+//                                    row x 248077 x 5120 in a loop: 540 us at 1.25 GHz).
 //
 // n, the number of rows that have a loss, is only known on the device (`live`): the kernels read it there.
 //
@@ -12,7 +17,7 @@
 // of 64-deep K blocks; warp 1 of the even CTA issues the pair's MMAs (M = 256, N = 256, K = 16: each CTA holds 128
 // rows of A and 128 columns of B, so an operand byte in shared memory feeds twice the products of a one-CTA tile);
 // warps 2-5 drain the double-buffered accumulators. Outputs leave through swizzled staging buffers by TMA stores of 32
-// rows, one warp at a time. All waits are bounded (sm100.cuh); one that gives up sets *status.
+// rows, one warp at a time (LOGITS_N, DX_N: by coalesced stores). All waits are bounded (sm100.cuh); one that gives up sets *status.
 #pragma once
 #include <climits>
 #include "../common/common.cuh"
@@ -21,15 +26,29 @@
 
 namespace head {
 
-enum Mode : int { LOGITS = 0, DX = 1, DW = 2, DW32 = 3 };
+enum Mode : int { LOGITS = 0, DX = 1, DW = 2, DW32 = 3, LOGITS_N = 4, DX_N = 5 };
 
-constexpr int TILE = 256, BK = 64, STAGES = 5, THREADS = 192;
-constexpr int HALF_BYTES = 128 * BK * 2;           // one CTA's half of an operand block
-constexpr int STAGE_BYTES = 2 * HALF_BYTES;        // A half and B half
+constexpr int TILE = 256, BK = 64, THREADS = 192;
+constexpr int HALF_BYTES = 128 * BK * 2;           // one CTA's half of a 256-wide operand block
 constexpr int MN_CHUNK_BYTES = 64 * BK * 2;        // MN-major operands: 64-wide chunks of BK rows x 128 bytes
 constexpr int STAGING_BYTES = 32 * 128;            // 32 rows of 128 bytes, two buffers per epilogue warp
 constexpr int MASK_BYTES = 4 * 8 * 32 * 4;         // held columns of a tile: 8 words per row
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 8 * STAGING_BYTES + MASK_BYTES + 256 + 1024;
+
+template <int MODE, int NT>
+struct Cfg {
+  static constexpr bool NARROW = MODE == LOGITS_N || MODE == DX_N;
+  static_assert(NARROW ? NT == 32 || NT == 128 : NT == TILE, "tile widths");
+  static constexpr bool A_MN = MODE == DW || MODE == DW32 || MODE == DX_N;
+  static constexpr bool B_MN = MODE == DX || MODE == DW || MODE == DW32;
+  static constexpr int STAGE_BYTES = HALF_BYTES + NT / 2 * BK * 2;  // A half and B half
+  // narrow tiles only stream W: their ring holds about as many bytes of it as fit
+  static constexpr int STAGES = NT == 32 ? 11 : NT == 128 ? 8 : 5;
+  static constexpr int STAGING = NARROW ? 0 : 8 * STAGING_BYTES, MASKS = MODE == LOGITS ? MASK_BYTES : 0;
+  static constexpr int BAR_BYTES = 512;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + STAGING + MASKS + BAR_BYTES + 1024;
+  static constexpr int ACC_COLS = NT, TMEM_COLS = 2 * NT;
+  static constexpr uint32_t IDESC = sm100::idesc_bf16(256, NT, A_MN, B_MN);
+};
 
 struct Args {
   const int* live;  // rows with a loss, all chunks
@@ -43,6 +62,9 @@ struct Args {
   float2* part;     // [tiles of the vocabulary, part_ld]
   long part_ld;
   int store_e;
+  __nv_bfloat16* e; // LOGITS_N: the exponentials, [rows, ld_e]
+  long ld_e;
+  float* dx;        // DX_N: the partial sums
   int add;          // DW32: add to what is there
   int* status;
   uint4* poison;    // DW: the gradient's first 16 bytes, NaN if a wait gave up
@@ -71,12 +93,20 @@ struct Work {
       tiles_m = rows_m;
       tiles_n = (a.C + TILE - 1) / TILE;
       kblocks = (a.V + BK - 1) / BK;
+    } else if (MODE == LOGITS_N) {
+      tiles_m = n ? (a.V + TILE - 1) / TILE : 0;
+      tiles_n = 1;
+      kblocks = (a.C + BK - 1) / BK;
+    } else if (MODE == DX_N) {
+      tiles_m = n ? (a.C + TILE - 1) / TILE : 0;
+      tiles_n = 1;
+      kblocks = (a.V + BK - 1) / BK;
     } else {
       tiles_m = (a.V + TILE - 1) / TILE;
       tiles_n = (a.C + TILE - 1) / TILE;
       kblocks = max(1, (n + BK - 1) / BK);  // no live row: one block of zeros
     }
-    splits = MODE == DX ? a.splits : 1;
+    splits = MODE == DX || MODE == DX_N ? a.splits : 1;
     units = tiles_m * tiles_n * splits;
     if (MODE == DW32 && n == 0 && a.add) units = 0;
     unit = blockIdx.x >> 1;
@@ -86,12 +116,12 @@ struct Work {
     if (unit >= units) return false;
     int t = unit;
     split = 0;
-    if (MODE == DX) {  // one part of K at a time, so that the pairs running together share its rows of W in L2
+    if (MODE == DX || MODE == DX_N) {  // one part of K at a time, so that the pairs running together share its rows of W in L2
       const int tiles = tiles_m * tiles_n;
       split = t / tiles;
       t %= tiles;
     }
-    if (MODE == LOGITS || MODE == DX) {  // rows fastest: the tiles running together share their part of W
+    if (MODE != DW && MODE != DW32) {  // rows fastest: the tiles running together share their part of W
       tm = t % tiles_m;
       tn = t / tiles_m;
     } else {  // columns fastest: they share the larger dz
@@ -135,6 +165,37 @@ __device__ __forceinline__ bool held_mask(const Args& a, int row, int n, int col
   return true;
 }
 
+// Entries of one row's record in [first, first + 32), as bits.
+__device__ __forceinline__ uint32_t held_word(const int* s, int K, int first) {
+  int lo = 0, hi = K;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s[mid] < first) lo = mid; else hi = mid;
+  }
+  uint32_t word = 0;
+  for (; lo < K; ++lo) {
+    const int d = s[lo] - first;
+    if (d >= 32) break;
+    if (d >= 0) word |= 1u << d;
+  }
+  return word;
+}
+
+// Lane j: op over the lanes of v[j]. Each step halves the columns a lane holds: 31 shuffles for 32 columns.
+template <typename Op>
+__device__ __forceinline__ float columns(float (&v)[32], int lane, Op op) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    const bool upper = lane & s;
+#pragma unroll
+    for (int i = 0; i < s; ++i) {
+      const float send = upper ? v[i] : v[i + s], keep = upper ? v[i + s] : v[i];
+      v[i] = op(keep, __shfl_xor_sync(~0u, send, s));
+    }
+  }
+  return v[0];
+}
+
 __device__ __forceinline__ void drop_held(float (&v)[32], uint32_t word) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = word >> i & 1 ? -INFINITY : v[i];
@@ -145,16 +206,17 @@ __device__ __forceinline__ uint4* staged(uint8_t* buf, int lane, int q) {
   return reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4));
 }
 
-template <int MODE>
+template <int MODE, int NT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 pair_kernel(const __grid_constant__ Maps maps, const Args args) {
-  constexpr bool A_MN = MODE == DW || MODE == DW32, B_MN = MODE != LOGITS;
-  constexpr uint32_t IDESC = sm100::idesc_bf16(256, 256, A_MN, B_MN);
+  using C_ = Cfg<MODE, NT>;
+  constexpr bool A_MN = C_::A_MN, B_MN = C_::B_MN;
+  constexpr int STAGES = C_::STAGES, STAGE_BYTES = C_::STAGE_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = sm100::align_smem_1024(smem_raw);
   uint8_t* staging = smem + STAGES * STAGE_BYTES;
-  uint32_t* masks = reinterpret_cast<uint32_t*>(staging + 8 * STAGING_BYTES);
-  uint64_t* full = reinterpret_cast<uint64_t*>(staging + 8 * STAGING_BYTES + MASK_BYTES);
+  uint32_t* masks = reinterpret_cast<uint32_t*>(staging + C_::STAGING);
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + C_::STAGING + C_::MASKS);
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
   uint64_t* tempty = tfull + 2;
@@ -182,7 +244,7 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
     sm100::prefetch_tmap(&maps.out);
   }
   if (warp == 1) {
-    sm100::tmem_alloc_pair(tmem_slot, 512);
+    sm100::tmem_alloc_pair(tmem_slot, C_::TMEM_COLS);
     sm100::tmem_relinquish_pair();
   }
   sm100::tc_fence_before();
@@ -202,7 +264,7 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
       uint32_t phase = 0;
       bool ok = true;
       while (ok && work.next(tm, tn, split, k0, k1)) {
-        const int am = tm * TILE + cta * 128, bn = tn * TILE + cta * 128;
+        const int am = tm * TILE + cta * 128, bn = tn * NT + cta * (NT / 2);
         for (int kb = k0; kb < k1; ++kb) {
           if (!sm100::mbar_wait(&empty[stage], phase ^ 1, abort)) {
             ok = false;
@@ -241,7 +303,7 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
       while (ok && work.next(tm, tn, split, k0, k1)) {
         if (!sm100::mbar_wait(&tempty[acc], acc_phase ^ 1, abort)) break;
         sm100::tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * 256;
+        const uint32_t d_tmem = tmem_base + acc * C_::ACC_COLS;
         for (int kb = k0; kb < k1; ++kb) {
           if (!sm100::mbar_wait(&full[stage], phase, abort)) {
             ok = false;
@@ -256,7 +318,7 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
                                         : sm100::smem_desc(a_base + ks * 32, 16, 1024);
             const uint64_t bdesc = B_MN ? sm100::smem_desc(b_base + ks * 2048, MN_CHUNK_BYTES, 1024)
                                         : sm100::smem_desc(b_base + ks * 32, 16, 1024);
-            sm100::mma_bf16_pair(d_tmem, adesc, bdesc, IDESC, kb != k0 || ks != 0);
+            sm100::mma_bf16_pair(d_tmem, adesc, bdesc, C_::IDESC, kb != k0 || ks != 0);
           }
           sm100::mma_commit_pair(&empty[stage]);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -282,7 +344,7 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
       if (MODE == LOGITS) masked = held_mask(args, row0 + lane, n, col0, mask);
       if (!__all_sync(~0u, sm100::mbar_wait(&tfull[acc], acc_phase, abort))) break;
       sm100::tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
+      const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * C_::ACC_COLS;
       // staging buffer of the next store: its previous store has been read
       auto next_buffer = [&]() {
         if (lane == 0) sm100::bulk_wait_read<1>();
@@ -300,7 +362,51 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
           sm100::bulk_commit();
         }
       };
-      if (MODE == LOGITS) {
+      if (MODE == LOGITS_N) {
+        const int v_at = row0 + lane;  // this thread's entry of the vocabulary; the columns are rows of X
+#pragma unroll 1
+        for (int g = 0; g < NT / 32 && 32 * g < n; ++g) {
+          const int j = 32 * g + lane;
+          const uint32_t word = j < n ? held_word(args.sidx + (long)j * args.K, args.K, row0) : 0u;
+          const bool held = __any_sync(~0u, word != 0);
+          float v[32], t[32];
+          sm100::tmem_ld32(t_row + 32 * g, v);
+          sm100::tmem_wait_ld();
+          if (held) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (__shfl_sync(~0u, word, i) >> lane & 1) v[i] = -INFINITY;
+          }
+          if (v_at >= args.V) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) t[i] = v[i];
+          const float m = columns(t, lane, [](float a, float b) { return fmaxf(a, b); });
+          const float m2 = m == -INFINITY ? 0.f : m * args.scale2;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            v[i] = ex2(fmaf(v[i], args.scale2, -__shfl_sync(~0u, m2, i)));
+            if (args.store_e && 32 * g + i < n && v_at < args.V)
+              args.e[(32 * g + i) * args.ld_e + v_at] = __float2bfloat16_rn(v[i]);
+          }
+          const float sum = columns(v, lane, [](float a, float b) { return a + b; });
+          if (j < n) args.part[(row0 / 32) * args.part_ld + j] = make_float2(m == -INFINITY ? m : m2, sum);
+        }
+      } else if (MODE == DX_N) {
+        const int c_at = row0 + lane;
+#pragma unroll 1
+        for (int g = 0; g < NT / 32 && 32 * g < n; ++g) {
+          float v[32];
+          sm100::tmem_ld32(t_row + 32 * g, v);
+          sm100::tmem_wait_ld();
+          float* out = args.dx + ((long)split * args.split_rows + 32 * g) * args.C + c_at;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * g + i < n && c_at < args.C) out[(long)i * args.C] = v[i];
+        }
+      } else if (MODE == LOGITS) {
         float m = -INFINITY;
 #pragma unroll 1
         for (int c = 0; c < 8; ++c) {
@@ -385,7 +491,7 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
   sm100::cluster_sync();  // neither CTA's shared memory or TMEM is used by the other any more
   if (warp == 1) {
     sm100::tc_fence_after();
-    sm100::tmem_dealloc_pair(tmem_base, 512);
+    sm100::tmem_dealloc_pair(tmem_base, C_::TMEM_COLS);
   }
   if (threadIdx.x == 0 && *abort) {
     atomicExch(args.status, 1);

@@ -205,11 +205,11 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
 }
 
 // ---------------------------------------------------------------- losses of the valid rows of a chunk
-// Block of MERGE_ROWS rows: its threads merge the tiles' statistics (in a fixed order: each row's tiles go round-robin
-// to MERGE_GROUPS threads), then one warp per row forms the loss and the gradient's coefficients: d/dz_v = tail
+// Block of ROWS rows (four, or one of the few rows whose statistics are finer): its threads merge the tiles' statistics
+// (in a fixed order: each row's tiles go round-robin to MERGE_THREADS / ROWS threads), then one warp per row forms the loss and the gradient's coefficients: d/dz_v = tail
 // exp2(z_v - lse2) outside the record, coef[k] for its held entries, both times scale and the row's upstream gradient
 // (given per row, or 1, or 1 / rows with a loss).
-constexpr int MERGE_ROWS = 4, MERGE_GROUPS = 64;
+constexpr int MERGE_THREADS = 256;
 struct MergeArgs {
   const float2* part;
   long part_ld;
@@ -236,20 +236,22 @@ __device__ __forceinline__ float2 merge2(float2 a, float2 b) {
   return make_float2(m, (a.x == m ? a.y : a.y * exp2f(a.x - m)) + (b.x == m ? b.y : b.y * exp2f(b.x - m)));
 }
 
+template <int ROWS>
 __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
-  __shared__ float2 merged[MERGE_GROUPS][MERGE_ROWS];
+  constexpr int GROUPS = MERGE_THREADS / ROWS;
+  __shared__ float2 merged[GROUPS][ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int n = min(max(p.counts->valid - p.row0, 0), p.rows);
-  const int first = blockIdx.x * MERGE_ROWS;
+  const int first = blockIdx.x * ROWS;
   if (first < n) {
-    const int j = threadIdx.x % MERGE_ROWS, group = threadIdx.x / MERGE_ROWS;
+    const int j = threadIdx.x % ROWS, group = threadIdx.x / ROWS;
     const float2* part = p.part + min(first + j, n - 1);
     float2 sum = make_float2(-INFINITY, 0.f);
-    for (int i = group; i < p.tiles; i += 4 * MERGE_GROUPS) {
+    for (int i = group; i < p.tiles; i += 4 * GROUPS) {
       float2 t[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        t[u] = i + u * MERGE_GROUPS < p.tiles ? part[(i + u * MERGE_GROUPS) * p.part_ld] : make_float2(-INFINITY, 0.f);
+        t[u] = i + u * GROUPS < p.tiles ? part[(i + u * GROUPS) * p.part_ld] : make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int u = 0; u < 4; ++u) sum = merge2(sum, t[u]);
     }
@@ -257,13 +259,15 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
   }
   __syncthreads();
   const int j = warp;
-  if (j < MERGE_ROWS && first + j < n) {
+  if (j < ROWS && first + j < n) {
     const int r = first + j;
     const long place = p.row0 + r, row = p.row_of[place];
     const int* sidx = p.sidx + place * p.K;
     const float* slogp = p.slogp + place * p.K;
     const float* hit = p.hit + place * p.K;
-    float2 all = merge2(merged[lane][j], merged[lane + 32][j]);
+    float2 all = merged[lane][j];
+#pragma unroll
+    for (int i = 32; i < GROUPS; i += 32) all = merge2(all, merged[lane + i][j]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1)
       all = merge2(all, make_float2(__shfl_xor_sync(~0u, all.x, off), __shfl_xor_sync(~0u, all.y, off)));
@@ -323,11 +327,12 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
 }
 
 // The last block to finish also adds up the rows' losses, in a fixed order (mean: over rows with a loss).
-__global__ void __launch_bounds__(MERGE_ROWS * MERGE_GROUPS) merge_kernel(const MergeArgs p) {
+template <int ROWS>
+__global__ void __launch_bounds__(MERGE_THREADS) merge_kernel(const MergeArgs p) {
   rt::grid_wait();
-  __shared__ double part[MERGE_ROWS * MERGE_GROUPS / 32];
+  __shared__ double part[MERGE_THREADS / 32];
   __shared__ bool last;
-  merge_rows(p);
+  merge_rows<ROWS>(p);
   if (!p.loss) return;
   __threadfence();
   __syncthreads();
@@ -348,12 +353,12 @@ __global__ void __launch_bounds__(MERGE_ROWS * MERGE_GROUPS) merge_kernel(const 
 }
 
 // ---------------------------------------------------------------- gradient of the logits
-// In place: exponentials of a chunk's rows (relative to their tile's maximum) -> dz, one warp per row and tile; the block
+// In place: exponentials of a chunk's rows (relative to the maximum of their `group` columns) -> dz, one warp per row and tile; the block
 // of 32 tiles also puts their held entries in their places; rows that fill the last block of 64 become zero. A read and a write
 // of every value: 0.18 ms for 1024 x 248077 (5.7 TB/s), where forming the logits again would cost 1.8 ms.
 __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict__ e, long ld, int V, int tiles,
                                                        int row0, int rows, const Counts* __restrict__ counts,
-                                                       const float2* __restrict__ part, long part_ld,
+                                                       const float2* __restrict__ part, long part_ld, int group,
                                                        const float* __restrict__ lse2, const float* __restrict__ tail,
                                                        int K, const int* __restrict__ sidx,
                                                        const float* __restrict__ coef) {
@@ -373,9 +378,9 @@ __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict
     if (c < ld) {
       uint4* at = reinterpret_cast<uint4*>(out + c);
       float v[8] = {};
-      if (live) {
+      if (live && c < V) {
         rt::unpack8(*at, v);
-        const float m = part[t * part_ld + r].x, f = m == -INFINITY ? 0.f : a * exp2f(m - l);
+        const float m = part[c / group * part_ld + r].x, f = m == -INFINITY ? 0.f : a * exp2f(m - l);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= f;
       }
@@ -466,16 +471,20 @@ int pairs() {
   return n;
 }
 
-// Parts of K = V for dX. A wave of tiles takes kblocks / S blocks of 512 cycles and fills `pairs` pairs, or part of them
+// Calls of up to this many rows run the products as W . X^T, with the rows as the tiles' columns (head_gemm.cuh).
+constexpr long NARROW_ROWS = 128;
+
+// Parts of K = V for dX. A wave of tiles takes kblocks / S blocks of 512 cycles (700 to read W, for few rows) and fills `pairs` pairs, or part of them
 // in the last wave; each part adds a write and a read of rows x C fp32 partial sums (16 bytes per value at about 5
 // TB/s = 2800 bytes a cycle).
 int dx_splits(long rows, long V, int C) {
   const long tiles = up(rows, 256) / 256 * (up(C, 256) / 256), kblocks = up(V, 64) / 64;
+  const double block = rows <= NARROW_ROWS ? 700 : 512;
   int best = 1;
   double least = 1e300;
   for (int S = 1; S <= 64 && S <= std::max(1L, kblocks / 16); ++S) {
     const long waves = (tiles * S + pairs() - 1) / pairs();
-    const double cycles = waves * ((double)kblocks / S * 512 + 3000) + (double)S * rows * C * 16 / 2800;
+    const double cycles = waves * ((double)kblocks / S * block + 3000) + (double)S * rows * C * 16 / 2800;
     if (cycles < least * 0.995) {
       least = cycles;
       best = S;
@@ -487,7 +496,8 @@ int dx_splits(long rows, long V, int C) {
 // Offsets in floats. Each is a multiple of 1 KB: a TMA box row of 128 bytes that straddles two lines costs twice the L2
 // accesses (dW of 1024 tokens: 2.8 ms from a 16-byte aligned dz, 1.8 ms from an aligned one).
 struct Layout {
-  long rows, ld_e, tiles, splits, split_rows;  // rows of a chunk, row stride of the exponentials, tiles of the vocabulary
+  // rows of a chunk, row stride of the exponentials, 256-wide tiles of the vocabulary, groups of columns with statistics
+  long rows, ld_e, tiles, groups, splits, split_rows;
   bool dw32;
   long kind, slot, row_of, counts, x, sidx, slogp, hit, coef, lse2, tail, part, e, dx, dw, total;
 };
@@ -502,6 +512,7 @@ Layout layout(long T, long V, int C, int K, bool grad_h, bool grad_w) {
   const bool grad = grad_h || grad_w;
   l.ld_e = up(V, 64);
   l.tiles = up(V, 256) / 256;
+  l.groups = T <= NARROW_ROWS ? l.tiles * 8 : l.tiles;
   l.rows = std::min(up(T, 64),
                     grad ? std::min(CHUNK_ROWS, std::max(256L, CHUNK_VALUES / l.ld_e / 256 * 256)) : SCORE_ROWS);
   l.dw32 = grad_w && l.rows < T;
@@ -518,7 +529,7 @@ Layout layout(long T, long V, int C, int K, bool grad_h, bool grad_w) {
   l.coef = take(grad ? T * K : 0);
   l.lse2 = take(T);
   l.tail = take(T);
-  l.part = take(2 * l.tiles * l.rows);
+  l.part = take(2 * l.groups * l.rows);
   l.e = take(grad ? l.rows * l.ld_e / 2 : 0);
   l.dx = take(l.splits * l.split_rows * C);
   l.dw = take(l.dw32 ? V * C : 0);
@@ -533,19 +544,20 @@ bool map2d(CUtensorMap* map, bool f32, const void* base, long inner, long outer,
                       strides, box);
 }
 
-template <int MODE>
+template <int MODE, int NT = head::TILE>
 cudaError_t launch(const head::Maps& maps, const head::Args& args, long units, cudaStream_t s) {
   static std::atomic<uint64_t> set{0};  // per device: the shared-memory size has been raised
   int dev = 0;
   RT_CUDA_CHECK(cudaGetDevice(&dev));
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (!bit || !(set.load(std::memory_order_acquire) & bit)) {
-    RT_CUDA_CHECK(cudaFuncSetAttribute(head::pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       head::SMEM_BYTES));
+    RT_CUDA_CHECK(cudaFuncSetAttribute(head::pair_kernel<MODE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       head::Cfg<MODE, NT>::SMEM_BYTES));
     set.fetch_or(bit, std::memory_order_acq_rel);
   }
   const unsigned grid = 2 * (unsigned)std::min<long>(units, pairs());
-  return rt::launch_after(head::pair_kernel<MODE>, grid, head::THREADS, head::SMEM_BYTES, s, maps, args);
+  return rt::launch_after(head::pair_kernel<MODE, NT>, grid, head::THREADS, head::Cfg<MODE, NT>::SMEM_BYTES, s, maps,
+                          args);
 }
 
 }  // namespace
@@ -599,14 +611,18 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   args.K = K;
   args.scale2 = scale2 * mma_gain(C);
   args.part = part;
+  args.e = e;
+  args.ld_e = l.ld_e;
+  args.dx = work + l.dx;
   args.part_ld = l.rows;
   args.store_e = grad;
   args.splits = (int)std::max(1L, l.splits);
   args.split_rows = (int)l.split_rows;
   args.status = &counts->failed;
+  const bool narrow = T <= NARROW_ROWS, few = T <= 32;  // one chunk
   int merge_blocks = 0;
   for (long row0 = 0; row0 < T; row0 += l.rows)
-    merge_blocks += (int)((std::min(l.rows, up(T - row0, 64)) + MERGE_ROWS - 1) / MERGE_ROWS);
+    merge_blocks += (int)(std::min(l.rows, up(T - row0, 64)) / (narrow ? 1 : 4));  // multiples of 64
   for (long row0 = 0; row0 < T; row0 += l.rows) {
     const long rows = std::min(l.rows, up(T - row0, 64));  // packed rows of x are filled up to a block of 64
     __nv_bfloat16* xc = x + row0 * C;
@@ -614,27 +630,32 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
     args.rows = (int)l.rows;
     args.sidx = ints(l.sidx) + row0 * K;
     args.add = row0 > 0;
-    if (!map2d(&logits.a, false, xc, C, rows, 2L * C, 128) ||
-        !map2d(&logits.b, false, p->weight, C, V, 2 * p->ld_weight, 128) ||
+    const long tiles_m = up(rows, 256) / 256, tiles_c = up(C, 256) / 256;
+    CUtensorMap* of_x = narrow ? &logits.b : &logits.a;
+    if (!map2d(of_x, false, xc, C, rows, 2L * C, few ? 16 : narrow ? 64 : 128) ||
+        !map2d(narrow ? &logits.a : &logits.b, false, p->weight, C, V, 2 * p->ld_weight, 128) ||
         !map2d(&logits.out, false, grad ? (void*)e : (void*)xc, grad ? V : C, rows, 2 * (grad ? l.ld_e : C), 32))
       return cudaErrorInvalidValue;
-    const long tiles_m = up(rows, 256) / 256, tiles_c = up(C, 256) / 256;
-    RT_CUDA_CHECK(launch<head::LOGITS>(logits, args, tiles_m * l.tiles, s));
-    MergeArgs m{part, l.rows, (int)l.tiles, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, merge_blocks, T,
+    RT_CUDA_CHECK((few      ? launch<head::LOGITS_N, 32>(logits, args, l.tiles, s)
+                   : narrow ? launch<head::LOGITS_N, 128>(logits, args, l.tiles, s)
+                            : launch<head::LOGITS>(logits, args, tiles_m * l.tiles, s)));
+    MergeArgs m{part, l.rows, (int)l.groups, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, merge_blocks, T,
                 counts, ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->scale, p->row_grad, p->row_loss,
                 p->reduction ? p->loss : nullptr, work + l.lse2, work + l.tail, grad ? work + l.coef : nullptr};
-    RT_CUDA_CHECK(rt::launch_after(merge_kernel, (unsigned)((rows + MERGE_ROWS - 1) / MERGE_ROWS),
-                                   MERGE_ROWS * MERGE_GROUPS, 0, s, m));
+    RT_CUDA_CHECK(rt::launch_after(narrow ? merge_kernel<1> : merge_kernel<4>,
+                                   (unsigned)(narrow ? rows : (rows + 3) / 4), MERGE_THREADS, 0, s, m));
     if (grad)
       RT_CUDA_CHECK(rt::launch_after(gradient_kernel, dim3((unsigned)((l.tiles + 31) / 32), (unsigned)rows), 256, 0, s, e,
-                                     l.ld_e, (int)V, (int)l.tiles, (int)row0, (int)l.rows, counts, part, l.rows,
+                                     l.ld_e, (int)V, (int)l.tiles, (int)row0, (int)l.rows, counts, part, l.rows, narrow ? 32 : 256,
                                      work + l.lse2, work + l.tail, K, ints(l.sidx), work + l.coef));
     if (p->dhidden) {
-      if (!map2d(&dx.a, false, e, V, rows, 2 * l.ld_e, 128) ||
-          !map2d(&dx.b, false, p->weight, C, V, 2 * p->ld_weight, 64) ||
+      if (!map2d(narrow ? &dx.b : &dx.a, false, e, V, rows, 2 * l.ld_e, few ? 16 : narrow ? 64 : 128) ||
+          !map2d(narrow ? &dx.a : &dx.b, false, p->weight, C, V, 2 * p->ld_weight, 64) ||
           !map2d(&dx.out, true, work + l.dx, C, l.splits * l.split_rows, 4L * C, 32))
         return cudaErrorInvalidValue;
-      RT_CUDA_CHECK(launch<head::DX>(dx, args, tiles_m * tiles_c * l.splits, s));
+      RT_CUDA_CHECK((few      ? launch<head::DX_N, 32>(dx, args, tiles_c * l.splits, s)
+                     : narrow ? launch<head::DX_N, 128>(dx, args, tiles_c * l.splits, s)
+                              : launch<head::DX>(dx, args, tiles_m * tiles_c * l.splits, s)));
       RT_CUDA_CHECK(rt::launch_after(dhidden_kernel, (unsigned)rows, 256, 0, s, work + l.dx, (int)l.splits, l.split_rows,
                                      C, (int)row0, (int)l.rows, counts, ints(l.row_of),
                                      reinterpret_cast<__nv_bfloat16*>(p->dhidden)));
