@@ -72,29 +72,6 @@ RT_DEVICE void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "me
 template <int N>
 RT_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// First statement of a kernel launched by launch_after: lets the next such kernel's blocks start, and waits until the
-// kernel before has finished and its writes are visible. As every kernel of a chain waits, each sees all before it.
-RT_DEVICE void grid_wait() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
-// Launch whose blocks may start before the kernel ahead of it in the stream has ended: the kernel calls grid_wait().
-template <typename... P, typename... A>
-cudaError_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
-  cudaLaunchAttribute after;
-  after.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  after.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
-  config.blockDim = block;
-  config.dynamicSmemBytes = smem;
-  config.stream = stream;
-  config.attrs = &after;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
-}
-
 }  // namespace rt
 
 // Host-side status helpers.

@@ -252,7 +252,6 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
   sm100::cluster_sync();
   sm100::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  rt::grid_wait();  // all above runs beside the end of the kernel before
   const int n = min(max(*args.live - args.row0, 0), args.rows);
   Work<MODE> work(args, n);
   int tm, tn, split, k0, k1;
@@ -329,6 +328,8 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
       }
       sm100::mma_commit_pair(drain);
       sm100::mbar_wait_bounded(drain, 0);
+    } else if (cta == 1 && lane == 0) {
+      sm100::mbar_wait_bounded(drain, 0);  // the last arrival from the other CTA lands before shared memory goes away
     }
   } else {
     // ---------------------------------------------------------------- epilogue (warps 2..5, both CTAs)

@@ -39,7 +39,6 @@ __device__ __forceinline__ int row_kind(int entries) { return entries & 2 ? 2 : 
 
 // One warp per row: kind[row] of a record of K entries.
 __global__ void kinds_kernel(const long* __restrict__ idx, long rows, int K, long V, int* __restrict__ kind) {
-  rt::grid_wait();
   const long row = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   if (row >= rows) return;
   int any = 0;
@@ -59,7 +58,6 @@ struct Counts {
 __global__ void __launch_bounds__(1024) pack_kernel(const int* __restrict__ kind, const long* __restrict__ targets,
                                                     long ignore, long V, long rows, int* __restrict__ slot,
                                                     Counts* __restrict__ counts) {
-  rt::grid_wait();
   __shared__ int warps[2][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int valid = 0, bad = 0;
@@ -130,7 +128,6 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
                                                      int* __restrict__ sidx, float* __restrict__ slogp,
                                                      float* __restrict__ hit, float* __restrict__ row_loss,
                                                      uint4* __restrict__ dhidden) {
-  rt::grid_wait();
   extern __shared__ unsigned long long keys[];
   const long row = blockIdx.x;
   const int C8 = C / 8;
@@ -329,7 +326,6 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
 // The last block to finish also adds up the rows' losses, in a fixed order (mean: over rows with a loss).
 template <int ROWS>
 __global__ void __launch_bounds__(MERGE_THREADS) merge_kernel(const MergeArgs p) {
-  rt::grid_wait();
   __shared__ double part[MERGE_THREADS / 32];
   __shared__ bool last;
   merge_rows<ROWS>(p);
@@ -362,7 +358,6 @@ __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict
                                                        const float* __restrict__ lse2, const float* __restrict__ tail,
                                                        int K, const int* __restrict__ sidx,
                                                        const float* __restrict__ coef) {
-  rt::grid_wait();
   const int n = min(max(counts->valid - row0, 0), rows), r = blockIdx.y;
   if (r >= max((n + 63) / 64 * 64, 64)) return;
   const int lane = threadIdx.x & 31;
@@ -400,7 +395,6 @@ __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict
 __global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ partial, int splits, long split_rows,
                                                       int C, int row0, int rows, const Counts* __restrict__ counts,
                                                       const int* __restrict__ row_of, __nv_bfloat16* __restrict__ out) {
-  rt::grid_wait();
   const int n = min(max(counts->valid - row0, 0), rows), r = blockIdx.x;
   if (r >= n) return;
   const float failed = counts->failed ? NAN : 0.f;  // a product gave up a wait
@@ -421,7 +415,6 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ 
 
 // The weight's gradient of a product that gave up a wait (the one-chunk kernel leaves its NaN itself).
 __global__ void failed_kernel(const Counts* __restrict__ counts, __nv_bfloat16* __restrict__ dweight) {
-  rt::grid_wait();
   if (counts->failed && threadIdx.x < 8) dweight[threadIdx.x] = __float2bfloat16_rn(NAN);
 }
 
@@ -556,8 +549,8 @@ cudaError_t launch(const head::Maps& maps, const head::Args& args, long units, c
     set.fetch_or(bit, std::memory_order_acq_rel);
   }
   const unsigned grid = 2 * (unsigned)std::min<long>(units, pairs());
-  return rt::launch_after(head::pair_kernel<MODE, NT>, grid, head::THREADS, head::Cfg<MODE, NT>::SMEM_BYTES, s, maps,
-                          args);
+  head::pair_kernel<MODE, NT><<<grid, head::THREADS, head::Cfg<MODE, NT>::SMEM_BYTES, s>>>(maps, args);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -592,16 +585,17 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   const bool brief = T * K <= SHORT_ENTRIES;
   if (!brief) {
     if (p->log_probs) kinds_kernel<<<(unsigned)((T * 32 + 255) / 256), 256, 0, s>>>(p->index, T, K, V, ints(l.kind));
-    RT_CUDA_CHECK(rt::launch_after(pack_kernel, 1, 1024, 0, s, p->log_probs ? ints(l.kind) : nullptr, p->index, p->ignore,
-                                   V, T, ints(l.slot), counts));
+    pack_kernel<<<1, 1024, 0, s>>>(p->log_probs ? ints(l.kind) : nullptr, p->index, p->ignore, V, T, ints(l.slot),
+                                   counts);
   }
   int Kp = 1;
   while (Kp < K) Kp <<= 1;
-  RT_CUDA_CHECK(rt::launch_after(
-      gather_kernel, (unsigned)(T + 64), 256, Kp * 8, s, p->index, p->log_probs, K, Kp, T, reinterpret_cast<const __nv_bfloat16*>(p->hidden), p->ld_hidden,
-      reinterpret_cast<const __nv_bfloat16*>(p->weight), p->ld_weight, C, scale2, V, p->ignore, brief,
-      ints(l.slot), counts, ints(l.row_of), reinterpret_cast<uint4*>(x), ints(l.sidx), work + l.slogp, work + l.hit, p->row_loss,
-      reinterpret_cast<uint4*>(p->dhidden)));
+  gather_kernel<<<(unsigned)(T + 64), 256, Kp * 8, s>>>(
+      p->index, p->log_probs, K, Kp, T, reinterpret_cast<const __nv_bfloat16*>(p->hidden), p->ld_hidden,
+      reinterpret_cast<const __nv_bfloat16*>(p->weight), p->ld_weight, C, scale2, V, p->ignore, brief, ints(l.slot),
+      counts, ints(l.row_of), reinterpret_cast<uint4*>(x), ints(l.sidx), work + l.slogp, work + l.hit, p->row_loss,
+      reinterpret_cast<uint4*>(p->dhidden));
+  RT_CUDA_CHECK(cudaGetLastError());
 
   head::Maps logits, dx, dw;
   head::Args args{};
@@ -642,12 +636,13 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
     MergeArgs m{part, l.rows, (int)l.groups, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, merge_blocks, T,
                 counts, ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->scale, p->row_grad, p->row_loss,
                 p->reduction ? p->loss : nullptr, work + l.lse2, work + l.tail, grad ? work + l.coef : nullptr};
-    RT_CUDA_CHECK(rt::launch_after(narrow ? merge_kernel<1> : merge_kernel<4>,
-                                   (unsigned)(narrow ? rows : (rows + 3) / 4), MERGE_THREADS, 0, s, m));
+    if (narrow) merge_kernel<1><<<(unsigned)rows, MERGE_THREADS, 0, s>>>(m);
+    else merge_kernel<4><<<(unsigned)(rows + 3) / 4, MERGE_THREADS, 0, s>>>(m);
     if (grad)
-      RT_CUDA_CHECK(rt::launch_after(gradient_kernel, dim3((unsigned)((l.tiles + 31) / 32), (unsigned)rows), 256, 0, s, e,
-                                     l.ld_e, (int)V, (int)l.tiles, (int)row0, (int)l.rows, counts, part, l.rows, narrow ? 32 : 256,
-                                     work + l.lse2, work + l.tail, K, ints(l.sidx), work + l.coef));
+      gradient_kernel<<<dim3((unsigned)((l.tiles + 31) / 32), (unsigned)rows), 256, 0, s>>>(
+          e, l.ld_e, (int)V, (int)l.tiles, (int)row0, (int)l.rows, counts, part, l.rows, narrow ? 32 : 256,
+          work + l.lse2, work + l.tail, K, ints(l.sidx), work + l.coef);
+    RT_CUDA_CHECK(cudaGetLastError());
     if (p->dhidden) {
       if (!map2d(narrow ? &dx.b : &dx.a, false, e, V, rows, 2 * l.ld_e, few ? 16 : narrow ? 64 : 128) ||
           !map2d(narrow ? &dx.a : &dx.b, false, p->weight, C, V, 2 * p->ld_weight, 64) ||
@@ -656,9 +651,9 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
       RT_CUDA_CHECK((few      ? launch<head::DX_N, 32>(dx, args, tiles_c * l.splits, s)
                      : narrow ? launch<head::DX_N, 128>(dx, args, tiles_c * l.splits, s)
                               : launch<head::DX>(dx, args, tiles_m * tiles_c * l.splits, s)));
-      RT_CUDA_CHECK(rt::launch_after(dhidden_kernel, (unsigned)rows, 256, 0, s, work + l.dx, (int)l.splits, l.split_rows,
-                                     C, (int)row0, (int)l.rows, counts, ints(l.row_of),
-                                     reinterpret_cast<__nv_bfloat16*>(p->dhidden)));
+      dhidden_kernel<<<(unsigned)rows, 256, 0, s>>>(work + l.dx, (int)l.splits, l.split_rows, C, (int)row0, (int)l.rows,
+                                                    counts, ints(l.row_of),
+                                                    reinterpret_cast<__nv_bfloat16*>(p->dhidden));
     }
     if (p->dweight) {
       void* out = l.dw32 ? (void*)(work + l.dw) : p->dweight;

@@ -277,7 +277,6 @@ __global__ void __launch_bounds__(THREADS, 4) top_kernel(const T* __restrict__ l
   __shared__ float2 warps[WARPS];
   __shared__ unsigned short groups[MAX_GROUPS];
   const int tid = threadIdx.x, lane = tid & 31;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge's blocks may start
   const long row = blockIdx.y;
   const int lo = (int)((long)a.V * blockIdx.x / a.segments), n = (int)((long)a.V * (blockIdx.x + 1) / a.segments) - lo;
   const T* z = logits + row * a.ld + lo;
@@ -467,7 +466,6 @@ __global__ void __launch_bounds__(MERGE_THREADS) top_merge_kernel(const TopArgs 
   __shared__ int counters[3], found;
   __shared__ unsigned peak, bound;
   __shared__ float2 sums[MERGE_THREADS / 32];
-  rt::grid_wait();
   const long row = blockIdx.x;
   const int tid = threadIdx.x, total = a.segments * a.k, parts = a.k <= MERGE_THREADS / 2 ? 1 : 4;
   const unsigned long long* in = a.entries + row * total;
@@ -609,7 +607,6 @@ extern "C" cudaError_t rt_top_log_probs(int dtype, const void* logits, long rows
     const auto* z = static_cast<const float*>(logits);
     RT_CUDA_CHECK((values / 4 <= MAX_KEYS ? launch<float, 1>(z, rows, a, s) : launch<float, BATCH>(z, rows, a, s)));
   }
-  if (a.segments > 1)
-    RT_CUDA_CHECK(rt::launch_after(top_merge_kernel, (unsigned)rows, MERGE_THREADS, a.capacity * 8, s, a));
-  return cudaSuccess;
+  if (a.segments > 1) top_merge_kernel<<<(unsigned)rows, MERGE_THREADS, a.capacity * 8, s>>>(a);
+  return cudaGetLastError();
 }
