@@ -2,7 +2,8 @@
 // accumulators in TMEM, one persistent kernel each.
 //
 //   LOGITS  z = X . W^T              X [n, C] live rows, W [V, C]; z stays on chip: per row and tile the epilogue
-//                                    leaves (max, sum of exponentials) and, for gradients, the exponentials in bf16
+//                                    leaves (max, sum of exponentials) and, for gradients, how far each logit lies
+//                                    below that maximum (see depth)
 //   DX      dX = dz . W              dz [n, V]; K = V is cut into `splits` parts, each an fp32 partial sum
 //   DW      dW = dz^T . X            bf16, or fp32 added up over chunks of rows
 //   LOGITS_N, DX_N                   the first two for up to NT = 32 or 128 rows, as z^T = W . X^T and dX^T = W^T . dz^T:
@@ -62,7 +63,7 @@ struct Args {
   float2* part;     // [tiles of the vocabulary, part_ld]
   long part_ld;
   int store_e;
-  __nv_bfloat16* e; // LOGITS_N: the exponentials, [rows, ld_e]
+  unsigned short* e; // LOGITS_N: the logits' depths, [rows, ld_e]
   long ld_e;
   float* dx;        // DX_N: the partial sums
   int add;          // DW32: add to what is there
@@ -78,6 +79,22 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// A logit t <= 0 octaves (units of log2) from its tile's maximum as a 16-bit number of 1/512 octaves: the exponential it
+// stands for is off by 7e-4 at most, a fifth of bf16's rounding, down to 2^-128. Here as the low half of an fp32 word
+// (2^23 + depth, so that one fused multiply-add rounds).
+constexpr float DEPTH_STEPS = 512.f, DEPTH_BASE = 8388608.f;
+__device__ __forceinline__ uint32_t depth(float t) {
+  return __float_as_uint(fminf(fmaf(t, -DEPTH_STEPS, DEPTH_BASE), DEPTH_BASE + 65535.f));
+}
+__device__ __forceinline__ uint4 pack_depths(const float* t) {
+  uint4 u;
+  u.x = __byte_perm(depth(t[0]), depth(t[1]), 0x5410);
+  u.y = __byte_perm(depth(t[2]), depth(t[3]), 0x5410);
+  u.z = __byte_perm(depth(t[4]), depth(t[5]), 0x5410);
+  u.w = __byte_perm(depth(t[6]), depth(t[7]), 0x5410);
+  return u;
 }
 
 template <int MODE>
@@ -388,9 +405,10 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
           const float m2 = m == -INFINITY ? 0.f : m * args.scale2;
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            v[i] = ex2(fmaf(v[i], args.scale2, -__shfl_sync(~0u, m2, i)));
+            v[i] = fmaf(v[i], args.scale2, -__shfl_sync(~0u, m2, i));
             if (args.store_e && 32 * g + i < n && v_at < args.V)
-              args.e[(32 * g + i) * args.ld_e + v_at] = __float2bfloat16_rn(v[i]);
+              args.e[(32 * g + i) * args.ld_e + v_at] = (unsigned short)depth(v[i]);
+            v[i] = ex2(v[i]);
           }
           const float sum = columns(v, lane, [](float a, float b) { return a + b; });
           if (j < n) args.part[(row0 / 32) * args.part_ld + j] = make_float2(m == -INFINITY ? m : m2, sum);
@@ -431,17 +449,17 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
             sm100::tmem_wait_ld();
             if (masked) drop_held(v, mask[(c + h) * 32]);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = ex2(fmaf(v[i], args.scale2, -m2));
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              s0 += v[i];
-              s1 += v[i + 1];
-              s2 += v[i + 2];
-              s3 += v[i + 3];
-            }
+            for (int i = 0; i < 32; ++i) v[i] = fmaf(v[i], args.scale2, -m2);
             if (store) {
 #pragma unroll
-              for (int q = 0; q < 4; ++q) *staged(b, lane, 4 * h + q) = rt::pack8(v + 8 * q);
+              for (int q = 0; q < 4; ++q) *staged(b, lane, 4 * h + q) = pack_depths(v + 8 * q);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              s0 += ex2(v[i]);
+              s1 += ex2(v[i + 1]);
+              s2 += ex2(v[i + 2]);
+              s3 += ex2(v[i + 3]);
             }
           }
           if (store) send(b, col0 + 32 * c, row0, false);

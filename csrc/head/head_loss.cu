@@ -12,9 +12,9 @@
 //
 // Launches of one call: the rows that have a loss are counted and packed (gather_kernel: their hidden states, sorted
 // records and held logits), z = X W^T leaves per row and 256-column tile its maximum and sum of exponentials
-// (head_gemm.cuh), merge_kernel forms the losses. With gradients the same product also leaves the exponentials in bf16,
-// relative to their tile's maximum; gradient_kernel turns them into dz in place, and dX = dz W, dW = dz^T X follow.
-// That is 6 T V C operations, against 8 T V C where the logits are formed a second time, for T V bf16 values of
+// (head_gemm.cuh), merge_kernel forms the losses. With gradients the same product also leaves each logit's depth below
+// its tile's maximum in 16 bits; gradient_kernel turns them into dz (bf16) in place, and dX = dz W, dW = dz^T X follow.
+// That is 6 T V C operations, against 8 T V C where the logits are formed a second time, for T V 16-bit values of
 // workspace; CHUNK_VALUES bounds it, and more rows run in chunks whose dW adds up in fp32. Rows without a loss cost
 // nothing but their packing, and what they hold never meets the other rows. A product that gave up a bounded wait leaves
 // NaN in the losses, or in the gradient it was forming.
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) merge_kernel(const MergeArgs p)
 }
 
 // ---------------------------------------------------------------- gradient of the logits
-// In place: exponentials of a chunk's rows (relative to the maximum of their `group` columns) -> dz, one warp per row and tile; the block
+// In place: depths of a chunk's logits (below the maximum of their `group` columns) -> dz, one warp per row and tile; the block
 // of 32 tiles also puts their held entries in their places; rows that fill the last block of 64 become zero. A read and a write
 // of every value: 0.18 ms for 1024 x 248077 (5.7 TB/s), where forming the logits again would cost 1.8 ms.
 __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict__ e, long ld, int V, int tiles,
@@ -374,10 +374,14 @@ __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict
       uint4* at = reinterpret_cast<uint4*>(out + c);
       float v[8] = {};
       if (live && c < V) {
-        rt::unpack8(*at, v);
-        const float m = part[c / group * part_ld + r].x, f = m == -INFINITY ? 0.f : a * exp2f(m - l);
+        const uint4 u = *at;
+        const float m = part[c / group * part_ld + r].x, top = m == -INFINITY ? m : m - l;
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= f;
+        for (int j = 0; j < 8; ++j) {  // 2^23 + depth as a float, and back
+          const float d = __uint_as_float(__byte_perm(w[j / 2], 0x4b000000u, j & 1 ? 0x7632 : 0x7610)) - head::DEPTH_BASE;
+          v[j] = a * head::ex2(fmaf(d, -1.f / head::DEPTH_STEPS, top));
+        }
       }
       *at = rt::pack8(v);
     }
@@ -450,7 +454,7 @@ float mma_gain(int C) { return 1.f + (float)(C / 16) * 0x1p-26f; }
 
 constexpr long up(long n, long to) { return (n + to - 1) / to * to; }
 
-// Rows of a chunk: with gradients their exponentials take up to 2 GiB of bf16, without their statistics take 8 bytes per
+// Rows of a chunk: with gradients their logits' depths take up to 2 GiB, without their statistics take 8 bytes per
 // row and tile.
 constexpr long CHUNK_VALUES = 1L << 30, CHUNK_ROWS = 32768;
 constexpr long SCORE_ROWS = 16384;
@@ -489,7 +493,7 @@ int dx_splits(long rows, long V, int C) {
 // Offsets in floats. Each is a multiple of 1 KB: a TMA box row of 128 bytes that straddles two lines costs twice the L2
 // accesses (dW of 1024 tokens: 2.8 ms from a 16-byte aligned dz, 1.8 ms from an aligned one).
 struct Layout {
-  // rows of a chunk, row stride of the exponentials, 256-wide tiles of the vocabulary, groups of columns with statistics
+  // rows of a chunk, row stride of the depths and of dz, 256-wide tiles of the vocabulary, groups of columns with statistics
   long rows, ld_e, tiles, groups, splits, split_rows;
   bool dw32;
   long kind, slot, row_of, counts, x, sidx, slogp, hit, coef, lse2, tail, part, e, dx, dw, total;
@@ -605,7 +609,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   args.K = K;
   args.scale2 = scale2 * mma_gain(C);
   args.part = part;
-  args.e = e;
+  args.e = reinterpret_cast<unsigned short*>(e);
   args.ld_e = l.ld_e;
   args.dx = work + l.dx;
   args.part_ld = l.rows;
