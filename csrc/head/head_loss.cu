@@ -118,7 +118,8 @@ __device__ __forceinline__ int place_in_short(const long* idx, bool record, int 
 // state goes to its place in `x`; its entries are sorted by vocabulary index (INT_MAX behind the last) with their
 // log-probabilities, and their logits in units of log2 are summed here: they enter the loss with a weight of about one,
 // where all others enter it through the sum of exponentials, so they come from fp32 fused multiply-adds, which round,
-// instead of from the tensor cores, which truncate (see mma_gain). Rows without a gradient get their zeros here.
+// instead of from the tensor cores, which truncate (see mma_gain). Rows without a gradient get their zeros here. Where
+// there are few rows, the entries of a row are shared out over the blocks of its y index.
 __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ idx, const float* __restrict__ logp,
                                                      int K, int Kp, long rows, const __nv_bfloat16* __restrict__ hidden,
                                                      long ldh, const __nv_bfloat16* __restrict__ w, long ldw, int C,
@@ -141,21 +142,24 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
     valid = counts->valid;
     place = row < rows ? slot[row] : 0;
   }
+  const bool lead = blockIdx.y == 0;
   if (row >= rows) {
+    if (!lead) return;
     const long n = valid, fill = n + (row - rows);
     if (fill < max((n + 63) / 64 * 64, 64L))
       for (int c = threadIdx.x; c < C8; c += blockDim.x) x[fill * C8 + c] = zero;
     return;
   }
   if (place < 0) {
+    if (!lead) return;
     if (threadIdx.x == 0) row_loss[row] = place == -1 ? 0.f : NAN;
     if (dhidden)
       for (int c = threadIdx.x; c < C8; c += blockDim.x) dhidden[row * C8 + c] = zero;
     return;
   }
-  if (threadIdx.x == 0) row_of[place] = (int)row;
+  if (lead && threadIdx.x == 0) row_of[place] = (int)row;
   const uint4* src = reinterpret_cast<const uint4*>(hidden + row * ldh);
-  for (int c = threadIdx.x; c < C8; c += blockDim.x) x[place * C8 + c] = __ldg(src + c);
+  for (int c = threadIdx.x; lead && c < C8; c += blockDim.x) x[place * C8 + c] = __ldg(src + c);
   for (int k = threadIdx.x; k < Kp; k += blockDim.x) {
     int v = INT_MAX;
     float lp = 0.f;
@@ -179,11 +183,12 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
       __syncthreads();
     }
   const int lane = threadIdx.x & 31;
-  for (int k = threadIdx.x >> 5; k < K; k += blockDim.x >> 5) {
+  for (int k = (threadIdx.x >> 5) + 8 * blockIdx.y; k < K; k += 8 * gridDim.y) {
     const int v = (int)(keys[k] >> 32);
     float sum = 0.f;
     if (v != INT_MAX) {
       const uint4* wr = reinterpret_cast<const uint4*>(w + (long)v * ldw);
+#pragma unroll 4
       for (int c = lane; c < C8; c += 32) {
         float a[8], b[8];
         rt::unpack8(__ldg(src + c), a);
@@ -594,7 +599,8 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   }
   int Kp = 1;
   while (Kp < K) Kp <<= 1;
-  gather_kernel<<<(unsigned)(T + 64), 256, Kp * 8, s>>>(
+  const unsigned share = (unsigned)std::max(1L, std::min((K + 7L) / 8, 296 / T));  // blocks of a row: two per SM in all
+  gather_kernel<<<dim3((unsigned)(T + 64), share), 256, Kp * 8, s>>>(
       p->index, p->log_probs, K, Kp, T, reinterpret_cast<const __nv_bfloat16*>(p->hidden), p->ld_hidden,
       reinterpret_cast<const __nv_bfloat16*>(p->weight), p->ld_weight, C, scale2, V, p->ignore, brief, ints(l.slot),
       counts, ints(l.row_of), reinterpret_cast<uint4*>(x), ints(l.sidx), work + l.slogp, work + l.hit, p->row_loss,
