@@ -1,16 +1,16 @@
-// The three matrix products of the vocabulary-head losses on CTA pairs: tiles of 256 x 256 (256 x NT for few rows), fp32
-// accumulators in TMEM, one persistent kernel each.
+// The three matrix products of the vocabulary-head losses on CTA pairs: tiles of 256 x 256 (256 x NT for few rows),
+// fp32 accumulators in TMEM, one persistent kernel each.
 //
 //   LOGITS  z = X . W^T              X [n, C] live rows, W [V, C]; z stays on chip: per row and tile the epilogue
 //                                    leaves (max, sum of exponentials) and, for gradients, how far each logit lies
 //                                    below that maximum (see depth)
 //   DX      dX = dz . W              dz [n, V]; K = V is cut into `splits` parts, each an fp32 partial sum
 //   DW      dW = dz^T . X            bf16, or fp32 added up over chunks of rows
-//   LOGITS_N, DX_N                   the first two for up to NT = 32 or 128 rows, as z^T = W . X^T and dX^T = W^T . dz^T:
-//                                    the rows are the tile's columns, so the tensor cores do 1/8 or 1/2 of the work of
-//                                    a 256-row tile that is mostly padding. These calls are bound by reading W; with
-//                                    padded tiles the 1 kW power cap halved the clock and with it the bandwidth (one
-//                                    row x 248077 x 5120 in a loop: 540 us at 1.25 GHz).
+//   LOGITS_N, DX_N                   the first two for up to NT = 32 or 128 rows, as z^T = W . X^T and
+//                                    dX^T = W^T . dz^T: the rows are the tile's columns, so the tensor cores do 1/8 or
+//                                    1/2 of the work of a 256-row tile that is mostly padding. These calls are bound by
+//                                    reading W; with padded tiles the 1 kW power cap held the clock at 1.25 GHz and the
+//                                    bandwidth at 4.7 TB/s (one row x 248077 x 5120 in a loop: 540 us; now 405 us).
 //
 // n, the number of rows that have a loss, is only known on the device (`live`): the kernels read it there.
 //
@@ -18,7 +18,8 @@
 // of 64-deep K blocks; warp 1 of the even CTA issues the pair's MMAs (M = 256, N = 256, K = 16: each CTA holds 128
 // rows of A and 128 columns of B, so an operand byte in shared memory feeds twice the products of a one-CTA tile);
 // warps 2-5 drain the double-buffered accumulators. Outputs leave through swizzled staging buffers by TMA stores of 32
-// rows, one warp at a time (LOGITS_N, DX_N: by coalesced stores). All waits are bounded (sm100.cuh); one that gives up sets *status.
+// rows, one warp at a time (LOGITS_N, DX_N: by coalesced stores). All waits are bounded (sm100.cuh); one that gives up
+// sets *status.
 #pragma once
 #include <climits>
 #include "../common/common.cuh"
@@ -81,9 +82,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// A logit t <= 0 octaves (units of log2) from its tile's maximum as a 16-bit number of 1/512 octaves: the exponential it
-// stands for is off by 7e-4 at most, a fifth of bf16's rounding, down to 2^-128. Here as the low half of an fp32 word
-// (2^23 + depth, so that one fused multiply-add rounds).
+// A logit t <= 0 octaves (units of log2) from its tile's maximum as a 16-bit number of 1/512 octaves: the exponential
+// it stands for is off by 7e-4 at most, a fifth of bf16's rounding, down to 2^-128. Here as the low half of an fp32
+// word (2^23 + depth, so that one fused multiply-add rounds).
 constexpr float DEPTH_STEPS = 512.f, DEPTH_BASE = 8388608.f;
 __device__ __forceinline__ uint32_t depth(float t) {
   return __float_as_uint(fminf(fmaf(t, -DEPTH_STEPS, DEPTH_BASE), DEPTH_BASE + 65535.f));
@@ -133,7 +134,7 @@ struct Work {
     if (unit >= units) return false;
     int t = unit;
     split = 0;
-    if (MODE == DX || MODE == DX_N) {  // one part of K at a time, so that the pairs running together share its rows of W in L2
+    if (MODE == DX || MODE == DX_N) {  // one part of K at a time: the pairs running together share its rows of W in L2
       const int tiles = tiles_m * tiles_n;
       split = t / tiles;
       t %= tiles;

@@ -16,8 +16,8 @@
 // its tile's maximum in 16 bits; gradient_kernel turns them into dz (bf16) in place, and dX = dz W, dW = dz^T X follow.
 // That is 6 T V C operations, against 8 T V C where the logits are formed a second time, for T V 16-bit values of
 // workspace; CHUNK_VALUES bounds it, and more rows run in chunks whose dW adds up in fp32. Rows without a loss cost
-// nothing but their packing, and what they hold never meets the other rows. A product that gave up a bounded wait leaves
-// NaN in the losses, or in the gradient it was forming.
+// nothing but their packing, and what they hold never meets the other rows. A product that gave up a bounded wait
+// leaves NaN in the losses, or in the gradient it was forming.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -35,7 +35,8 @@ __device__ __forceinline__ int entry_kind(long id, bool record, long ignore, lon
   if (record ? id < 0 : id == ignore) return 0;
   return id < 0 || id >= V ? 2 : 1;
 }
-__device__ __forceinline__ int row_kind(int entries) { return entries & 2 ? 2 : entries; }  // of the entries' kinds or'd
+// From its entries' kinds or'd.
+__device__ __forceinline__ int row_kind(int entries) { return entries & 2 ? 2 : entries; }
 
 // One warp per row: kind[row] of a record of K entries.
 __global__ void kinds_kernel(const long* __restrict__ idx, long rows, int K, long V, int* __restrict__ kind) {
@@ -208,9 +209,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
 
 // ---------------------------------------------------------------- losses of the valid rows of a chunk
 // Block of ROWS rows (four, or one of the few rows whose statistics are finer): its threads merge the tiles' statistics
-// (in a fixed order: each row's tiles go round-robin to MERGE_THREADS / ROWS threads), then one warp per row forms the loss and the gradient's coefficients: d/dz_v = tail
-// exp2(z_v - lse2) outside the record, coef[k] for its held entries, both times scale and the row's upstream gradient
-// (given per row, or 1, or 1 / rows with a loss).
+// (in a fixed order: each row's tiles go round-robin to MERGE_THREADS / ROWS threads), then one warp per row forms the
+// loss and the gradient's coefficients: d/dz_v = tail exp2(z_v - lse2) outside the record, coef[k] for its held
+// entries, both times scale and the row's upstream gradient (given per row, or 1, or 1 / rows with a loss).
 constexpr int MERGE_THREADS = 256;
 struct MergeArgs {
   const float2* part;
@@ -354,9 +355,10 @@ __global__ void __launch_bounds__(MERGE_THREADS) merge_kernel(const MergeArgs p)
 }
 
 // ---------------------------------------------------------------- gradient of the logits
-// In place: depths of a chunk's logits (below the maximum of their `group` columns) -> dz, one warp per row and tile; the block
-// of 32 tiles also puts their held entries in their places; rows that fill the last block of 64 become zero. A read and a write
-// of every value: 0.18 ms for 1024 x 248077 (5.7 TB/s), where forming the logits again would cost 1.8 ms.
+// In place: depths of a chunk's logits (below the maximum of their `group` columns) -> dz, one warp per row and tile;
+// the block of 32 tiles also puts their held entries in their places; rows that fill the last block of 64 become zero.
+// A read and a write of every value: 0.18 ms for 1024 x 248077 (5.7 TB/s), where forming the logits again would cost
+// 1.8 ms.
 __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict__ e, long ld, int V, int tiles,
                                                        int row0, int rows, const Counts* __restrict__ counts,
                                                        const float2* __restrict__ part, long part_ld, int group,
@@ -384,7 +386,8 @@ __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {  // 2^23 + depth as a float, and back
-          const float d = __uint_as_float(__byte_perm(w[j / 2], 0x4b000000u, j & 1 ? 0x7632 : 0x7610)) - head::DEPTH_BASE;
+          const uint32_t word = __byte_perm(w[j / 2], 0x4b000000u, j & 1 ? 0x7632 : 0x7610);
+          const float d = __uint_as_float(word) - head::DEPTH_BASE;
           v[j] = a * head::ex2(fmaf(d, -1.f / head::DEPTH_STEPS, top));
         }
       }
@@ -476,9 +479,9 @@ int pairs() {
 // Calls of up to this many rows run the products as W . X^T, with the rows as the tiles' columns (head_gemm.cuh).
 constexpr long NARROW_ROWS = 128;
 
-// Parts of K = V for dX. A wave of tiles takes kblocks / S blocks of 512 cycles (700 to read W, for few rows) and fills `pairs` pairs, or part of them
-// in the last wave; each part adds a write and a read of rows x C fp32 partial sums (16 bytes per value at about 5
-// TB/s = 2800 bytes a cycle).
+// Parts of K = V for dX. A wave of tiles takes kblocks / S blocks of 512 cycles (700 to read W, for few rows) and fills
+// `pairs` pairs, or part of them in the last wave; each part adds a write and a read of rows x C fp32 partial sums (16
+// bytes per value at about 5 TB/s = 2800 bytes a cycle).
 int dx_splits(long rows, long V, int C) {
   const long tiles = up(rows, 256) / 256 * (up(C, 256) / 256), kblocks = up(V, 64) / 64;
   const double block = rows <= NARROW_ROWS ? 700 : 512;
@@ -498,7 +501,8 @@ int dx_splits(long rows, long V, int C) {
 // Offsets in floats. Each is a multiple of 1 KB: a TMA box row of 128 bytes that straddles two lines costs twice the L2
 // accesses (dW of 1024 tokens: 2.8 ms from a 16-byte aligned dz, 1.8 ms from an aligned one).
 struct Layout {
-  // rows of a chunk, row stride of the depths and of dz, 256-wide tiles of the vocabulary, groups of columns with statistics
+  // rows of a chunk, row stride of the depths and of dz, 256-wide tiles of the vocabulary, groups of columns with
+  // statistics, and for dX the parts of K and the rows between their partial sums
   long rows, ld_e, tiles, groups, splits, split_rows;
   bool dw32;
   long kind, slot, row_of, counts, x, sidx, slogp, hit, coef, lse2, tail, part, e, dx, dw, total;

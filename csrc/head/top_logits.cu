@@ -2,14 +2,14 @@
 //
 // One read of the logits. A row is streamed in groups of 8 or 32 values, whose maxima stay in shared memory, while the
 // softmax's denominator is summed. A value t that k of the maxima reach is reached by k logits at least, so the result
-// lies in the groups whose maximum reaches t. t is the k-th largest of 1.5 k maxima or more over several groups each, found
-// by one warp's bisection of their order-preserving keys; the groups that reach it (about 1.4 k at most) are read again, and
-// their values from t up are sorted as unique 64-bit keys (value above, lower index first below). Rows whose equal or
-// special values defeat the bounds (thousands of equal maxima, infinities, NaN) take a radix descent over the whole
-// row instead.
+// lies in the groups whose maximum reaches t. t is the k-th largest of 1.5 k maxima or more over several groups each,
+// found by one warp's bisection of their order-preserving keys; the groups that reach it (about 1.4 k at most) are read
+// again, and their values from t up are sorted as unique 64-bit keys (value above, lower index first below). Rows whose
+// equal or special values defeat the bounds (thousands of equal maxima, infinities, NaN) take a radix descent over the
+// whole row instead.
 //
-// Bound by memory: per value one packed maximum's half, unpacking, multiply-add, ex2 and add (about 5 issue slots of the
-// 11 that the bandwidth leaves). Several blocks per SM, so that one streams while another selects. Few rows are cut
+// Bound by memory: per value one packed maximum's half, unpacking, multiply-add, ex2 and add (about 5 issue slots of
+// the 11 that the bandwidth leaves). Several blocks per SM, so that one streams while another selects. Few rows are cut
 // into segments over as many blocks, whose k candidates a second kernel merges.
 #include <algorithm>
 #include <climits>
@@ -539,8 +539,8 @@ int capacity_for(int k) {
 }
 
 // Segments of a row. One block takes a row of 32003 values in 10 us and of 248077 in 20 us, and merging segments costs
-// another launch of about 8 us, so only a few long rows are cut (8 segments of 1 x 248077 bf16, k 64: 18.7 us), and rows
-// with more vectors than a segment's maxima have room for (past a million values, a long record may not fit: 0).
+// another launch of about 8 us, so only a few long rows are cut (8 segments of 1 x 248077 bf16, k 64: 18.7 us), and
+// rows with more vectors than a segment's maxima have room for (past a million values, a long record may not fit: 0).
 int segments_for(int dtype, long rows, long V, int k) {
   const int vec = dtype == 1 ? 8 : 4;
   const long least = (V / vec + (long)MAX_KEYS * BATCH - 1) / ((long)MAX_KEYS * BATCH);
