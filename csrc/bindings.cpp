@@ -561,15 +561,8 @@ struct HeadLossFunction : public torch::autograd::Function<HeadLossFunction> {
     auto r = run_head_loss(hidden, weight, index, log_probs, call, at::Tensor(), reduction && grad_h,
                            reduction && grad_w);
     ctx->save_for_backward({hidden, weight, index, log_probs.has_value() ? *log_probs : at::Tensor()});
-    ctx->saved_data["ignore"] = ignore;
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["tail"] = tail;
-    ctx->saved_data["reduction"] = reduction;
-    ctx->saved_data["grad_h"] = grad_h;
-    ctx->saved_data["grad_w"] = grad_w;
-    ctx->saved_data["ready"] = reduction != 0;
-    if (r.dhidden.defined()) ctx->saved_data["dhidden"] = r.dhidden;
-    if (r.dweight.defined()) ctx->saved_data["dweight"] = r.dweight;
+    ctx->saved_data["call"] = c10::ivalue::Tuple::create({ignore, scale, tail, reduction, grad_h, grad_w});
+    if (reduction) ctx->saved_data["ready"] = std::vector<at::Tensor>{r.dhidden, r.dweight};
     return r.loss;
   }
 
@@ -577,17 +570,18 @@ struct HeadLossFunction : public torch::autograd::Function<HeadLossFunction> {
                                                  torch::autograd::variable_list upstreams) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "the head losses have no second derivative (create_graph)");
     auto& data = ctx->saved_data;
-    const HeadLossCall call{data["ignore"].toInt(), data["scale"].toDouble(), data["tail"].toBool(),
-                            data["reduction"].toInt()};
-    const bool grad_h = data["grad_h"].toBool(), grad_w = data["grad_w"].toBool();
+    const auto args = data.at("call").toTuple();
+    const auto& a = args->elements();
+    const HeadLossCall call{a[0].toInt(), a[1].toDouble(), a[2].toBool(), a[3].toInt()};
+    const bool grad_h = a[4].toBool(), grad_w = a[5].toBool();
     const at::Tensor upstream = upstreams[0].to(at::kFloat).contiguous();
     at::Tensor dh, dw;
-    if (data["ready"].toBool()) {
-      if (grad_h) dh = data["dhidden"].toTensor();
-      if (grad_w) dw = data["dweight"].toTensor();
-      data["ready"] = false;
-      data.erase("dhidden");
-      data.erase("dweight");
+    const auto ready = data.find("ready");
+    if (ready != data.end()) {
+      const auto grads = ready->second.toTensorVector();
+      if (grad_h) dh = grads[0];
+      if (grad_w) dw = grads[1];
+      data.erase(ready);
     } else {
       const auto saved = ctx->get_saved_variables();
       c10::optional<at::Tensor> log_probs;

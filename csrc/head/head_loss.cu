@@ -298,8 +298,8 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
       L += __shfl_xor_sync(~0u, L, off);
     }
     // rest is relative to m, heldz to peak
-    const float Z = heldz + (m == -INFINITY ? rest : rest * exp2f(m - peak));
-    const double l2 = (double)peak + log2((double)Z);
+    const double Z = (double)heldz + (double)(m == -INFINITY ? rest : rest * exp2f(m - peak));
+    const double l2 = (double)peak + log2(Z);
     const double lse = l2 * 0.6931471805599453;
     const double r1 = p.tail_class && P < 1. ? 1. - P : 0.;
     const double weight = P + r1;
