@@ -370,3 +370,63 @@ def test_more_rows_than_a_chunk(ignored):
     loss = linear_cross_entropy(hidden, weight, targets, reduction="none")
     expected, _, _ = _oracle(hidden, weight, targets[:, None], None, -100, 1.0, 0)
     torch.testing.assert_close(loss.double(), expected, rtol=1e-5, atol=1e-4)
+
+
+@cuda
+def test_offsets_beyond_32_bits():
+    """A weight of 2.2e9 entries and logits of 2.2e9: the first and last rows against 64 bits."""
+    V, C, T = 430003, 5120, 40
+    g = torch.Generator(device="cuda").manual_seed(8)
+    weight = torch.empty(V, C, device="cuda", dtype=torch.bfloat16).normal_(0, 1.4 / math.sqrt(C), generator=g)
+    hidden = torch.randn(T, C, device="cuda", generator=g).to(torch.bfloat16)
+    targets = torch.randint(V - 2000, V, (T,), device="cuda", generator=g)
+    z = torch.cat([hidden.double() @ part.double().t() for part in weight.split(50000)], 1)
+    q = torch.softmax(z, -1)
+    dz = q.scatter_add(1, targets[:, None], torch.full((T, 1), -1.0, device="cuda", dtype=torch.float64)) / T
+    h, w = hidden.requires_grad_(), weight.requires_grad_()
+    loss = linear_cross_entropy(h, w, targets)
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    x = hidden.detach().double()
+    err = (C / 16 + 16) * 2.0 ** -23 * x.norm(dim=-1).max().item() * 1.6
+    expected = torch.nn.functional.cross_entropy(z, targets)
+    torch.testing.assert_close(loss.detach().double(), expected, rtol=1e-5, atol=2 * err)
+    last = slice(V - 2000, V)
+    tol = 3 * U + 4 * err
+    for rows in (slice(0, 64), last):
+        _within(dw[rows], dz[:, rows].t() @ x, tol * (dz[:, rows].abs().t() @ x.abs()))
+    expected = sum(dz[:, a:a + 50000] @ weight[a:a + 50000].detach().double() for a in range(0, V, 50000))
+    bound = sum(dz[:, a:a + 50000].abs() @ weight[a:a + 50000].detach().double().abs() for a in range(0, V, 50000))
+    _within(dh, expected, tol * bound)
+    del weight, w, dw, z, q, dz
+    logits = torch.empty(8700, 248077, device="cuda", dtype=torch.bfloat16).normal_(0, 2, generator=g)
+    log_probs, index = top_log_probs(logits, 7)
+    for row in (0, 8699):
+        expected, order = _top(logits[row:row + 1], 7)
+        assert torch.equal(index[row:row + 1], order)
+        torch.testing.assert_close(log_probs[row:row + 1].double(), expected, rtol=0, atol=1e-4)
+
+
+@cuda
+def test_calls_in_a_cuda_graph():
+    hidden, weight, targets, g = _inputs(96, 3000, 256)
+    hidden.requires_grad_()
+    weight.requires_grad_()
+
+    def call():
+        loss = linear_cross_entropy(hidden, weight, targets)
+        return (loss.detach(), *torch.autograd.grad(loss, (hidden, weight)), *top_log_probs(hidden.detach(), 5))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    with torch.no_grad():
+        targets.copy_(targets.flip(0))
+        hidden.mul_(1.5)
+    graph.replay()
+    for a, b in zip(out, call()):
+        assert torch.equal(a, b)
