@@ -33,7 +33,7 @@ enum Mode : int { LOGITS = 0, DX = 1, DW = 2, DW32 = 3, LOGITS_N = 4, DX_N = 5 }
 constexpr int TILE = 256, BK = 64, THREADS = 192;
 constexpr int HALF_BYTES = 128 * BK * 2;           // one CTA's half of a 256-wide operand block
 constexpr int MN_CHUNK_BYTES = 64 * BK * 2;        // MN-major operands: 64-wide chunks of BK rows x 128 bytes
-constexpr int STAGING_BYTES = 32 * 128;            // 32 rows of 128 bytes, two buffers per epilogue warp
+constexpr int STAGING_BYTES = 32 * 128;            // 32 rows of 128 bytes, one buffer per epilogue warp
 constexpr int MASK_BYTES = 4 * 8 * 32 * 4;         // held columns of a tile: 8 words per row
 
 template <int MODE, int NT>
@@ -43,9 +43,11 @@ struct Cfg {
   static constexpr bool A_MN = MODE == DW || MODE == DW32 || MODE == DX_N;
   static constexpr bool B_MN = MODE == DX || MODE == DW || MODE == DW32;
   static constexpr int STAGE_BYTES = HALF_BYTES + NT / 2 * BK * 2;  // A half and B half
-  // narrow tiles only stream W: their ring holds about as many bytes of it as fit
-  static constexpr int STAGES = NT == 32 ? 11 : NT == 128 ? 8 : 5;
-  static constexpr int STAGING = NARROW ? 0 : 8 * STAGING_BYTES, MASKS = MODE == LOGITS ? MASK_BYTES : 0;
+  // narrow tiles only stream W: their ring holds about as many bytes of it as fit. 256 x 256 tiles: 6 stages and one
+  // staging buffer per warp took 1.90 / 2.05 / 2.01 ms (dW, dX, logits of 1024 rows in a loop), 5 stages and two
+  // buffers 1.97 / 2.06 / 2.02.
+  static constexpr int STAGES = NT == 32 ? 11 : NT == 128 ? 8 : 6;
+  static constexpr int STAGING = NARROW ? 0 : 4 * STAGING_BYTES, MASKS = MODE == LOGITS ? MASK_BYTES : 0;
   static constexpr int BAR_BYTES = 512;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + STAGING + MASKS + BAR_BYTES + 1024;
   static constexpr int ACC_COLS = NT, TMEM_COLS = 2 * NT;
@@ -352,9 +354,9 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
   } else {
     // ---------------------------------------------------------------- epilogue (warps 2..5, both CTAs)
     const int quarter = warp & 3;
-    uint8_t* buf = staging + 2 * quarter * STAGING_BYTES;
+    uint8_t* buf = staging + quarter * STAGING_BYTES;
     uint32_t* mask = masks + quarter * 8 * 32 + lane;
-    int acc = 0, flip = 0;
+    int acc = 0;
     uint32_t acc_phase = 0;
     while (work.next(tm, tn, split, k0, k1)) {
       const int row0 = tm * TILE + cta * 128 + quarter * 32;  // this warp's first row of the tile
@@ -366,11 +368,9 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
       const uint32_t t_row = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * C_::ACC_COLS;
       // staging buffer of the next store: its previous store has been read
       auto next_buffer = [&]() {
-        if (lane == 0) sm100::bulk_wait_read<1>();
+        if (lane == 0) sm100::bulk_wait_read<0>();
         __syncwarp();
-        uint8_t* b = buf + flip * STAGING_BYTES;
-        flip ^= 1;
-        return b;
+        return buf;
       };
       auto send = [&](uint8_t* b, int x, int y, bool add) {
         sm100::fence_async_shared();
