@@ -55,7 +55,7 @@ struct Cfg {
 };
 
 struct Args {
-  const int* live;  // rows with a loss, all chunks
+  const int* live;  // rows with a loss, all chunks (null: `rows` rows, whether they have one or not)
   int row0, rows;   // this chunk: live rows [row0, row0 + rows)
   int V, C;
   int splits, split_rows;  // DX: parts of K, and rows between their partial sums
@@ -63,6 +63,8 @@ struct Args {
   float scale2;     // logits to units of log2
   int K;            // held entries per row
   const int* sidx;  // [rows, K] ascending, INT_MAX behind the last
+  const long* targets;  // LOGITS_N without `live`: the rows' targets in their place, and
+  int* counts;      // four counters that the call's next kernel finds zero
   float2* part;     // [tiles of the vocabulary, part_ld]
   long part_ld;
   int store_e;
@@ -272,7 +274,9 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
   sm100::cluster_sync();
   sm100::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int n = min(max(*args.live - args.row0, 0), args.rows);
+  const bool direct = MODE == LOGITS_N && !args.live;
+  if (direct && blockIdx.x == 0 && threadIdx.x < 4) args.counts[threadIdx.x] = 0;
+  const int n = direct ? args.rows : min(max(*args.live - args.row0, 0), args.rows);
   Work<MODE> work(args, n);
   int tm, tn, split, k0, k1;
 
@@ -386,7 +390,13 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
 #pragma unroll 1
         for (int g = 0; g < NT / 32 && 32 * g < n; ++g) {
           const int j = 32 * g + lane;
-          const uint32_t word = j < n ? held_word(args.sidx + (long)j * args.K, args.K, row0) : 0u;
+          uint32_t word = 0;
+          if (direct) {
+            const long d = j < n ? args.targets[j] - row0 : -1;
+            if (d >= 0 && d < 32) word = 1u << d;
+          } else if (j < n) {
+            word = held_word(args.sidx + (long)j * args.K, args.K, row0);
+          }
           const bool held = __any_sync(~0u, word != 0);
           float v[32], t[32];
           sm100::tmem_ld32(t_row + 32 * g, v);

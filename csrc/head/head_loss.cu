@@ -16,7 +16,8 @@
 // its tile's maximum in 16 bits; gradient_kernel turns them into dz (bf16) in place, and dX = dz W, dW = dz^T X follow.
 // That is 6 T V C operations, against 8 T V C where the logits are formed a second time, for T V 16-bit values of
 // workspace; CHUNK_VALUES bounds it, and more rows run in chunks whose dW adds up in fp32. Rows without a loss cost
-// nothing but their packing, and what they hold never meets the other rows. A product that gave up a bounded wait
+// nothing but their packing, and what they hold never meets the other rows. A few rows' cross entropy without gradients is
+// not packed and takes two launches. A product that gave up a bounded wait
 // leaves NaN in the losses, or in the gradient it was forming.
 #include <algorithm>
 #include <atomic>
@@ -28,6 +29,7 @@
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr double LN2 = 0.6931471805599453;
 
 // ---------------------------------------------------------------- rows with a loss
 // Kind of each row: 0 no entry (no loss), 1 valid, 2 an index outside the vocabulary (loss NaN, gradient zero).
@@ -116,6 +118,20 @@ __device__ __forceinline__ int place_in_short(const long* idx, bool record, int 
   return kind == 1 ? scratch[0] : -kind - (kind == 0);
 }
 
+// One warp: x . w over 8 c8 values by fp32 fused multiply-adds.
+__device__ __forceinline__ float row_dot(const uint4* x, const uint4* w, int c8, int lane) {
+  float sum = 0.f;
+#pragma unroll 4
+  for (int c = lane; c < c8; c += 32) {
+    float a[8], b[8];
+    rt::unpack8(__ldg(x + c), a);
+    rt::unpack8(__ldg(w + c), b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum = fmaf(a[j], b[j], sum);
+  }
+  return rt::warp_sum(sum);
+}
+
 // One block per row, and 64 more for the zero rows that fill the packed rows' last block of 64. A valid row's hidden
 // state goes to its place in `x`; its entries are sorted by vocabulary index (INT_MAX behind the last) with their
 // log-probabilities, and their logits in units of log2 are summed here: they enter the loss with a weight of about one,
@@ -187,19 +203,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
   const int lane = threadIdx.x & 31;
   for (int k = (threadIdx.x >> 5) + 8 * blockIdx.y; k < K; k += 8 * gridDim.y) {
     const int v = (int)(keys[k] >> 32);
-    float sum = 0.f;
-    if (v != INT_MAX) {
-      const uint4* wr = reinterpret_cast<const uint4*>(w + (long)v * ldw);
-#pragma unroll 4
-      for (int c = lane; c < C8; c += 32) {
-        float a[8], b[8];
-        rt::unpack8(__ldg(src + c), a);
-        rt::unpack8(__ldg(wr + c), b);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fmaf(a[j], b[j], sum);
-      }
-      sum = rt::warp_sum(sum);
-    }
+    const float sum = v == INT_MAX ? 0.f : row_dot(src, reinterpret_cast<const uint4*>(w + (long)v * ldw), C8, lane);
     if (lane == 0) {
       sidx[place * K + k] = v;
       slogp[place * K + k] = __uint_as_float((unsigned)keys[k]);
@@ -290,7 +294,7 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
       heldz += exp2f(z2 - peak);
       const double q = exp((double)lp);
       P += q;
-      if (!(q <= 0.)) L += q * ((double)lp - (double)z2 * 0.6931471805599453);
+      if (!(q <= 0.)) L += q * ((double)lp - (double)z2 * LN2);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
@@ -301,12 +305,12 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
     // rest is relative to m, heldz to peak
     const double Z = (double)heldz + (double)(m == -INFINITY ? rest : rest * exp2f(m - peak));
     const double l2 = (double)peak + log2(Z);
-    const double lse = l2 * 0.6931471805599453;
+    const double lse = l2 * LN2;
     const double r1 = p.tail_class && P < 1. ? 1. - P : 0.;
     const double weight = P + r1;
     double a = weight, value = L + P * lse;
     if (r1 > 0. && !(rest <= 0.f)) {  // an empty rest of the vocabulary has no class
-      const double lr = ((double)m + log2((double)rest)) * 0.6931471805599453 - lse;  // log of the student's rest
+      const double lr = ((double)m + log2((double)rest)) * LN2 - lse;  // log of the student's rest
       value += r1 * (log(r1) - lr);
       a -= r1 * exp(-lr);
     }
@@ -353,6 +357,84 @@ __global__ void __launch_bounds__(MERGE_THREADS) merge_kernel(const MergeArgs p)
     for (int w = 1; w < (int)blockDim.x / 32; ++w) s += part[w];
     *p.loss = (float)(p.mean ? s / (double)max(p.counts->counted, 1) : s);
   }
+}
+
+// Cross entropy of a few rows without gradients, whose rows were not gathered: block per row, whose last warp sums its
+// target's logit beside the merge. Same operations in the same order as merge_kernel<1>, and so the same bits. The last block adds up the rows' losses as in merge_kernel.
+struct ScoreArgs {
+  const float2* part;
+  long part_ld;
+  int tiles, mean;
+  const long* targets;
+  long ignore, V;
+  const __nv_bfloat16* hidden;
+  long ldh;
+  const __nv_bfloat16* w;
+  long ldw;
+  int C;
+  float scale2;
+  Counts* counts;
+  float* row_loss;
+  float* loss;
+};
+__global__ void __launch_bounds__(MERGE_THREADS + 32) score_kernel(const ScoreArgs p) {
+  __shared__ float2 merged[MERGE_THREADS];
+  __shared__ float target_z2;
+  __shared__ bool last;
+  const int tid = threadIdx.x, lane = tid & 31, row = blockIdx.x, rows = gridDim.x;
+  const long target = p.targets[row];
+  const int kind = entry_kind(target, false, p.ignore, p.V);
+  if (kind == 1 && tid >= MERGE_THREADS) {
+    const float dot = row_dot(reinterpret_cast<const uint4*>(p.hidden + row * p.ldh),
+                              reinterpret_cast<const uint4*>(p.w + target * p.ldw), p.C / 8, lane);
+    if (lane == 0) target_z2 = dot * p.scale2;
+  } else if (kind == 1) {
+    float2 sum = make_float2(-INFINITY, 0.f);
+    for (int i = tid; i < p.tiles; i += 8 * MERGE_THREADS) {
+      float2 t[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        t[u] = i + u * MERGE_THREADS < p.tiles ? p.part[(i + u * MERGE_THREADS) * p.part_ld + row]
+                                               : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum = merge2(sum, t[u]);
+    }
+    merged[tid] = sum;
+  }
+  __syncthreads();
+  if (tid < 32) {
+    float value = kind ? NAN : 0.f;
+    if (kind == 1) {
+      float2 all = merged[lane];
+#pragma unroll
+      for (int i = 32; i < MERGE_THREADS; i += 32) all = merge2(all, merged[lane + i]);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1)
+        all = merge2(all, make_float2(__shfl_xor_sync(~0u, all.x, off), __shfl_xor_sync(~0u, all.y, off)));
+      const float z2 = target_z2, peak = fmaxf(all.x, z2);
+      const double Z = (double)exp2f(z2 - peak) +
+                       (double)(all.x == -INFINITY ? all.y : all.y * exp2f(all.x - peak));
+      if (!p.counts->failed) value = (float)(((double)peak + log2(Z)) * LN2 - (double)z2 * LN2);
+    }
+    if (lane == 0) p.row_loss[row] = value;
+  }
+  if (!p.loss) return;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last = atomicAdd(&p.counts->done, 1) == rows - 1;
+  __syncthreads();
+  if (!last || tid >= 32) return;
+  __threadfence();
+  double s = 0.;
+  int counted = 0;
+  for (int t = lane; t < rows; t += 32) {
+    s += (double)__ldcg(p.row_loss + t);
+    counted += p.targets[t] != p.ignore;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(~0u, s, off);
+  counted = __reduce_add_sync(~0u, counted);
+  if (lane == 0) *p.loss = (float)(p.mean ? s / (double)max(counted, 1) : s);
 }
 
 // ---------------------------------------------------------------- gradient of the logits
@@ -596,6 +678,33 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(work + l.e);
   float2* part = reinterpret_cast<float2*>(work + l.part);
   const float scale2 = p->scale * LOG2E;
+  const bool narrow = T <= NARROW_ROWS, few = T <= 32;  // one chunk
+  if (narrow && !grad && !p->log_probs) {  // scores: two launches, the rows where they are
+    head::Maps maps;
+    head::Args args{};
+    args.rows = (int)T;
+    args.V = (int)V;
+    args.C = C;
+    args.K = 1;
+    args.scale2 = scale2 * mma_gain(C);
+    args.part = part;
+    args.part_ld = l.rows;
+    args.targets = p->index;
+    args.counts = &counts->valid;
+    args.status = &counts->failed;
+    if (!map2d(&maps.a, false, p->weight, C, V, 2 * p->ld_weight, 128) ||
+        !map2d(&maps.b, false, p->hidden, C, T, 2 * p->ld_hidden, few ? 16 : 64) ||
+        !map2d(&maps.out, false, p->hidden, C, T, 2 * p->ld_hidden, 32))
+      return cudaErrorInvalidValue;
+    RT_CUDA_CHECK((few ? launch<head::LOGITS_N, 32>(maps, args, l.tiles, s)
+                       : launch<head::LOGITS_N, 128>(maps, args, l.tiles, s)));
+    const ScoreArgs score{part, l.rows, (int)l.groups, p->reduction == 2, p->index, p->ignore, V,
+                          reinterpret_cast<const __nv_bfloat16*>(p->hidden), p->ld_hidden,
+                          reinterpret_cast<const __nv_bfloat16*>(p->weight), p->ld_weight, C, scale2, counts,
+                          p->row_loss, p->reduction ? p->loss : nullptr};
+    score_kernel<<<(unsigned)T, MERGE_THREADS + 32, 0, s>>>(score);
+    return cudaGetLastError();
+  }
   const bool brief = T * K <= SHORT_ENTRIES;
   if (!brief) {
     if (p->log_probs) kinds_kernel<<<(unsigned)((T * 32 + 255) / 256), 256, 0, s>>>(p->index, T, K, V, ints(l.kind));
@@ -628,7 +737,6 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   args.splits = (int)std::max(1L, l.splits);
   args.split_rows = (int)l.split_rows;
   args.status = &counts->failed;
-  const bool narrow = T <= NARROW_ROWS, few = T <= 32;  // one chunk
   int merge_blocks = 0;
   for (long row0 = 0; row0 < T; row0 += l.rows)
     merge_blocks += (int)(std::min(l.rows, up(T - row0, 64)) / (narrow ? 1 : 4));  // multiples of 64
