@@ -360,7 +360,8 @@ __global__ void __launch_bounds__(MERGE_THREADS) merge_kernel(const MergeArgs p)
 }
 
 // Cross entropy of a few rows without gradients, whose rows were not gathered: block per row, whose last warp sums its
-// target's logit beside the merge. Same operations in the same order as merge_kernel<1>, and so the same bits. The last block adds up the rows' losses as in merge_kernel.
+// target's logit beside the merge. Same operations in the same order as merge_kernel<1>, and so the same bits. The last
+// block adds up the rows' losses as in merge_kernel.
 struct ScoreArgs {
   const float2* part;
   long part_ld;
@@ -585,8 +586,8 @@ int dx_splits(long rows, long V, int C) {
 // accesses (dW of 1024 tokens: 2.8 ms from a 16-byte aligned dz, 1.8 ms from an aligned one).
 struct Layout {
   // rows of a chunk, row stride of the depths and of dz, 256-wide tiles of the vocabulary, groups of columns with
-  // statistics, and for dX the parts of K and the rows between their partial sums
-  long rows, ld_e, tiles, groups, splits, split_rows;
+  // statistics and values between them, and for dX the parts of K and the rows between their partial sums
+  long rows, ld_e, tiles, groups, part_ld, splits, split_rows;
   bool dw32;
   long kind, slot, row_of, counts, x, sidx, slogp, hit, coef, lse2, tail, part, e, dx, dw, total;
 };
@@ -618,7 +619,8 @@ Layout layout(long T, long V, int C, int K, bool grad_h, bool grad_w) {
   l.coef = take(grad ? T * K : 0);
   l.lse2 = take(T);
   l.tail = take(T);
-  l.part = take(2 * l.groups * l.rows);
+  l.part_ld = std::min(T, l.rows);  // one row x 7760 groups: score_kernel 12 us, with values 512 bytes apart 21 us
+  l.part = take(2 * l.groups * l.part_ld);
   l.e = take(grad ? l.rows * l.ld_e / 2 : 0);
   l.dx = take(l.splits * l.split_rows * C);
   l.dw = take(l.dw32 ? V * C : 0);
@@ -688,7 +690,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
     args.K = 1;
     args.scale2 = scale2 * mma_gain(C);
     args.part = part;
-    args.part_ld = l.rows;
+    args.part_ld = l.part_ld;
     args.targets = p->index;
     args.counts = &counts->valid;
     args.status = &counts->failed;
@@ -698,7 +700,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
       return cudaErrorInvalidValue;
     RT_CUDA_CHECK((few ? launch<head::LOGITS_N, 32>(maps, args, l.tiles, s)
                        : launch<head::LOGITS_N, 128>(maps, args, l.tiles, s)));
-    const ScoreArgs score{part, l.rows, (int)l.groups, p->reduction == 2, p->index, p->ignore, V,
+    const ScoreArgs score{part, l.part_ld, (int)l.groups, p->reduction == 2, p->index, p->ignore, V,
                           reinterpret_cast<const __nv_bfloat16*>(p->hidden), p->ld_hidden,
                           reinterpret_cast<const __nv_bfloat16*>(p->weight), p->ld_weight, C, scale2, counts,
                           p->row_loss, p->reduction ? p->loss : nullptr};
@@ -732,7 +734,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   args.e = reinterpret_cast<unsigned short*>(e);
   args.ld_e = l.ld_e;
   args.dx = work + l.dx;
-  args.part_ld = l.rows;
+  args.part_ld = l.part_ld;
   args.store_e = grad;
   args.splits = (int)std::max(1L, l.splits);
   args.split_rows = (int)l.split_rows;
@@ -756,14 +758,14 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
     RT_CUDA_CHECK((few      ? launch<head::LOGITS_N, 32>(logits, args, l.tiles, s)
                    : narrow ? launch<head::LOGITS_N, 128>(logits, args, l.tiles, s)
                             : launch<head::LOGITS>(logits, args, tiles_m * l.tiles, s)));
-    MergeArgs m{part, l.rows, (int)l.groups, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, merge_blocks, T,
+    MergeArgs m{part, l.part_ld, (int)l.groups, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, merge_blocks, T,
                 counts, ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->scale, p->row_grad, p->row_loss,
                 p->reduction ? p->loss : nullptr, work + l.lse2, work + l.tail, grad ? work + l.coef : nullptr};
     if (narrow) merge_kernel<1><<<(unsigned)rows, MERGE_THREADS, 0, s>>>(m);
     else merge_kernel<4><<<(unsigned)(rows + 3) / 4, MERGE_THREADS, 0, s>>>(m);
     if (grad)
       gradient_kernel<<<dim3((unsigned)((l.tiles + 31) / 32), (unsigned)rows), 256, 0, s>>>(
-          e, l.ld_e, (int)V, (int)l.tiles, (int)row0, (int)l.rows, counts, part, l.rows, narrow ? 32 : 256,
+          e, l.ld_e, (int)V, (int)l.tiles, (int)row0, (int)l.rows, counts, part, l.part_ld, narrow ? 32 : 256,
           work + l.lse2, work + l.tail, K, ints(l.sidx), work + l.coef);
     RT_CUDA_CHECK(cudaGetLastError());
     if (p->dhidden) {
