@@ -16,9 +16,9 @@
 // its tile's maximum in 16 bits; gradient_kernel turns them into dz (bf16) in place, and dX = dz W, dW = dz^T X follow.
 // That is 6 T V C operations, against 8 T V C where the logits are formed a second time, for T V 16-bit values of
 // workspace; CHUNK_VALUES bounds it, and more rows run in chunks whose dW adds up in fp32. Rows without a loss cost
-// nothing but their packing, and what they hold never meets the other rows. A few rows' cross entropy without gradients is
-// not packed and takes two launches. A product that gave up a bounded wait
-// leaves NaN in the losses, or in the gradient it was forming.
+// nothing but their packing, and what they hold never meets the other rows. The cross entropy of a few rows without
+// gradients is not packed and takes two launches. A product that gave up a bounded wait leaves NaN in the losses, or in
+// the gradient it was forming.
 #include <algorithm>
 #include <atomic>
 #include <climits>

@@ -430,3 +430,28 @@ def test_calls_in_a_cuda_graph():
     graph.replay()
     for a, b in zip(out, call()):
         assert torch.equal(a, b)
+
+
+@cuda
+@pytest.mark.parametrize("T", [1, 31, 32, 33, 128, 129])
+def test_scores_equal_the_losses_of_a_training_call(T):
+    """Without gradients few rows take a path of their own: the same bits per token, whatever masked rows hold, and the
+    same sums but for the order of 64-bit additions."""
+    hidden, weight, targets, _ = _inputs(T, 1500, 136)
+    targets[T // 2:T // 2 + 3] = -100
+    hidden[T // 2] = math.nan
+    if T > 8:
+        hidden[T // 2 + 1] = math.inf
+        targets[2], targets[5] = 1500, -7
+    for reduction in ("none", "sum", "mean"):
+        score = linear_cross_entropy(hidden, weight, targets, reduction=reduction)
+        loss = linear_cross_entropy(hidden.clone().requires_grad_(), weight, targets, reduction=reduction).detach()
+        tolerance = 0 if reduction == "none" else 1e-6
+        torch.testing.assert_close(score, loss, rtol=tolerance, atol=0, equal_nan=True)
+    if T > 8:
+        targets[2] = targets[5] = 3
+    for reduction in ("sum", "mean"):
+        score = linear_cross_entropy(hidden, weight, targets, reduction=reduction)
+        loss = linear_cross_entropy(hidden.clone().requires_grad_(), weight, targets, reduction=reduction).detach()
+        assert torch.isfinite(score)
+        torch.testing.assert_close(score, loss, rtol=1e-6, atol=0)
