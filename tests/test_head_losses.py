@@ -147,3 +147,51 @@ def test_refusals():
             top_log_probs(teacher, k)
     with pytest.raises(ValueError, match="temperature"):
         top_log_probs(teacher, 2, temperature=-1.0)
+
+
+def test_c_entries_refuse_before_any_cuda_call():
+    """Sizes, counts and alignments out of range return cudaErrorInvalidValue; stand-in addresses are never used."""
+    import ctypes
+    import glob
+    from pathlib import Path
+    found = glob.glob(str(Path(__file__).resolve().parents[1] / "rwkv_theseus_b200" / "_C*.so"))
+    if not found:
+        pytest.skip("extension not built")
+    lib = ctypes.CDLL(found[0])
+    vp, lg, it, fl = ctypes.c_void_p, ctypes.c_long, ctypes.c_int, ctypes.c_float
+    lib.rt_top_log_probs.argtypes = [it, vp, lg, lg, lg, it, fl, vp, vp, vp, vp]
+    lib.rt_top_workspace_bytes.argtypes, lib.rt_top_workspace_bytes.restype = [it, lg, lg, it], lg
+    lib.rt_head_loss.argtypes = [vp, vp, vp]
+    lib.rt_scale_bf16.argtypes = [ctypes.POINTER(vp), ctypes.POINTER(lg), vp, vp]
+    good = 0x10000
+
+    def top(rows=4, V=100, k=5, work=good):
+        return lib.rt_top_log_probs(1, good, rows, V, V, k, 1.0, good, good, work, None)
+
+    assert top(k=0) == top(k=101) == top(k=1025, V=5000) == top(V=0) == top(rows=-1) == 1
+    assert top(rows=0) == 0
+    assert top(rows=1, V=1 << 22, work=None) == 1                     # cut into segments, which need their workspace
+    assert top(rows=1, V=1 << 24, k=1024) == 1 and lib.rt_top_workspace_bytes(1, 1, 1 << 24, 1024) == -1
+
+    class HeadLoss(ctypes.Structure):
+        _fields_ = [("hidden", vp), ("ld_hidden", lg), ("weight", vp), ("ld_weight", lg), ("index", vp),
+                    ("log_probs", vp), ("rows", lg), ("vocab", lg), ("width", it), ("K", it), ("ignore", lg),
+                    ("scale", fl), ("tail", it), ("reduction", it), ("row_grad", vp), ("row_loss", vp), ("loss", vp),
+                    ("dhidden", vp), ("dweight", vp)]
+
+    def head(work=good, **changes):
+        call = HeadLoss(hidden=good, ld_hidden=64, weight=good, ld_weight=64, index=good, rows=4, vocab=100, width=64,
+                        K=1, ignore=-100, scale=1.0, row_loss=good)
+        for name, value in changes.items():
+            setattr(call, name, value)
+        return lib.rt_head_loss(ctypes.byref(call), work, None)
+
+    assert lib.rt_head_loss(None, good, None) == 1 and head(work=None) == 1 and head(work=good + 8) == 1
+    for changes in (dict(rows=-1), dict(rows=(1 << 24) + 1), dict(vocab=0), dict(vocab=2 ** 31), dict(width=60),
+                    dict(K=0), dict(K=2), dict(K=1025, log_probs=good), dict(ld_hidden=60), dict(ld_weight=60),
+                    dict(hidden=None), dict(weight=None), dict(hidden=good + 2), dict(weight=good + 8),
+                    dict(dhidden=good + 4), dict(dweight=good + 2)):
+        assert head(**changes) == 1, changes
+    assert head(rows=0) == 0                                           # no reduction, no weight gradient: nothing to do
+    assert lib.rt_scale_bf16((vp * 2)(good + 2, None), (lg * 2)(8, 0), good, None) == 1
+    assert lib.rt_scale_bf16((vp * 2)(None, None), (lg * 2)(0, 0), good, None) == 0
