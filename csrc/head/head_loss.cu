@@ -439,12 +439,12 @@ __global__ void __launch_bounds__(MERGE_THREADS + 32) score_kernel(const ScoreAr
 }
 
 // ---------------------------------------------------------------- gradient of the logits
-// In place: depths of a chunk's logits (below the maximum of their `group` columns) -> dz, one warp per row and tile;
-// the block of 32 tiles also puts their held entries in their places; rows that fill the last block of 64 become zero.
-// A read and a write of every value: 0.18 ms for 1024 x 248077 (5.7 TB/s), where forming the logits again would cost
-// 1.8 ms.
-__global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict__ e, long ld, int V, int tiles,
-                                                       int row0, int rows, const Counts* __restrict__ counts,
+// In place: depths of a chunk's logits (below the maximum of their `group` columns) -> dz, one warp per row and 256
+// columns; the block of 32 such tiles also puts their held entries in their places; rows that fill the last block of 64
+// become zero. A read and a write of every value: 0.16 ms for 992 x 248077 (6.2 TB/s), where forming the logits again
+// would cost 1.8 ms. dz is rounded to bf16 here, once: it is a tensor-core operand next.
+__global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict__ e, long ld, int V, int row0,
+                                                       int rows, const Counts* __restrict__ counts,
                                                        const float2* __restrict__ part, long part_ld, int group,
                                                        const float* __restrict__ lse2, const float* __restrict__ tail,
                                                        int K, const int* __restrict__ sidx,
@@ -456,27 +456,33 @@ __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict
   const float l = live ? lse2[row0 + r] : 0.f, a = live ? tail[row0 + r] : 0.f;
   sidx += (long)(row0 + r) * K;
   coef += (long)(row0 + r) * K;
+  __nv_bfloat16* out = e + r * ld;
+  uint4 depths[4];
+  float m[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {  // all loads first: nothing says that the stores leave them alone
+    const int c = ((blockIdx.x * 4 + u) * 8 + (threadIdx.x >> 5)) * 256 + lane * 8;
+    if (live && c < V) {
+      depths[u] = *reinterpret_cast<const uint4*>(out + c);
+      m[u] = part[c / group * part_ld + r].x;
+    }
+  }
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    const int t = (blockIdx.x * 4 + u) * 8 + (threadIdx.x >> 5), c = t * 256 + lane * 8;
-    if (t >= tiles) continue;
-    __nv_bfloat16* out = e + r * ld;
-    if (c < ld) {
-      uint4* at = reinterpret_cast<uint4*>(out + c);
-      float v[8] = {};
-      if (live && c < V) {
-        const uint4 u = *at;
-        const float m = part[c / group * part_ld + r].x, top = m == -INFINITY ? m : m - l;
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const int c = ((blockIdx.x * 4 + u) * 8 + (threadIdx.x >> 5)) * 256 + lane * 8;
+    if (c >= ld) continue;
+    float v[8] = {};
+    if (live && c < V) {
+      const float top = m[u] == -INFINITY ? m[u] : m[u] - l;
+      const uint32_t w[4] = {depths[u].x, depths[u].y, depths[u].z, depths[u].w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {  // 2^23 + depth as a float, and back
-          const uint32_t word = __byte_perm(w[j / 2], 0x4b000000u, j & 1 ? 0x7632 : 0x7610);
-          const float d = __uint_as_float(word) - head::DEPTH_BASE;
-          v[j] = a * head::ex2(fmaf(d, -1.f / head::DEPTH_STEPS, top));
-        }
+      for (int j = 0; j < 8; ++j) {  // 2^23 + depth as a float, and back
+        const uint32_t word = __byte_perm(w[j / 2], 0x4b000000u, j & 1 ? 0x7632 : 0x7610);
+        const float d = __uint_as_float(word) - head::DEPTH_BASE;
+        v[j] = a * head::ex2(fmaf(d, -1.f / head::DEPTH_STEPS, top));
       }
-      *at = rt::pack8(v);
     }
+    *reinterpret_cast<uint4*>(out + c) = rt::pack8(v);
   }
   if (!live) return;
   __syncthreads();
@@ -765,7 +771,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
     else merge_kernel<4><<<(unsigned)(rows + 3) / 4, MERGE_THREADS, 0, s>>>(m);
     if (grad)
       gradient_kernel<<<dim3((unsigned)((l.tiles + 31) / 32), (unsigned)rows), 256, 0, s>>>(
-          e, l.ld_e, (int)V, (int)l.tiles, (int)row0, (int)l.rows, counts, part, l.part_ld, narrow ? 32 : 256,
+          e, l.ld_e, (int)V, (int)row0, (int)l.rows, counts, part, l.part_ld, narrow ? 32 : 256,
           work + l.lse2, work + l.tail, K, ints(l.sidx), work + l.coef);
     RT_CUDA_CHECK(cudaGetLastError());
     if (p->dhidden) {
