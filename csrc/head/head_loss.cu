@@ -286,12 +286,11 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, off));
     const float peak = fmaxf(m, top);
-    float heldz = 0.f;
-    double P = 0., L = 0.;
+    double heldz = 0., P = 0., L = 0.;
     for (int k = lane; k < p.K; k += 32) {
       if (sidx[k] == INT_MAX) continue;
       const float z2 = hit[k], lp = slogp[k];
-      heldz += exp2f(z2 - peak);
+      heldz += exp2((double)z2 - (double)peak);
       const double q = exp((double)lp);
       P += q;
       if (!(q <= 0.)) L += q * ((double)lp - (double)z2 * LN2);
@@ -302,8 +301,9 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
       P += __shfl_xor_sync(~0u, P, off);
       L += __shfl_xor_sync(~0u, L, off);
     }
-    // rest is relative to m, heldz to peak
-    const double Z = (double)heldz + (double)(m == -INFINITY ? rest : rest * exp2f(m - peak));
+    // rest is relative to m, heldz to peak. In fp64: a KL is a small difference of these, and fp32's exp2f alone put
+    // -4e-8 on a mean of 0.018.
+    const double Z = heldz + (m == -INFINITY ? rest : rest * exp2((double)m - (double)peak));
     const double l2 = (double)peak + log2(Z);
     const double lse = l2 * LN2;
     const double r1 = p.tail_class && P < 1. ? 1. - P : 0.;
@@ -413,8 +413,8 @@ __global__ void __launch_bounds__(MERGE_THREADS + 32) score_kernel(const ScoreAr
       for (int off = 16; off > 0; off >>= 1)
         all = merge2(all, make_float2(__shfl_xor_sync(~0u, all.x, off), __shfl_xor_sync(~0u, all.y, off)));
       const float z2 = target_z2, peak = fmaxf(all.x, z2);
-      const double Z = (double)exp2f(z2 - peak) +
-                       (double)(all.x == -INFINITY ? all.y : all.y * exp2f(all.x - peak));
+      const double Z = exp2((double)z2 - (double)peak) +
+                       (all.x == -INFINITY ? all.y : all.y * exp2((double)all.x - (double)peak));
       if (!p.counts->failed) value = (float)(((double)peak + log2(Z)) * LN2 - (double)z2 * LN2);
     }
     if (lane == 0) p.row_loss[row] = value;
