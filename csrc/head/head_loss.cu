@@ -6,9 +6,12 @@
 // Z = sum_v exp z_v and Z_rest = sum_{v not in S} exp z_v:
 //   loss  = sum_S p (log p - z_v + log Z) + r (log r - log Z_rest + log Z)
 //   d/dz_v = w exp(z_v) / Z - p_v                       (v in S)
-//          = exp(z_v) / Z (w - r Z / Z_rest)            (v not in S)
+//          = exp(z_v) / Z_rest (w Z_rest / Z - r)       (v not in S, r > 0)
+//          = exp(z_v) / Z w                             (v not in S, r = 0)
 // Z_rest is summed without the held entries instead of as Z minus them, so a row that is sure of its target keeps the
-// relative precision of 1 - q. All sums and row statistics are fp32 (the few held terms of a row: double).
+// relative precision of 1 - q. The second form has factors of at most one however small Z_rest / Z is; as exp(z_v) / Z
+// (w - r Z / Z_rest) its factors leave fp32's range at Z_rest / Z = e^-87.
+// All sums and row statistics are fp32 (the few held terms of a row: double).
 //
 // Launches of one call: the rows that have a loss are counted and packed (gather_kernel: their hidden states, sorted
 // records and held logits), z = X W^T leaves per row and 256-column tile its maximum and sum of exponentials
@@ -215,8 +218,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
 // ---------------------------------------------------------------- losses of the valid rows of a chunk
 // Block of ROWS rows (four, or one of the few rows whose statistics are finer): its threads merge the tiles' statistics
 // (in a fixed order: each row's tiles go round-robin to MERGE_THREADS / ROWS threads), then one warp per row forms the
-// loss and the gradient's coefficients: d/dz_v = tail exp2(z_v - lse2) outside the record, coef[k] for its held
-// entries, both times scale and the row's upstream gradient (given per row, or 1, or 1 / rows with a loss).
+// loss and the gradient's coefficients: d/dz_v = tail exp2(z_v - base2) outside the record (base2 = log2 Z_rest with a
+// rest's class, else log2 Z), coef[k] for its held entries, both times scale and the row's upstream gradient (given per
+// row, or 1, or 1 / rows with a loss).
 constexpr int MERGE_THREADS = 256;
 struct MergeArgs {
   const float2* part;
@@ -233,7 +237,7 @@ struct MergeArgs {
   const float* grad;
   float* row_loss;
   float* loss;  // null: the rows' losses are the result
-  float* lse2;
+  float* base2;
   float* tail;
   float* coef;
 };
@@ -308,16 +312,17 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
     const double lse = l2 * LN2;
     const double r1 = p.tail_class && P < 1. ? 1. - P : 0.;
     const double weight = P + r1;
-    double a = weight, value = L + P * lse;
+    double a = weight, value = L + P * lse, base = l2;
     if (r1 > 0. && !(rest <= 0.f)) {  // an empty rest of the vocabulary has no class
-      const double lr = ((double)m + log2((double)rest)) * LN2 - lse;  // log of the student's rest
+      base = (double)m + log2((double)rest);
+      const double lr = base * LN2 - lse;  // log of the student's rest
       value += r1 * (log(r1) - lr);
-      a -= r1 * exp(-lr);
+      a = weight * exp(lr) - r1;
     }
     const float g = p.scale * (p.grad ? p.grad[row] : (p.mean ? 1.f / (float)max(p.counts->counted, 1) : 1.f));
     if (lane == 0) {
       p.row_loss[row] = p.counts->failed ? NAN : (float)value;
-      p.lse2[place] = (float)l2;
+      p.base2[place] = (float)base;
       p.tail[place] = g * (float)a;
     }
     if (!p.coef) return;
@@ -446,14 +451,14 @@ __global__ void __launch_bounds__(MERGE_THREADS + 32) score_kernel(const ScoreAr
 __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict__ e, long ld, int V, int row0,
                                                        int rows, const Counts* __restrict__ counts,
                                                        const float2* __restrict__ part, long part_ld, int group,
-                                                       const float* __restrict__ lse2, const float* __restrict__ tail,
+                                                       const float* __restrict__ base2, const float* __restrict__ tail,
                                                        int K, const int* __restrict__ sidx,
                                                        const float* __restrict__ coef) {
   const int n = min(max(counts->valid - row0, 0), rows), r = blockIdx.y;
   if (r >= max((n + 63) / 64 * 64, 64)) return;
   const int lane = threadIdx.x & 31;
   const bool live = r < n;
-  const float l = live ? lse2[row0 + r] : 0.f, a = live ? tail[row0 + r] : 0.f;
+  const float l = live ? base2[row0 + r] : 0.f, a = live ? tail[row0 + r] : 0.f;
   sidx += (long)(row0 + r) * K;
   coef += (long)(row0 + r) * K;
   __nv_bfloat16* out = e + r * ld;
@@ -595,7 +600,7 @@ struct Layout {
   // statistics and values between them, and for dX the parts of K and the rows between their partial sums
   long rows, ld_e, tiles, groups, part_ld, splits, split_rows;
   bool dw32;
-  long kind, slot, row_of, counts, x, sidx, slogp, hit, coef, lse2, tail, part, e, dx, dw, total;
+  long kind, slot, row_of, counts, x, sidx, slogp, hit, coef, base2, tail, part, e, dx, dw, total;
 };
 Layout layout(long T, long V, int C, int K, bool grad_h, bool grad_w) {
   Layout l;
@@ -623,7 +628,7 @@ Layout layout(long T, long V, int C, int K, bool grad_h, bool grad_w) {
   l.slogp = take(T * K);
   l.hit = take(T * K);
   l.coef = take(grad ? T * K : 0);
-  l.lse2 = take(T);
+  l.base2 = take(T);
   l.tail = take(T);
   l.part_ld = std::min(T, l.rows);  // one row x 7760 groups: score_kernel 12 us, with values 512 bytes apart 21 us
   l.part = take(2 * l.groups * l.part_ld);
@@ -766,13 +771,13 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
                             : launch<head::LOGITS>(logits, args, tiles_m * l.tiles, s)));
     MergeArgs m{part, l.part_ld, (int)l.groups, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, merge_blocks, T,
                 counts, ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->scale, p->row_grad, p->row_loss,
-                p->reduction ? p->loss : nullptr, work + l.lse2, work + l.tail, grad ? work + l.coef : nullptr};
+                p->reduction ? p->loss : nullptr, work + l.base2, work + l.tail, grad ? work + l.coef : nullptr};
     if (narrow) merge_kernel<1><<<(unsigned)rows, MERGE_THREADS, 0, s>>>(m);
     else merge_kernel<4><<<(unsigned)(rows + 3) / 4, MERGE_THREADS, 0, s>>>(m);
     if (grad)
       gradient_kernel<<<dim3((unsigned)((l.tiles + 31) / 32), (unsigned)rows), 256, 0, s>>>(
           e, l.ld_e, (int)V, (int)row0, (int)l.rows, counts, part, l.part_ld, narrow ? 32 : 256,
-          work + l.lse2, work + l.tail, K, ints(l.sidx), work + l.coef);
+          work + l.base2, work + l.tail, K, ints(l.sidx), work + l.coef);
     RT_CUDA_CHECK(cudaGetLastError());
     if (p->dhidden) {
       if (!map2d(narrow ? &dx.b : &dx.a, false, e, V, rows, 2 * l.ld_e, few ? 16 : narrow ? 64 : 128) ||

@@ -1,0 +1,41 @@
+"""Corners of the vocabulary-head operators on the GPU against 64-bit formulas: students that are sure of their record.
+
+Tolerances are those of test_head_losses_gpu.py (u = 2^-8; a gradient is off by (3 u + 4 dz) times the same product of
+absolute values, dz the bound of a logit's error) unless a test derives its own.
+"""
+import pytest
+import torch
+
+from test_head_losses_gpu import _check
+
+pytestmark = pytest.mark.gpu
+cuda = pytest.mark.skipif(not torch.cuda.is_available(), reason="CUDA unavailable")
+
+
+def _sure(T, V, gap, mass, entries=4):
+    """Rows whose student is `gap` nats surer of its `entries` recorded tokens than of the rest, where the teacher's
+    record holds `mass`. Feature j of the width stands for the j-th group of tokens and is zero for all others."""
+    g = torch.Generator(device="cuda").manual_seed(T + V + int(gap))
+    weight = torch.randn(V, 64, device="cuda", generator=g) * 0.15
+    hidden = torch.randn(T, 64, device="cuda", generator=g)
+    weight[:, :8] = 0.0
+    hidden[:, :8] = 0.0
+    for j in range(8):
+        weight[j * entries:(j + 1) * entries, j] = 1.0
+    group = torch.randint(0, 8, (T,), device="cuda", generator=g)
+    hidden[torch.arange(T, device="cuda"), group] = gap
+    index = group[:, None] * entries + torch.arange(entries, device="cuda")
+    p = torch.rand(T, entries, device="cuda", generator=g) + 0.2
+    return hidden.to(torch.bfloat16), weight.to(torch.bfloat16), index, (p / p.sum(-1, keepdim=True) * mass).log()
+
+
+@cuda
+@pytest.mark.parametrize("T", [5, 100, 150])
+@pytest.mark.parametrize("gap", [80.0, 100.0, 300.0])
+@pytest.mark.parametrize("mass,entries", [(0.5, 4), (0.9, 1), (0.999999, 4)])
+def test_a_student_that_is_sure_of_its_record(T, gap, mass, entries):
+    """The rest of the vocabulary has a probability of e^-gap, and is all that pushes mass back to it."""
+    hidden, weight, index, log_probs = _sure(T, 1003, gap, mass, entries)
+    _check(hidden, weight, index, log_probs, 1.0, True, "mean")
+    _check(hidden, weight, index, log_probs, 0.5, True, "none")
+    _check(hidden, weight, index, log_probs, 1.0, False, "mean")
