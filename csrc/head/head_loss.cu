@@ -2,8 +2,8 @@
 // log-probabilities, with the gradients of the hidden states and of the head's weight.
 //
 // With z_tv = scale x_t . W_v, a row's record is a set S of held entries (v, log p_v); the cross entropy's record is
-// its target with p = 1. With P = sum_S p, r = max(0, 1 - P) (the rest as one more class, or 0 without it), w = P + r,
-// Z = sum_v exp z_v and Z_rest = sum_{v not in S} exp z_v:
+// its target with p = 1. With P = sum_S p, r = max(0, 1 - P) (the rest as one more class; 0 without that class, or
+// where S is the whole vocabulary), w = P + r, Z = sum_v exp z_v and Z_rest = sum_{v not in S} exp z_v:
 //   loss  = sum_S p (log p - z_v + log Z) + r (log r - log Z_rest + log Z)
 //   d/dz_v = w exp(z_v) / Z - p_v                       (v in S)
 //          = exp(z_v) / Z_rest (w Z_rest / Z - r)       (v not in S, r > 0)
@@ -310,10 +310,10 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
     const double Z = heldz + (m == -INFINITY ? rest : rest * exp2((double)m - (double)peak));
     const double l2 = (double)peak + log2(Z);
     const double lse = l2 * LN2;
-    const double r1 = p.tail_class && P < 1. ? 1. - P : 0.;
+    const double r1 = p.tail_class && P < 1. && !(rest <= 0.f) ? 1. - P : 0.;  // an empty rest has no class
     const double weight = P + r1;
     double a = weight, value = L + P * lse, base = l2;
-    if (r1 > 0. && !(rest <= 0.f)) {  // an empty rest of the vocabulary has no class
+    if (r1 > 0.) {
       base = (double)m + log2((double)rest);
       const double lr = base * LN2 - lse;  // log of the student's rest
       value += r1 * (log(r1) - lr);

@@ -1,12 +1,15 @@
-"""Corners of the vocabulary-head operators on the GPU against 64-bit formulas: students that are sure of their record.
+"""Corners of the vocabulary-head operators on the GPU against 64-bit formulas: students that are sure of their record,
+records of the whole vocabulary.
 
 Tolerances are those of test_head_losses_gpu.py (u = 2^-8; a gradient is off by (3 u + 4 dz) times the same product of
 absolute values, dz the bound of a logit's error) unless a test derives its own.
 """
+import math
+
 import pytest
 import torch
 
-from test_head_losses_gpu import _check
+from test_head_losses_gpu import _check, _inputs, _record
 
 pytestmark = pytest.mark.gpu
 cuda = pytest.mark.skipif(not torch.cuda.is_available(), reason="CUDA unavailable")
@@ -39,3 +42,15 @@ def test_a_student_that_is_sure_of_its_record(T, gap, mass, entries):
     _check(hidden, weight, index, log_probs, 1.0, True, "mean")
     _check(hidden, weight, index, log_probs, 0.5, True, "none")
     _check(hidden, weight, index, log_probs, 1.0, False, "mean")
+
+
+@cuda
+@pytest.mark.parametrize("T", [5, 100, 150])
+@pytest.mark.parametrize("V", [8, 64, 700])
+def test_a_record_of_the_whole_vocabulary_without_all_its_mass(T, V):
+    """Nothing is left for the rest's class, in the loss and in its gradient."""
+    hidden, weight, _, g = _inputs(T, V, 64)
+    log_probs, index = _record(hidden, weight, V, 1.0, g)
+    _check(hidden, weight, index, log_probs + math.log(0.6), 1.0, True, "mean")
+    log_probs[:, 1:3] = -math.inf
+    _check(hidden, weight, index, log_probs, 1.0, True, "none")
