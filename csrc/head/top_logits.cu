@@ -56,13 +56,13 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // Two fp32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
-      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
       : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -242,10 +242,10 @@ struct TopArgs {
 
 // list[0, n), n >= min(k, available): the row's result from its candidates and denominator.
 __device__ void write_row(const TopArgs& a, long row, unsigned long long* list, int n, float2 ms) {
-  const float lse = ms.x * a.scale + logf(ms.y);
+  const float log_sum = logf(ms.y);
   auto put = [&](int rank, unsigned long long e) {
     a.index[row * a.k + rank] = (long)(int)~(unsigned)e;
-    a.logp[row * a.k + rank] = key_value((unsigned)(e >> 32)) * a.scale - lse;
+    a.logp[row * a.k + rank] = (key_value((unsigned)(e >> 32)) - ms.x) * a.scale - log_sum;
   };
   if (n <= 512) {  // place = number of larger entries
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
@@ -329,16 +329,17 @@ __global__ void __launch_bounds__(THREADS, 4) top_kernel(const T* __restrict__ l
       s *= m == -INFINITY ? 0.f : ex2((m - top) * c);
       m = top;
     }
-    const float mc = m == -INFINITY ? 0.f : -m * c;
+    // c (f - m) and not c f - c m: a mask of the type's lowest value times c is beyond fp32
+    const float less = m == -INFINITY ? 0.f : -m;
     float2 sum = make_float2(0.f, 0.f);
-    const float2 c2 = make_float2(c, c), mc2 = make_float2(mc, mc);
+    const float2 c2 = make_float2(c, c), less2 = make_float2(less, less);
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
       float f[VEC];
       unpack(u[b], f);
 #pragma unroll
       for (int j = 0; j < VEC; j += 2) {
-        const float2 y = fma2(make_float2(f[j], f[j + 1]), c2, mc2);
+        const float2 y = mul2(add2(make_float2(f[j], f[j + 1]), less2), c2);
         sum = add2(sum, make_float2(ex2(y.x), ex2(y.y)));
       }
     }

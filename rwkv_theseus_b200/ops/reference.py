@@ -138,4 +138,6 @@ def top_log_probs(logits, k, scale):
     """k largest log-probabilities of softmax(scale * logits) and their indices, equal logits by the lowest index."""
     z = logits.float() if logits.dtype != torch.float64 else logits
     index = torch.sort(z, dim=-1, descending=True, stable=True)[1][..., :k]
-    return torch.log_softmax(z * scale, -1).gather(-1, index), index
+    wide = z.double()  # masks of the lowest value leave fp32's range when they are scaled
+    below = (wide - wide.amax(-1, keepdim=True)) * scale
+    return torch.log_softmax(below, -1).gather(-1, index).to(z.dtype), index

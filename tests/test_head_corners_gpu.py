@@ -1,5 +1,5 @@
 """Corners of the vocabulary-head operators on the GPU against 64-bit formulas: students that are sure of their record,
-records of the whole vocabulary.
+records of the whole vocabulary, masks of the type's lowest value.
 
 Tolerances are those of test_head_losses_gpu.py (u = 2^-8; a gradient is off by (3 u + 4 dz) times the same product of
 absolute values, dz the bound of a logit's error) unless a test derives its own.
@@ -9,6 +9,7 @@ import math
 import pytest
 import torch
 
+from rwkv_theseus_b200.losses import top_log_probs
 from test_head_losses_gpu import _check, _inputs, _record
 
 pytestmark = pytest.mark.gpu
@@ -54,3 +55,28 @@ def test_a_record_of_the_whole_vocabulary_without_all_its_mass(T, V):
     _check(hidden, weight, index, log_probs + math.log(0.6), 1.0, True, "mean")
     log_probs[:, 1:3] = -math.inf
     _check(hidden, weight, index, log_probs, 1.0, True, "none")
+
+
+@cuda
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [700, 20011, 248077])
+@pytest.mark.parametrize("temperature", [0.5, 1.0, 2.0])
+def test_top_log_probs_of_masks_of_the_lowest_value(dtype, V, temperature):
+    """Logits masked by the type's lowest number: most of a row, all but one entry, all of it, and beside the largest.
+    Expected in 64 bits, rounded to fp32 (a masked entry may be -inf there); the bound is that of test_head_losses_gpu.py
+    for the unmasked logits, and the magnitude's rounding for the masked ones."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    logits = torch.randn(6, V, device="cuda", generator=g).mul_(3).to(dtype)
+    logits[0, : V // 2] = low
+    logits[1, 20:] = low
+    logits[2, 1:] = low
+    logits[3] = low
+    logits[4, 7] = high
+    logits[5, ::2], logits[5, 1::2] = low, -math.inf
+    got, index = top_log_probs(logits, 30, temperature)
+    z = logits.double()
+    order = torch.sort(z, dim=-1, descending=True, stable=True)[1][:, :30]
+    expected = torch.log_softmax(z / temperature, -1).gather(1, order).float()
+    assert torch.equal(index, order)
+    torch.testing.assert_close(got, expected, rtol=2.0 ** -21, atol=8 * 2.0 ** -24 * (20 / temperature + 32))
