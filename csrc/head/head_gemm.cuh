@@ -86,6 +86,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// A tile's maximum m in units of log2, rounded up: fmaf(v, scale2, -m2) is then never above 0 for v <= m, where depth()
+// would wrap around (rounded to nearest it is, from logits of 1e4 on). 0 for a tile of -inf.
+__device__ __forceinline__ float tile_top(float m, float scale2) {
+  return m == -INFINITY ? 0.f : __fmul_ru(m, scale2);
+}
+
 // A logit t <= 0 octaves (units of log2) from its tile's maximum as a 16-bit number of 1/512 octaves: the exponential
 // it stands for is off by 7e-4 at most, a fifth of bf16's rounding, down to 2^-128. Here as the low half of an fp32
 // word (2^23 + depth, so that one fused multiply-add rounds).
@@ -413,7 +419,7 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) t[i] = v[i];
           const float m = columns(t, lane, [](float a, float b) { return fmaxf(a, b); });
-          const float m2 = m == -INFINITY ? 0.f : m * args.scale2;
+          const float m2 = tile_top(m, args.scale2);
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             v[i] = fmaf(v[i], args.scale2, -__shfl_sync(~0u, m2, i));
@@ -447,7 +453,7 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) m = fmaxf(m, v[i]);
         }
-        const float m2 = m == -INFINITY ? 0.f : m * args.scale2;
+        const float m2 = tile_top(m, args.scale2);
         float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll 1
         for (int c = 0; c < 8; c += 2) {

@@ -1,5 +1,5 @@
 """Corners of the vocabulary-head operators on the GPU against 64-bit formulas: students that are sure of their record,
-records of the whole vocabulary, masks of the type's lowest value.
+records of the whole vocabulary, logits of any size, masks of the type's lowest value.
 
 Tolerances are those of test_head_losses_gpu.py (u = 2^-8; a gradient is off by (3 u + 4 dz) times the same product of
 absolute values, dz the bound of a logit's error) unless a test derives its own.
@@ -9,8 +9,8 @@ import math
 import pytest
 import torch
 
-from rwkv_theseus_b200.losses import top_log_probs
-from test_head_losses_gpu import _check, _inputs, _record
+from rwkv_theseus_b200.losses import linear_cross_entropy, top_log_probs
+from test_head_losses_gpu import U, _check, _inputs, _record
 
 pytestmark = pytest.mark.gpu
 cuda = pytest.mark.skipif(not torch.cuda.is_available(), reason="CUDA unavailable")
@@ -58,13 +58,34 @@ def test_a_record_of_the_whole_vocabulary_without_all_its_mass(T, V):
 
 
 @cuda
+@pytest.mark.parametrize("T", [20, 100, 150])
+def test_the_largest_of_very_large_logits(T):
+    """Two equal logits share each row, one of them its target; all others are far below. They are exact (one product
+    and zeros), so the other one's gradient is 1/2 up to the 16-bit form of its logit (2^-10 octaves, 7e-4) and two
+    roundings to bf16."""
+    hidden = torch.zeros(T, 64, device="cuda")
+    hidden[:, 0] = torch.linspace(8192, 32000, T, device="cuda").to(torch.bfloat16)
+    weight = torch.zeros(600, 64, device="cuda")
+    weight[5, 0], weight[300, 0], weight[300, 1] = 1.0, 1.0, 1.0
+    hidden = hidden.to(torch.bfloat16).requires_grad_()
+    weight = weight.to(torch.bfloat16).requires_grad_()
+    loss = linear_cross_entropy(hidden, weight, torch.full((T,), 5, device="cuda"), reduction="sum")
+    dh, dw = torch.autograd.grad(loss, (hidden, weight))
+    half = torch.full((T,), 0.5, device="cuda", dtype=torch.float64)
+    torch.testing.assert_close(dh[:, 1].double(), half, rtol=0, atol=0.5 * (7e-4 + 2 * U))
+    half = 0.5 * hidden[:, 0].detach().double().sum()
+    torch.testing.assert_close(dw[300, 0].double(), half, rtol=7e-4 + 2 * U, atol=0)
+    torch.testing.assert_close(dw[5, 0].double(), -half, rtol=7e-4 + 2 * U, atol=0)
+
+
+@cuda
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("V", [700, 20011, 248077])
 @pytest.mark.parametrize("temperature", [0.5, 1.0, 2.0])
 def test_top_log_probs_of_masks_of_the_lowest_value(dtype, V, temperature):
     """Logits masked by the type's lowest number: most of a row, all but one entry, all of it, and beside the largest.
-    Expected in 64 bits, rounded to fp32 (a masked entry may be -inf there); the bound is that of test_head_losses_gpu.py
-    for the unmasked logits, and the magnitude's rounding for the masked ones."""
+    Expected in 64 bits, rounded to fp32 (a masked entry may be -inf there); the bound is that of
+    test_head_losses_gpu.py for the unmasked logits, and the magnitude's rounding for the masked ones."""
     g = torch.Generator(device="cuda").manual_seed(V)
     low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
     logits = torch.randn(6, V, device="cuda", generator=g).mul_(3).to(dtype)
