@@ -312,7 +312,7 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
     const double lse = l2 * LN2;
     const double r1 = p.tail_class && P < 1. && !(rest <= 0.f) ? 1. - P : 0.;  // an empty rest has no class
     const double weight = P + r1;
-    double a = weight, value = L + P * lse, base = l2;
+    double a = Z == Z ? weight : NAN, value = L + P * lse, base = l2;  // NaN logits: also where a tile has no maximum
     if (r1 > 0.) {
       base = (double)m + log2((double)rest);
       const double lr = base * LN2 - lse;  // log of the student's rest

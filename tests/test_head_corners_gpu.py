@@ -1,5 +1,5 @@
 """Corners of the vocabulary-head operators on the GPU against 64-bit formulas: students that are sure of their record,
-records of the whole vocabulary, logits of any size, masks of the type's lowest value.
+records of the whole vocabulary, logits of any size, masks of the type's lowest value, NaN.
 
 Tolerances are those of test_head_losses_gpu.py (u = 2^-8; a gradient is off by (3 u + 4 dz) times the same product of
 absolute values, dz the bound of a logit's error) unless a test derives its own.
@@ -101,3 +101,16 @@ def test_top_log_probs_of_masks_of_the_lowest_value(dtype, V, temperature):
     expected = torch.log_softmax(z / temperature, -1).gather(1, order).float()
     assert torch.equal(index, order)
     torch.testing.assert_close(got, expected, rtol=2.0 ** -21, atol=8 * 2.0 ** -24 * (20 / temperature + 32))
+
+
+@cuda
+@pytest.mark.parametrize("T", [20, 150])
+def test_a_weight_without_numbers(T):
+    """Logits that are NaN have NaN gradients, held or not."""
+    hidden, weight, targets, _ = _inputs(T, 700, 64)
+    weight[:, 3] = math.nan
+    hidden.requires_grad_()
+    weight.requires_grad_()
+    loss = linear_cross_entropy(hidden, weight, targets)
+    dh, dw = torch.autograd.grad(loss, (hidden, weight))
+    assert torch.isnan(loss) and torch.isnan(dh).all() and torch.isnan(dw).all()
