@@ -109,12 +109,13 @@ def attention(q, k_all, v_all, offset):
 def head_loss(hidden, weight, index, log_probs, ignore, scale, tail, reduction):
     """Vocabulary-head loss against a record (see ``losses.linear_topk_kl``), in fp32 (fp64 for fp64 operands)."""
     wide = torch.float64 if hidden.dtype == torch.float64 else torch.float32
-    z = (hidden.to(wide) @ weight.to(wide).t()) * scale
-    log_q = z - z.logsumexp(-1, keepdim=True)
     held = (index != ignore) if log_probs is None else (index >= 0)
     if bool((held & ((index < 0) | (index >= weight.shape[0]))).any()):
         raise IndexError(f"vocabulary index outside 0..{weight.shape[0] - 1}")
     valid = held.any(-1)
+    # what a row without an entry holds never meets the weight, whose gradient it would make NaN
+    z = (hidden.to(wide).masked_fill(~valid[..., None], 0.0) @ weight.to(wide).t()) * scale
+    log_q = z - z.logsumexp(-1, keepdim=True)
     logp = torch.zeros(index.shape, dtype=wide, device=z.device) if log_probs is None else log_probs.to(wide)
     logp = logp.masked_fill(~held, float("-inf"))
     p = logp.exp()
