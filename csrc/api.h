@@ -93,6 +93,9 @@ struct RtHeadLoss {
 };
 long rt_head_loss_workspace_floats(long rows, long vocab, int width, int K, int grad_h, int grad_w);
 cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream_t stream);
+// With the caller's status word: set to 1 by a product that gives up a bounded wait, never cleared, and while it is set
+// the losses, dhidden and the first 16 bytes of dweight are NaN (without it the call keeps its own).
+cudaError_t rt_head_loss_status(const RtHeadLoss* p, float* work, int* status, cudaStream_t stream);
 cudaError_t rt_scale_bf16(void* const x[2], const long n[2], const float* factor, cudaStream_t stream);
 cudaError_t rt_top_log_probs(int dtype, const void* logits, long rows, long V, long ld, int k, float scale,
                              float* logp, long* index, void* work, cudaStream_t stream);

@@ -73,7 +73,7 @@ struct Args {
   float* dx;        // DX_N: the partial sums
   int add;          // DW32: add to what is there
   int* status;
-  uint4* poison;    // DW: the gradient's first 16 bytes, NaN if a wait gave up
+  uint4* poison;    // DW: the gradient's first 16 bytes, NaN if a wait of this or of an earlier product gave up
 };
 
 struct Maps {
@@ -529,9 +529,16 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
     sm100::tc_fence_after();
     sm100::tmem_dealloc_pair(tmem_base, C_::TMEM_COLS);
   }
-  if (threadIdx.x == 0 && *abort) {
-    atomicExch(args.status, 1);
-    if (MODE == DW) *args.poison = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+  if (threadIdx.x == 0) {
+    const bool gave_up = *abort;
+    if (gave_up) atomicExch(args.status, 1);
+    if (MODE == DW && (gave_up || blockIdx.x == 0)) {
+      // Block 0 has stored the tile with these bytes. It looks at the status after that, and a block that gave up sets
+      // the status before it writes them: whichever comes last leaves NaN.
+      __threadfence();
+      if (gave_up || *reinterpret_cast<volatile int*>(args.status))
+        *args.poison = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+    }
   }
 }
 

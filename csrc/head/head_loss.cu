@@ -20,8 +20,8 @@
 // That is 6 T V C operations, against 8 T V C where the logits are formed a second time, for T V 16-bit values of
 // workspace; CHUNK_VALUES bounds it, and more rows run in chunks whose dW adds up in fp32. Rows without a loss cost
 // nothing but their packing, and what they hold never meets the other rows. The cross entropy of a few rows without
-// gradients is not packed and takes two launches. A product that gave up a bounded wait leaves NaN in the losses, or in
-// the gradient it was forming.
+// gradients is not packed and takes two launches. A product that gave up a bounded wait leaves NaN in all that is
+// formed after it: the losses, dX, and the first 16 bytes of dW.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -53,8 +53,8 @@ __global__ void kinds_kernel(const long* __restrict__ idx, long rows, int K, lon
   if ((threadIdx.x & 31) == 0) kind[row] = row_kind(any);
 }
 
-// What the rows' losses and gradients are taken over: valid rows, rows with a loss, a product that gave up a wait, and
-// blocks of merge_kernel that are done.
+// What the rows' losses and gradients are taken over: valid rows, rows with a loss, a product that gave up a wait
+// (where the caller has no status word), and blocks of merge_kernel that are done.
 struct Counts {
   int valid, counted, failed, done;
 };
@@ -229,6 +229,7 @@ struct MergeArgs {
   int blocks;  // of all chunks
   long all_rows;
   Counts* counts;
+  const int* failed;  // a product gave up a wait
   const int* row_of;
   const int* sidx;
   const float* slogp;
@@ -321,7 +322,7 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
     }
     const float g = p.scale * (p.grad ? p.grad[row] : (p.mean ? 1.f / (float)max(p.counts->counted, 1) : 1.f));
     if (lane == 0) {
-      p.row_loss[row] = p.counts->failed ? NAN : (float)value;
+      p.row_loss[row] = *p.failed ? NAN : (float)value;
       p.base2[place] = (float)base;
       p.tail[place] = g * (float)a;
     }
@@ -380,6 +381,7 @@ struct ScoreArgs {
   int C;
   float scale2;
   Counts* counts;
+  const int* failed;
   float* row_loss;
   float* loss;
 };
@@ -420,7 +422,7 @@ __global__ void __launch_bounds__(MERGE_THREADS + 32) score_kernel(const ScoreAr
       const float z2 = target_z2, peak = fmaxf(all.x, z2);
       const double Z = exp2((double)z2 - (double)peak) +
                        (all.x == -INFINITY ? all.y : all.y * exp2((double)all.x - (double)peak));
-      if (!p.counts->failed) value = (float)(((double)peak + log2(Z)) * LN2 - (double)z2 * LN2);
+      if (!*p.failed) value = (float)(((double)peak + log2(Z)) * LN2 - (double)z2 * LN2);
     }
     if (lane == 0) p.row_loss[row] = value;
   }
@@ -501,15 +503,16 @@ __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict
 // dhidden[row_of[place]] = bf16 of the row's partial sums, added in order.
 __global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ partial, int splits, long split_rows,
                                                       int C, int row0, int rows, const Counts* __restrict__ counts,
-                                                      const int* __restrict__ row_of, __nv_bfloat16* __restrict__ out) {
+                                                      const int* failed, const int* __restrict__ row_of,
+                                                      __nv_bfloat16* __restrict__ out) {
   const int n = min(max(counts->valid - row0, 0), rows), r = blockIdx.x;
   if (r >= n) return;
-  const float failed = counts->failed ? NAN : 0.f;  // a product gave up a wait
+  const float from = *failed ? NAN : 0.f;  // a product gave up a wait
   uint4* dst = reinterpret_cast<uint4*>(out + (long)row_of[row0 + r] * C);
   for (int c = threadIdx.x; c < C / 8; c += blockDim.x) {
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = failed;
+    for (int j = 0; j < 8; ++j) v[j] = from;
     for (int s = 0; s < splits; ++s) {
       const float4* src = reinterpret_cast<const float4*>(partial + ((long)s * split_rows + r) * C) + 2 * c;
       const float4 x = __ldg(src), y = __ldg(src + 1);
@@ -520,9 +523,9 @@ __global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ 
   }
 }
 
-// The weight's gradient of a product that gave up a wait (the one-chunk kernel leaves its NaN itself).
-__global__ void failed_kernel(const Counts* __restrict__ counts, __nv_bfloat16* __restrict__ dweight) {
-  if (counts->failed && threadIdx.x < 8) dweight[threadIdx.x] = __float2bfloat16_rn(NAN);
+// The weight's gradient where a product gave up a wait (the one-chunk kernel leaves its NaN itself).
+__global__ void failed_kernel(const int* failed, __nv_bfloat16* __restrict__ dweight) {
+  if (*failed && threadIdx.x < 8) dweight[threadIdx.x] = __float2bfloat16_rn(NAN);
 }
 
 // x *= *factor for up to two tensors, nothing at all for a factor of one (the usual upstream gradient of a loss).
@@ -669,6 +672,10 @@ extern "C" long rt_head_loss_workspace_floats(long rows, long V, int C, int K, i
 }
 
 extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream_t s) {
+  return rt_head_loss_status(p, work, nullptr, s);
+}
+
+extern "C" cudaError_t rt_head_loss_status(const RtHeadLoss* p, float* work, int* status, cudaStream_t s) {
   if (!p || !work) return cudaErrorInvalidValue;
   const long T = p->rows, V = p->vocab;
   const int C = p->width, K = p->K;
@@ -687,6 +694,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   const Layout l = layout(T, V, C, K, p->dhidden != nullptr, p->dweight != nullptr);
   auto ints = [&](long at) { return reinterpret_cast<int*>(work + at); };
   Counts* counts = reinterpret_cast<Counts*>(work + l.counts);
+  int* failed = status ? status : &counts->failed;
   __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(work + l.x);
   __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(work + l.e);
   float2* part = reinterpret_cast<float2*>(work + l.part);
@@ -704,7 +712,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
     args.part_ld = l.part_ld;
     args.targets = p->index;
     args.counts = &counts->valid;
-    args.status = &counts->failed;
+    args.status = failed;
     if (!map2d(&maps.a, false, p->weight, C, V, 2 * p->ld_weight, 128) ||
         !map2d(&maps.b, false, p->hidden, C, T, 2 * p->ld_hidden, few ? 16 : 64) ||
         !map2d(&maps.out, false, p->hidden, C, T, 2 * p->ld_hidden, 32))
@@ -714,7 +722,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
     const ScoreArgs score{part, l.part_ld, (int)l.groups, p->reduction == 2, p->index, p->ignore, V,
                           reinterpret_cast<const __nv_bfloat16*>(p->hidden), p->ld_hidden,
                           reinterpret_cast<const __nv_bfloat16*>(p->weight), p->ld_weight, C, scale2, counts,
-                          p->row_loss, p->reduction ? p->loss : nullptr};
+                          failed, p->row_loss, p->reduction ? p->loss : nullptr};
     score_kernel<<<(unsigned)T, MERGE_THREADS + 32, 0, s>>>(score);
     return cudaGetLastError();
   }
@@ -749,7 +757,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   args.store_e = grad;
   args.splits = (int)std::max(1L, l.splits);
   args.split_rows = (int)l.split_rows;
-  args.status = &counts->failed;
+  args.status = failed;
   int merge_blocks = 0;
   for (long row0 = 0; row0 < T; row0 += l.rows)
     merge_blocks += (int)(std::min(l.rows, up(T - row0, 64)) / (narrow ? 1 : 4));  // multiples of 64
@@ -770,8 +778,9 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
                    : narrow ? launch<head::LOGITS_N, 128>(logits, args, l.tiles, s)
                             : launch<head::LOGITS>(logits, args, tiles_m * l.tiles, s)));
     MergeArgs m{part, l.part_ld, (int)l.groups, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, merge_blocks, T,
-                counts, ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->scale, p->row_grad, p->row_loss,
-                p->reduction ? p->loss : nullptr, work + l.base2, work + l.tail, grad ? work + l.coef : nullptr};
+                counts, failed, ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->scale, p->row_grad,
+                p->row_loss, p->reduction ? p->loss : nullptr, work + l.base2, work + l.tail,
+                grad ? work + l.coef : nullptr};
     if (narrow) merge_kernel<1><<<(unsigned)rows, MERGE_THREADS, 0, s>>>(m);
     else merge_kernel<4><<<(unsigned)(rows + 3) / 4, MERGE_THREADS, 0, s>>>(m);
     if (grad)
@@ -788,7 +797,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
                      : narrow ? launch<head::DX_N, 128>(dx, args, tiles_c * l.splits, s)
                               : launch<head::DX>(dx, args, tiles_m * tiles_c * l.splits, s)));
       dhidden_kernel<<<(unsigned)rows, 256, 0, s>>>(work + l.dx, (int)l.splits, l.split_rows, C, (int)row0, (int)l.rows,
-                                                    counts, ints(l.row_of),
+                                                    counts, failed, ints(l.row_of),
                                                     reinterpret_cast<__nv_bfloat16*>(p->dhidden));
     }
     if (p->dweight) {
@@ -803,7 +812,7 @@ extern "C" cudaError_t rt_head_loss(const RtHeadLoss* p, float* work, cudaStream
   }
   if (l.dw32) {
     RT_CUDA_CHECK(rt_to_bf16(work + l.dw, p->dweight, V * C, s));
-    failed_kernel<<<1, 32, 0, s>>>(counts, reinterpret_cast<__nv_bfloat16*>(p->dweight));
+    failed_kernel<<<1, 32, 0, s>>>(failed, reinterpret_cast<__nv_bfloat16*>(p->dweight));
   }
   return cudaGetLastError();
 }

@@ -4,6 +4,7 @@ records of the whole vocabulary, logits of any size, masks of the type's lowest 
 Tolerances are those of test_head_losses_gpu.py (u = 2^-8; a gradient is off by (3 u + 4 dz) times the same product of
 absolute values, dz the bound of a logit's error) unless a test derives its own.
 """
+import ctypes
 import math
 
 import pytest
@@ -114,3 +115,52 @@ def test_a_weight_without_numbers(T):
     loss = linear_cross_entropy(hidden, weight, targets)
     dh, dw = torch.autograd.grad(loss, (hidden, weight))
     assert torch.isnan(loss) and torch.isnan(dh).all() and torch.isnan(dw).all()
+
+
+class _Call(ctypes.Structure):
+    """RtHeadLoss of csrc/api.h."""
+    _fields_ = [("hidden", ctypes.c_void_p), ("ld_hidden", ctypes.c_long), ("weight", ctypes.c_void_p),
+                ("ld_weight", ctypes.c_long), ("index", ctypes.c_void_p), ("log_probs", ctypes.c_void_p),
+                ("rows", ctypes.c_long), ("vocab", ctypes.c_long), ("width", ctypes.c_int), ("K", ctypes.c_int),
+                ("ignore", ctypes.c_long), ("scale", ctypes.c_float), ("tail", ctypes.c_int),
+                ("reduction", ctypes.c_int), ("row_grad", ctypes.c_void_p), ("row_loss", ctypes.c_void_p),
+                ("loss", ctypes.c_void_p), ("dhidden", ctypes.c_void_p), ("dweight", ctypes.c_void_p)]
+
+
+@cuda
+@pytest.mark.parametrize("T,grad_h,grad_w", [(5, False, False), (5, True, True), (5, False, True), (150, True, True),
+                                             (150, False, True), (33000, False, True)])
+def test_a_product_that_gave_up_a_wait_leaves_nan(T, grad_h, grad_w):
+    """The status word as such a product leaves it, set before the call: no number comes back that looks like a result.
+    Unset, the entry does what the public function does. (No kernel is kept waiting here.)"""
+    from rwkv_theseus_b200.ops import native
+    lib = ctypes.CDLL(native().__file__)
+    floats = lib.rt_head_loss_workspace_floats
+    floats.restype, floats.argtypes = ctypes.c_long, [ctypes.c_long] * 2 + [ctypes.c_int] * 4
+    run = lib.rt_head_loss_status
+    run.argtypes = [ctypes.c_void_p] * 4
+    hidden, weight, targets, _ = _inputs(T, 300, 64)
+    targets[1] = -100
+    live = targets != -100
+    rows, loss = torch.empty(T, device="cuda"), torch.empty((), device="cuda")
+    dh, dw = torch.empty_like(hidden), torch.empty_like(weight)
+    work = torch.empty(floats(T, 300, 64, 1, grad_h, grad_w), device="cuda")
+    for fault in (0, 1):
+        status = torch.full((1,), fault, device="cuda", dtype=torch.int32)
+        call = _Call(hidden.data_ptr(), 64, weight.data_ptr(), 64, targets.data_ptr(), None, T, 300, 64, 1, -100,
+                     1.0, 0, 2, None, rows.data_ptr(), loss.data_ptr(), dh.data_ptr() if grad_h else None,
+                     dw.data_ptr() if grad_w else None)
+        assert run(ctypes.byref(call), work.data_ptr(), status.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert status.item() == fault
+        if fault:
+            assert torch.isnan(loss) and torch.isnan(rows[live]).all()
+            assert not grad_h or torch.isnan(dh[live]).all()
+            assert not grad_w or torch.isnan(dw[0, :8]).all()
+        else:
+            h, w = hidden.clone().requires_grad_(grad_h), weight.clone().requires_grad_(grad_w)
+            expected = linear_cross_entropy(h, w, targets)
+            assert torch.equal(loss, expected.detach())
+            wanted = [(h, dh)] * grad_h + [(w, dw)] * grad_w
+            for (_, got), grad in zip(wanted, torch.autograd.grad(expected, [t for t, _ in wanted]) if wanted else ()):
+                assert torch.equal(got, grad)
