@@ -12,6 +12,7 @@
 // the 11 that the bandwidth leaves). Several blocks per SM, so that one streams while another selects. Few rows are cut
 // into segments over as many blocks, whose k candidates a second kernel merges.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include "../api.h"
 #include "../common/common.cuh"
@@ -533,10 +534,16 @@ __global__ void __launch_bounds__(MERGE_THREADS) top_merge_kernel(const TopArgs 
   write_row(a, row, list, found, ms);
 }
 
-int capacity_for(int k) {
+constexpr int capacity_for(int k) {
   int c = 1024;
   while (c < 4 * k) c <<= 1;
   return c;
+}
+// Dynamic shared memory of a block whose segment has `vecs` vectors.
+template <typename T, int U>
+constexpr size_t smem_for(int capacity, long vecs) {
+  const long steps = (vecs + BATCH * THREADS - 1) / (BATCH * THREADS);
+  return (size_t)capacity * 8 + (size_t)steps * THREADS * (U == 1 ? BATCH : 1) * sizeof(typename Key<T>::type);
 }
 
 // Segments of a row. One block takes a row of 32003 values in 10 us and of 248077 in 20 us, and merging segments costs
@@ -554,11 +561,18 @@ template <typename T, int U>
 cudaError_t launch(const T* logits, long rows, const TopArgs& a, cudaStream_t s) {
   constexpr int VEC = 16 / sizeof(T);
   const long longest = (a.V + a.segments - 1) / a.segments;
-  const long steps = (longest / VEC + BATCH * THREADS - 1) / (BATCH * THREADS);
-  const size_t smem = (size_t)a.capacity * 8 + (size_t)steps * THREADS * (U == 1 ? BATCH : 1) *
-                                                   sizeof(typename Key<T>::type);
-  if (smem > 40 * 1024)  // 48 KB without asking, static arrays included
-    RT_CUDA_CHECK(cudaFuncSetAttribute(top_kernel<T, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const size_t smem = smem_for<T, U>(a.capacity, longest / VEC);
+  // The longest segment and record; the limit belongs to the device and not to the call, so it is raised once.
+  constexpr size_t most = smem_for<T, U>(capacity_for(RT_HEAD_MAX_RECORD), (long)MAX_KEYS * (U == 1 ? 1 : BATCH) + 1);
+  if (smem > most) return cudaErrorInvalidValue;
+  static std::atomic<uint64_t> set{0};  // devices
+  int dev = 0;
+  RT_CUDA_CHECK(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!bit || !(set.load(std::memory_order_acquire) & bit)) {
+    RT_CUDA_CHECK(cudaFuncSetAttribute(top_kernel<T, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+    set.fetch_or(bit, std::memory_order_acq_rel);
+  }
   for (long r = 0; r < rows; r += 65535) {
     const long some = std::min(rows - r, 65535L);
     TopArgs b = a;

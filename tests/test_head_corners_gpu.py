@@ -6,6 +6,7 @@ absolute values, dz the bound of a logit's error) unless a test derives its own.
 """
 import ctypes
 import math
+import threading
 
 import pytest
 import torch
@@ -164,3 +165,31 @@ def test_a_product_that_gave_up_a_wait_leaves_nan(T, grad_h, grad_w):
             wanted = [(h, dh)] * grad_h + [(w, dw)] * grad_w
             for (_, got), grad in zip(wanted, torch.autograd.grad(expected, [t for t, _ in wanted]) if wanted else ()):
                 assert torch.equal(got, grad)
+
+
+@cuda
+def test_top_log_probs_from_two_threads():
+    """Records of different lengths at once: a launch's shared memory is not what the other thread last asked for."""
+    from rwkv_theseus_b200.ops import native
+    run = ctypes.CDLL(native().__file__).rt_top_log_probs
+    long, pointer = ctypes.c_long, ctypes.c_void_p
+    run.argtypes = [ctypes.c_int, pointer, long, long, long, ctypes.c_int, ctypes.c_float] + [pointer] * 4
+    V = 32003
+    logits = torch.randn(2, V, device="cuda")
+    codes = {}
+
+    def call(k):
+        values = torch.empty(2, k, device="cuda")
+        index = torch.empty(2, k, device="cuda", dtype=torch.int64)
+        stream = torch.cuda.Stream()
+        codes[k] = {run(0, logits.data_ptr(), 2, V, V, k, 1.0, values.data_ptr(), index.data_ptr(), None,
+                        stream.cuda_stream) for _ in range(3000)}
+        stream.synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=call, args=(k,)) for k in (200, 1024)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert codes == {200: {0}, 1024: {0}}
