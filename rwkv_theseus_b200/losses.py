@@ -59,6 +59,12 @@ def kl_sum(student_logits, teacher_logits):
     return (teacher.exp() * (teacher - student)).sum()
 
 
+def _check_temperature(temperature):
+    """Its inverse times a logit has to stay in fp32's range, and a mask of -inf has to stay one."""
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"temperature must be positive (1e-30 to 1e30), got {temperature}")
+
+
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
@@ -113,8 +119,7 @@ def linear_topk_kl(hidden, weight, indices, log_probs, temperature=1.0, tail=Tru
         raise ValueError(f"a record holds 1 to 1024 entries per token, got {tuple(indices.shape)}")
     if not log_probs.is_floating_point():
         raise TypeError("log_probs must be floating point")
-    if not temperature > 0:
-        raise ValueError("temperature must be positive")
+    _check_temperature(temperature)
     return _head_loss(hidden, weight, indices, log_probs.detach(), -1, 1.0 / temperature, tail, reduction)
 
 
@@ -124,8 +129,7 @@ def top_log_probs(logits, k, temperature=1.0):
     are bf16 or fp32 and k is at most 1024."""
     if logits.dim() < 1 or not 1 <= k <= min(logits.shape[-1], 1024):
         raise ValueError(f"k must be in 1..min(V, 1024), got {k} for logits {tuple(logits.shape)}")
-    if not temperature > 0:
-        raise ValueError("temperature must be positive")
+    _check_temperature(temperature)
     if logits.is_cuda:
         if logits.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("top_log_probs takes bf16 or fp32 logits on CUDA")

@@ -42,3 +42,14 @@ def test_masked_rows_hold_anything(dtype, value):
         for a, b in zip(*results):
             assert torch.equal(a, b)
         assert not results[1][1][masked].any()
+
+
+@pytest.mark.parametrize("temperature", [math.inf, math.nan, 1e-31, 1e31])
+def test_temperatures_that_leave_no_scale(temperature):
+    """1 / temperature times a logit has to stay a number of fp32's range (at infinity 0 x -inf is none)."""
+    hidden, weight = torch.randn(3, 8), torch.randn(20, 8)
+    log_probs, indices = top_log_probs(torch.randn(3, 20), 4)
+    with pytest.raises(ValueError, match="temperature"):
+        linear_topk_kl(hidden, weight, indices, log_probs, temperature)
+    with pytest.raises(ValueError, match="temperature"):
+        top_log_probs(torch.randn(3, 20), 4, temperature)
