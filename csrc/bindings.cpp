@@ -478,6 +478,9 @@ at::Tensor kl_rows(at::Tensor student, at::Tensor teacher) {
   return out;
 }
 
+// A dual tensor of forward-mode differentiation (level 0 is the only one there is).
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
+
 // ---- vocabulary-head losses (see RtHeadLoss). index [..., K] with log_probs like it, or targets [...] without.
 struct HeadLossCall {
   int64_t ignore;
@@ -605,6 +608,7 @@ struct HeadLossFunction : public torch::autograd::Function<HeadLossFunction> {
 at::Tensor head_loss(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& index,
                      const c10::optional<at::Tensor>& log_probs, int64_t ignore, double scale, bool tail,
                      int64_t reduction) {
+  TORCH_CHECK(!has_tangent(hidden) && !has_tangent(weight), "the head losses have no forward-mode derivative");
   const bool on = at::GradMode::is_enabled(), grad_h = on && hidden.requires_grad(),
              grad_w = on && weight.requires_grad();
   if (!grad_h && !grad_w)
@@ -616,6 +620,7 @@ at::Tensor head_loss(const at::Tensor& hidden, const at::Tensor& weight, const a
 // The k largest log-probabilities of softmax(scale * logits) over the last axis and their indices, largest first, equal
 // logits by the lowest index.
 std::tuple<at::Tensor, at::Tensor> top_log_probs(const at::Tensor& logits, int64_t k, double scale) {
+  TORCH_CHECK(!has_tangent(logits), "top_log_probs has no forward-mode derivative");
   TORCH_CHECK(logits.is_cuda() && logits.dim() >= 1, "top_log_probs: CUDA logits [..., V]");
   c10::cuda::CUDAGuard guard(logits.device());
   const int dtype = dtype_code(logits);

@@ -10,6 +10,7 @@ import threading
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from rwkv_theseus_b200.losses import linear_cross_entropy, top_log_probs
 from test_head_losses_gpu import U, _check, _inputs, _record
@@ -193,3 +194,18 @@ def test_top_log_probs_from_two_threads():
     for thread in threads:
         thread.join()
     assert codes == {200: {0}, 1024: {0}}
+
+
+@cuda
+def test_forward_mode_derivatives_are_refused():
+    """A tangent is not dropped without a word, whether or not the tensor also wants a gradient."""
+    hidden, weight, targets, _ = _inputs(5, 300, 64)
+    with forward_ad.dual_level():
+        h, w = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (hidden, weight))
+        learning = forward_ad.make_dual(hidden.clone().requires_grad_(), torch.ones_like(hidden))
+        for pair in ((h, weight), (hidden, w), (learning, weight)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                linear_cross_entropy(*pair, targets)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            top_log_probs(h, 3)
+    assert torch.isfinite(linear_cross_entropy(hidden, weight, targets))
