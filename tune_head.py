@@ -44,8 +44,8 @@ def run(checkpoint, output, steps, chunks=32, top=64, temperature=1.0, kl_weight
     before, tokens = score(runner, held_out, device)
     losses = tune_head(model, train, states, records, device, steps, lr, kl_weight, temperature)
     after = score(runner, held_out, device)[0]
-    report = {"tokens": tokens, "teacher": teacher, "before": before, "after": after, "first_loss": losses[0],
-              "last_loss": losses[-1]}
+    report = {"tokens": tokens, "teacher": teacher, "before": before, "after": after,
+              "first_loss": losses[0] if losses else None, "last_loss": losses[-1] if losses else None}
     if output:
         save_export(model.cpu(), output, cfg, meta["order"], meta["base_fingerprint"], checkpoint=directory)
     return report
@@ -55,7 +55,7 @@ def main(argv=None):
     p = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     p.add_argument("--checkpoint", required=True, help="complete checkpoint, its run directory or 'latest'")
     p.add_argument("--output", help="directory of the export (omit to report only)")
-    p.add_argument("--steps", type=int, default=200)
+    p.add_argument("--steps", type=int, default=200, help="0: the scores alone")
     p.add_argument("--chunks", type=int, default=32, help="training chunks to record and tune on")
     p.add_argument("--top", type=int, default=64, help="recorded log-probabilities per token")
     p.add_argument("--temperature", type=float, default=1.0)
