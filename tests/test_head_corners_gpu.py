@@ -12,8 +12,8 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from rwkv_theseus_b200.losses import linear_cross_entropy, top_log_probs
-from test_head_losses_gpu import U, _check, _inputs, _record
+from rwkv_theseus_b200.losses import linear_cross_entropy, linear_topk_kl, top_log_probs
+from test_head_losses_gpu import U, _check, _inputs, _oracle, _record, _within
 
 pytestmark = pytest.mark.gpu
 cuda = pytest.mark.skipif(not torch.cuda.is_available(), reason="CUDA unavailable")
@@ -209,3 +209,92 @@ def test_forward_mode_derivatives_are_refused():
         with pytest.raises(RuntimeError, match="forward-mode"):
             top_log_probs(h, 3)
     assert torch.isfinite(linear_cross_entropy(hidden, weight, targets))
+
+
+@cuda
+@pytest.mark.parametrize("T", [4, 150])
+@pytest.mark.parametrize("C", [64, 5120])
+def test_logits_without_rounding(T, C):
+    """One-hot hidden states: each logit is one product and zeros, so the tensor cores round nothing, and what undoes
+    their rounding elsewhere (C / 16 x 2^-26 of a logit) is all of the error but for fp32's: the scale's two roundings
+    and the result's (4 x 2^-24 of a logit), and the sum of exponentials (2^-22 each, at most 70 additions of a thread)."""
+    g = torch.Generator(device="cuda").manual_seed(C)
+    weight = (torch.randn(700, C, device="cuda", generator=g)).to(torch.bfloat16)
+    hidden = torch.zeros(T, C, device="cuda", dtype=torch.bfloat16)
+    hidden[torch.arange(T, device="cuda"), torch.randint(0, C, (T,), device="cuda", generator=g)] = 10.0
+    targets = torch.randint(0, 700, (T,), device="cuda", generator=g)
+    z = hidden.double() @ weight.double().t()
+    expected = torch.nn.functional.cross_entropy(z, targets, reduction="none")
+    got = linear_cross_entropy(hidden, weight, targets, reduction="none").double()
+    bound = z.abs().max().item() * (C // 16 * 2.0 ** -26 + 4 * 2.0 ** -24) + 2.0 ** -22 + 70 * 2.0 ** -24
+    assert ((got - expected).abs() <= bound).all(), ((got - expected).abs().max().item(), bound)
+
+
+@cuda
+@pytest.mark.parametrize("T", [96, 300])
+@pytest.mark.parametrize("K,tail", [(0, False), (8, False), (8, True)])
+def test_the_norm_of_the_gradients_errors(T, K, tail):
+    """What the logits' gradient, rounded to bf16 once, and a rounded result cost, is what the gradients may be off by:
+    the errors' norm against that of the same two roundings in 64 bits, with the 16-bit form of the logits (6.8e-4 of an
+    exponential at most, independent of each other) beside it, and a tenth for the sample."""
+    hidden, weight, targets, g = _inputs(T, 2000, 256)
+    log_probs, index = (None, targets[:, None]) if K == 0 else _record(hidden, weight, K, 1.0, g)
+    _, dz, _ = _oracle(hidden, weight, index, log_probs, -100, 1.0, tail)
+    h, w = hidden.clone().requires_grad_(), weight.clone().requires_grad_()
+    loss = (linear_cross_entropy(h, w, targets, reduction="sum") if K == 0 else
+            linear_topk_kl(h, w, index, log_probs, tail=tail, reduction="sum"))
+    x, W, rounded = hidden.double(), weight.double(), dz.to(torch.bfloat16).double()
+    for got, exact, once, spread in zip(
+            torch.autograd.grad(loss, (h, w)), (dz @ W, dz.t() @ x), (rounded @ W, rounded.t() @ x),
+            (dz.square() @ W.square(), dz.square().t() @ x.square())):
+        allowed = (once.to(torch.bfloat16).double() - exact).norm().square() + 6.8e-4 ** 2 * spread.sum()
+        assert (got.double() - exact).norm() <= 1.1 * allowed.sqrt()
+
+
+@cuda
+@pytest.mark.parametrize("T", [300, 1100])
+def test_the_weights_gradient_alone(T):
+    """What tuning a head asks for, in tiles of rows: with the gradient of the hidden states the same bits."""
+    hidden, weight, targets, g = _inputs(T, 1500, 136)
+    targets[: T // 4] = -100
+    log_probs, index = _record(hidden, weight, 12, 1.0, g)
+    for call in (lambda h, w: linear_cross_entropy(h, w, targets),
+                 lambda h, w: linear_topk_kl(h, w, index, log_probs)):
+        w = weight.clone().requires_grad_()
+        alone = torch.autograd.grad(call(hidden, w), w)[0]
+        h = hidden.clone().requires_grad_()
+        assert torch.equal(alone, torch.autograd.grad(call(h, w), (h, w))[1])
+    _, dz, valid = _oracle(hidden, weight, index, log_probs, -100, 1.0, True)
+    dz, x = dz / valid.sum(), hidden.double()
+    xmax, wmax = (t.float().norm(dim=-1).max().item() for t in (hidden, weight))
+    tol = 3 * U + 4 * (136 / 16 + 16) * 2.0 ** -23 * xmax * wmax
+    _within(alone, dz.t() @ x, tol * (dz.abs().t() @ x.abs()))
+
+
+@cuda
+@pytest.mark.parametrize("T", [70, 300])
+def test_both_losses_in_one_graph(T):
+    """A weighted sum of the two, as head tuning forms it: each gradient is rounded once more for its factor, and their
+    sum once."""
+    hidden, weight, targets, g = _inputs(T, 1500, 136)
+    targets[::5] = -100
+    log_probs, index = _record(hidden, weight, 12, 2.0, g)
+    index[::3] = -1
+    h, w = hidden.clone().requires_grad_(), weight.clone().requires_grad_()
+    loss = 0.3 * linear_topk_kl(h, w, index, log_probs, 2.0) + 0.7 * linear_cross_entropy(h, w, targets)
+    grads = torch.autograd.grad(loss, (h, w))
+    x, W = hidden.double(), weight.double()
+    xmax, wmax = (t.norm(dim=-1).max().item() for t in (x, W))
+    err = (136 / 16 + 16) * 2.0 ** -23 * xmax * wmax
+    expected, bound, value = [0, 0], [0, 0], 0
+    parts = ((0.3, index, log_probs, 0.5, True), (0.7, targets[:, None], None, 1.0, False))
+    for factor, ids, logp, scale, tail in parts:
+        rows, dz, valid = _oracle(hidden, weight, ids, logp, -100, scale, tail)
+        value += factor * rows.sum() / valid.sum()
+        dz = dz * (factor * scale / valid.sum())
+        for i, (a, b) in enumerate(((dz, W), (dz.t(), x))):
+            expected[i] = expected[i] + a @ b
+            bound[i] = bound[i] + (4 * U + 4 * err) * (a.abs() @ b.abs())
+    torch.testing.assert_close(loss.detach().double(), value, rtol=1e-5, atol=2 * err + 1e-6)
+    for got, e, b in zip(grads, expected, bound):
+        _within(got, e, b + U * (e.abs() + b))
