@@ -11,7 +11,8 @@
 // Z_rest is summed without the held entries instead of as Z minus them, so a row that is sure of its target keeps the
 // relative precision of 1 - q. The second form has factors of at most one however small Z_rest / Z is; as exp(z_v) / Z
 // (w - r Z / Z_rest) its factors leave fp32's range at Z_rest / Z = e^-87.
-// All sums and row statistics are fp32 (the few held terms of a row: double).
+// Sums within a tile and over a row's tiles are fp32. What joins a row's rest and its held entries (Z, log Z, the loss
+// and the gradient's coefficients) and the sum of the rows' losses are fp64: a KL is a small difference of these.
 //
 // Launches of one call: the rows that have a loss are counted and packed (gather_kernel: their hidden states, sorted
 // records and held logits), z = X W^T leaves per row and 256-column tile its maximum and sum of exponentials
@@ -528,7 +529,9 @@ __global__ void failed_kernel(const int* failed, __nv_bfloat16* __restrict__ dwe
   if (*failed && threadIdx.x < 8) dweight[threadIdx.x] = __float2bfloat16_rn(NAN);
 }
 
-// x *= *factor for up to two tensors, nothing at all for a factor of one (the usual upstream gradient of a loss).
+// x *= *factor for up to two tensors, nothing at all for a factor of one (the usual upstream gradient of a loss). A
+// factor that is no power of two rounds the gradients to bf16 a second time: it is only known in backward, and fp32
+// gradients kept until then would take twice the weight's memory (5 GB at the 27B head).
 struct ScaleArgs {
   __nv_bfloat16* x[2];
   long n[2];
@@ -555,7 +558,9 @@ __global__ void scale_kernel(const ScaleArgs p, const float* __restrict__ factor
 // The tensor cores round each of the C / 16 partial sums of a logit towards zero. Given the sum z, the partial sums are
 // (k / n) z on average, each loses half a unit in its last place, and the expected loss is n 2^-26 z (measured: 4.84e-6
 // z at width 5120, 1.82e-6 at 2048, 0.86e-6 at 1024, on random operands; the rest of the error has no preferred side).
-// Undoing it takes the error of log Z from 9.6e-6 to 2e-7 at width 5120.
+// Undoing it takes the error of log Z from 9.6e-6 to 2e-7 at width 5120. Where the products add up exactly (one-hot
+// hidden states, small whole numbers) there is nothing to undo, and n 2^-26 of the logit is the error: 4.8e-6 at width
+// 5120, as large as without the correction on other operands.
 float mma_gain(int C) { return 1.f + (float)(C / 16) * 0x1p-26f; }
 
 constexpr long up(long n, long to) { return (n + to - 1) / to * to; }

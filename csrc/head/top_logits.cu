@@ -8,9 +8,9 @@
 // equal or special values defeat the bounds (thousands of equal maxima, infinities, NaN) take a radix descent over the
 // whole row instead.
 //
-// Bound by memory: per value one packed maximum's half, unpacking, multiply-add, ex2 and add (about 5 issue slots of
-// the 11 that the bandwidth leaves). Several blocks per SM, so that one streams while another selects. Few rows are cut
-// into segments over as many blocks, whose k candidates a second kernel merges.
+// Bound by memory: per value one packed maximum's half, unpacking, packed subtraction, product and sum, and ex2
+// (about 5.5 issue slots of the 11 that the bandwidth leaves). Several blocks per SM, so that one streams while
+// another selects. Few rows are cut into segments over as many blocks, whose k candidates a second kernel merges.
 #include <algorithm>
 #include <atomic>
 #include <climits>
