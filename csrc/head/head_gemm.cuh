@@ -72,6 +72,7 @@ struct Args {
   long ld_e;
   float* dx;        // DX_N: the partial sums
   int add;          // DW32: add to what is there
+  const float* factor;  // DW, DW32: of the whole product
   int* status;
   uint4* poison;    // DW: the gradient's first 16 bytes, NaN if a wait of this or of an earlier product gave up
 };
@@ -367,6 +368,7 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
     const int quarter = warp & 3;
     uint8_t* buf = staging + quarter * STAGING_BYTES;
     uint32_t* mask = masks + quarter * 8 * 32 + lane;
+    const float factor = MODE == DW || MODE == DW32 ? *args.factor : 1.f;
     int acc = 0;
     uint32_t acc_phase = 0;
     while (work.next(tm, tn, split, k0, k1)) {
@@ -495,6 +497,8 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
             sm100::tmem_ld32(t_row + (c + h) * 32, v);
             sm100::tmem_wait_ld();
 #pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= factor;
+#pragma unroll
             for (int q = 0; q < 4; ++q) *staged(b, lane, 4 * h + q) = rt::pack8(v + 8 * q);
           }
           send(b, col0 + 32 * c, row0, false);
@@ -509,6 +513,10 @@ pair_kernel(const __grid_constant__ Maps maps, const Args args) {
           float v[32];
           sm100::tmem_ld32(t_row + c * 32, v);
           sm100::tmem_wait_ld();
+          if (MODE == DW32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= factor;
+          }
 #pragma unroll
           for (int q = 0; q < 8; ++q)
             *staged(b, lane, q) = make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]),

@@ -56,21 +56,41 @@ __global__ void kinds_kernel(const long* __restrict__ idx, long rows, int K, lon
 
 // What the rows' losses and gradients are taken over: valid rows, rows with a loss, a product that gave up a wait
 // (where the caller has no status word), and blocks of merge_kernel that are done.
+// `factor` is what all rows' gradients have in common (scale, the mean's 1 / rows with a loss, the largest upstream
+// gradient of a row): dX and dW are multiplied by it in fp32. In dz it would round the target entries of all rows,
+// which are nearly -factor, the same way: up to 0.4% of the whole gradient. `unit`: the upstream gradient that counts
+// as one.
 struct Counts {
   int valid, counted, failed, done;
+  float factor, unit;
+};
+
+struct Upstream {
+  float scale;
+  int mean;
+  const float* rows;  // or null
+  __device__ __forceinline__ float of(long row) const { return rows ? fabsf(rows[row]) : 0.f; }
+  // top: the largest of the valid rows
+  __device__ __forceinline__ Counts counts(int valid, int counted, float top) const {
+    const float unit = top > 0.f && top < INFINITY ? top : 1.f;
+    return Counts{valid, counted, 0, 0, rows ? scale * unit : mean ? scale / (float)max(counted, 1) : scale, unit};
+  }
 };
 
 // One block: slot[row] = place of a valid row among the valid ones, or -1 (no loss), -2 (outside the vocabulary). The
 // kinds come from `kind`, or from targets.
 __global__ void __launch_bounds__(1024) pack_kernel(const int* __restrict__ kind, const long* __restrict__ targets,
-                                                    long ignore, long V, long rows, int* __restrict__ slot,
-                                                    Counts* __restrict__ counts) {
-  __shared__ int warps[2][32];
+                                                    long ignore, long V, long rows, const Upstream up,
+                                                    int* __restrict__ slot, Counts* __restrict__ counts) {
+  __shared__ int warps[2][32], top_bits;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int valid = 0, bad = 0;
+  float top = 0.f;
+  if (threadIdx.x == 0) top_bits = 0;
   for (long base = 0; base < rows; base += 1024) {
     const long t = base + threadIdx.x;
     const int k = t >= rows ? 0 : kind ? kind[t] : entry_kind(targets[t], false, ignore, V);
+    if (k == 1) top = fmaxf(top, up.of(t));
     const unsigned good = __ballot_sync(~0u, k == 1), outside = __ballot_sync(~0u, k == 2);
     if (lane == 0) {
       warps[0][warp] = __popc(good);
@@ -85,7 +105,9 @@ __global__ void __launch_bounds__(1024) pack_kernel(const int* __restrict__ kind
     if (t < rows) slot[t] = k == 1 ? at : -k - (k == 0);
     __syncthreads();
   }
-  if (threadIdx.x == 0) *counts = Counts{valid, valid + bad, 0, 0};
+  if (up.rows) atomicMax(&top_bits, __float_as_int(top));  // not negative: ordered like the numbers
+  __syncthreads();
+  if (threadIdx.x == 0) *counts = up.counts(valid, valid + bad, __int_as_float(top_bits));
 }
 
 // The same for the block of one row of a short call (at most SHORT_ENTRIES in all its records), which counts the rows
@@ -93,8 +115,9 @@ __global__ void __launch_bounds__(1024) pack_kernel(const int* __restrict__ kind
 // (16 targets: 3.4 us against 1.9 + 3.0 in two launches; 1024 targets: 27 against 2.2 + 18.5.)
 constexpr int SHORT_ENTRIES = 512;
 __device__ __forceinline__ int place_in_short(const long* idx, bool record, int K, long rows, long row, long ignore,
-                                              long V, Counts* counts, int* scratch, int& valid) {
+                                              long V, const Upstream& up, Counts* counts, int* scratch, int& valid) {
   int before = 0, all = 0, bad = 0;
+  float top = 0.f;
   for (long t = threadIdx.x; t < rows; t += blockDim.x) {
     int any = 0;
     for (int k = 0; k < K; ++k) any |= entry_kind(idx[t * K + k], record, ignore, V);
@@ -103,8 +126,10 @@ __device__ __forceinline__ int place_in_short(const long* idx, bool record, int 
     all += kind == 1;
     bad += kind == 2;
     if (t == row) scratch[3] = kind;
+    if (row == 0 && kind == 1) top = fmaxf(top, up.of(t));
   }
   if (threadIdx.x < 3) scratch[threadIdx.x] = 0;
+  if (threadIdx.x == 3) scratch[4] = 0;
   __syncthreads();
   before = __reduce_add_sync(~0u, before);
   all = __reduce_add_sync(~0u, all);
@@ -114,9 +139,10 @@ __device__ __forceinline__ int place_in_short(const long* idx, bool record, int 
     atomicAdd(&scratch[1], all);
     atomicAdd(&scratch[2], bad);
   }
+  if (row == 0 && up.rows) atomicMax(&scratch[4], __float_as_int(top));
   __syncthreads();
   valid = scratch[1];
-  if (row == 0 && threadIdx.x == 0) *counts = Counts{valid, valid + scratch[2], 0, 0};
+  if (row == 0 && threadIdx.x == 0) *counts = up.counts(valid, valid + scratch[2], __int_as_float(scratch[4]));
   if (row >= rows) return 0;
   const int kind = scratch[3];
   return kind == 1 ? scratch[0] : -kind - (kind == 0);
@@ -146,8 +172,9 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
                                                      int K, int Kp, long rows, const __nv_bfloat16* __restrict__ hidden,
                                                      long ldh, const __nv_bfloat16* __restrict__ w, long ldw, int C,
                                                      float scale2, long V, long ignore, bool brief,
-                                                     const int* __restrict__ slot, Counts* __restrict__ counts,
-                                                     int* __restrict__ row_of, uint4* __restrict__ x,
+                                                     const Upstream up, const int* __restrict__ slot,
+                                                     Counts* __restrict__ counts, int* __restrict__ row_of,
+                                                     uint4* __restrict__ x,
                                                      int* __restrict__ sidx, float* __restrict__ slogp,
                                                      float* __restrict__ hit, float* __restrict__ row_loss,
                                                      uint4* __restrict__ dhidden) {
@@ -155,11 +182,11 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
   const long row = blockIdx.x;
   const int C8 = C / 8;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  __shared__ int scratch[4];
+  __shared__ int scratch[5];
   int valid;
   long place;
   if (brief) {
-    place = place_in_short(idx, logp != nullptr, K, rows, row, ignore, V, counts, scratch, valid);
+    place = place_in_short(idx, logp != nullptr, K, rows, row, ignore, V, up, counts, scratch, valid);
   } else {
     valid = counts->valid;
     place = row < rows ? slot[row] : 0;
@@ -220,8 +247,8 @@ __global__ void __launch_bounds__(256) gather_kernel(const long* __restrict__ id
 // Block of ROWS rows (four, or one of the few rows whose statistics are finer): its threads merge the tiles' statistics
 // (in a fixed order: each row's tiles go round-robin to MERGE_THREADS / ROWS threads), then one warp per row forms the
 // loss and the gradient's coefficients: d/dz_v = tail exp2(z_v - base2) outside the record (base2 = log2 Z_rest with a
-// rest's class, else log2 Z), coef[k] for its held entries, both times scale and the row's upstream gradient (given per
-// row, or 1, or 1 / rows with a loss).
+// rest's class, else log2 Z), coef[k] for its held entries, both times the row's upstream gradient in units of the
+// call's (see Counts).
 constexpr int MERGE_THREADS = 256;
 struct MergeArgs {
   const float2* part;
@@ -235,8 +262,7 @@ struct MergeArgs {
   const int* sidx;
   const float* slogp;
   const float* hit;
-  float scale;
-  const float* grad;
+  const float* grad;  // upstream gradients of the rows, or null
   float* row_loss;
   float* loss;  // null: the rows' losses are the result
   float* base2;
@@ -321,7 +347,7 @@ __device__ __forceinline__ void merge_rows(const MergeArgs& p) {
       value += r1 * (log(r1) - lr);
       a = weight * exp(lr) - r1;
     }
-    const float g = p.scale * (p.grad ? p.grad[row] : (p.mean ? 1.f / (float)max(p.counts->counted, 1) : 1.f));
+    const float g = p.grad ? p.grad[row] / p.counts->unit : 1.f;
     if (lane == 0) {
       p.row_loss[row] = *p.failed ? NAN : (float)value;
       p.base2[place] = (float)base;
@@ -501,25 +527,27 @@ __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict
   }
 }
 
-// dhidden[row_of[place]] = bf16 of the row's partial sums, added in order.
+// dhidden[row_of[place]] = bf16 of factor times the row's partial sums, added in order.
 __global__ void __launch_bounds__(256) dhidden_kernel(const float* __restrict__ partial, int splits, long split_rows,
                                                       int C, int row0, int rows, const Counts* __restrict__ counts,
                                                       const int* failed, const int* __restrict__ row_of,
                                                       __nv_bfloat16* __restrict__ out) {
   const int n = min(max(counts->valid - row0, 0), rows), r = blockIdx.x;
   if (r >= n) return;
-  const float from = *failed ? NAN : 0.f;  // a product gave up a wait
+  const float factor = *failed ? NAN : counts->factor;  // a product gave up a wait
   uint4* dst = reinterpret_cast<uint4*>(out + (long)row_of[row0 + r] * C);
   for (int c = threadIdx.x; c < C / 8; c += blockDim.x) {
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = from;
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
     for (int s = 0; s < splits; ++s) {
       const float4* src = reinterpret_cast<const float4*>(partial + ((long)s * split_rows + r) * C) + 2 * c;
       const float4 x = __ldg(src), y = __ldg(src + 1);
       v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
       v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= factor;
     dst[c] = rt::pack8(v);
   }
 }
@@ -630,7 +658,7 @@ Layout layout(long T, long V, int C, int K, bool grad_h, bool grad_w) {
   l.kind = take(T);
   l.slot = take(T);
   l.row_of = take(T);
-  l.counts = take(4);
+  l.counts = take(sizeof(Counts) / 4);
   l.x = take(up(T, 64) * C / 2);
   l.sidx = take(T * K);
   l.slogp = take(T * K);
@@ -732,19 +760,20 @@ extern "C" cudaError_t rt_head_loss_status(const RtHeadLoss* p, float* work, int
     return cudaGetLastError();
   }
   const bool brief = T * K <= SHORT_ENTRIES;
+  const Upstream upstream{p->scale, p->reduction == 2, p->row_grad};
   if (!brief) {
     if (p->log_probs) kinds_kernel<<<(unsigned)((T * 32 + 255) / 256), 256, 0, s>>>(p->index, T, K, V, ints(l.kind));
-    pack_kernel<<<1, 1024, 0, s>>>(p->log_probs ? ints(l.kind) : nullptr, p->index, p->ignore, V, T, ints(l.slot),
-                                   counts);
+    pack_kernel<<<1, 1024, 0, s>>>(p->log_probs ? ints(l.kind) : nullptr, p->index, p->ignore, V, T, upstream,
+                                   ints(l.slot), counts);
   }
   int Kp = 1;
   while (Kp < K) Kp <<= 1;
   const unsigned share = (unsigned)std::max(1L, std::min((K + 7L) / 8, 296 / T));  // blocks of a row: two per SM in all
   gather_kernel<<<dim3((unsigned)(T + 64), share), 256, Kp * 8, s>>>(
       p->index, p->log_probs, K, Kp, T, reinterpret_cast<const __nv_bfloat16*>(p->hidden), p->ld_hidden,
-      reinterpret_cast<const __nv_bfloat16*>(p->weight), p->ld_weight, C, scale2, V, p->ignore, brief, ints(l.slot),
-      counts, ints(l.row_of), reinterpret_cast<uint4*>(x), ints(l.sidx), work + l.slogp, work + l.hit, p->row_loss,
-      reinterpret_cast<uint4*>(p->dhidden));
+      reinterpret_cast<const __nv_bfloat16*>(p->weight), p->ld_weight, C, scale2, V, p->ignore, brief, upstream,
+      ints(l.slot), counts, ints(l.row_of), reinterpret_cast<uint4*>(x), ints(l.sidx), work + l.slogp, work + l.hit,
+      p->row_loss, reinterpret_cast<uint4*>(p->dhidden));
   RT_CUDA_CHECK(cudaGetLastError());
 
   head::Maps logits, dx, dw;
@@ -783,8 +812,8 @@ extern "C" cudaError_t rt_head_loss_status(const RtHeadLoss* p, float* work, int
                    : narrow ? launch<head::LOGITS_N, 128>(logits, args, l.tiles, s)
                             : launch<head::LOGITS>(logits, args, tiles_m * l.tiles, s)));
     MergeArgs m{part, l.part_ld, (int)l.groups, (int)row0, (int)l.rows, K, p->tail, p->reduction == 2, merge_blocks, T,
-                counts, failed, ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->scale, p->row_grad,
-                p->row_loss, p->reduction ? p->loss : nullptr, work + l.base2, work + l.tail,
+                counts, failed, ints(l.row_of), ints(l.sidx), work + l.slogp, work + l.hit, p->row_grad, p->row_loss,
+                p->reduction ? p->loss : nullptr, work + l.base2, work + l.tail,
                 grad ? work + l.coef : nullptr};
     if (narrow) merge_kernel<1><<<(unsigned)rows, MERGE_THREADS, 0, s>>>(m);
     else merge_kernel<4><<<(unsigned)(rows + 3) / 4, MERGE_THREADS, 0, s>>>(m);
@@ -812,6 +841,7 @@ extern "C" cudaError_t rt_head_loss_status(const RtHeadLoss* p, float* work, int
         return cudaErrorInvalidValue;
       const long units = l.tiles * tiles_c;
       args.poison = static_cast<uint4*>(p->dweight);
+      args.factor = &counts->factor;
       RT_CUDA_CHECK(l.dw32 ? launch<head::DW32>(dw, args, units, s) : launch<head::DW>(dw, args, units, s));
     }
   }
