@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(MERGE_THREADS + 32) score_kernel(const ScoreAr
 // ---------------------------------------------------------------- gradient of the logits
 // In place: depths of a chunk's logits (below the maximum of their `group` columns) -> dz, one warp per row and 256
 // columns; the block of 32 such tiles also puts their held entries in their places; rows that fill the last block of 64
-// become zero. A read and a write of every value: 0.16 ms for 992 x 248077 (6.2 TB/s), where forming the logits again
+// become zero. A read and a write of every value: 0.16 ms for 992 x 248077 (6.0 TB/s), where forming the logits again
 // would cost 1.8 ms. dz is rounded to bf16 here, once: it is a tensor-core operand next.
 __global__ void __launch_bounds__(256) gradient_kernel(__nv_bfloat16* __restrict__ e, long ld, int V, int row0,
                                                        int rows, const Counts* __restrict__ counts,

@@ -11,11 +11,11 @@ first two take hidden states and the head's weight and never keep the logits, th
 that the second learns from.
 
 On CUDA the two losses are fp32 and off by about 2e-7 of a logit (width / 16 x 2^-26 of it where its products add up
-without rounding, 4.8e-6 at width 5120). Their gradients are bf16: the logits' gradient is rounded to bf16 once, the
-result once, and once more for an upstream factor that is no power of two. A loss that is summed or averaged while
-gradients are recorded forms them in the forward call, all that are required, and keeps them until its backward (outside
-saved-tensor hooks): score under ``torch.no_grad()``. reduction "none" forms them in backward. There is no second and no
-forward-mode derivative. ``top_log_probs`` has no gradient.
+without rounding, 4.8e-6 at width 5120). Their gradients are bf16: the logits' gradient is rounded to bf16 once (without
+the factors that all tokens share), the result once, and once more for an upstream factor that is no power of two. A
+loss that is summed or averaged while gradients are recorded forms them in the forward call, all that are required, and
+keeps them until its backward (outside saved-tensor hooks): score under ``torch.no_grad()``. reduction "none" forms them
+in backward. There is no second and no forward-mode derivative. ``top_log_probs`` has no gradient.
 """
 import math
 
