@@ -101,6 +101,38 @@ cudaError_t rt_top_log_probs(int dtype, const void* logits, long rows, long V, l
                              float* logp, long* index, void* work, cudaStream_t stream);
 long rt_top_workspace_bytes(int dtype, long rows, long V, int k);
 
+// Beam search (csrc/beam/): selection over beams and vocabulary, rows of states that follow their parents.
+long rt_beam_select_workspace_bytes(long groups, int K, long V);
+cudaError_t rt_beam_select(int dtype, const void* logits, long groups, int K, long V, long ld_group, long ld_beam,
+                           const float* scores, const int* lengths, const bool* finished, int end_token,
+                           double penalty, long* tokens, long* parents, float* out_scores, int* out_lengths,
+                           bool* out_finished, void* work, cudaStream_t stream);
+cudaError_t rt_reorder_rows(void* const* base, const long* bytes, int n, const long* parents, long groups, int K,
+                            cudaStream_t stream);
+
+// Paged key/value cache (csrc/paged/): pool [pages, blocks, 2, heads, page, dim] bf16, table [rows, width] int32.
+struct RtPool {
+  void* pool;
+  int pages, blocks, heads, page, dim, rows, width;
+};
+long rt_advance_workspace_bytes(int rows);
+cudaError_t rt_advance_pages(const struct RtPool* p, const int* table, const int* lengths, const int* refs, int tokens,
+                             const long* parents, int K, const bool* live, int* new_table, int* new_lengths,
+                             int* new_refs, int* status, int keep_status, void* work, cudaStream_t stream);
+long rt_compact_workspace_bytes(int pages);
+cudaError_t rt_compact_pages(const struct RtPool* p, const int* table, const int* refs, int* new_table, int* new_refs,
+                             int* used, void* work, cudaStream_t stream);
+cudaError_t rt_store_pages(const struct RtPool* p, int block, const int* table, const int* lengths, const void* keys,
+                           const long* key_strides, const void* values, const long* value_strides, int T, int every,
+                           cudaStream_t stream);
+cudaError_t rt_append_heads(const struct RtPool* p, int block, const int* table, const int* lengths, const void* x,
+                            long ld, const float* q_weight, const float* k_weight, const float* inv_freq, int half,
+                            int heads, float eps, void* q, cudaStream_t stream);
+long rt_paged_attention_workspace_floats(const struct RtPool* p, int heads, int group);
+cudaError_t rt_paged_attention(const struct RtPool* p, int block, const int* table, const int* lengths, const void* q,
+                               long q_row, long q_head, int heads, const void* gate, long gate_row, long gate_head,
+                               int group, void* out, float* work, cudaStream_t stream);
+
 // Teacher-block kernels (bf16 activations, fp32 parameters).
 cudaError_t rt_rmsnorm_1p(const void* x, const void* h, const float* w, void* sum_out, void* out, long rows, int C,
                           float eps, cudaStream_t stream);

@@ -766,6 +766,198 @@ at::Tensor flash_attention(at::Tensor q, at::Tensor keys, at::Tensor values, at:
   return out;
 }
 
+// ------------------------------------------------------------------ beam search
+// The Python layer (beams.py, paged.py) has checked shapes, types and devices.
+std::vector<at::Tensor> beam_select(at::Tensor logits, at::Tensor scores, at::Tensor lengths, at::Tensor finished,
+                                    int64_t end_token, double penalty) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 3, "beam_select: logits must be CUDA [groups, beams, vocabulary]");
+  c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t G = logits.size(0), K = logits.size(1), V = logits.size(2);
+  TORCH_CHECK(K >= 1 && K <= 32 && V >= 1 && V <= (1 << 22), "beam_select: 1 to 32 beams and a vocabulary of 2^22 at most");
+  TORCH_CHECK(end_token >= -1 && end_token < V, "beam_select: end_token outside the vocabulary");
+  TORCH_CHECK(scores.scalar_type() == at::kFloat && lengths.scalar_type() == at::kInt &&
+                  finished.scalar_type() == at::kBool && scores.numel() == G * K && lengths.numel() == G * K &&
+                  finished.numel() == G * K && scores.device() == logits.device() &&
+                  lengths.device() == logits.device() && finished.device() == logits.device(),
+              "beam_select: scores fp32, lengths int32 and finished bool, one per beam");
+  if (logits.stride(2) != 1 && V > 1) logits = logits.contiguous();
+  scores = scores.contiguous();
+  lengths = lengths.contiguous();
+  finished = finished.contiguous();
+  auto longs = scores.options().dtype(at::kLong);
+  auto tokens = at::empty({G, K}, longs), parents = at::empty({G, K}, longs);
+  auto out_scores = at::empty({G, K}, scores.options()), out_lengths = at::empty({G, K}, lengths.options());
+  auto out_finished = at::empty({G, K}, finished.options());
+  auto work = at::empty({rt_beam_select_workspace_bytes(G, K, V)}, scores.options().dtype(at::kByte));
+  check_cuda(rt_beam_select(dtype_code(logits), logits.data_ptr(), G, K, V, logits.stride(0), logits.stride(1),
+                            scores.data_ptr<float>(), lengths.data_ptr<int>(), finished.data_ptr<bool>(),
+                            (int)end_token, penalty, reinterpret_cast<long*>(tokens.data_ptr<int64_t>()),
+                            reinterpret_cast<long*>(parents.data_ptr<int64_t>()), out_scores.data_ptr<float>(),
+                            out_lengths.data_ptr<int>(), out_finished.data_ptr<bool>(), work.data_ptr(),
+                            stream_of(logits)),
+             "beam_select");
+  return {tokens, parents, out_scores, out_lengths, out_finished};
+}
+
+void reorder_rows_(std::vector<at::Tensor> states, at::Tensor parents) {
+  TORCH_CHECK(parents.is_cuda() && parents.scalar_type() == at::kLong && parents.dim() == 2 && parents.is_contiguous() &&
+                  parents.size(1) >= 1 && parents.size(1) <= 32,
+              "reorder_rows_: parents must be contiguous CUDA int64 [groups, 1 to 32 beams]");
+  c10::cuda::CUDAGuard guard(parents.device());
+  std::vector<void*> base;
+  std::vector<long> bytes;
+  for (const at::Tensor& t : states) {
+    TORCH_CHECK(t.device() == parents.device() && t.is_contiguous() && t.dim() >= 1 && t.size(0) == parents.numel() &&
+                    t.numel() > 0,
+                "reorder_rows_: states must be contiguous tensors of one row per beam");
+    base.push_back(t.data_ptr());
+    bytes.push_back(t.numel() / t.size(0) * (long)t.element_size());
+  }
+  check_cuda(rt_reorder_rows(base.data(), bytes.data(), (int)base.size(),
+                             reinterpret_cast<const long*>(parents.data_ptr<int64_t>()), parents.size(0),
+                             (int)parents.size(1), stream_of(parents)),
+             "reorder_rows_");
+}
+
+RtPool pool_of(const at::Tensor& pool, const at::Tensor& table) {
+  check_bf16(pool, "pool");
+  TORCH_CHECK(pool.dim() == 6 && pool.size(2) == 2 && pool.numel() > 0 && pool.size(0) < (1 << 30) &&
+                  pool.size(1) * pool.size(3) < (1 << 20),
+              "pool must be [pages, blocks, 2, heads, page, dim]");
+  TORCH_CHECK(pool.size(4) == 16 || pool.size(4) == 32 || pool.size(4) == 64, "a page holds 16, 32 or 64 tokens");
+  TORCH_CHECK(pool.size(5) == 64 || pool.size(5) == 128 || pool.size(5) == 256, "head size must be 64, 128 or 256");
+  TORCH_CHECK(table.device() == pool.device() && table.scalar_type() == at::kInt && table.is_contiguous() &&
+                  table.dim() == 2 && table.numel() > 0 && table.size(0) <= 1024 && table.size(1) < (1 << 24),
+              "table must be contiguous int32 [1 to 1024 rows, width] on the pool's device");
+  return {pool.data_ptr(), (int)pool.size(0), (int)pool.size(1), (int)pool.size(3), (int)pool.size(4),
+          (int)pool.size(5), (int)table.size(0), (int)table.size(1)};
+}
+
+int* ints(const at::Tensor& t, const at::Tensor& pool, int64_t numel, const char* name) {
+  TORCH_CHECK(t.device() == pool.device() && t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() == numel,
+              name, " must be ", numel, " contiguous int32 on the pool's device");
+  return t.data_ptr<int>();
+}
+
+std::vector<at::Tensor> advance_pages(at::Tensor pool, at::Tensor table, at::Tensor lengths, at::Tensor refs,
+                                      int64_t tokens, c10::optional<at::Tensor> parents,
+                                      c10::optional<at::Tensor> live, c10::optional<std::vector<at::Tensor>> out) {
+  const RtPool p = pool_of(pool, table);
+  c10::cuda::CUDAGuard guard(pool.device());
+  TORCH_CHECK(tokens >= 0 && tokens <= (1 << 30), "advance_pages: tokens out of range");
+  int K = 1;
+  if (parents.has_value()) {
+    TORCH_CHECK(parents->device() == pool.device() && parents->scalar_type() == at::kLong && parents->dim() == 2 &&
+                    parents->is_contiguous() && parents->numel() == p.rows,
+                "advance_pages: parents must be contiguous int64 [groups, beams]");
+    K = (int)parents->size(1);
+  }
+  TORCH_CHECK(!live.has_value() || (live->device() == pool.device() && live->scalar_type() == at::kBool &&
+                                    live->is_contiguous() && live->numel() == p.rows),
+              "advance_pages: live must be one bool per row");
+  const bool given = out.has_value();
+  if (!given)
+    out = std::vector<at::Tensor>{at::empty_like(table), at::empty_like(lengths), at::empty_like(refs),
+                                  at::empty({1}, lengths.options())};
+  TORCH_CHECK(out->size() == 4, "advance_pages: out is (table, lengths, refs, status)");
+  const at::Tensor &t = (*out)[0], &l = (*out)[1], &r = (*out)[2], &st = (*out)[3];
+  auto work = at::empty({rt_advance_workspace_bytes(p.rows)}, table.options().dtype(at::kByte));
+  check_cuda(rt_advance_pages(&p, table.data_ptr<int>(), ints(lengths, pool, p.rows, "lengths"),
+                              ints(refs, pool, p.pages, "refs"), (int)tokens,
+                              parents.has_value() ? reinterpret_cast<const long*>(parents->data_ptr<int64_t>()) : nullptr,
+                              K, live.has_value() ? live->data_ptr<bool>() : nullptr,
+                              ints(t, pool, (int64_t)p.rows * p.width, "out table"), ints(l, pool, p.rows, "out lengths"),
+                              ints(r, pool, p.pages, "out refs"), ints(st, pool, 1, "out status"), given,
+                              work.data_ptr(), stream_of(pool)),
+             "advance_pages");
+  return *out;
+}
+
+std::vector<at::Tensor> compact_pages(at::Tensor pool, at::Tensor table, at::Tensor refs,
+                                      c10::optional<std::vector<at::Tensor>> out) {
+  const RtPool p = pool_of(pool, table);
+  c10::cuda::CUDAGuard guard(pool.device());
+  if (!out.has_value()) out = std::vector<at::Tensor>{at::empty_like(table), at::empty_like(refs)};
+  TORCH_CHECK(out->size() == 2, "compact_pages: out is (table, refs)");
+  auto used = at::empty({1}, refs.options());
+  auto work = at::empty({rt_compact_workspace_bytes(p.pages)}, table.options().dtype(at::kByte));
+  check_cuda(rt_compact_pages(&p, table.data_ptr<int>(), ints(refs, pool, p.pages, "refs"),
+                              ints((*out)[0], pool, (int64_t)p.rows * p.width, "out table"),
+                              ints((*out)[1], pool, p.pages, "out refs"), used.data_ptr<int>(), work.data_ptr(),
+                              stream_of(pool)),
+             "compact_pages");
+  return {(*out)[0], (*out)[1], used};
+}
+
+void store_pages(at::Tensor pool, int64_t block, at::Tensor table, at::Tensor lengths, at::Tensor keys,
+                 at::Tensor values) {
+  const RtPool p = pool_of(pool, table);
+  c10::cuda::CUDAGuard guard(pool.device());
+  long strides[2][3];
+  for (int i = 0; i < 2; ++i) {
+    at::Tensor& x = i ? values : keys;
+    TORCH_CHECK(x.device() == pool.device() && x.scalar_type() == at::kBFloat16 && x.dim() == 4 &&
+                    x.sizes() == keys.sizes() && x.size(0) >= 1 && p.rows % x.size(0) == 0 && x.size(2) == p.heads &&
+                    x.size(3) == p.dim && x.size(1) <= (1 << 30),
+                "store_pages: keys and values must be bf16 [rows / beams, tokens, heads, dim]");
+    if (x.stride(3) != 1) x = x.contiguous();
+    for (int d = 0; d < 3; ++d) strides[i][d] = x.stride(d);
+  }
+  check_cuda(rt_store_pages(&p, (int)block, table.data_ptr<int>(), ints(lengths, pool, p.rows, "lengths"),
+                            keys.data_ptr(), strides[0], values.data_ptr(), strides[1], (int)keys.size(1),
+                            p.rows / (int)keys.size(0), stream_of(pool)),
+             "store_pages");
+}
+
+at::Tensor append_heads(at::Tensor x, at::Tensor pool, int64_t block, at::Tensor table, at::Tensor lengths,
+                        at::Tensor q_weight, at::Tensor k_weight, at::Tensor inv_freq, int64_t heads, double eps) {
+  const RtPool p = pool_of(pool, table);
+  c10::cuda::CUDAGuard guard(pool.device());
+  TORCH_CHECK(heads >= 1 && heads <= (1 << 16) && x.device() == pool.device() && x.scalar_type() == at::kBFloat16 &&
+                  x.dim() == 2 && x.size(0) == p.rows && x.size(1) == (2 * heads + 2 * p.heads) * p.dim,
+              "append_heads: x must be bf16 [rows, (2 heads + 2 kv heads) dim]");
+  for (const at::Tensor* w : {&q_weight, &k_weight, &inv_freq})
+    TORCH_CHECK(w->device() == pool.device() && w->scalar_type() == at::kFloat && w->is_contiguous() && w->dim() == 1,
+                "append_heads: weights and frequencies must be fp32 vectors");
+  TORCH_CHECK(q_weight.numel() == p.dim && k_weight.numel() == p.dim && 2 * inv_freq.numel() <= p.dim,
+              "append_heads: weights of one head and at most dim / 2 frequencies");
+  if (x.stride(1) != 1) x = x.contiguous();
+  auto q = at::empty({p.rows, heads, p.dim}, x.options());
+  check_cuda(rt_append_heads(&p, (int)block, table.data_ptr<int>(), ints(lengths, pool, p.rows, "lengths"), x.data_ptr(),
+                             x.stride(0), q_weight.data_ptr<float>(), k_weight.data_ptr<float>(),
+                             inv_freq.data_ptr<float>(), (int)inv_freq.numel(), (int)heads, (float)eps, q.data_ptr(),
+                             stream_of(pool)),
+             "append_heads");
+  return q;
+}
+
+at::Tensor paged_attention(at::Tensor q, at::Tensor pool, int64_t block, at::Tensor table, at::Tensor lengths,
+                           c10::optional<at::Tensor> gate, int64_t group) {
+  const RtPool p = pool_of(pool, table);
+  c10::cuda::CUDAGuard guard(pool.device());
+  TORCH_CHECK(q.device() == pool.device() && q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.size(0) == p.rows &&
+                  q.size(2) == p.dim && q.size(1) >= 1 && q.size(1) % p.heads == 0 && q.size(1) <= 64L * p.heads,
+              "paged_attention: q must be bf16 [rows, heads, dim], 1 to 64 heads per key head");
+  TORCH_CHECK(group >= 1 && group <= p.rows && p.rows % group == 0, "paged_attention: rows are no groups of ", group);
+  if (q.stride(2) != 1) q = q.contiguous();
+  at::Tensor g;
+  if (gate.has_value()) {
+    g = *gate;
+    TORCH_CHECK(g.device() == pool.device() && g.scalar_type() == at::kBFloat16 && g.sizes() == q.sizes(),
+                "paged_attention: gate must be like q");
+    if (g.stride(2) != 1) g = g.contiguous();
+  }
+  auto out = at::empty(q.sizes(), q.options());
+  const int heads = (int)q.size(1);
+  auto work = at::empty({rt_paged_attention_workspace_floats(&p, heads, (int)group)}, q.options().dtype(at::kFloat));
+  check_cuda(rt_paged_attention(&p, (int)block, table.data_ptr<int>(), ints(lengths, pool, p.rows, "lengths"),
+                                q.data_ptr(), q.stride(0), q.stride(1), heads, g.defined() ? g.data_ptr() : nullptr,
+                                g.defined() ? g.stride(0) : 0, g.defined() ? g.stride(1) : 0, (int)group, out.data_ptr(),
+                                work.data_ptr<float>(), stream_of(pool)),
+             "paged_attention");
+  return out;
+}
+
 // Native executor of one fused TimeMix student micro-step (reference theseus/timemix.py:66-89 forward, with the
 // hand-written backward): mix, the r/k/v and LoRA GEMMs, pre-WKV, WKV7, post-WKV, the output GEMM with the loss in
 // its epilogue, and the backward of all of it, issued from C++ on the current stream (about 40 launches; the Python
@@ -1021,6 +1213,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       }, "dst = src with this package's kernel");
   m.def("to_bf16_", &to_bf16_);
   m.def("flash_attention", &flash_attention);
+  m.def("beam_select", &beam_select, "one step of beam search: (tokens, parents, scores, lengths, finished)");
+  m.def("reorder_rows_", &reorder_rows_, "rows of many tensors replaced by their parents' rows in place");
+  m.def("advance_pages", &advance_pages, "rows take over their parents' pages and get room for more tokens");
+  m.def("compact_pages", &compact_pages, "pages in use moved to the front of their pool");
+  m.def("store_pages", &store_pages, "keys and values as the last tokens of rows");
+  m.def("append_heads", &append_heads, "norm and rotation of queries and keys, keys and values into their pages");
+  m.def("paged_attention", &paged_attention, "attention of one token per row over its pages");
   m.def("exchange_update", &exchange_update, "peer-memory reduce-scatter + clip + AdamW + all-gather of one layer");
   m.def("exchange_shard", &exchange_shard);
   m.def("exchange_signal_words", []() { return rt_exchange_signal_words(); });

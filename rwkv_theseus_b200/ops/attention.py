@@ -46,6 +46,18 @@ def core_attention(q, k_all, v_all, offset):
     return out.transpose(1, 2)
 
 
+def paged_block(module, proj, inv_freq, T, paged):
+    """Gated attention of one token per row over a paged cache, from the block's input projection ``proj`` [rows,
+    q | gate per head, k, v]; ``paged`` is (``paged.PagedCache``, its block, rows per group). Any device."""
+    if T != 1:
+        raise ValueError(f"a paged cache takes one token per step, got {T}")
+    cache, block, group = paged
+    Hq, D = module.cfg.num_attention_heads, module.cfg.head_dim
+    q = cache.append_(block, proj, module.q_norm.weight, module.k_norm.weight, inv_freq, Hq, module.q_norm.eps)
+    gate = proj[:, :2 * Hq * D].view(-1, Hq, 2 * D)[..., D:]
+    return cache.attend(block, q, gate, group).view(-1, 1, Hq * D)
+
+
 def attention_block(module, x, rope, state):
     cfg = module.cfg
     B, T, C = x.shape
@@ -54,6 +66,8 @@ def attention_block(module, x, rope, state):
     rot = cfg.rotary_dim
     x2 = x.reshape(B * T, C)
     proj = linear(x2, fused_weight(module, ("q_proj", "k_proj", "v_proj"), "_qkv_weight"))  # one GEMM: q|g, k, v
+    if state is not None and "paged" in state:
+        return linear(paged_block(module, proj, inv_freq, T, state["paged"]), module.o_proj.weight)
     nq, nk = module.q_proj.weight.shape[0], module.k_proj.weight.shape[0]
     qg = proj[:, :nq]                                       # [BT, Hq * 2D]: per head [q | gate]
     k = proj[:, nq:nq + nk]

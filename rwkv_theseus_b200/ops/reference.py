@@ -142,3 +142,166 @@ def top_log_probs(logits, k, scale):
     wide = z.double()  # masks of the lowest value leave fp32's range when they are scaled
     below = (wide - wide.amax(-1, keepdim=True)) * scale
     return torch.log_softmax(below, -1).gather(-1, index).to(z.dtype), index
+
+
+def place_children(parents):
+    """Slots of a group's K chosen candidates, given by rank (``parents`` [G, K]): a parent's best child keeps the
+    parent's slot, the others fill the slots that are left in order. Returns [G, K]: the rank that each slot takes."""
+    held = torch.empty_like(parents)
+    for g, row in enumerate(parents.tolist()):
+        slots = {}
+        for rank, parent in enumerate(row):
+            slots.setdefault(parent, rank)
+        rest = [rank for rank in range(len(row)) if rank not in slots.values()]
+        for slot in range(len(row)):
+            held[g, slot] = slots[slot] if slot in slots else rest.pop(0)
+    return held
+
+
+def beam_select(logits, scores, lengths, finished, end_token, length_penalty):
+    """One step of beam search over [G, K, V] (see ``beams.beam_select``), ranked in 64 bits."""
+    G, K, V = logits.shape
+    value = scores.double()[..., None] + torch.log_softmax(logits.double(), -1)
+    fit = scores.isfinite()
+    value = value.masked_fill(~((value < float("inf")) & (fit & ~finished)[..., None]), float("-inf"))
+    if end_token >= 0:
+        value[..., end_token] = torch.where(finished & fit, scores.double(), value[..., end_token])
+    length = lengths + (~finished).to(lengths.dtype)
+    rank = (value / length.clamp_min(1).double().pow(length_penalty)[..., None]).flatten(1)
+    best = rank.sort(dim=1, descending=True, stable=True)[1][:, :K]
+    best = best.gather(1, place_children(best // V))
+    parents, tokens = best // V, best % V
+    return (tokens, parents, value.flatten(1).gather(1, best).float(), length.gather(1, parents),
+            finished.gather(1, parents) | (tokens == end_token))
+
+
+def parent_rows(parents):
+    """Rows [G * K] of the parents [G, K]; an index outside a group stands for the slot itself."""
+    G, K = parents.shape
+    own = torch.arange(K, device=parents.device).expand(G, K)
+    inside = torch.where((parents >= 0) & (parents < K), parents, own)
+    return (inside + torch.arange(G, device=parents.device)[:, None] * K).flatten()
+
+
+def advance_pages(pool, table, lengths, refs, tokens, parents, live):
+    """Row after row, as ``paged.advance_pages`` defines it. Returns (table, lengths, refs, status)."""
+    pages, page, (R, width) = pool.shape[0], pool.shape[4], table.shape
+    old, length, count = table.tolist(), lengths.tolist(), refs.tolist()
+    status = 0
+    source = list(range(R))
+    if parents is not None:
+        source = parent_rows(parents).tolist()
+        status = 4 * bool(((parents < 0) | (parents >= parents.shape[1])).any())
+    alive = [True] * R if live is None else live.flatten().tolist()
+    new = [list(old[source[r]]) if alive[r] else [-1] * width for r in range(R)]
+    length = [min(max(length[source[r]], 0), width * page) if alive[r] else 0 for r in range(R)]
+    for rows, change in ((old, -1), (new, 1)):
+        for row in rows:
+            for entry in row:
+                if 0 <= entry < pages:
+                    count[entry] += change
+    free = iter([p for p in range(pages) if count[p] <= 0])
+
+    def take():
+        nonlocal status
+        found = next(free, -1)
+        if found < 0:
+            status |= 1
+        else:
+            count[found] = 1
+        return found
+
+    for r in range(R):
+        if not alive[r] or tokens == 0:
+            continue
+        have, need, fill = -(-length[r] // page), -(-(length[r] + tokens) // page), length[r] % page
+        if need > width:
+            status |= 2
+            continue
+        last = new[r][have - 1] if fill else -1
+        if 0 <= last < pages and count[last] > 1:
+            new[r][have - 1] = found = take()
+            count[last] -= 1
+            if found >= 0:
+                pool[found, ..., :fill, :] = pool[last, ..., :fill, :]
+        for slot in range(have, need):
+            new[r][slot] = take()
+        length[r] += tokens
+    return (torch.tensor(new, dtype=torch.int32).view(R, width), torch.tensor(length, dtype=torch.int32),
+            torch.tensor(count, dtype=torch.int32), torch.tensor([status], dtype=torch.int32))
+
+
+def compact_pages(pool, table, refs):
+    """Pages in use moved into the free ones before them (see ``paged.compact_pages``). Returns (table, refs, used)."""
+    taken = refs > 0
+    used = int(taken.sum())
+    holes = (~taken[:used]).nonzero()[:, 0]
+    behind = taken[used:].nonzero()[:, 0] + used
+    pool[holes] = pool[behind]
+    target = torch.arange(len(refs))
+    target[behind] = holes
+    inside = (table >= 0) & (table < len(refs))
+    table = torch.where(inside, target[table.long().clamp(0, len(refs) - 1)].to(torch.int32), table)
+    refs = refs.clone()
+    refs[holes] = refs[behind]
+    refs[behind] = 0
+    return table, refs, torch.tensor([used], dtype=torch.int32)
+
+
+def _slots(pool, table, positions):
+    """(valid, page, slot) of the positions [R, T] of each row."""
+    page = pool.shape[4]
+    at = (positions.clamp_min(0) // page).long()
+    inside = (positions >= 0) & (at < table.shape[1])
+    entry = table.gather(1, at.clamp_max(table.shape[1] - 1)).long()
+    return inside & (entry >= 0) & (entry < pool.shape[0]), entry, (positions.clamp_min(0) % page).long()
+
+
+def store_pages(pool, block, table, lengths, keys, values):
+    """``keys``, ``values`` [N, T, H, D] as the last T tokens of every (R / N)-th row."""
+    N, T = keys.shape[:2]
+    every = table.shape[0] // N
+    positions = lengths[::every, None] - T + torch.arange(T)
+    valid, entry, slot = _slots(pool, table[::every], positions)
+    for kind, x in enumerate((keys, values)):
+        pool[entry[valid], block, kind, :, slot[valid]] = x[valid].to(pool.dtype)
+
+
+def append_heads(x, pool, block, table, lengths, q_weight, k_weight, inv_freq, heads, eps):
+    """Norm and rotation of a token's queries and keys, keys and values into their pages (see ``paged.append_heads``)."""
+    H, D = pool.shape[3], pool.shape[5]
+    R = x.shape[0]
+    q = x[:, :2 * heads * D].reshape(R, heads, 2 * D)[..., :D]
+    k, v = x[:, 2 * heads * D:].reshape(R, 2, H, D).unbind(1)
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    angle = (lengths - 1).clamp_min(0).double()[:, None] * inv_freq.double()
+    cos, sin = torch.cat([angle, angle], -1).cos().to(wide), torch.cat([angle, angle], -1).sin().to(wide)
+
+    def turned(y, weight):
+        y = y.to(wide)
+        y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps) * (1.0 + weight.to(wide))
+        return apply_rope(y[None], cos, sin)[0]  # rows as time: its [B, T, H, D] has one angle per T
+
+    q, k = turned(q, q_weight), turned(k, k_weight)
+    store_pages(pool, block, table, lengths, k[:, None], v[:, None])
+    return q.to(x.dtype)
+
+
+def paged_attention(q, pool, block, table, lengths, gate):
+    """One token per row over the keys of its pages (see ``paged.paged_attention``)."""
+    R, Hq, D = q.shape
+    H, page, width = pool.shape[3], pool.shape[4], table.shape[1]
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    out = torch.zeros(R, Hq, D, dtype=wide)
+    positions = torch.arange(width * page).expand(R, -1)
+    valid, entry, slot = _slots(pool, table, positions)
+    valid = valid & (positions < lengths[:, None])
+    for r in range(R):
+        if not valid[r].any():
+            continue
+        k, v = (pool[entry[r][valid[r]], block, kind, :, slot[r][valid[r]]].to(wide) for kind in (0, 1))  # [n, H, D]
+        s = torch.einsum("hgd,nhd->hgn", q[r].to(wide).view(H, -1, D), k) * D ** -0.5
+        out[r] = torch.einsum("hgn,nhd->hgd", torch.softmax(s, -1), v).reshape(Hq, D)
+    if gate is not None:
+        out = out * torch.sigmoid(gate.to(wide))
+    return out.to(q.dtype)

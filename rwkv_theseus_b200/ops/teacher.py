@@ -146,6 +146,10 @@ def gated_attention(module, x, rope, state):
     if _cuda(x):
         from .attention import attention_block
         return attention_block(module, x, rope, state)
+    if state is not None and "paged" in state:
+        from .attention import paged_block
+        proj = torch.cat([linear(x[:, -1], w.weight) for w in (module.q_proj, module.k_proj, module.v_proj)], -1)
+        return linear(paged_block(module, proj, rope[2], T, state["paged"]), module.o_proj.weight)
     cos, sin = rope[0], rope[1]
     qg = linear(x, module.q_proj.weight).view(B, T, Hq, 2 * D)
     q, gate = qg[..., :D], qg[..., D:]
