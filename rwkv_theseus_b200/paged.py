@@ -171,7 +171,7 @@ def paged_attention(q, pool, block, table, lengths, gate=None, group=1):
     """Attention [R, Hq, dim] of one token per row over the ``lengths`` tokens of its pages in one block, scaled by
     dim^-0.5; query head h reads key head h // (Hq / heads). ``gate`` [R, Hq, dim]: the result is multiplied by its
     sigmoid. A row without tokens has zeros. ``group``: that many consecutive rows are beams of one prompt; a page
-    that several of them hold is read once (the result does not depend on it)."""
+    that several of them hold is read once (a matter of speed, and of the order in which sums are formed)."""
     _check(pool, table, lengths, block=block)
     R, H, D = table.shape[0], pool.shape[3], pool.shape[5]
     if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % H or q.shape[1] > 64 * H:
