@@ -2,18 +2,18 @@
 //
 // Bound by memory: every page that a row or its group's other beams hold has to be read once. So a block takes the
 // rows of a group together (one key head, every splits-th tile of 64 keys): of each tile it loads the pages that
-// differ between the rows, and each of them meets the queries of all rows that hold it. Roles:
-//   warp 8      finds the tile's distinct pages (a lane per row) and brings their keys and values in with TMA (128-byte
-//               swizzle, boxes of 64 components) into a ring of tiles;
-//   warps 0-3, 4-7   two groups, which take the ring's units (a tile of keys and of values) in turn, each with its own
-//               running maximum, sum and output, so that one group's barriers hide behind the other's products.
-// The products are transposed: S^T = K Q^T has the keys as the 16 rows of a matrix instruction and the (up to 8) query
-// heads of one row as its 8 columns, so a tile in registers serves all rows that hold its page and rows that do not
-// cost nothing; O^T = V^T P^T likewise, V^T by transposing loads. A warp forms the scores of 16 keys for all queries and
-// the outputs of a quarter of the components; P goes through shared memory in bf16 (2^-8 of each weight at most, the
-// rounding that the operands of the product need), sums and outputs stay fp32. At 8 queries these are mma.sync's
-// shapes: with 128 rows of queries a tcgen05 tile would be padded 16-fold, and its transposed form would need P in the
-// swizzled layout and the outputs rescaled in TMEM, for products that take half of the time that the loads take.
+// differ between the rows, and each of them meets the queries of all rows that hold it (up to 64 queries; rows that do
+// not hold it get the weight 0). Roles (192 threads):
+//   warp 2      finds the tile's distinct pages (a lane per row) and brings their keys and values into a ring with TMA
+//               (128-byte swizzle, boxes of 64 components);
+//   warp 3      issues S = Q K^T (M = 128, N = 64) into one of two TMEM buffers and O += P V (N = dim), V read MN-major.
+//               The queries are rows 0-63 of the tile; what the products make of the rows behind them, which are whatever
+//               lies in shared memory there, stays in TMEM lanes that nobody reads;
+//   warps 0, 1, 4, 5   softmax, two threads per query (32 keys each): scores against the query's reference, which is
+//               raised (O rescaled in TMEM) only where a score exceeds it by 2^8; P in bf16 (2^-8 of each weight at most,
+//               which the product needs; sums and outputs are fp32) as a swizzled tile.
+// The same with mma.sync (16 keys x 8 queries per instruction) took 76 us for eight beams of 32 k tokens at the 27B
+// heads: its operand loads alone are 2300 cycles of shared memory per tile, against 2700 that the tile's bytes leave.
 //
 // Keys that a row does not see (behind its last token, or in a missing page) get the weight 0 whatever they hold:
 // their scores are replaced, their values zeroed in shared memory.
@@ -29,13 +29,14 @@
 namespace {
 
 using bf16 = __nv_bfloat16;
-constexpr int TILE = 64, MAX_TILES = 8;  // keys of a unit; 8-query tiles of a block
-constexpr int MAX_SPLITS = 148;
+constexpr int TILE = 64, QUERIES = 64, THREADS = 192;  // keys of a unit, queries of a block
+constexpr int MAX_SPLITS = 296, UNITS = 8;
+constexpr float HEADROOM = 8.f;  // log2 that a score may exceed its reference by before that is raised
 
 struct AttendArgs {
   int pages, panels, first, kv_heads, page, width, splits;
   int rows, group, together, subgroups;  // rows of a block at most, blocks per group of beams
-  int heads, per_kv, tiles_per_row;
+  int heads, per_kv;
   const int* table;
   const int* lengths;
   const bf16* q;
@@ -46,43 +47,35 @@ struct AttendArgs {
   float scale_log2;
   bf16* out;
   float* sums;     // [rows, heads, splits, dim]
-  float2* stats;   // [rows, heads, splits]: maximum, sum of exponentials
+  float2* stats;   // [rows, heads, splits]: reference in log2 units, sum of exponentials
+};
+
+// A unit: a tile's pages as some rows hold them.
+struct Unit {
+  uint32_t members;  // rows; 0: no more units
+  int valid;         // keys before the rows' end
+  uint32_t there;    // 16-key blocks whose page exists
+  uint64_t queries;  // of the members
 };
 
 template <int D> struct Shape {
-  static constexpr int HALF = TILE * D * 2;                    // bytes of a tile of keys or of values
-  static constexpr int SLOTS = D == 256 ? 5 : D == 128 ? 6 : 8;
-  static constexpr int MTILES = D / 64;                        // of 16 components per warp
+  static constexpr int BOX = TILE * 128;                            // 64 components of a tile's keys or values
+  static constexpr int HALF = TILE * D * 2;                         // all of them
+  static constexpr int RING = D == 256 ? 5 : D == 128 ? 4 : 8;      // tiles of keys or values (two blocks per SM below 256)
+  static constexpr int P = 0, P_BYTES = QUERIES * 128;              // two tiles of weights [64][64 keys]
+  // products read 64 rows more than a tile of weights or queries has: what follows has to be as long
+  static constexpr int Q = P + 2 * P_BYTES;                         // [D / 64][64][64]
+  static constexpr int KV = Q + QUERIES * D * 2;
+  static constexpr int TABLE = KV + RING * HALF;                    // [32 rows][4][16 tiles]
+  static constexpr int MAX = TABLE + 32 * 4 * 16 * 4;               // [64 queries][2]
+  static constexpr int UNIT = MAX + QUERIES * 2 * 4;
+  static constexpr int BARS = UNIT + UNITS * 24;
+  static constexpr int BYTES = BARS + 8 * (2 * RING + UNITS + 8) + 16 + 1024;
+  static constexpr uint32_t S = D, COLUMNS = D == 256 ? 512 : 256;  // TMEM: O, then two buffers of scores
+  static constexpr uint32_t IDESC_S = sm100::idesc_bf16(128, TILE, false, false);
+  static constexpr uint32_t IDESC_O = sm100::idesc_bf16(128, D, false, true);
 };
-// Eight tiles of queries need more registers than an even split gives (168): there the loading warp's warpgroup is
-// whole and hands some of its registers over, 4 x 40 + 8 x 232 of the 12 x 168 that the block has.
-constexpr int threads(int NT) { return NT == 8 ? 384 : 288; }
-constexpr int GIVEN = 40, TAKEN = 232;
-static_assert(4 * GIVEN + 8 * TAKEN <= 12 * 168, "registers handed over");
-template <int D, int NT> constexpr int smem_bytes() {
-  return Shape<D>::SLOTS * Shape<D>::HALF + NT * 8 * D * 2 + 2 * NT * 8 * TILE * 2 + 2 * 4 * NT * 8 * 4 +
-         Shape<D>::SLOTS * 32 + 64 + 1024;
-}
 
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void stsm2_t(uint32_t addr, uint32_t a, uint32_t b) {
-  asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1,%2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
-}
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -92,107 +85,122 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// Barrier of a group of 128 threads.
-__device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ void both_sync() { asm volatile("bar.sync 3, 256;" ::: "memory"); }
-// A group's, and whether any of them says so.
-__device__ __forceinline__ bool group_any(int id, bool v) {
+// Barrier of the 128 softmax threads, and whether any of them says so.
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool softmax_any(bool v) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %2, 0;\n\t"
-      "bar.red.or.pred q, %1, 128, p;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(id), "r"((uint32_t)v)
+      : "r"((uint32_t)v)
       : "memory");
   return r != 0;
 }
+// D += A B in the TMEM lanes whose bit is set among the first 64 (the others are not written, whatever the product is).
+__device__ __forceinline__ void mma_lanes(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t lo, uint32_t hi) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %7, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %6}, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(~lo), "r"(~hi), "r"(~0u), "r"(1u)
+      : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// A unit of the ring, in the slot of its keys.
-struct Unit {
-  uint32_t tiles;  // of queries that hold its page; 0: no more units
-  int valid;       // keys before the rows' end
-  uint32_t there;  // 16-key blocks whose page exists
-};
-
-// Grid (splits, key heads, groups x subgroups). NT: 8-query tiles.
-template <int D, int NT>
-__global__ void __launch_bounds__(threads(NT), 1) attend_kernel(const __grid_constant__ CUtensorMap map, const AttendArgs a) {
-  constexpr int THREADS = threads(NT);
-  constexpr int SLOTS = Shape<D>::SLOTS, HALF = Shape<D>::HALF, MT = Shape<D>::MTILES, BOXES = D / 64;
+// Grid (splits, key heads, groups x subgroups).
+template <int D>
+__global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__ CUtensorMap map, const AttendArgs a) {
+  using Sh = Shape<D>;
+  constexpr int RING = Sh::RING, HALF = Sh::HALF, BOX = Sh::BOX, BOXES = D / 64;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = sm100::align_smem_1024(raw);
-  uint8_t* sQ = smem + SLOTS * HALF;                                   // [NT * 8][D], 16-byte chunks swizzled by row
-  uint8_t* sP = sQ + NT * 8 * D * 2;                                   // per group [NT * 8][64 keys], likewise
-  float* sMax = reinterpret_cast<float*>(sP + 2 * NT * 8 * TILE * 2);  // per group [4 warps][NT * 8]
-  Unit* units = reinterpret_cast<Unit*>(sMax + 2 * 4 * NT * 8);        // [SLOTS]
-  uint64_t* full = reinterpret_cast<uint64_t*>(units + SLOTS + (SLOTS & 1));
-  uint64_t* empty = full + SLOTS;
-  volatile int* abort = reinterpret_cast<volatile int*>(empty + SLOTS);
+  uint8_t *sP = smem + Sh::P, *sQ = smem + Sh::Q, *sKV = smem + Sh::KV;
+  int* sTable = reinterpret_cast<int*>(smem + Sh::TABLE);
+  float* sMax = reinterpret_cast<float*>(smem + Sh::MAX);
+  Unit* units = reinterpret_cast<Unit*>(smem + Sh::UNIT);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sh::BARS);  // a tile of the ring has landed
+  uint64_t* empty = full + RING;                                  // its products are done
+  uint64_t* known = empty + RING;                                 // [UNITS] a unit's description is there
+  uint64_t* q_full = known + UNITS;
+  uint64_t* s_full = q_full + 1;  // [2]
+  uint64_t* p_full = s_full + 2;  // [2]
+  uint64_t* o_done = p_full + 2;  // [2]
+  uint64_t* drain = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = blockIdx.x, kv = blockIdx.y, g = blockIdx.z / a.subgroups, sub = blockIdx.z % a.subgroups;
   const int row0 = g * a.group + sub * a.together, rows = min(a.together, a.group - sub * a.together);
   if (tid == 0) {
-    for (int i = 0; i < SLOTS; ++i) {
+    for (int i = 0; i < RING; ++i) {
       sm100::mbar_init(&full[i], 1);
-      sm100::mbar_init(&empty[i], 4);
+      sm100::mbar_init(&empty[i], 1);
     }
+    for (int i = 0; i < UNITS; ++i) sm100::mbar_init(&known[i], 1);
+    sm100::mbar_init(q_full, 128);
+    for (int i = 0; i < 2; ++i) {
+      sm100::mbar_init(&s_full[i], 1);
+      sm100::mbar_init(&p_full[i], 128);
+      sm100::mbar_init(&o_done[i], 1);
+    }
+    sm100::mbar_init(drain, 1);
     *abort = 0;
     sm100::fence_barrier_init();
   }
-  // queries: row r's head h is query r * tiles_per_row * 8 + h; the others are zero
-  const int row_queries = a.tiles_per_row * 8;
-  for (int i = tid; i < NT * 8 * (D / 8); i += THREADS) {
-    const int n = i / (D / 8), c = i % (D / 8), r = n / row_queries, h = n % row_queries;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < rows && h < a.per_kv) {
-      const bf16* x = a.q + (row0 + r) * a.q_row + (long)(kv * a.per_kv + h) * a.q_head + c * 8;
-      if (a.q_vec) {
-        v = *reinterpret_cast<const uint4*>(x);
-      } else {
-        bf16* e = reinterpret_cast<bf16*>(&v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = x[j];
-      }
-    }
-    *reinterpret_cast<uint4*>(sQ + n * D * 2 + ((c ^ (n & 7)) << 4)) = v;
+  if (warp == 3) {
+    sm100::tmem_alloc(tmem_slot, Sh::COLUMNS);
+    sm100::tmem_relinquish();
   }
+  sm100::tc_fence_before();
   __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 8) {
-    if (NT == 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(GIVEN));
-    if (warp > 8) return;
-    // ------------------------------------------------------------ producer
+  if (warp == 2) {
+    // ------------------------------------------------------------ loads
+    if (lane == 0) sm100::prefetch_tmap(&map);
     const int capacity = a.width * a.page, span = TILE / a.page;  // pages of a tile
     const int length = lane < rows ? min(max(a.lengths[row0 + lane], 0), capacity) : 0;
     const int longest = __reduce_max_sync(~0u, length);
-    const int* table = a.table + (long)(row0 + (lane < rows ? lane : 0)) * a.width;
     const int count = (longest + TILE - 1) / TILE;
-    auto entries = [&](int i, int (&e)[4]) {  // this row's pages of a tile, -1: none
+    // The rows' pages of the block's next 16 tiles, a lane per tile, so that their loads wait for memory together
+    // (-1: no such page); sTable[(row * 4 + j) * 16 + tile].
+    auto look_up = [&](int first, int step) {
+      const int i = first + lane * step;
+      for (int r0 = 0; r0 < rows; r0 += 8) {
+        int e[8][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        e[j] = -1;
-        if (j < span && i < count && i * TILE + j * a.page < length) {
-          const int p = table[i * span + j];
-          if (p >= 0 && p < a.pages) e[j] = p;
+        for (int r = 0; r < 8; ++r) {
+          const int n = __shfl_sync(~0u, length, (r0 + r) & 31);  // 0 behind the last row
+          const int* table = a.table + (long)(row0 + r0 + r) * a.width;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            e[r][j] = lane < 16 && j < span && i < count && i * TILE + j * a.page < n ? table[i * span + j] : -1;
         }
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (lane < 16) sTable[((r0 + r) * 4 + j) * 16 + lane] = e[r][j] < a.pages ? max(e[r][j], -1) : -1;
       }
+      __syncwarp();
     };
-    if (lane == 0) sm100::prefetch_tmap(&map);
-    int next[4], entry = 0;
-    entries(split, next);
+    const uint64_t one = a.per_kv == 64 ? ~0ull : (1ull << a.per_kv) - 1;  // the queries of row 0
+    int entry = 0, unit = 0;  // tiles of the ring (keys, values, keys, ...) and units so far
     bool ok = true;
-    auto wait_empty = [&](int slot) {
-      if (entry >= SLOTS && !sm100::mbar_wait(&empty[slot], (entry / SLOTS - 1) & 1, abort)) ok = false;
-      ok = __all_sync(~0u, ok);
-    };
-    for (int i = split; i < count && ok; i += a.splits) {
+    // The tiles are dealt out to the splits in turn; of the last 16, where beams have gone apart, the units one by one.
+    const int tail = max(count - 16, 0);
+    int dealt = tail;  // units before the next one, where they are dealt out
+    for (int i = split < tail ? split : tail, t = 0; i < count && ok; t = (t + 1) & 15) {
+      const bool single = i >= tail;
+      if (t == 0) look_up(i, single ? 1 : a.splits);
       int e[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) e[j] = next[j];
-      entries(i + a.splits, next);
+      for (int j = 0; j < 4; ++j) e[j] = lane < rows ? sTable[(lane * 4 + j) * 16 + t] : -1;
       const int valid = min(max(length - i * TILE, 0), TILE);
       unsigned same = __match_any_sync(~0u, valid);
       bool any = false;
@@ -206,26 +214,30 @@ __global__ void __launch_bounds__(threads(NT), 1) attend_kernel(const __grid_con
       unsigned left = __ballot_sync(~0u, any && valid > 0);
       while (left && ok) {
         const int leader = __ffs(left) - 1;
-        const unsigned members = __shfl_sync(~0u, same, leader);
-        left &= ~members;
         Unit u;
+        u.members = __shfl_sync(~0u, same, leader);
         u.valid = __shfl_sync(~0u, valid, leader);
         u.there = __shfl_sync(~0u, there, leader);
-        u.tiles = 0;
-        for (unsigned r = members; r; r &= r - 1)
-          u.tiles |= ((1u << a.tiles_per_row) - 1) << ((__ffs(r) - 1) * a.tiles_per_row);
+        left &= ~u.members;
+        if (single && dealt++ % a.splits != split) continue;
+        u.queries = 0;
+        for (uint32_t k = u.members; k; k &= k - 1) u.queries |= one << ((__ffs(k) - 1) * a.per_kv);
         int p[4], here = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           p[j] = __shfl_sync(~0u, e[j], leader);
           here += p[j] >= 0;
         }
-        for (int kind = 0; kind < 2 && ok; ++kind, ++entry) {
-          const int slot = entry % SLOTS;
-          wait_empty(slot);
+        for (int kind = 0; kind < 2; ++kind) {
+          const int slot = entry % RING;
+          ok = __all_sync(~0u, entry < RING || sm100::mbar_wait(&empty[slot], (entry / RING - 1) & 1, abort));
           if (!ok) break;
           if (lane == 0) {
-            if (kind == 0) units[slot] = u;
+            if (kind == 0) {
+              // eight units before this one the softmax is done: the ring holds four at most
+              units[unit % UNITS] = u;
+              sm100::mbar_arrive(&known[unit % UNITS]);
+            }
             sm100::mbar_expect_tx(&full[slot], here * a.page * D * 2);
           }
           __syncwarp();
@@ -233,283 +245,351 @@ __global__ void __launch_bounds__(threads(NT), 1) attend_kernel(const __grid_con
           const int page = j == 0 ? p[0] : j == 1 ? p[1] : j == 2 ? p[2] : p[3];
           if (j < span && page >= 0) {
             const int y = (page * a.panels + a.first + kind * a.kv_heads + kv) * a.page;
-            sm100::tma_load_2d(smem + slot * HALF + box * (TILE * 128) + j * a.page * 128, &map, &full[slot], box * 64, y);
+            sm100::tma_load_2d(sKV + slot * HALF + box * BOX + j * a.page * 128, &map, &full[slot], box * 64, y);
           }
           __syncwarp();
+          ++entry;
         }
+        ++unit;
+      }
+      __syncwarp();
+      if (single) {
+        ++i;
+      } else if ((i += a.splits) >= tail) {
+        i = tail;
+        t = 15;  // looked up anew
       }
     }
-    // both groups' ends
-    for (int i = 0; i < 2 && ok; ++i) {
-      const int slot = entry % SLOTS;
-      wait_empty(slot);
-      if (ok && lane == 0) {
-        units[slot].tiles = 0;
-        sm100::mbar_arrive(&full[slot]);
-      }
-      entry += 2;
+    if (ok && lane == 0) {
+      units[unit % UNITS].members = 0;
+      sm100::mbar_arrive(&known[unit % UNITS]);
     }
-    if (!ok)  // copies in flight have to land before the block ends
-      for (int i = max(entry - SLOTS, 0); i < entry; ++i) sm100::mbar_wait_bounded(&full[i % SLOTS], (i / SLOTS) & 1);
-    return;
-  }
-
-  // -------------------------------------------------------------- groups
-  if (NT == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TAKEN));
-  const int grp = warp >> 2, w = warp & 3;
-  float o[NT][MT][4], m[NT][2], l[NT][2];
+    // copies in flight have to land before the block ends (all have where the products were done)
+    if (!ok)
+      for (int i = max(entry - RING, 0); i < entry; ++i) sm100::mbar_wait_bounded(&full[i % RING], (i / RING) & 1);
+  } else if (warp == 3) {
+    // ------------------------------------------------------------ products
+    if (sm100::elect_one()) {
+      const uint32_t qb = sm100::smem_u32(sQ);
+      bool ok = sm100::mbar_wait(q_full, 0, abort), last = false;
+      auto scores = [&](int u) {  // of unit u, unless there is none
+        if (!sm100::mbar_wait(&known[u % UNITS], (u / UNITS) & 1, abort)) return false;
+        if (units[u % UNITS].members == 0) {
+          last = true;
+          return true;
+        }
+        const int entry = 2 * u, slot = entry % RING;
+        if (!sm100::mbar_wait(&full[slot], (entry / RING) & 1, abort)) return false;
+        sm100::tc_fence_after();
+        const uint32_t kb = sm100::smem_u32(sKV + slot * HALF);
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t ad = sm100::smem_desc(qb + (k >> 2) * BOX + (k & 3) * 32, 16, 1024);
+          const uint64_t bd = sm100::smem_desc(kb + (k >> 2) * BOX + (k & 3) * 32, 16, 1024);
+          sm100::mma_bf16(tmem + Sh::S + (u & 1) * TILE, ad, bd, Sh::IDESC_S, k > 0);
+        }
+        sm100::mma_commit(&s_full[u & 1]);
+        sm100::mma_commit(&empty[slot]);
+        return true;
+      };
+      if (ok) ok = scores(0);
+      int end = last ? 0 : 1;  // units whose scores are formed
+      if (ok && !last) {
+        ok = scores(1);
+        end += !last;
+      }
+      for (int u = 0; ok && u < end; ++u) {
+        const int entry = 2 * u + 1, slot = entry % RING;
+        if (!sm100::mbar_wait(&p_full[u & 1], (u >> 1) & 1, abort)) break;
+        if (!sm100::mbar_wait(&full[slot], (entry / RING) & 1, abort)) break;
+        sm100::tc_fence_after();
+        const uint64_t queries = units[u % UNITS].queries;
+        const uint32_t pb = sm100::smem_u32(sP + (u & 1) * Sh::P_BYTES), vb = sm100::smem_u32(sKV + slot * HALF);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.f;
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.f;
-  }
-  {
-    const uint32_t q_base = sm100::smem_u32(sQ), p_base = sm100::smem_u32(sP) + grp * NT * 8 * TILE * 2;
-    float* top = sMax + grp * 4 * NT * 8;
-    const int bar = 1 + grp, t2 = 2 * (lane & 3);
-    for (int u = grp;; u += 2) {
-      const int ke = 2 * u, ks = ke % SLOTS, vs = (ke + 1) % SLOTS;
-      // what ends the loop is agreed on at the group's first barrier, whichever thread's wait gives up
-      bool bad = __any_sync(~0u, !sm100::mbar_wait(&full[ks], (ke / SLOTS) & 1, abort));
-      const Unit unit = units[ks];
-      const bool done = bad || unit.tiles == 0;
-      const uint32_t k_base = sm100::smem_u32(smem) + ks * HALF, v_base = sm100::smem_u32(smem) + vs * HALF;
-      float s[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-      if (!done) {
-        const int r = w * 16 + (lane & 15);
-        const uint32_t row = k_base + r * 128;
-#pragma unroll 4
-        for (int kk = 0; kk < D / 32; ++kk) {
-          uint32_t a0[4], a1[4];
-          const uint32_t box = row + (kk >> 1) * (TILE * 128);
-          const int c = (kk & 1) * 4 + (lane >> 4);
-          ldsm4(a0, box + ((c ^ (r & 7)) << 4));
-          ldsm4(a1, box + (((c + 2) ^ (r & 7)) << 4));
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            if (unit.tiles >> n & 1) {
-              uint32_t b[4];
-              const int x = lane & 7;
-              ldsm4(b, q_base + (n * 8 + x) * D * 2 + (((kk * 4 + (lane >> 3)) ^ x) << 4));
-              mma(s[n], a0, b[0], b[1]);
-              mma(s[n], a1, b[2], b[3]);
-            }
+        for (int k = 0; k < TILE / 16; ++k) {
+          const uint64_t ad = sm100::smem_desc(pb + k * 32, 16, 1024);
+          const uint64_t bd = sm100::smem_desc(vb + k * 2048, BOX, 1024);
+          mma_lanes(tmem, ad, bd, Sh::IDESC_O, (uint32_t)queries, (uint32_t)(queries >> 32));
+        }
+        sm100::mma_commit(&o_done[u & 1]);
+        sm100::mma_commit(&empty[slot]);
+        if (!last) {
+          ok = scores(u + 2);
+          end += !last;
         }
       }
-      if (!done) {
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&empty[ks]);
-        // keys lane / 4 and lane / 4 + 8 of this warp's 16, queries t2 and t2 + 1 of each tile
-        const int key = w * 16 + (lane >> 2);
-        const bool block = unit.there >> w & 1, see0 = block && key < unit.valid, see1 = block && key + 8 < unit.valid;
+      sm100::mma_commit(drain);
+      sm100::mbar_wait_bounded(drain, 0);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int half = warp >> 2, n = (warp & 1) * 32 + lane, st128 = (half * 2 + (warp & 1)) * 32 + lane;
+    const int row = n / a.per_kv, h = n % a.per_kv;
+    const bool used = row < rows;  // a query, of row0 + row
+    // queries into the product's layout; those that do not exist have weights 0
+    {
+      constexpr int EACH = QUERIES * D / 8 / 128;  // 16-byte words of a thread
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          if (unit.tiles >> n & 1) {
-            if (!see0) s[n][0] = s[n][1] = -INFINITY;
-            if (!see1) s[n][2] = s[n][3] = -INFINITY;
-            float x = fmaxf(s[n][0], s[n][2]), y = fmaxf(s[n][1], s[n][3]);
+      for (int k0 = 0; k0 < EACH; k0 += 8) {
+        uint4 v[8];
 #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) {
-              x = fmaxf(x, __shfl_xor_sync(~0u, x, off));
-              y = fmaxf(y, __shfl_xor_sync(~0u, y, off));
+        for (int k = 0; k < 8; ++k) {
+          const int i = (k0 + k) * 128 + st128, m = i / (D / 8), c = i % (D / 8), r = m / a.per_kv;
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (k0 + k < EACH && r < rows) {
+            const bf16* x = a.q + (row0 + r) * a.q_row + (long)(kv * a.per_kv + m % a.per_kv) * a.q_head + c * 8;
+            if (a.q_vec) {
+              v[k] = *reinterpret_cast<const uint4*>(x);
+            } else {
+              bf16* e = reinterpret_cast<bf16*>(&v[k]);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) e[j] = x[j];
             }
-            if (lane < 4) *reinterpret_cast<float2*>(top + w * NT * 8 + n * 8 + t2) = make_float2(x, y);
           }
-        bad = !sm100::mbar_wait(&full[vs], ((ke + 1) / SLOTS) & 1, abort);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int i = (k0 + k) * 128 + st128, m = i / (D / 8), c = i % (D / 8);
+          if (k0 + k < EACH) *reinterpret_cast<uint4*>(sQ + (c >> 3) * BOX + m * 128 + (((c & 7) ^ (m & 7)) << 4)) = v[k];
+        }
       }
-      if (group_any(bar, done || bad)) break;
-      const bool partial = unit.valid < TILE || unit.there != 15u;
-      if (partial) {
-        const int t = tid & 127;
-        for (int i = t; i < TILE * D / 8; i += 128) {  // boxes of 64 rows of 8 chunks
+      fence_proxy_async();
+      sm100::mbar_arrive(q_full);
+    }
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 1) * 32) << 16);
+    {  // products add to O from the first on (the first product waits for these threads' first weights)
+      float zero[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) zero[i] = 0.f;
+#pragma unroll 1
+      for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) sm100::tmem_st32(lanes + c, zero);
+      sm100::tmem_wait_st();
+    }
+    float m = -INFINITY, l = 0.f;
+    int u = 0;
+    bool bad = false;
+    for (;; ++u) {
+      const int st = u & 1;
+      // what ends the loop is agreed on at the first barrier, whichever thread's wait gives up
+      if (!bad) bad = !sm100::mbar_wait(&known[u % UNITS], (u / UNITS) & 1, abort);
+      bad = __any_sync(~0u, bad);
+      const Unit unit = units[u % UNITS];
+      bool done = bad || unit.members == 0;
+      if (!done) done = bad = __any_sync(~0u, !sm100::mbar_wait(&s_full[st], (u >> 1) & 1, abort));
+      const bool member = used && (unit.members >> row & 1), partial = unit.valid < TILE || unit.there != 15u;
+      float s[32];
+      bool higher = false;  // a score far above the reference (or NaN, or the first): look at the maxima
+      if (!done) {
+        sm100::tc_fence_after();
+        sm100::tmem_ld32(lanes + Sh::S + st * TILE + half * 32, s);
+        sm100::tmem_wait_ld();
+        if (partial) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (half * 32 + i >= unit.valid || !(unit.there >> (half * 2 + i / 16) & 1)) s[i] = -INFINITY;
+        }
+        if (member) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            s[i] *= a.scale_log2;
+            higher |= !(s[i] - m <= HEADROOM);
+          }
+        }
+      }
+      if (softmax_any(done || higher)) {
+        if (softmax_any(done)) break;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
+        sMax[n * 2 + half] = top;
+        softmax_sync();
+        top = fmaxf(m, fmaxf(sMax[n * 2], sMax[n * 2 + 1]));
+        const float keep = !member || top == m ? 1.f : ex2(m - top);  // (m of -inf: sums and outputs are 0 so far)
+        if (member) {
+          m = top;
+          l *= keep;
+        }
+        if (u > 0) {  // O must hold what came before it is rescaled
+          bad = __any_sync(~0u, !sm100::mbar_wait(&o_done[(u - 1) & 1], ((u - 1) >> 1) & 1, abort));
+          if (!bad && __any_sync(~0u, keep != 1.f)) {
+            sm100::tc_fence_after();
+#pragma unroll 1
+            for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
+              float o[32];
+              sm100::tmem_ld32(lanes + c, o);
+              sm100::tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] *= keep;
+              sm100::tmem_st32(lanes + c, o);
+            }
+            sm100::tmem_wait_st();
+          }
+        }
+      }
+      // the buffer of weights was last read by the product of unit u - 2
+      if (u >= 2) bad |= __any_sync(~0u, !sm100::mbar_wait(&o_done[st], ((u - 2) >> 1) & 1, abort));
+      if (partial) {  // values that nobody sees
+        const int entry = 2 * u + 1, slot = entry % RING;
+        bad |= __any_sync(~0u, !sm100::mbar_wait(&full[slot], (entry / RING) & 1, abort));
+        for (int i = st128; i < TILE * D / 8; i += 128) {  // boxes of 64 rows of 8 words
           const int r = i / 8 % TILE;
           if (r >= unit.valid || !(unit.there >> (r / 16) & 1))
-            *reinterpret_cast<uint4*>(smem + vs * HALF + i * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(sKV + slot * HALF + i * 16) = make_uint4(0, 0, 0, 0);
         }
       }
+      const float base = m == -INFINITY ? 0.f : m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint8_t* weights = sP + st * Sh::P_BYTES + n * 128;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-        if (unit.tiles >> n & 1) {
-          float2 mx = make_float2(m[n][0], m[n][1]);
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        if (member) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 x = *reinterpret_cast<const float2*>(top + i * NT * 8 + n * 8 + t2);
-            mx.x = fmaxf(mx.x, x.x);
-            mx.y = fmaxf(mx.y, x.y);
+            const float x = ex2(s[c * 8 + 2 * i] - base), y = ex2(s[c * 8 + 2 * i + 1] - base);
+            sum[i] += x + y;
+            w[i] = pack(x, y);
           }
-          // (relative to 0 while nothing is seen: every weight is 0 then)
-          const float bx = mx.x == -INFINITY ? 0.f : mx.x, by = mx.y == -INFINITY ? 0.f : mx.y;
-          const float kx = ex2((m[n][0] - bx) * a.scale_log2), ky = ex2((m[n][1] - by) * a.scale_log2);
-          m[n][0] = mx.x;
-          m[n][1] = mx.y;
-          s[n][0] = ex2((s[n][0] - bx) * a.scale_log2);
-          s[n][1] = ex2((s[n][1] - by) * a.scale_log2);
-          s[n][2] = ex2((s[n][2] - bx) * a.scale_log2);
-          s[n][3] = ex2((s[n][3] - by) * a.scale_log2);
-          l[n][0] = l[n][0] * kx + (s[n][0] + s[n][2]);
-          l[n][1] = l[n][1] * ky + (s[n][1] + s[n][3]);
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            o[n][t][0] *= kx;
-            o[n][t][1] *= ky;
-            o[n][t][2] *= kx;
-            o[n][t][3] *= ky;
-          }
-          // transposed: row = query, column = key
-          const int x = lane & 7;
-          stsm2_t(p_base + (n * 8 + x) * TILE * 2 + (((w * 2 + ((lane >> 3) & 1)) ^ x) << 4), pack(s[n][0], s[n][1]),
-                  pack(s[n][2], s[n][3]));
         }
-      group_sync(bar);
-#pragma unroll
-      for (int kp = 0; kp < 2; ++kp) {
-        uint32_t v[2][MT][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            const int d = w * (D / 4) + t * 16, r = (kp * 2 + h) * 16 + (lane & 7) + (lane >> 4) * 8;
-            const int c = (d & 63) / 8 + ((lane >> 3) & 1);
-            ldsm4_t(v[h][t], v_base + (d >> 6) * (TILE * 128) + r * 128 + ((c ^ (r & 7)) << 4));
-          }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          if (unit.tiles >> n & 1) {
-            uint32_t b[4];
-            const int x = lane & 7;
-            ldsm4(b, p_base + (n * 8 + x) * TILE * 2 + (((kp * 4 + (lane >> 3)) ^ x) << 4));
-#pragma unroll
-            for (int t = 0; t < MT; ++t) {
-              mma(o[n][t], v[0][t], b[0], b[1]);
-              mma(o[n][t], v[1][t], b[2], b[3]);
-            }
-          }
+        *reinterpret_cast<uint4*>(weights + (((half * 4 + c) ^ (n & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      if (partial) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // zeros, then the next copy
-      __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&empty[vs]);
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      fence_proxy_async();
+      sm100::tc_fence_before();
+      sm100::mbar_arrive(&p_full[st]);
+    }
+    // ---- result: u units were seen (bad: it is none)
+    if (u > 0 && !bad) bad = !sm100::mbar_wait(&o_done[(u - 1) & 1], ((u - 1) >> 1) & 1, abort);
+    sMax[n * 2 + half] = l;
+    bad = softmax_any(bad || *abort);
+    sm100::tc_fence_after();
+    const long at = ((long)(row0 + row) * a.heads + kv * a.per_kv + h) * a.splits + split;
+    if (used && half == 0) a.stats[at] = make_float2(m, bad ? NAN : sMax[n * 2] + sMax[n * 2 + 1]);
+    // rows through shared memory (16 bytes apart beyond their size), half of a row with one copy; the ring has had its use
+    float* line = reinterpret_cast<float*>(sKV) + n * (D + 4) + half * (D / 2);
+#pragma unroll 1
+    for (int c = 0; c < D / 2; c += 32) {
+      float o[32];
+      sm100::tmem_ld32(lanes + half * (D / 2) + c, o);
+      sm100::tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(line + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+    }
+    fence_proxy_async();
+    if (used && !bad) {
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.sums + at * D + half * (D / 2)),
+                   "r"(sm100::smem_u32(line)), "r"(D * 2)
+                   : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
   }
-  both_sync();
-  if (*abort)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) l[n][0] = l[n][1] = NAN;  // a wait that gave up: no result
-
-  // ---- the groups' results joined: the second's through shared memory, sums over the warps' keys
-  float* out1 = reinterpret_cast<float*>(smem);                   // [NT * 8][D] of the second group
-  float2* ml = reinterpret_cast<float2*>(smem + NT * 8 * D * 4);  // [2 groups][4 warps][NT * 8]: maximum, sum
-  {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float x = l[n][j];
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) x += __shfl_xor_sync(~0u, x, off);
-        if (lane < 4) ml[(grp * 4 + w) * NT * 8 + n * 8 + 2 * lane + j] = make_float2(m[n][j], x);
-      }
-    }
-    if (grp == 1)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int d = w * (D / 4) + t * 16 + (lane >> 2) + (i >> 1) * 8, q = n * 8 + 2 * (lane & 3) + (i & 1);
-            out1[q * D + d] = o[n][t][i];
-          }
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (warp == 3) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, Sh::COLUMNS);
   }
-  both_sync();
-  if (grp == 1) return;
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int q = n * 8 + 2 * (lane & 3) + j, r = q / row_queries, h = q % row_queries;
-      if (r >= rows || h >= a.per_kv) continue;
-      const float m0 = ml[q].x, m1 = ml[4 * NT * 8 + q].x, mx = fmaxf(m0, m1), base = mx == -INFINITY ? 0.f : mx;
-      const float w0 = ex2((m0 - base) * a.scale_log2), w1 = ex2((m1 - base) * a.scale_log2);
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum += w0 * ml[i * NT * 8 + q].y + w1 * ml[(4 + i) * NT * 8 + q].y;
-      const long at = ((long)(row0 + r) * a.heads + kv * a.per_kv + h) * a.splits + split;
-      if (w == 0 && (lane >> 2) == 0) a.stats[at] = make_float2(mx, sum);
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int d = w * (D / 4) + t * 16 + (lane >> 2) + i * 8;
-          a.sums[at * D + d] = w0 * o[n][t][2 * i + j] + w1 * out1[q * D + d];
-        }
-    }
 }
 
-// Block per (row, query head), a thread per component.
-__global__ void join_kernel(const AttendArgs a, int D) {
+// Block of 256 threads per (row, query head): the splits' weights first, then their sums, a thread per four components of
+// every (256 / (D / 4))-th split, so that all of them are loaded at once.
+__global__ void __launch_bounds__(256) join_kernel(const AttendArgs a, int D) {
+  __shared__ float weight[MAX_SPLITS], scratch[32];
+  __shared__ float4 parts[256];
   const long rh = blockIdx.x;
-  const int head = rh % a.heads, row = rh / a.heads, c = threadIdx.x;
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int i = 0; i < a.splits; ++i) m = fmaxf(m, a.stats[rh * a.splits + i].x);
-  for (int i = 0; i < a.splits; ++i) {
-    const float2 st = a.stats[rh * a.splits + i];
-    if (st.y == 0.f) continue;
-    const float w = st.x == m ? 1.f : ex2((st.x - m) * a.scale_log2);
-    l += w * st.y;
-    o += w * a.sums[(rh * a.splits + i) * D + c];
+  const int head = rh % a.heads, row = rh / a.heads, tid = threadIdx.x, wide = D / 4, c = tid % wide, first = tid / wide;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float2 st[2];
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = j * 256 + tid;
+    st[j] = i < a.splits ? a.stats[rh * a.splits + i] : make_float2(-INFINITY, 0.f);
+    m = fmaxf(m, st[j].x);
   }
-  o = l == 0.f ? 0.f : o / l;
-  if (a.gate) o *= rt::sigmoidf_(rt::to_f(a.gate[row * a.gate_row + head * a.gate_head + c]));
-  a.out[rh * D + c] = __float2bfloat16_rn(o);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, off));
+  if ((tid & 31) == 0) scratch[tid >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, scratch[w]);
+  float l = 0.f;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = j * 256 + tid;
+    // (a split that saw nothing has the sum 0 and the reference -inf)
+    const float w = st[j].y == 0.f ? 0.f : st[j].x == m ? 1.f : ex2(st[j].x - m);
+    if (i < a.splits) weight[i] = w;
+    l += w * st[j].y;
+  }
+  l = rt::block_sum(l, scratch);
+  const float4* sums = reinterpret_cast<const float4*>(a.sums) + rh * a.splits * wide + c;
+  const int step = 256 / wide;
+#pragma unroll 10
+  for (int i = first; i < a.splits; i += step) {
+    const float w = weight[i];
+    const float4 x = sums[(long)i * wide];
+    o.x += w * x.x;
+    o.y += w * x.y;
+    o.z += w * x.z;
+    o.w += w * x.w;
+  }
+  parts[tid] = o;
+  __syncthreads();
+  if (tid >= wide) return;
+  for (int i = 1; i < step; ++i) {
+    const float4 x = parts[i * wide + tid];
+    o.x += x.x;
+    o.y += x.y;
+    o.z += x.z;
+    o.w += x.w;
+  }
+  float v[4] = {o.x, o.y, o.z, o.w};
+  __nv_bfloat16 r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float y = l == 0.f ? 0.f : v[j] / l;
+    if (a.gate) y *= rt::sigmoidf_(rt::to_f(a.gate[row * a.gate_row + head * a.gate_head + tid * 4 + j]));
+    r[j] = __float2bfloat16_rn(y);
+  }
+  *reinterpret_cast<uint2*>(a.out + rh * D + tid * 4) = *reinterpret_cast<const uint2*>(r);
 }
 
-// How a call is cut: rows of a group that fit a block's query tiles together, evenly; splits of the keys so that the
-// blocks fill the SMs once (one block each), but no finer than the cache's tiles.
+// How a call is cut: rows of a group that fit a block's queries (and a lane each) together, evenly; splits of the keys
+// so that the blocks fill the SMs once, but no finer than the cache's tiles.
 struct Plan {
-  int tiles_per_row, together, subgroups, splits;
+  int together, subgroups, splits;
 };
 Plan plan_for(const RtPool* p, int heads, int group) {
   Plan x;
-  x.tiles_per_row = (heads / p->heads + 7) / 8;
-  const int most = std::max(1, MAX_TILES / x.tiles_per_row);
+  const int most = std::min(32, QUERIES / (heads / p->heads));
   x.subgroups = (group + most - 1) / most;
   x.together = (group + x.subgroups - 1) / x.subgroups;
   x.subgroups = (group + x.together - 1) / x.together;
   const long blocks = (long)(p->rows / group) * x.subgroups * p->heads;
   const long tiles = ((long)p->width * p->page + TILE - 1) / TILE;
-  x.splits = (int)std::max(1L, std::min({tiles, 148 / blocks, (long)MAX_SPLITS}));
+  x.splits = (int)std::max(1L, std::min({tiles, (p->dim == 256 ? 148 : 296) / blocks, (long)MAX_SPLITS}));
   return x;
 }
 
-template <int D, int NT>
+template <int D>
 cudaError_t launch(const CUtensorMap& map, const AttendArgs& a, const Plan& x, cudaStream_t s) {
-  constexpr int bytes = smem_bytes<D, NT>();
-  static_assert(bytes <= 227 * 1024, "shared memory of a block");
-  static_assert(NT * 8 * D * 4 + 8 * NT * 8 * 8 <= Shape<D>::SLOTS * Shape<D>::HALF, "the join fits the ring");
+  constexpr int bytes = Shape<D>::BYTES;
+  static_assert(bytes <= (D == 256 ? 227 : 113) * 1024, "shared memory of a block");
   // The limit belongs to the device and not to the call, so it is raised once.
   static std::atomic<uint64_t> set{0};  // devices
   int dev = 0;
   RT_CUDA_CHECK(cudaGetDevice(&dev));
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (!bit || !(set.load(std::memory_order_acquire) & bit)) {
-    RT_CUDA_CHECK(cudaFuncSetAttribute(attend_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    RT_CUDA_CHECK(cudaFuncSetAttribute(attend_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     set.fetch_or(bit, std::memory_order_acq_rel);
   }
   const dim3 grid((unsigned)x.splits, (unsigned)a.kv_heads, (unsigned)(a.rows / a.group * x.subgroups));
-  attend_kernel<D, NT><<<grid, threads(NT), bytes, s>>>(map, a);
+  attend_kernel<D><<<grid, THREADS, bytes, s>>>(map, a);
   return cudaGetLastError();
-}
-template <int D>
-cudaError_t launch(const CUtensorMap& map, const AttendArgs& a, const Plan& x, cudaStream_t s) {
-  const int tiles = x.together * x.tiles_per_row;
-  if (tiles <= 1) return launch<D, 1>(map, a, x, s);
-  if (tiles <= 2) return launch<D, 2>(map, a, x, s);
-  if (tiles <= 4) return launch<D, 4>(map, a, x, s);
-  return launch<D, 8>(map, a, x, s);
 }
 
 }  // namespace
@@ -519,12 +599,12 @@ extern "C" long rt_paged_attention_workspace_floats(const RtPool* p, int heads, 
 }
 
 // q [rows, heads, dim] and gate (or null) with strides in elements, unit inner stride; out contiguous; work:
-// rt_paged_attention_workspace_floats, 8-byte aligned. Results are NaN if a bounded wait gave up.
+// rt_paged_attention_workspace_floats, 16-byte aligned. Results are NaN if a bounded wait gave up.
 extern "C" cudaError_t rt_paged_attention(const RtPool* p, int block, const int* table, const int* lengths,
                                           const void* q, long q_row, long q_head, int heads, const void* gate,
                                           long gate_row, long gate_head, int group, void* out, float* work,
                                           cudaStream_t s) {
-  if (block < 0 || block >= p->blocks || heads < 1 || heads % p->heads || heads > 64 * p->heads || group < 1 ||
+  if (block < 0 || block >= p->blocks || heads < 1 || heads % p->heads || heads > QUERIES * p->heads || group < 1 ||
       p->rows < 1 || p->rows % group || p->heads > 65535 || (p->page != 16 && p->page != 32 && p->page != 64) ||
       (long)p->width * p->page > INT_MAX - TILE || reinterpret_cast<uintptr_t>(p->pool) % 16)
     return cudaErrorInvalidValue;
@@ -545,7 +625,6 @@ extern "C" cudaError_t rt_paged_attention(const RtPool* p, int block, const int*
   a.subgroups = x.subgroups;
   a.heads = heads;
   a.per_kv = heads / p->heads;
-  a.tiles_per_row = x.tiles_per_row;
   a.table = table;
   a.lengths = lengths;
   a.q = static_cast<const bf16*>(q);
@@ -557,8 +636,8 @@ extern "C" cudaError_t rt_paged_attention(const RtPool* p, int block, const int*
   a.gate_head = gate_head;
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)p->dim);
   a.out = static_cast<bf16*>(out);
-  a.stats = reinterpret_cast<float2*>(work);
-  a.sums = work + 2L * p->rows * heads * x.splits;
+  a.sums = work;
+  a.stats = reinterpret_cast<float2*>(work + (long)p->rows * heads * x.splits * p->dim);
   // the pool as rows of one token's key or value in one head; a box is a page's rows of 64 components
   CUtensorMap map;
   const uint64_t dims[2] = {(uint64_t)p->dim, (uint64_t)lines}, strides[1] = {(uint64_t)p->dim * 2};
@@ -568,6 +647,6 @@ extern "C" cudaError_t rt_paged_attention(const RtPool* p, int block, const int*
   else if (p->dim == 128) RT_CUDA_CHECK(launch<128>(map, a, x, s));
   else if (p->dim == 256) RT_CUDA_CHECK(launch<256>(map, a, x, s));
   else return cudaErrorInvalidValue;
-  join_kernel<<<(unsigned)(p->rows * heads), p->dim, 0, s>>>(a, p->dim);
+  join_kernel<<<(unsigned)(p->rows * heads), 256, 0, s>>>(a, p->dim);
   return cudaGetLastError();
 }
