@@ -5,9 +5,9 @@
 //
 // Within a beam the order is that of its logits, so a block per (beam, segment of the vocabulary) needs no softmax to
 // find the segment's K best: it holds the segment in registers, forms the segment's maximum and sum of exponentials
-// (terms in fp32, added up over threads in fp64), takes the K-th largest of its threads' maxima as a bound that K
-// values reach, and sorts the few values that do. A second kernel, one block per group, joins the sums, ranks the
-// segments' candidates in fp64 and draws the K best. Ranks of different beams differ by the fp32 exponentials' error
+// (terms in fp32, added up over threads in fp64), takes a bound from its threads' maxima that K values reach, and sorts
+// the few values that do. A second kernel, one block per group, joins the sums, ranks the segments' candidates in fp64
+// and keeps the K best. Ranks of different beams differ by the fp32 exponentials' error
 // at worst (about 1e-7), those of one beam only by their logits.
 //
 // A finished beam is a list of its own: itself at the end token, then nothing (-inf) at the other tokens; a beam
@@ -19,11 +19,14 @@
 
 namespace {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
-constexpr int LIST = 1024;            // candidates of a segment
-constexpr int SEGMENT = 16384 - 64;   // values of a segment at most (its ends need not be aligned)
-constexpr int MAX_SEGMENTS = 256;
-constexpr int MERGE_THREADS = 256, MERGE_WARPS = MERGE_THREADS / 32;
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int LIST = 512;            // candidates of a segment
+constexpr int HELD = 8192;           // values of a block in registers
+constexpr int SEGMENT = HELD - 64;   // of a segment at most (its ends need not be aligned)
+constexpr int MAX_SEGMENTS = 512;
+constexpr int MERGE_THREADS = 1024, MERGE_WARPS = MERGE_THREADS / 32;
+constexpr int MERGE_LIST = 1024;     // candidates of a group
+constexpr float LOG2E = 1.4426950408889634f;
 
 // Order-preserving 32-bit key of a logit: -0 equals +0; 0 is below all of them. (Of a NaN any: its beam has no rank.)
 __device__ __forceinline__ unsigned order_key(float v) {
@@ -44,6 +47,12 @@ __device__ __forceinline__ unsigned long long rank_key(double v) {
 __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) { rt::unpack8(u, f); }
 __device__ __forceinline__ void unpack(const uint4& u, float (&f)[4]) {
   f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 struct SelectArgs {
@@ -80,14 +89,36 @@ __device__ __forceinline__ int block_count(int n, int* counter) {
   return *counter;
 }
 
+// The K largest entries of z[0, n) into list, unsorted (many equal values): they are unique, so the K-th largest is found
+// bit by bit, with a read of the segment for each. Returns how many there are.
 template <typename T>
-__global__ void __launch_bounds__(THREADS) select_rows_kernel(const SelectArgs a) {
-  constexpr int VEC = 16 / sizeof(T), NV = 16384 / (THREADS * VEC);
+__device__ __noinline__ int take_by_bits(const T* z, int lo, int n, int K, unsigned long long* list) {
+  __shared__ int counter;
+  unsigned long long least = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const unsigned long long c = least | 1ull << bit;
+    int reach = 0;
+    for (int v = threadIdx.x; v < n; v += THREADS) reach += entry(order_key(rt::to_f<T>(z[v])), lo + v) >= c;
+    if (block_count(reach, &counter) >= K) least = c;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) counter = 0;
+  __syncthreads();
+  for (int v = threadIdx.x; v < n; v += THREADS) {
+    const unsigned long long e = entry(order_key(rt::to_f<T>(z[v])), lo + v);
+    if (e >= least) list[atomicAdd(&counter, 1)] = e;
+  }
+  __syncthreads();
+  return counter;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 4) select_rows_kernel(const SelectArgs a) {
+  constexpr int VEC = 16 / sizeof(T), NV = HELD / (THREADS * VEC);
   __shared__ unsigned long long list[LIST];
-  __shared__ unsigned maxima[THREADS];
   __shared__ float warp_top[WARPS];
   __shared__ double warp_sum[WARPS];
-  __shared__ unsigned bound;
+  __shared__ unsigned warp_bound[WARPS];
   __shared__ int found;
   const long row = blockIdx.x / a.segments;
   const int seg = blockIdx.x % a.segments, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -122,10 +153,22 @@ __global__ void __launch_bounds__(THREADS) select_rows_kernel(const SelectArgs a
         bad |= !(f[j] < INFINITY);
       }
     }
-  maxima[tid] = single >= 0 || tid < nvec ? order_key(top) : 0u;
+  const unsigned mine = single >= 0 || tid < nvec ? order_key(top) : 0u;
   float m = top;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  // ---- bound: of the warps whose threads all have values, each one's k-th largest of its threads' maxima, the smallest
+  // of which K values reach (none where there is no such warp)
+  const int whole = min(nvec / 32, WARPS);
+  if (warp < whole) {
+    unsigned key = mine, t = 0;
+    for (int k = (a.K + whole - 1) / whole; k > 0; --k) {
+      t = __reduce_max_sync(~0u, key);
+      const unsigned equal = __ballot_sync(~0u, key == t);
+      if (lane == __ffs(equal) - 1) key = 0;
+    }
+    if (lane == 0) warp_bound[warp] = t;
+  }
   if (lane == 0) warp_top[warp] = m;
   bad = __syncthreads_or(bad);
   m = warp_top[0];
@@ -140,38 +183,44 @@ __global__ void __launch_bounds__(THREADS) select_rows_kernel(const SelectArgs a
     return;
   }
 
-  // ---- sum of exponentials
-  float s = 0.f;
+  // ---- sum of exponentials (differences before products: a mask of the type's lowest value may leave fp32's range)
+  float s[2] = {0.f, 0.f};
   if (m > -INFINITY) {
-    if (one > -INFINITY) s = expf(one - m);
+    if (single >= 0) s[0] = ex2((one - m) * LOG2E);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if (i * THREADS + tid < nvec) {
         float f[VEC];
         unpack(u[i], f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s += expf(f[j] - m);
+        for (int j = 0; j < VEC; ++j) s[j & 1] += ex2((f[j] - m) * LOG2E);
       }
   }
-  double d = s;
+  double d = (double)s[0] + (double)s[1];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(~0u, d, o);
   if (lane == 0) warp_sum[warp] = d;
+  unsigned bound = 0;
+  for (int w = 0; w < whole; ++w) bound = w ? min(bound, warp_bound[w]) : warp_bound[0];
 
-  // ---- bound: the K-th largest of the threads' maxima, bit by bit (1, which every value reaches, where fewer have one)
-  if (warp == 0) {
-    unsigned key[WARPS];
+  // ---- candidates
+  if (mine && mine >= bound) {
+    const float least = bound ? key_value(bound) : -INFINITY;
+    auto take = [&](float f, int index) {
+      if (f >= least) {
+        const int to = atomicAdd(&found, 1);
+        if (to < LIST) list[to] = entry(order_key(f), index);
+      }
+    };
+    if (single >= 0) take(one, lo + single);
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) key[i] = maxima[i * 32 + lane];
-    unsigned t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const unsigned c = t | 1u << bit;
-      int reach = 0;
+    for (int i = 0; i < NV; ++i)
+      if (i * THREADS + tid < nvec) {
+        float f[VEC];
+        unpack(u[i], f);
 #pragma unroll
-      for (int i = 0; i < WARPS; ++i) reach += key[i] >= c;
-      if (__reduce_add_sync(~0u, reach) >= a.K) t = c;
-    }
-    if (lane == 0) bound = max(t, 1u);
+        for (int j = 0; j < VEC; ++j) take(f[j], lo + head + (i * THREADS + tid) * VEC + j);
+      }
   }
   __syncthreads();
   if (tid == 0) {
@@ -180,46 +229,7 @@ __global__ void __launch_bounds__(THREADS) select_rows_kernel(const SelectArgs a
     a.tops[at] = m;
     a.sums[at] = total;
   }
-
-  // ---- candidates
-  auto each = [&](auto&& take) {
-    if (single >= 0) take(entry(order_key(one), lo + single));
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (i * THREADS + tid < nvec) {
-        float f[VEC];
-        unpack(u[i], f);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) take(entry(order_key(f[j]), lo + head + (i * THREADS + tid) * VEC + j));
-      }
-  };
-  unsigned long long least = (unsigned long long)bound << 32;
-  auto collect = [&]() {
-    if (maxima[tid] >= (unsigned)(least >> 32) && maxima[tid])
-      each([&](unsigned long long e) {
-        if (e >= least) {
-          const int to = atomicAdd(&found, 1);
-          if (to < LIST) list[to] = e;
-        }
-      });
-    __syncthreads();
-  };
-  collect();
-  if (found > LIST) {  // many equal values: the K-th largest of the unique entries, bit by bit
-    __shared__ int counter;
-    unsigned long long t = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const unsigned long long c = t | 1ull << bit;
-      int reach = 0;
-      each([&](unsigned long long e) { reach += e >= c; });
-      if (block_count(reach, &counter) >= a.K) t = c;
-    }
-    least = t;
-    if (tid == 0) found = 0;
-    __syncthreads();
-    collect();
-  }
-  const int have = found;
+  const int have = found <= LIST ? found : take_by_bits(z, lo, n, a.K, list);
   unsigned long long* out = a.entries + at * a.K;
   for (int i = tid; i < have; i += THREADS) {  // place = number of larger entries
     const unsigned long long e = list[i];
@@ -230,56 +240,72 @@ __global__ void __launch_bounds__(THREADS) select_rows_kernel(const SelectArgs a
   for (int i = have + tid; i < a.K; i += THREADS) out[i] = 0;
 }
 
-// Block per group. Its lists (one per beam and segment, sorted) are drawn from K times: the best of their heads.
+// Block per group: the K best of its lists (one per beam and segment, sorted, K entries each). Their
+// heads give a bound that K candidates reach; the candidates that do are few, and each counts those before it. Where
+// equal heads make them too many, the best head is drawn K times instead.
 __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const SelectArgs a) {
   extern __shared__ unsigned char taken[];  // of each list
   __shared__ double base[32], norm[32];     // value = base + (z - top); rank = value / norm
   __shared__ float row_top[32];
   __shared__ int kind[32];                  // 0 running, 1 finished, 2 nothing
-  __shared__ unsigned long long warp_rank[MERGE_WARPS];
-  __shared__ long warp_flat[MERGE_WARPS];
-  __shared__ unsigned long long best_rank;
-  __shared__ long best_flat, chosen[32];
+  __shared__ int next_length[32];
+  __shared__ bool ended[32];
+  __shared__ unsigned long long list_rank[MERGE_LIST], best_rank, warp_rank[MERGE_WARPS];
+  __shared__ long list_flat[MERGE_LIST], best_flat, warp_flat[MERGE_WARPS], chosen[32];
+  __shared__ double list_value[MERGE_LIST];
+  __shared__ unsigned warp_bound[MERGE_WARPS], heads[MERGE_THREADS];
+  __shared__ float row_least[32];
+  __shared__ int found;
   __shared__ double values[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.K, S = a.segments, lists = K * S;
   const long first = (long)blockIdx.x * K;
-  for (int i = tid; i < lists; i += MERGE_THREADS) taken[i] = 0;
+  if (tid == 0) found = 0;
   for (int b = warp; b < K; b += MERGE_WARPS) {
     const long row = first + b;
-    const bool run = running(a, row);
-    float top = -INFINITY;
-    if (run)
-      for (int i = lane; i < S; i += 32) top = fmaxf(top, a.tops[row * S + i]);
+    const float score = a.scores[row];
+    const bool finished = a.finished[row], run = !finished && isfinite(score);
+    const int length = a.lengths[row] + (finished ? 0 : 1);
+    float t[4], top = -INFINITY;
+    double s[4], sum = 0.0;
+    for (int i0 = 0; i0 < S && run; i0 += 128) {  // (one round for up to 128 segments: the values stay)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    double sum = 0.0;
-    if (run && top > -INFINITY)
-      for (int i = lane; i < S; i += 32) {
-        const float t = a.tops[row * S + i];
-        if (t > -INFINITY) sum += a.sums[row * S + i] * exp((double)t - (double)top);
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * 32 + lane;
+        t[j] = i < S ? a.tops[row * S + i] : -INFINITY;
+        s[j] = i < S ? a.sums[row * S + i] : 0.0;
       }
+      float more = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) more = fmaxf(more, __shfl_xor_sync(~0u, more, o));
+      if (more > top) {
+        sum *= top == -INFINITY ? 0.0 : exp((double)top - (double)more);
+        top = more;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (s[j] != 0.0) sum += s[j] * (t[j] == top ? 1.0 : exp((double)t[j] - (double)top));  // NaN stays
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     if (lane == 0) {
-      const double score = a.scores[row];
       const bool fit = sum > 0.0 && isfinite(sum) && isfinite(top);
-      kind[b] = run && fit ? 0 : a.finished[row] && isfinite(score) ? 1 : 2;
-      base[b] = score - (kind[b] == 0 ? log(sum) : 0.0);
+      kind[b] = run && fit ? 0 : finished && isfinite(score) ? 1 : 2;
+      base[b] = (double)score - (kind[b] == 0 ? log(sum) : 0.0);
       row_top[b] = top;
-      const int length = a.lengths[row] + (a.finished[row] ? 0 : 1);
-      norm[b] = pow((double)max(length, 1), a.penalty);
+      next_length[b] = length;
+      ended[b] = finished;
+      norm[b] = a.penalty == 0.0 ? 1.0 : pow((double)max(length, 1), a.penalty);
     }
   }
   __syncthreads();
-  // head of list i (rank key 0: none left)
-  auto head = [&](int i, unsigned long long& rank, long& flat, double& value) {
-    const int b = i / S, seg = i % S;
-    int j = taken[i];
+  // j-th entry of list i (rank key 0: there is none)
+  auto item = [&](int i, int j, unsigned long long& rank, long& flat, double& value) {
+    const int b = i / S, seg = i - b * S;
     rank = 0;
     flat = LONG_MAX;
+    value = -INFINITY;
     if (j >= K) return;
     int token;
-    value = -INFINITY;
     if (kind[b] == 0) {
       const unsigned long long e = a.entries[((first + b) * S + seg) * K + j];
       if (e == 0) return;
@@ -298,60 +324,169 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     rank = rank_key(value / norm[b]);
     flat = (long)b * a.V + token;
   };
-  unsigned long long rank = 0;
-  long flat = LONG_MAX;
-  int mine = -1;
-  double value = 0.0;
-  auto refresh = [&]() {
-    rank = 0;
-    flat = LONG_MAX;
-    mine = -1;
-    for (int i = tid; i < lists; i += MERGE_THREADS) {
+  // the upper half of a rank's key keeps its order. A warp's lists are spread over all beams, as they are not alike
+  // (a thread may stand for several lists); each warp's k-th largest head, as in a segment
+  const int whole = min((lists + 31) / 32, MERGE_WARPS);
+  if (warp < whole) {
+    unsigned head = 0, t = 0;
+    for (int i = lane * whole + warp; i < lists; i += 32 * whole) {
       unsigned long long r;
       long f;
-      double v = 0.0;
-      head(i, r, f, v);
-      if (r > rank || (r == rank && f < flat)) {
-        rank = r;
-        flat = f;
-        mine = i;
-        value = v;
+      double v;
+      item(i, 0, r, f, v);
+      head = max(head, (unsigned)(r >> 32));
+    }
+    const unsigned best = head;
+    for (int k = (K + whole - 1) / whole; k > 0; --k) {
+      t = __reduce_max_sync(~0u, head);
+      const unsigned equal = __ballot_sync(~0u, head == t);
+      if (lane == __ffs(equal) - 1) head = 0;
+    }
+    if (lane == 0) warp_bound[warp] = t;
+    heads[warp * 32 + lane] = best;
+  }
+  __syncthreads();
+  unsigned least = __reduce_min_sync(~0u, lane < whole ? warp_bound[lane] : ~0u);
+  if (whole > 4) {  // (many lists: a bound that is theirs and not each warp's; below four warps it would cost more than it saves)
+    if (warp == 0) {
+      unsigned key[MERGE_WARPS], above = 0;
+#pragma unroll
+      for (int i = 0; i < MERGE_WARPS; ++i) {
+        key[i] = i < whole ? heads[i * 32 + lane] : 0u;
+        above = max(above, key[i]);
+      }
+      unsigned below = least;  // K heads reach it
+      above = __reduce_max_sync(~0u, above) + 1;
+      while (above - below > 1) {
+        const unsigned mid = below + (above - below) / 2;
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < MERGE_WARPS; ++i) reach += key[i] >= mid;
+        reach = __reduce_add_sync(~0u, reach);
+        if (reach < K) {
+          above = mid;
+        } else {
+          below = mid;
+          if (reach <= K + K / 4) break;
+        }
+      }
+      if (lane == 0) warp_bound[0] = below;
+    }
+    __syncthreads();
+    least = warp_bound[0];
+  }
+  least = max(least, 1u);
+  auto offer = [&](int i, int j) {
+    unsigned long long r;
+    long f;
+    double v;
+    item(i, j, r, f, v);
+    if ((unsigned)(r >> 32) >= least) {
+      const int to = atomicAdd(&found, 1);
+      if (to < MERGE_LIST) {
+        list_rank[to] = r;
+        list_flat[to] = f;
+        list_value[to] = v;
       }
     }
   };
-  refresh();
-  for (int n = 0; n < K; ++n) {
-    unsigned long long r = rank;
-    long f = flat;
+  // A row's candidates that can reach the bound have a logit of about (bound norm - base) + top; they are few, and only
+  // they are ranked. (The margin is far above the rounding of these steps; what it lets through is ranked in vain.)
+  if (tid < K) {
+    const unsigned long long key = (unsigned long long)least << 32;
+    const double at_least = __longlong_as_double((long long)(key >> 63 ? key & ~(1ull << 63) : ~key)) * norm[tid] - base[tid] +
+                            (double)row_top[tid];
+    // (NaN, of a bound below all numbers, lets everything through)
+    row_least[tid] = __double2float_rd(at_least - fabs(at_least) * 1e-6 - 1e-3);
+  }
+  __syncthreads();
+  // a lane per entry, 32 / K lists per warp
+  const int per = 32 / K, sub = lane / K, j = lane - sub * K;
+  for (int i0 = warp * per + sub; i0 < lists; i0 += 8 * MERGE_WARPS * per) {
+    unsigned long long in[8];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long r2 = __shfl_xor_sync(~0u, r, o);
-      const long f2 = __shfl_xor_sync(~0u, f, o);
-      if (r2 > r || (r2 == r && f2 < f)) {
-        r = r2;
-        f = f2;
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + k * MERGE_WARPS * per;
+      in[k] = sub < per && i < lists && kind[i / S] == 0 ? a.entries[(first * S + i) * K + j] : 0ull;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + k * MERGE_WARPS * per;
+      if (in[k] && !(key_value((unsigned)(in[k] >> 32)) < row_least[i / S])) offer(i, j);
+    }
+  }
+  for (int e = tid; e < K * K; e += MERGE_THREADS)
+    if (kind[e / K] != 0) offer(e / K * S, e % K);
+  __syncthreads();
+  const int have = found;
+  if (have <= MERGE_LIST) {
+    if (tid < have) {
+      const unsigned long long r = list_rank[tid];
+      const long f = list_flat[tid];
+      int place = 0;
+      for (int j = 0; j < have; ++j) place += list_rank[j] > r || (list_rank[j] == r && list_flat[j] < f);
+      if (place < K) {
+        chosen[place] = f;
+        values[place] = list_value[tid];
       }
     }
-    if (lane == 0) {
-      warp_rank[warp] = r;
-      warp_flat[warp] = f;
-    }
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < MERGE_WARPS; ++w)
-        if (warp_rank[w] > r || (warp_rank[w] == r && warp_flat[w] < f)) {
-          r = warp_rank[w];
-          f = warp_flat[w];
+  } else {
+    for (int i = tid; i < lists; i += MERGE_THREADS) taken[i] = 0;
+    unsigned long long rank;
+    long flat;
+    int mine;
+    double value;
+    auto refresh = [&]() {  // the best head of this thread's lists
+      rank = 0;
+      flat = LONG_MAX;
+      mine = -1;
+      for (int i = tid; i < lists; i += MERGE_THREADS) {
+        unsigned long long r;
+        long f;
+        double v;
+        item(i, taken[i], r, f, v);
+        if (r > rank || (r == rank && f < flat)) {
+          rank = r;
+          flat = f;
+          mine = i;
+          value = v;
         }
-      best_rank = r;
-      best_flat = f;
-    }
-    __syncthreads();
-    if (mine >= 0 && flat == best_flat && rank == best_rank) {
-      chosen[n] = flat;
-      values[n] = value;
-      ++taken[mine];
-      refresh();
+      }
+    };
+    refresh();
+    for (int n = 0; n < K; ++n) {
+      unsigned long long r = rank;
+      long f = flat;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const unsigned long long r2 = __shfl_xor_sync(~0u, r, o);
+        const long f2 = __shfl_xor_sync(~0u, f, o);
+        if (r2 > r || (r2 == r && f2 < f)) {
+          r = r2;
+          f = f2;
+        }
+      }
+      if (lane == 0) {
+        warp_rank[warp] = r;
+        warp_flat[warp] = f;
+      }
+      __syncthreads();
+      if (tid == 0) {
+        for (int w = 1; w < MERGE_WARPS; ++w)
+          if (warp_rank[w] > r || (warp_rank[w] == r && warp_flat[w] < f)) {
+            r = warp_rank[w];
+            f = warp_flat[w];
+          }
+        best_rank = r;
+        best_flat = f;
+      }
+      __syncthreads();
+      if (mine >= 0 && flat == best_flat && rank == best_rank) {
+        chosen[n] = flat;
+        values[n] = value;
+        ++taken[mine];
+        refresh();
+      }
     }
   }
   __syncthreads();
@@ -370,18 +505,18 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     for (int skip = __popc(others & ((1u << lane) - 1)); skip > 0; --skip) left &= left - 1;
     slot = __ffs(left) - 1;
   }
-  const long token = chosen[lane] % a.V, to = first + slot, from = first + parent;
+  const long token = chosen[lane] % a.V, to = first + slot;
   a.tokens[to] = token;
   a.parents[to] = parent;
   a.out_scores[to] = (float)values[lane];
-  a.out_lengths[to] = a.lengths[from] + (a.finished[from] ? 0 : 1);
-  a.out_finished[to] = a.finished[from] || token == a.end_token;
+  a.out_lengths[to] = next_length[parent];
+  a.out_finished[to] = ended[parent] || token == a.end_token;
 }
 
-// Segments of a beam's vocabulary: enough to fill the SMs twice, of 2048 values at least.
+// Segments of a beam's vocabulary: enough for four blocks per SM, of 1024 values at least.
 int segments_for(long rows, long V) {
   const long least = (V + SEGMENT - 1) / SEGMENT;
-  const long spread = std::min((296 + rows - 1) / rows, V / 2048);
+  const long spread = std::min({(592 + rows - 1) / rows, V / 1024, 128L});
   return (int)std::max({1L, least, spread});
 }
 
