@@ -113,7 +113,7 @@ __device__ __noinline__ int take_by_bits(const T* z, int lo, int n, int K, unsig
 }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 4) select_rows_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(THREADS, 5) select_rows_kernel(const SelectArgs a) {
   constexpr int VEC = 16 / sizeof(T), NV = HELD / (THREADS * VEC);
   __shared__ unsigned long long list[LIST];
   __shared__ float warp_top[WARPS];

@@ -12,7 +12,7 @@
 namespace {
 
 using bf16 = __nv_bfloat16;
-constexpr int THREADS = 1024, WARPS = THREADS / 32, MAX_ROWS = 1024;
+constexpr int THREADS = 1024, WARPS = THREADS / 32, MAX_ROWS = 1024, SMALL_POOL = 5120;
 
 // Exclusive prefix sum over the block and its total. Two barriers.
 __device__ __forceinline__ int block_prefix(int v, int* warp_sums, int& total) {
@@ -51,18 +51,26 @@ struct AdvanceArgs {
   int4* copies;         // [rows]: (from, to, tokens, -); from = -1: none
 };
 
+// SMALL: the counts fit shared memory, which takes three waits for memory out of the chain that this kernel is bound by.
+template <bool SMALL>
 __global__ void __launch_bounds__(THREADS) advance_kernel(const AdvanceArgs a) {
   __shared__ int source[MAX_ROWS];  // row whose history a row takes over, -1: none (not live)
+  __shared__ int before[MAX_ROWS];  // its last slot (of the partly filled page), -1: none
   __shared__ int last[MAX_ROWS];    // partly filled page that a row appends to, -1: none
   __shared__ int wants[MAX_ROWS];   // exclusive prefix of the pages that rows take
   __shared__ int slot[MAX_ROWS];    // where a row's first taken page goes
   __shared__ int target[MAX_ROWS];  // that page, -1: none found
+  __shared__ int counts[SMALL ? SMALL_POOL : 1];
   __shared__ int warp_sums[WARPS];
   __shared__ int bits;
   const int tid = threadIdx.x, R = a.rows;
+  int* refs = SMALL ? counts : a.new_refs;
+  auto count_of = [&](int p) { return SMALL ? counts[p] : __ldcg(&a.new_refs[p]); };
   if (tid == 0) bits = 0;
+  if (SMALL || a.new_refs != a.refs)
+    for (int p = tid; p < a.pages; p += THREADS) refs[p] = a.refs[p];
   __syncthreads();
-  int length = 0;
+  int length = 0, row_source = -1;
   if (tid < R) {
     int from = tid;
     if (a.parents) {
@@ -70,58 +78,63 @@ __global__ void __launch_bounds__(THREADS) advance_kernel(const AdvanceArgs a) {
       if (p >= 0 && p < a.K) from = tid / a.K * a.K + (int)p;
       else atomicOr(&bits, 4);
     }
-    const bool live = !a.live || a.live[tid];
-    source[tid] = live ? from : -1;
-    if (live) length = min(max(a.lengths[from], 0), a.width * a.page);
+    if (!a.live || a.live[tid]) {
+      row_source = from;
+      length = min(max(a.lengths[from], 0), a.width * a.page);
+    }
   }
-  if (a.new_refs != a.refs)
-    for (int p = tid; p < a.pages; p += THREADS) a.new_refs[p] = a.refs[p];
+  const int fill = length % a.page, have = (length + a.page - 1) / a.page;
+  const long need = ((long)length + a.tokens + a.page - 1) / a.page;
+  bool grows = row_source >= 0 && a.tokens > 0;
+  if (grows && need > a.width) {
+    atomicOr(&bits, 2);
+    grows = false;
+  }
+  if (tid < R) {
+    source[tid] = row_source;
+    before[tid] = grows && fill ? have - 1 : -1;
+    last[tid] = -1;
+  }
   __syncthreads();
 
   // ---- histories: all rows of some columns are read before any is written
-  const int columns = THREADS / R, c_in = tid / R, r_in = tid % R;
+  const int columns = THREADS / R, c_in = tid / R, r_in = tid - c_in * R;
   const bool busy = c_in < columns;
-  const int from = busy ? source[r_in] : -1;
-  for (int c0 = 0; c0 < a.width; c0 += columns) {
-    const int c = c0 + c_in;
-    const bool on = busy && c < a.width;
-    int old = -1, now = -1;
-    if (on) {
-      old = a.table[(long)r_in * a.width + c];
-      if (from >= 0) now = from == r_in ? old : a.table[(long)from * a.width + c];
+  const int from = busy ? source[r_in] : -1, at = busy ? before[r_in] : -1;
+  constexpr int U = 4;
+  for (int c0 = 0; c0 < a.width; c0 += U * columns) {
+    int old[U], now[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int c = c0 + k * columns + c_in;
+      const bool on = busy && c < a.width;
+      old[k] = on ? a.table[(long)r_in * a.width + c] : -1;
+      now[k] = on && from >= 0 && from != r_in ? a.table[(long)from * a.width + c] : -1;
+      if (from == r_in) now[k] = old[k];
     }
     __syncthreads();
-    if (on) {
-      if (now != old) {
-        if (old >= 0 && old < a.pages) atomicSub(&a.new_refs[old], 1);
-        if (now >= 0 && now < a.pages) atomicAdd(&a.new_refs[now], 1);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int c = c0 + k * columns + c_in;
+      if (!busy || c >= a.width) continue;
+      if (now[k] != old[k]) {
+        if (old[k] >= 0 && old[k] < a.pages) atomicSub(&refs[old[k]], 1);
+        if (now[k] >= 0 && now[k] < a.pages) atomicAdd(&refs[now[k]], 1);
       }
-      a.new_table[(long)r_in * a.width + c] = now;
+      a.new_table[(long)r_in * a.width + c] = now[k];
+      if (c == at && now[k] < a.pages) last[r_in] = now[k];
     }
   }
   __threadfence_block();
   __syncthreads();
 
   // ---- what each row takes: a page of its own for a shared partly filled one, and the pages behind it
-  const int fill = length % a.page, have = (length + a.page - 1) / a.page;
-  const long need = ((long)length + a.tokens + a.page - 1) / a.page;
-  bool grows = tid < R && source[tid] >= 0 && a.tokens > 0;
-  if (grows && need > a.width) {
-    atomicOr(&bits, 2);
-    grows = false;
-  }
-  int mine = -1;
-  if (grows && fill) {
-    mine = a.new_table[(long)tid * a.width + have - 1];
-    if (mine >= a.pages) mine = -1;
-  }
-  if (tid < R) last[tid] = mine;
-  __syncthreads();
+  const int mine = tid < R ? last[tid] : -1;
   bool copy = false;
   if (mine >= 0) {
-    int before = 0;  // rows above that share it: each has left it by then
-    for (int r = 0; r < tid; ++r) before += last[r] == mine;
-    copy = __ldcg(&a.new_refs[mine]) - before > 1;
+    int earlier = 0;  // rows above that share it: each has left it by then
+    for (int r = 0; r < tid; ++r) earlier += last[r] == mine;
+    copy = count_of(mine) - earlier > 1;
   }
   const int takes = grows ? (int)copy + (int)need - have : 0;
   int total = 0;
@@ -132,14 +145,14 @@ __global__ void __launch_bounds__(THREADS) advance_kernel(const AdvanceArgs a) {
     target[tid] = -1;
   }
   for (int i = 0; i < takes; ++i) a.new_table[(long)tid * a.width + have - (int)copy + i] = -1;  // until found
-  if (copy) atomicSub(&a.new_refs[mine], 1);
+  if (copy) atomicSub(&refs[mine], 1);
   __syncthreads();
 
   // ---- the lowest free pages, to rows in order (a page is looked at once, so taking one disturbs no other)
   int found = 0;
   for (int p0 = 0; p0 < a.pages && found < total; p0 += THREADS) {
     const int p = p0 + tid;
-    const bool free = p < a.pages && __ldcg(&a.new_refs[p]) <= 0;
+    const bool free = p < a.pages && count_of(p) <= 0;
     int here;
     const int n = found + block_prefix(free, warp_sums, here);
     if (free && n < total) {
@@ -149,10 +162,10 @@ __global__ void __launch_bounds__(THREADS) advance_kernel(const AdvanceArgs a) {
         if (wants[mid] <= n) lo = mid;
         else hi = mid - 1;
       }
-      const int at = n - wants[lo];
-      a.new_refs[p] = 1;
-      a.new_table[(long)lo * a.width + slot[lo] + at] = p;
-      if (at == 0) target[lo] = p;
+      const int k = n - wants[lo];
+      refs[p] = 1;
+      a.new_table[(long)lo * a.width + slot[lo] + k] = p;
+      if (k == 0) target[lo] = p;
     }
     found += here;
   }
@@ -161,10 +174,26 @@ __global__ void __launch_bounds__(THREADS) advance_kernel(const AdvanceArgs a) {
     a.copies[tid] = make_int4(copy && target[tid] >= 0 ? mine : -1, target[tid], fill, 0);
     a.new_lengths[tid] = length + (grows ? a.tokens : 0);
   }
+  if (SMALL)
+    for (int p = tid; p < a.pages; p += THREADS) a.new_refs[p] = counts[p];
   if (tid == 0) {
     if (found < total) bits |= 1;
     *a.status = bits | (a.keep_status ? *a.status : 0);
   }
+}
+
+// Copies of a warp's or block's vectors, several in flight per thread.
+template <int U>
+__device__ __forceinline__ void copy_vectors(uint4* to, const uint4* from, long n, int first, int step) {
+  long i = first;
+  for (; i + (U - 1) * (long)step < n; i += U * (long)step) {
+    uint4 v[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) v[k] = from[i + k * (long)step];
+#pragma unroll
+    for (int k = 0; k < U; ++k) to[i + k * (long)step] = v[k];
+  }
+  for (; i < n; i += step) to[i] = from[i];
 }
 
 // The first `tokens` tokens of a page in every block and head, for each row's copy. Grid (parts, rows).
@@ -174,9 +203,8 @@ __global__ void __launch_bounds__(256) copy_tokens_kernel(bf16* pool, const int4
   const long size = (long)page * dim / 8;  // vectors of a panel: one block's keys or values of one head
   const uint4* from = reinterpret_cast<const uint4*>(pool) + (long)c.x * panels * size;
   uint4* to = reinterpret_cast<uint4*>(pool) + (long)c.y * panels * size;
-  const int used = c.z * dim / 8;
   for (int h = blockIdx.x; h < panels; h += gridDim.x)
-    for (int i = threadIdx.x; i < used; i += blockDim.x) to[h * size + i] = from[h * size + i];
+    copy_vectors<8>(to + h * size, from + h * size, c.z * dim / 8, threadIdx.x, blockDim.x);
 }
 
 struct CompactArgs {
@@ -251,9 +279,7 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(uint4* pool, const int2
   for (long w = blockIdx.x; w < work; w += gridDim.x) {
     const int2 m = moves[w / parts];
     const long lo = vectors * (w % parts) / parts, hi = vectors * (w % parts + 1) / parts;
-    const uint4* from = pool + m.x * vectors;
-    uint4* to = pool + m.y * vectors;
-    for (long i = lo + threadIdx.x; i < hi; i += blockDim.x) to[i] = from[i];
+    copy_vectors<8>(pool + m.y * vectors + lo, pool + m.x * vectors + lo, hi - lo, threadIdx.x, blockDim.x);
   }
 }
 
@@ -292,7 +318,11 @@ __global__ void __launch_bounds__(256) store_kernel(const StoreArgs a) {
     const long to = place_of(a.at, row, (long)a.at.lengths[row] - a.T + t, a.first + kind * a.heads + h);
     if (to < 0) continue;
     const bf16* x = a.x[kind] + n * a.batch[kind] + t * a.time[kind] + h * a.head[kind];
-    for (int c = lane; c < a.at.dim; c += 32) a.pool[to + c] = x[c];
+    if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+      if (lane * 8 < a.at.dim) *reinterpret_cast<uint4*>(a.pool + to + lane * 8) = *reinterpret_cast<const uint4*>(x + lane * 8);
+    } else {
+      for (int c = lane; c < a.at.dim; c += 32) a.pool[to + c] = x[c];
+    }
   }
 }
 
@@ -308,12 +338,13 @@ struct AppendArgs {
   int first;    // panel of the block's keys of head 0
   int rows, heads, kv_heads, half;
   float eps;
+  int vec;      // rows of x are 16-byte aligned
 };
 
 // One warp per (row, head): the query heads, then keys, then values. The angle position * frequency is reduced to a
 // turn in fp64 (in fp32 it is 0.01 off at position 2^17 already), its sine and cosine are fp32.
 __global__ void __launch_bounds__(128) append_kernel(const AppendArgs a) {
-  __shared__ float buf[4][256];
+  __shared__ __align__(16) float buf[4][256];
   const int lane = threadIdx.x % 32, D = a.at.dim, per = a.heads + 2 * a.kv_heads;
   const long item = (long)blockIdx.x * 4 + threadIdx.x / 32;
   if (item >= (long)a.rows * per) return;
@@ -328,31 +359,54 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs a) {
     if (to < 0) return;
     out = a.pool + to;
     if (kind == 2) {
-      for (int c = lane; c < D; c += 32) out[c] = x[c];
+      if (a.vec) {
+        if (lane * 8 < D) *reinterpret_cast<uint4*>(out + lane * 8) = *reinterpret_cast<const uint4*>(x + lane * 8);
+      } else {
+        for (int c = lane; c < D; c += 32) out[c] = x[c];
+      }
       return;
     }
   }
   float* s = buf[threadIdx.x / 32];
   const float* w = kind == 0 ? a.q_weight : a.k_weight;
   float sum = 0.f;
-  for (int c = lane; c < D; c += 32) {
-    const float v = rt::to_f(x[c]);
-    s[c] = v;
-    sum += v * v;
-  }
-  const float inv = rsqrtf(rt::warp_sum(sum) / D + a.eps);
-  for (int c = lane; c < D; c += 32) s[c] *= inv * (1.f + w[c]);
-  __syncwarp();
-  for (int c = lane; c < D; c += 32) {
-    float o = s[c];
-    if (c < 2 * a.half) {
-      const int i = c < a.half ? c : c - a.half;
-      const double turns = (double)max(position, 0L) * a.inv_freq[i] * 0.15915494309189535;
-      float sn, cs;
-      sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
-      o = c < a.half ? o * cs - s[c + a.half] * sn : o * cs + s[c - a.half] * sn;
+  if (a.vec) {  // eight components of each lane
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, g[8];
+    const int c = lane * 8;
+    if (c < D) {
+      rt::unpack8(*reinterpret_cast<const uint4*>(x + c), v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[k] = w[c + k];
     }
-    out[c] = __float2bfloat16_rn(o);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += v[k] * v[k];
+    const float inv = rsqrtf(rt::warp_sum(sum) / D + a.eps);
+    if (c < D)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[c + k] = v[k] * inv * (1.f + g[k]);
+  } else {
+    for (int c = lane; c < D; c += 32) {
+      const float v = rt::to_f(x[c]);
+      s[c] = v;
+      sum += v * v;
+    }
+    const float inv = rsqrtf(rt::warp_sum(sum) / D + a.eps);
+    for (int c = lane; c < D; c += 32) s[c] *= inv * (1.f + w[c]);
+  }
+  __syncwarp();
+  for (int i = lane; i < a.half; i += 32) {
+    const double turns = (double)max(position, 0L) * a.inv_freq[i] * 0.15915494309189535;
+    float sn, cs;
+    sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
+    const float x0 = s[i], x1 = s[i + a.half];
+    s[i] = x0 * cs - x1 * sn;
+    s[i + a.half] = x1 * cs + x0 * sn;
+  }
+  __syncwarp();
+  if (a.vec) {
+    if (lane * 8 < D) *reinterpret_cast<uint4*>(out + lane * 8) = rt::pack8(s + lane * 8);
+  } else {
+    for (int c = lane; c < D; c += 32) out[c] = __float2bfloat16_rn(s[c]);
   }
 }
 
@@ -378,7 +432,8 @@ extern "C" cudaError_t rt_advance_pages(const RtPool* p, const int* table, const
   if (!pool_fits(p) || tokens < 0 || K < 1 || p->rows % K) return cudaErrorInvalidValue;
   AdvanceArgs a{table, lengths, refs, new_table, new_lengths, new_refs, status, keep_status, parents, live,
                 p->rows, K, p->width, p->pages, p->page, tokens, static_cast<int4*>(work)};
-  advance_kernel<<<1, THREADS, 0, s>>>(a);
+  if (p->pages <= SMALL_POOL) advance_kernel<true><<<1, THREADS, 0, s>>>(a);
+  else advance_kernel<false><<<1, THREADS, 0, s>>>(a);
   RT_CUDA_CHECK(cudaGetLastError());
   if (tokens == 0) return cudaSuccess;
   const int panels = p->blocks * 2 * p->heads;
@@ -407,7 +462,7 @@ extern "C" cudaError_t rt_compact_pages(const RtPool* p, const int* table, const
   compact_kernel<<<1, THREADS, 0, s>>>(a);
   RT_CUDA_CHECK(cudaGetLastError());
   const long vectors = (long)p->blocks * 2 * p->heads * p->page * p->dim / 8;
-  const int parts = (int)std::min((vectors + 4095) / 4096, 4096L);
+  const int parts = (int)std::min((vectors + 2047) / 2048, 4096L);  // 32 KB: eight vectors per thread
   copy_pages_kernel<<<148 * 8, 256, 0, s>>>(static_cast<uint4*>(p->pool), a.moves, a.count, vectors, parts);
   return cudaGetLastError();
 }
@@ -447,7 +502,7 @@ extern "C" cudaError_t rt_append_heads(const RtPool* p, int block, const int* ta
     return cudaErrorInvalidValue;
   AppendArgs a{place(p, table, lengths), static_cast<const bf16*>(x), ld, q_weight, k_weight, inv_freq,
                static_cast<bf16*>(q), static_cast<bf16*>(p->pool), block * 2 * p->heads, p->rows, heads, p->heads, half,
-               eps};
+               eps, (reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ld * 2)) % 16 == 0};
   const long items = (long)p->rows * (heads + 2 * p->heads);
   append_kernel<<<(unsigned)((items + 3) / 4), 128, 0, s>>>(a);
   return cudaGetLastError();

@@ -19,7 +19,6 @@ from .validation import _logits
 MAX_BEAMS = 32  # of a group on CUDA
 
 
-@torch.no_grad()
 def beam_select(logits, scores, lengths, finished, end_token=-1, length_penalty=0.0):
     """(tokens int64, parents int64, scores fp32, lengths int32, finished bool), all [G, K]: one step of beam search
     for G groups of K beams.
@@ -62,22 +61,26 @@ def beam_select(logits, scores, lengths, finished, end_token=-1, length_penalty=
     return reference.beam_select(logits, scores, lengths, finished, end_token, length_penalty)
 
 
-@torch.no_grad()
 def reorder_states_(states, parents):
     """Rows of each tensor of ``states`` ([G * K, ...], contiguous, any type) replaced by their parents' rows, in
     place: slot k of group g takes what slot ``parents[g, k]`` held (int64 [G, K], any indices of the group; one
     outside it leaves its slot alone). Rows that stay are not touched. The tensors must not overlap."""
     states = list(states)
-    check_parents(parents, parents.numel(), parents.device)
-    rows = parents.numel()
+    rows, device = parents.numel(), parents.device
+    check_parents(parents, rows, device)
+    spans = []
     for state in states:
         if state.dim() < 1 or state.shape[0] != rows:
             raise ValueError(f"expected states of {rows} rows, got {tuple(state.shape)}")
         if not state.is_contiguous():
             raise ValueError("states must be contiguous")
-        if state.device != parents.device:
+        if state.device != device:
             raise ValueError("states and parents are on different devices")
-    spans = sorted((state.data_ptr(), state.data_ptr() + state.nbytes) for state in states if state.numel())
+        size = state.nbytes
+        if size:
+            start = state.data_ptr()
+            spans.append((start, start + size))
+    spans.sort()
     if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
         raise ValueError("states must not overlap")
     if not spans or parents.shape[1] == 1:
@@ -85,11 +88,13 @@ def reorder_states_(states, parents):
     if parents.is_cuda:
         if parents.shape[1] > MAX_BEAMS:
             raise ValueError(f"reorder_states_ takes at most {MAX_BEAMS} beams on CUDA, got {parents.shape[1]}")
-        native().reorder_rows_([state for state in states if state.numel()], parents.contiguous())
+        native().reorder_rows_(states if len(spans) == len(states) else [state for state in states if state.numel()],
+                               parents.contiguous())
         return
     source = reference.parent_rows(parents)
-    for state in states:
-        state.copy_(state[source])
+    with torch.no_grad():
+        for state in states:
+            state.copy_(state[source])
 
 
 def _spread(state, beams):

@@ -144,6 +144,7 @@ def top_log_probs(logits, k, scale):
     return torch.log_softmax(below, -1).gather(-1, index).to(z.dtype), index
 
 
+@torch.no_grad()
 def place_children(parents):
     """Slots of a group's K chosen candidates, given by rank (``parents`` [G, K]): a parent's best child keeps the
     parent's slot, the others fill the slots that are left in order. Returns [G, K]: the rank that each slot takes."""
@@ -158,6 +159,7 @@ def place_children(parents):
     return held
 
 
+@torch.no_grad()
 def beam_select(logits, scores, lengths, finished, end_token, length_penalty):
     """One step of beam search over [G, K, V] (see ``beams.beam_select``), ranked in 64 bits."""
     G, K, V = logits.shape
@@ -183,6 +185,7 @@ def parent_rows(parents):
     return (inside + torch.arange(G, device=parents.device)[:, None] * K).flatten()
 
 
+@torch.no_grad()
 def advance_pages(pool, table, lengths, refs, tokens, parents, live):
     """Row after row, as ``paged.advance_pages`` defines it. Returns (table, lengths, refs, status)."""
     pages, page, (R, width) = pool.shape[0], pool.shape[4], table.shape
@@ -231,6 +234,7 @@ def advance_pages(pool, table, lengths, refs, tokens, parents, live):
             torch.tensor(count, dtype=torch.int32), torch.tensor([status], dtype=torch.int32))
 
 
+@torch.no_grad()
 def compact_pages(pool, table, refs):
     """Pages in use moved into the free ones before them (see ``paged.compact_pages``). Returns (table, refs, used)."""
     taken = refs > 0
@@ -257,6 +261,7 @@ def _slots(pool, table, positions):
     return inside & (entry >= 0) & (entry < pool.shape[0]), entry, (positions.clamp_min(0) % page).long()
 
 
+@torch.no_grad()
 def store_pages(pool, block, table, lengths, keys, values):
     """``keys``, ``values`` [N, T, H, D] as the last T tokens of every (R / N)-th row."""
     N, T = keys.shape[:2]
@@ -267,6 +272,7 @@ def store_pages(pool, block, table, lengths, keys, values):
         pool[entry[valid], block, kind, :, slot[valid]] = x[valid].to(pool.dtype)
 
 
+@torch.no_grad()
 def append_heads(x, pool, block, table, lengths, q_weight, k_weight, inv_freq, heads, eps):
     """Norm and rotation of a token's queries and keys, keys and values into their pages (see ``paged.append_heads``)."""
     H, D = pool.shape[3], pool.shape[5]
@@ -287,6 +293,7 @@ def append_heads(x, pool, block, table, lengths, q_weight, k_weight, inv_freq, h
     return q.to(x.dtype)
 
 
+@torch.no_grad()
 def paged_attention(q, pool, block, table, lengths, gate):
     """One token per row over the keys of its pages (see ``paged.paged_attention``)."""
     R, Hq, D = q.shape

@@ -19,34 +19,38 @@ PAGES = (16, 32, 64)
 DIMS = (64, 128, 256)
 
 
+def _ints(name, part, shape, device):
+    if part.dtype != torch.int32 or not part.is_contiguous():
+        raise TypeError(f"{name} must be contiguous int32")
+    if part.shape != shape:
+        raise ValueError(f"{name} {tuple(part.shape)} does not match {tuple(shape)}")
+    if part.device != device:
+        raise ValueError(f"{name} is on {part.device}, the pool on {device}")
+
+
 def _check(pool, table, lengths=None, refs=None, block=None):
     """What all functions ask of a cache's tensors."""
-    if pool.dim() != 6 or pool.shape[2] != 2 or pool.numel() == 0:
-        raise ValueError(f"expected a pool [pages, blocks, 2, heads, page, dim], got {tuple(pool.shape)}")
-    if pool.shape[4] not in PAGES:
-        raise ValueError(f"a page holds {PAGES} tokens, got {pool.shape[4]}")
+    shape, held, device = pool.shape, table.shape, pool.device
+    if len(shape) != 6 or shape[2] != 2 or 0 in shape:
+        raise ValueError(f"expected a pool [pages, blocks, 2, heads, page, dim], got {tuple(shape)}")
+    if shape[4] not in PAGES:
+        raise ValueError(f"a page holds {PAGES} tokens, got {shape[4]}")
     if not pool.is_contiguous():
         raise ValueError("the pool must be contiguous")
-    if table.dim() != 2 or table.numel() == 0:
-        raise ValueError(f"expected a table [rows, width], got {tuple(table.shape)}")
-    for name, part, shape in (("table", table, table.shape), ("lengths", lengths, table.shape[:1]),
-                              ("refs", refs, pool.shape[:1])):
-        if part is None:
-            continue
-        if part.dtype != torch.int32 or not part.is_contiguous():
-            raise TypeError(f"{name} must be contiguous int32")
-        if part.shape != shape:
-            raise ValueError(f"{name} {tuple(part.shape)} does not match {tuple(shape)}")
-        if part.device != pool.device:
-            raise ValueError(f"{name} is on {part.device}, the pool on {pool.device}")
-    if block is not None and not 0 <= block < pool.shape[1]:
-        raise IndexError(f"block {block} of {pool.shape[1]}")
+    if len(held) != 2 or 0 in held:
+        raise ValueError(f"expected a table [rows, width], got {tuple(held)}")
+    _ints("table", table, held, device)
+    if lengths is not None:
+        _ints("lengths", lengths, held[:1], device)
+    if refs is not None:
+        _ints("refs", refs, shape[:1], device)
+    if block is not None and not 0 <= block < shape[1]:
+        raise IndexError(f"block {block} of {shape[1]}")
     if pool.is_cuda:
-        if pool.dtype != torch.bfloat16 or pool.shape[5] not in DIMS:
-            raise TypeError(f"the CUDA paged cache takes bf16 and head sizes {DIMS}, got {pool.dtype} and "
-                            f"{pool.shape[5]}")
-        if table.shape[0] > 1024:
-            raise ValueError(f"the CUDA paged cache has at most 1024 rows, got {table.shape[0]}")
+        if pool.dtype != torch.bfloat16 or shape[5] not in DIMS:
+            raise TypeError(f"the CUDA paged cache takes bf16 and head sizes {DIMS}, got {pool.dtype} and {shape[5]}")
+        if held[0] > 1024:
+            raise ValueError(f"the CUDA paged cache has at most 1024 rows, got {held[0]}")
 
 
 def _check_rows(name, part, pool, table, shape):
@@ -66,7 +70,6 @@ def check_parents(parents, rows, device):
         raise TypeError(f"parents must be int64 on {device}")
 
 
-@torch.no_grad()
 def advance_pages(pool, table, lengths, refs, tokens=1, parents=None, live=None, out=None):
     """(table, lengths, refs, status) after every row took over its parent's history and got room for ``tokens`` more.
 
@@ -107,7 +110,6 @@ def advance_pages(pool, table, lengths, refs, tokens=1, parents=None, live=None,
     return out
 
 
-@torch.no_grad()
 def compact_pages(pool, table, refs, out=None):
     """(table, refs, used): the pages in use moved to the front of the pool, whose first ``used`` [1] pages they are
     then. The lowest page behind them goes to the lowest free page among them, and so on; pages that lie there
@@ -127,7 +129,6 @@ def compact_pages(pool, table, refs, out=None):
     return out[0], out[1], result[2]
 
 
-@torch.no_grad()
 def store_pages(pool, block, table, lengths, keys, values):
     """Writes ``keys``, ``values`` [N, T, heads, dim] as the last T tokens of rows 0, R / N, 2 R / N, ... (the first of
     each group of beams); tokens before a row's first are dropped. For prompts, whose keys are rotated already."""
@@ -143,7 +144,6 @@ def store_pages(pool, block, table, lengths, keys, values):
         reference.store_pages(pool, block, table, lengths, keys, values)
 
 
-@torch.no_grad()
 def append_heads(x, pool, block, table, lengths, q_weight, k_weight, inv_freq, heads, eps):
     """Queries [R, heads, dim] of each row's newest token, whose key and value go into the row's pages, in one pass.
 
@@ -166,7 +166,6 @@ def append_heads(x, pool, block, table, lengths, q_weight, k_weight, inv_freq, h
     return reference.append_heads(x, pool, block, table, lengths, q_weight, k_weight, inv_freq, heads, eps)
 
 
-@torch.no_grad()
 def paged_attention(q, pool, block, table, lengths, gate=None, group=1):
     """Attention [R, Hq, dim] of one token per row over the ``lengths`` tokens of its pages in one block, scaled by
     dim^-0.5; query head h reads key head h // (Hq / heads). ``gate`` [R, Hq, dim]: the result is multiplied by its
