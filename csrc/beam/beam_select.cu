@@ -55,6 +55,26 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 struct SelectArgs {
   const void* logits;
   long ld_group, ld_beam;
@@ -120,11 +140,13 @@ __global__ void __launch_bounds__(THREADS, 5) select_rows_kernel(const SelectArg
   __shared__ double warp_sum[WARPS];
   __shared__ unsigned warp_bound[WARPS];
   __shared__ int found;
-  const long row = blockIdx.x / a.segments;
-  const int seg = blockIdx.x % a.segments, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // (32-bit divisions: those of 64 bits were half of this kernel's instructions; V x segments is below 2^32)
+  const unsigned segments = a.segments, row = blockIdx.x / segments, seg = blockIdx.x - row * segments;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (!running(a, row)) return;
-  const int lo = (int)((long)a.V * seg / a.segments), n = (int)((long)a.V * (seg + 1) / a.segments) - lo;
-  const T* z = static_cast<const T*>(a.logits) + row / a.K * a.ld_group + row % a.K * a.ld_beam + lo;
+  const int lo = (int)((unsigned)a.V * seg / segments), n = (int)((unsigned)a.V * (seg + 1) / segments) - lo;
+  const unsigned group = row / (unsigned)a.K;
+  const T* z = static_cast<const T*>(a.logits) + group * a.ld_group + (row - group * a.K) * a.ld_beam + lo;
   // aligned vectors, and the few values before and behind them, one per thread
   const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int)sizeof(T));
   const int nvec = (n - head) / VEC, tail = n - head - nvec * VEC;
@@ -132,27 +154,24 @@ __global__ void __launch_bounds__(THREADS, 5) select_rows_kernel(const SelectArg
   int single = -1;
   if (tid < head) single = tid;
   else if (tid >= 16 && tid < 16 + tail) single = n - tail + (tid - 16);
-  uint4 u[NV];
+  uint4 u[NV];  // -inf behind the last vector
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i * THREADS + tid < nvec) u[i] = __ldg(zv + i * THREADS + tid);
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+    u[i] = i * THREADS + tid < nvec ? __ldg(zv + i * THREADS + tid) : make_uint4(none, none, none, none);
+  }
   const float one = single >= 0 ? rt::to_f<T>(z[single]) : -INFINITY;
   if (tid == 0) found = 0;
 
-  // ---- maximum, and whether the segment holds what gives a beam no rank
+  // ---- maximum (of the numbers: a NaN or +inf, which leaves its beam without a rank, makes the sum below NaN)
   float top = one;
-  bool bad = !(one < INFINITY);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i * THREADS + tid < nvec) {
-      float f[VEC];
-      unpack(u[i], f);
+  for (int i = 0; i < NV; ++i) {
+    float f[VEC];
+    unpack(u[i], f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        top = fmaxf(top, f[j]);
-        bad |= !(f[j] < INFINITY);
-      }
-    }
+    for (int j = 0; j < VEC; ++j) top = fmaxf(top, f[j]);
+  }
   const unsigned mine = single >= 0 || tid < nvec ? order_key(top) : 0u;
   float m = top;
 #pragma unroll
@@ -170,33 +189,29 @@ __global__ void __launch_bounds__(THREADS, 5) select_rows_kernel(const SelectArg
     if (lane == 0) warp_bound[warp] = t;
   }
   if (lane == 0) warp_top[warp] = m;
-  bad = __syncthreads_or(bad);
+  __syncthreads();
   m = warp_top[0];
 #pragma unroll
   for (int w = 1; w < WARPS; ++w) m = fmaxf(m, warp_top[w]);
-  const long at = row * a.segments + seg;
-  if (bad) {
-    if (tid == 0) {
-      a.tops[at] = INFINITY;
-      a.sums[at] = NAN;
-    }
-    return;
-  }
+  const long at = blockIdx.x;
 
   // ---- sum of exponentials (differences before products: a mask of the type's lowest value may leave fp32's range)
-  float s[2] = {0.f, 0.f};
+  float2 sum2 = make_float2(0.f, 0.f);
   if (m > -INFINITY) {
-    if (single >= 0) s[0] = ex2((one - m) * LOG2E);
+    if (single >= 0) sum2.x = ex2((one - m) * LOG2E);
+    const float2 less = make_float2(-m, -m), scale = make_float2(LOG2E, LOG2E);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (i * THREADS + tid < nvec) {
-        float f[VEC];
-        unpack(u[i], f);
+    for (int i = 0; i < NV; ++i) {
+      float f[VEC];
+      unpack(u[i], f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s[j & 1] += ex2((f[j] - m) * LOG2E);
+      for (int j = 0; j < VEC; j += 2) {
+        const float2 y = mul2(add2(make_float2(f[j], f[j + 1]), less), scale);
+        sum2 = add2(sum2, make_float2(ex2(y.x), ex2(y.y)));
       }
+    }
   }
-  double d = (double)s[0] + (double)s[1];
+  double d = (double)sum2.x + (double)sum2.y;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(~0u, d, o);
   if (lane == 0) warp_sum[warp] = d;
@@ -214,13 +229,15 @@ __global__ void __launch_bounds__(THREADS, 5) select_rows_kernel(const SelectArg
     };
     if (single >= 0) take(one, lo + single);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (i * THREADS + tid < nvec) {
-        float f[VEC];
-        unpack(u[i], f);
+    for (int i = 0; i < NV; ++i) {
+      float f[VEC], best = -INFINITY;
+      unpack(u[i], f);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) best = fmaxf(best, f[j]);
+      if (best >= least && i * THREADS + tid < nvec)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) take(f[j], lo + head + (i * THREADS + tid) * VEC + j);
-      }
+    }
   }
   __syncthreads();
   if (tid == 0) {
@@ -260,20 +277,27 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.K, S = a.segments, lists = K * S;
   const long first = (long)blockIdx.x * K;
   if (tid == 0) found = 0;
+  const int whole = min((lists + 31) / 32, MERGE_WARPS), mine = lane * whole + warp;  // this thread's first list
+  const unsigned long long first_head = warp < whole && mine < lists ? a.entries[(first * S + mine) * K] : 0ull;
   for (int b = warp; b < K; b += MERGE_WARPS) {
     const long row = first + b;
-    const float score = a.scores[row];
-    const bool finished = a.finished[row], run = !finished && isfinite(score);
-    const int length = a.lengths[row] + (finished ? 0 : 1);
+    // (what rows that do not run leave unwritten is loaded with the rest, in one wait for memory, and not used)
     float t[4], top = -INFINITY;
     double s[4], sum = 0.0;
-    for (int i0 = 0; i0 < S && run; i0 += 128) {  // (one round for up to 128 segments: the values stay)
+    auto load = [&](int i0) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int i = i0 + j * 32 + lane;
         t[j] = i < S ? a.tops[row * S + i] : -INFINITY;
         s[j] = i < S ? a.sums[row * S + i] : 0.0;
       }
+    };
+    load(0);
+    const float score = a.scores[row];
+    const bool finished = a.finished[row], run = !finished && isfinite(score);
+    const int length = a.lengths[row] + (finished ? 0 : 1);
+    for (int i0 = 0; i0 < S && run; i0 += 128) {
+      if (i0) load(i0);
       float more = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) more = fmaxf(more, __shfl_xor_sync(~0u, more, o));
@@ -298,8 +322,9 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     }
   }
   __syncthreads();
-  // j-th entry of list i (rank key 0: there is none)
-  auto item = [&](int i, int j, unsigned long long& rank, long& flat, double& value) {
+  auto entry_of = [&](int i, int j) { return kind[i / S] == 0 && j < K ? a.entries[(first * S + i) * K + j] : 0ull; };
+  // j-th entry of list i, which is e where its row runs (rank key 0: there is none)
+  auto item = [&](int i, int j, unsigned long long e, unsigned long long& rank, long& flat, double& value) {
     const int b = i / S, seg = i - b * S;
     rank = 0;
     flat = LONG_MAX;
@@ -307,7 +332,6 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     if (j >= K) return;
     int token;
     if (kind[b] == 0) {
-      const unsigned long long e = a.entries[((first + b) * S + seg) * K + j];
       if (e == 0) return;
       token = (int)~(unsigned)e;
       const float z = key_value((unsigned)(e >> 32));
@@ -326,14 +350,13 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
   };
   // the upper half of a rank's key keeps its order. A warp's lists are spread over all beams, as they are not alike
   // (a thread may stand for several lists); each warp's k-th largest head, as in a segment
-  const int whole = min((lists + 31) / 32, MERGE_WARPS);
   if (warp < whole) {
     unsigned head = 0, t = 0;
-    for (int i = lane * whole + warp; i < lists; i += 32 * whole) {
+    for (int i = mine; i < lists; i += 32 * whole) {
       unsigned long long r;
       long f;
       double v;
-      item(i, 0, r, f, v);
+      item(i, 0, i == mine ? first_head : entry_of(i, 0), r, f, v);
       head = max(head, (unsigned)(r >> 32));
     }
     const unsigned best = head;
@@ -376,11 +399,11 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     least = warp_bound[0];
   }
   least = max(least, 1u);
-  auto offer = [&](int i, int j) {
+  auto offer = [&](int i, int j, unsigned long long e) {
     unsigned long long r;
     long f;
     double v;
-    item(i, j, r, f, v);
+    item(i, j, e, r, f, v);
     if ((unsigned)(r >> 32) >= least) {
       const int to = atomicAdd(&found, 1);
       if (to < MERGE_LIST) {
@@ -412,11 +435,11 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int i = i0 + k * MERGE_WARPS * per;
-      if (in[k] && !(key_value((unsigned)(in[k] >> 32)) < row_least[i / S])) offer(i, j);
+      if (in[k] && !(key_value((unsigned)(in[k] >> 32)) < row_least[i / S])) offer(i, j, in[k]);
     }
   }
   for (int e = tid; e < K * K; e += MERGE_THREADS)
-    if (kind[e / K] != 0) offer(e / K * S, e % K);
+    if (kind[e / K] != 0) offer(e / K * S, e % K, 0ull);
   __syncthreads();
   const int have = found;
   if (have <= MERGE_LIST) {
@@ -434,21 +457,21 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     for (int i = tid; i < lists; i += MERGE_THREADS) taken[i] = 0;
     unsigned long long rank;
     long flat;
-    int mine;
+    int best;
     double value;
     auto refresh = [&]() {  // the best head of this thread's lists
       rank = 0;
       flat = LONG_MAX;
-      mine = -1;
+      best = -1;
       for (int i = tid; i < lists; i += MERGE_THREADS) {
         unsigned long long r;
         long f;
         double v;
-        item(i, taken[i], r, f, v);
+        item(i, taken[i], entry_of(i, taken[i]), r, f, v);
         if (r > rank || (r == rank && f < flat)) {
           rank = r;
           flat = f;
-          mine = i;
+          best = i;
           value = v;
         }
       }
@@ -481,10 +504,10 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
         best_flat = f;
       }
       __syncthreads();
-      if (mine >= 0 && flat == best_flat && rank == best_rank) {
+      if (best >= 0 && flat == best_flat && rank == best_rank) {
         chosen[n] = flat;
         values[n] = value;
-        ++taken[mine];
+        ++taken[best];
         refresh();
       }
     }
@@ -494,7 +517,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
   // ---- slots: a parent's best child keeps the parent's, the others fill what is left in order
   const bool in = lane < K;
   const unsigned all = K == 32 ? ~0u : (1u << K) - 1;
-  const int parent = in ? (int)(chosen[lane] / a.V) : 32 + lane;
+  const int parent = in ? (int)((unsigned)chosen[lane] / (unsigned)a.V) : 32 + lane;
   const unsigned siblings = __match_any_sync(~0u, parent);
   const bool keeps = in && __ffs(siblings) - 1 == lane;
   unsigned left = all & ~__reduce_or_sync(~0u, in ? 1u << parent : 0u);
@@ -505,7 +528,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     for (int skip = __popc(others & ((1u << lane) - 1)); skip > 0; --skip) left &= left - 1;
     slot = __ffs(left) - 1;
   }
-  const long token = chosen[lane] % a.V, to = first + slot;
+  const long token = chosen[lane] - (long)parent * a.V, to = first + slot;
   a.tokens[to] = token;
   a.parents[to] = parent;
   a.out_scores[to] = (float)values[lane];
