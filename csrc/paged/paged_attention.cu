@@ -135,6 +135,12 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = blockIdx.x, kv = blockIdx.y, g = blockIdx.z / a.subgroups, sub = blockIdx.z % a.subgroups;
   const int row0 = g * a.group + sub * a.together, rows = min(a.together, a.group - sub * a.together);
+  const int capacity = a.width * a.page, span = TILE / a.page;  // pages of a tile
+  int length = 0;  // of row0 + lane, for the loads
+  if (warp == 2) {
+    sm100::prefetch_tmap(&map);
+    if (lane < rows) length = min(max(a.lengths[row0 + lane], 0), capacity);
+  }
   if (tid == 0) {
     for (int i = 0; i < RING; ++i) {
       sm100::mbar_init(&full[i], 1);
@@ -162,9 +168,6 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
 
   if (warp == 2) {
     // ------------------------------------------------------------ loads
-    if (lane == 0) sm100::prefetch_tmap(&map);
-    const int capacity = a.width * a.page, span = TILE / a.page;  // pages of a tile
-    const int length = lane < rows ? min(max(a.lengths[row0 + lane], 0), capacity) : 0;
     const int longest = __reduce_max_sync(~0u, length);
     const int count = (longest + TILE - 1) / TILE;
     // The rows' pages of the block's next 16 tiles, a lane per tile, so that their loads wait for memory together
@@ -493,68 +496,113 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
   }
 }
 
-// Block of 256 threads per (row, query head): the splits' weights first, then their sums, a thread per four components of
-// every (256 / (D / 4))-th split, so that all of them are loaded at once.
+__device__ __forceinline__ void finish(const AttendArgs& a, long rh, int D, int c, float4 o, float l, const float (&gate)[4]) {
+  const float scale = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
+  float v[4] = {o.x * scale, o.y * scale, o.z * scale, o.w * scale};
+  if (a.gate)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= rt::sigmoidf_(gate[j]);
+  __nv_bfloat162 r[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+  *reinterpret_cast<uint2*>(a.out + rh * D + c) = *reinterpret_cast<const uint2*>(r);
+}
+
+// Up to FEW splits: a thread per four components of a (row, query head), several of them per block, no barrier (1536 of
+// them with two splits: 15 us by the kernel below, one block each).
+constexpr int FEW = 8;
+__global__ void __launch_bounds__(256) join_few_kernel(const AttendArgs a, int D, long items) {
+  const int wide = D / 4;
+  const long rh = (long)blockIdx.x * (256 / wide) + threadIdx.x / wide;
+  if (rh >= items) return;
+  const int c = threadIdx.x % wide * 4, head = rh % a.heads, row = rh / a.heads;
+  float gate[4] = {0.f, 0.f, 0.f, 0.f};
+  if (a.gate)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) gate[j] = rt::to_f(a.gate[row * a.gate_row + head * a.gate_head + c + j]);
+  float4 x[FEW];
+  float2 st[FEW];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < FEW; ++i) {
+    const bool on = i < a.splits;
+    st[i] = on ? a.stats[rh * a.splits + i] : make_float2(-INFINITY, 0.f);
+    x[i] = on ? *reinterpret_cast<const float4*>(a.sums + (rh * a.splits + i) * D + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    m = fmaxf(m, st[i].x);
+  }
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < FEW; ++i) {
+    // (a split that saw nothing has the sum 0 and the reference -inf)
+    const float w = st[i].y == 0.f ? 0.f : st[i].x == m ? 1.f : ex2(st[i].x - m);
+    l += w * st[i].y;
+    o.x += w * x[i].x;
+    o.y += w * x[i].y;
+    o.z += w * x[i].z;
+    o.w += w * x[i].w;
+  }
+  finish(a, rh, D, c, o, l, gate);
+}
+
+// Block of 256 threads per (row, query head), a thread per four components of every (1024 / dim)-th split. Everything is
+// loaded at once: each warp forms the splits' weights for itself, so that one barrier is left, before the threads' sums
+// are added.
 __global__ void __launch_bounds__(256) join_kernel(const AttendArgs a, int D) {
-  __shared__ float weight[MAX_SPLITS], scratch[32];
+  constexpr int EACH = (MAX_SPLITS + 31) / 32, AHEAD = 10;
+  __shared__ float weights[8][MAX_SPLITS];
   __shared__ float4 parts[256];
   const long rh = blockIdx.x;
-  const int head = rh % a.heads, row = rh / a.heads, tid = threadIdx.x, wide = D / 4, c = tid % wide, first = tid / wide;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float2 st[2];
-  float m = -INFINITY;
+  const int head = rh % a.heads, row = rh / a.heads, tid = threadIdx.x, lane = tid & 31, wide = D / 4;
+  const int c = tid % wide, first = tid / wide, step = 256 / wide;
+  const float4* sums = reinterpret_cast<const float4*>(a.sums) + rh * a.splits * wide + c;
+  float4 x[AHEAD];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int i = j * 256 + tid;
+  for (int k = 0; k < AHEAD; ++k)
+    x[k] = first + k * step < a.splits ? sums[(long)(first + k * step) * wide] : make_float4(0.f, 0.f, 0.f, 0.f);
+  float gate[4] = {0.f, 0.f, 0.f, 0.f};
+  if (a.gate && tid < wide)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) gate[j] = rt::to_f(a.gate[row * a.gate_row + head * a.gate_head + tid * 4 + j]);
+  float2 st[EACH];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    const int i = j * 32 + lane;
     st[j] = i < a.splits ? a.stats[rh * a.splits + i] : make_float2(-INFINITY, 0.f);
     m = fmaxf(m, st[j].x);
   }
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, off));
-  if ((tid & 31) == 0) scratch[tid >> 5] = m;
-  __syncthreads();
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  float* weight = weights[tid >> 5];
 #pragma unroll
-  for (int w = 0; w < 8; ++w) m = fmaxf(m, scratch[w]);
-  float l = 0.f;
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int i = j * 256 + tid;
-    // (a split that saw nothing has the sum 0 and the reference -inf)
+  for (int j = 0; j < EACH; ++j) {
     const float w = st[j].y == 0.f ? 0.f : st[j].x == m ? 1.f : ex2(st[j].x - m);
-    if (i < a.splits) weight[i] = w;
+    if (j * 32 + lane < a.splits) weight[j * 32 + lane] = w;
     l += w * st[j].y;
   }
-  l = rt::block_sum(l, scratch);
-  const float4* sums = reinterpret_cast<const float4*>(a.sums) + rh * a.splits * wide + c;
-  const int step = 256 / wide;
-#pragma unroll 10
-  for (int i = first; i < a.splits; i += step) {
+  l = rt::warp_sum(l);
+  __syncwarp();
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](int i, const float4& v) {
     const float w = weight[i];
-    const float4 x = sums[(long)i * wide];
-    o.x += w * x.x;
-    o.y += w * x.y;
-    o.z += w * x.z;
-    o.w += w * x.w;
-  }
+    o.x += w * v.x;
+    o.y += w * v.y;
+    o.z += w * v.z;
+    o.w += w * v.w;
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (first + k * step < a.splits) add(first + k * step, x[k]);
+  for (int i = first + AHEAD * step; i < a.splits; i += step) add(i, sums[(long)i * wide]);
   parts[tid] = o;
   __syncthreads();
   if (tid >= wide) return;
   for (int i = 1; i < step; ++i) {
-    const float4 x = parts[i * wide + tid];
-    o.x += x.x;
-    o.y += x.y;
-    o.z += x.z;
-    o.w += x.w;
+    const float4 v = parts[i * wide + tid];
+    o.x += v.x;
+    o.y += v.y;
+    o.z += v.z;
+    o.w += v.w;
   }
-  float v[4] = {o.x, o.y, o.z, o.w};
-  __nv_bfloat16 r[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float y = l == 0.f ? 0.f : v[j] / l;
-    if (a.gate) y *= rt::sigmoidf_(rt::to_f(a.gate[row * a.gate_row + head * a.gate_head + tid * 4 + j]));
-    r[j] = __float2bfloat16_rn(y);
-  }
-  *reinterpret_cast<uint2*>(a.out + rh * D + tid * 4) = *reinterpret_cast<const uint2*>(r);
+  finish(a, rh, D, tid * 4, o, l, gate);
 }
 
 // How a call is cut: rows of a group that fit a block's queries (and a lane each) together, evenly; splits of the keys
@@ -647,6 +695,8 @@ extern "C" cudaError_t rt_paged_attention(const RtPool* p, int block, const int*
   else if (p->dim == 128) RT_CUDA_CHECK(launch<128>(map, a, x, s));
   else if (p->dim == 256) RT_CUDA_CHECK(launch<256>(map, a, x, s));
   else return cudaErrorInvalidValue;
-  join_kernel<<<(unsigned)(p->rows * heads), 256, 0, s>>>(a, p->dim);
+  const long items = (long)p->rows * heads, together = 1024 / p->dim;
+  if (x.splits <= FEW) join_few_kernel<<<(unsigned)((items + together - 1) / together), 256, 0, s>>>(a, p->dim, items);
+  else join_kernel<<<(unsigned)items, 256, 0, s>>>(a, p->dim);
   return cudaGetLastError();
 }
