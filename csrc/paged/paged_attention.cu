@@ -20,6 +20,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <type_traits>
 #include <cuda.h>
 #include "../api.h"
 #include "../common/common.cuh"
@@ -31,6 +32,7 @@ namespace {
 using bf16 = __nv_bfloat16;
 constexpr int TILE = 64, QUERIES = 64, THREADS = 192;  // keys of a unit, queries of a block
 constexpr int MAX_SPLITS = 296, UNITS = 8;
+constexpr int AHEAD = 8, APART = 16;  // tiles whose pages are looked up together; last tiles that may be dealt out by units
 constexpr float HEADROOM = 8.f;  // log2 that a score may exceed its reference by before that is raised
 
 struct AttendArgs {
@@ -66,8 +68,9 @@ template <int D> struct Shape {
   // products read 64 rows more than a tile of weights or queries has: what follows has to be as long
   static constexpr int Q = P + 2 * P_BYTES;                         // [D / 64][64][64]
   static constexpr int KV = Q + QUERIES * D * 2;
-  static constexpr int TABLE = KV + RING * HALF;                    // [32 rows][4][16 tiles]
-  static constexpr int MAX = TABLE + 32 * 4 * 16 * 4;               // [64 queries][2]
+  static constexpr int TABLE = KV + RING * HALF;                    // [32 rows][4][AHEAD tiles]
+  static constexpr int TAIL = TABLE + 32 * 4 * AHEAD * 4;           // [32 rows][4][APART tiles]
+  static constexpr int MAX = TAIL + 32 * 4 * APART * 4;             // [64 queries][2]
   static constexpr int UNIT = MAX + QUERIES * 2 * 4;
   static constexpr int BARS = UNIT + UNITS * 24;
   static constexpr int BYTES = BARS + 8 * (2 * RING + UNITS + 8) + 16 + 1024;
@@ -118,7 +121,7 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
   extern __shared__ uint8_t raw[];
   uint8_t* smem = sm100::align_smem_1024(raw);
   uint8_t *sP = smem + Sh::P, *sQ = smem + Sh::Q, *sKV = smem + Sh::KV;
-  int* sTable = reinterpret_cast<int*>(smem + Sh::TABLE);
+  int *sTable = reinterpret_cast<int*>(smem + Sh::TABLE), *sTail = reinterpret_cast<int*>(smem + Sh::TAIL);
   float* sMax = reinterpret_cast<float*>(smem + Sh::MAX);
   Unit* units = reinterpret_cast<Unit*>(smem + Sh::UNIT);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sh::BARS);  // a tile of the ring has landed
@@ -170,10 +173,14 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
     // ------------------------------------------------------------ loads
     const int longest = __reduce_max_sync(~0u, length);
     const int count = (longest + TILE - 1) / TILE;
-    // The rows' pages of the block's next 16 tiles, a lane per tile, so that their loads wait for memory together
-    // (-1: no such page); sTable[(row * 4 + j) * 16 + tile].
-    auto look_up = [&](int first, int step) {
+    // The rows' pages of N tiles, a lane per tile, so that their loads wait for memory together (-1: no such page);
+    // to[(row * 4 + j) * N + tile]. Returns whether the lane's tile is another one for some row than for the first.
+    auto look_up = [&](auto tiles, int first, int step, int* to) {
+      constexpr int N = decltype(tiles)::value;
       const int i = first + lane * step;
+      const int n0 = min(max(__shfl_sync(~0u, length, 0) - i * TILE, 0), TILE);
+      int e0[4];
+      bool apart = false;
       for (int r0 = 0; r0 < rows; r0 += 8) {
         int e[8][4];
 #pragma unroll
@@ -182,28 +189,38 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
           const int* table = a.table + (long)(row0 + r0 + r) * a.width;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            e[r][j] = lane < 16 && j < span && i < count && i * TILE + j * a.page < n ? table[i * span + j] : -1;
+            e[r][j] = lane < N && j < span && i < count && i * TILE + j * a.page < n ? table[i * span + j] : -1;
+          apart |= r0 + r < rows && min(max(n - i * TILE, 0), TILE) != n0;
         }
 #pragma unroll
         for (int r = 0; r < 8; ++r)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (lane < 16) sTable[((r0 + r) * 4 + j) * 16 + lane] = e[r][j] < a.pages ? max(e[r][j], -1) : -1;
+          for (int j = 0; j < 4; ++j) {
+            const int page = e[r][j] < a.pages ? max(e[r][j], -1) : -1;
+            if (r == 0 && r0 == 0) e0[j] = page;
+            apart |= r0 + r < rows && page != e0[j];
+            if (lane < N) to[((r0 + r) * 4 + j) * N + lane] = page;
+          }
       }
       __syncwarp();
+      return apart && lane < N && i < count;
     };
     const uint64_t one = a.per_kv == 64 ? ~0ull : (1ull << a.per_kv) - 1;  // the queries of row 0
     int entry = 0, unit = 0;  // tiles of the ring (keys, values, keys, ...) and units so far
     bool ok = true;
-    // The tiles are dealt out to the splits in turn; of the last 16, where beams have gone apart, the units one by one.
-    const int tail = max(count - 16, 0);
+    // The tiles are dealt out to the splits in turn; from the first of the last APART on where rows have gone apart, the
+    // units one by one.
+    const int window = max(count - APART, 0);
+    const unsigned apart = __ballot_sync(~0u, look_up(std::integral_constant<int, APART>{}, window, 1, sTail));
+    const int tail = apart ? window + __ffs(apart) - 1 : count;
     int dealt = tail;  // units before the next one, where they are dealt out
-    for (int i = split < tail ? split : tail, t = 0; i < count && ok; t = (t + 1) & 15) {
+    for (int i = split < tail ? split : tail, t = 0; i < count && ok; t = (t + 1) % AHEAD) {
       const bool single = i >= tail;
-      if (t == 0) look_up(i, single ? 1 : a.splits);
+      if (!single && i < window && t == 0) look_up(std::integral_constant<int, AHEAD>{}, i, a.splits, sTable);
       int e[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) e[j] = lane < rows ? sTable[(lane * 4 + j) * 16 + t] : -1;
+      for (int j = 0; j < 4; ++j)
+        e[j] = lane >= rows ? -1 : i >= window ? sTail[(lane * 4 + j) * APART + i - window] : sTable[(lane * 4 + j) * AHEAD + t];
       const int valid = min(max(length - i * TILE, 0), TILE);
       unsigned same = __match_any_sync(~0u, valid);
       bool any = false;
@@ -256,12 +273,8 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
         ++unit;
       }
       __syncwarp();
-      if (single) {
-        ++i;
-      } else if ((i += a.splits) >= tail) {
-        i = tail;
-        t = 15;  // looked up anew
-      }
+      if (single) ++i;
+      else i = min(i + a.splits, tail);
     }
     if (ok && lane == 0) {
       units[unit % UNITS].members = 0;
