@@ -213,19 +213,21 @@ class _StepGraph:
 
 @torch.no_grad()
 def beam_search(runner, prompt, new_tokens, beams=4, end_token=-1, length_penalty=0.0, prefill_chunk=4096, page=64,
-                graph=False):
+                on_token=None, graph=False):
     """The ``beams`` best continuations of each prompt of ``prompt`` [G, T] that a beam search finds, best first:
     (ids [G, beams, new_tokens], scores [G, beams], lengths [G, beams]).
 
     A continuation ends with ``end_token`` (its ids are followed by more of them, and its length counts the first) or
     after ``new_tokens``. Scores are sums of log-probabilities; the order is that of score / length^length_penalty
     (see ``beam_select``). ``page``: tokens in a page of the key/value cache (full-attention blocks that were not
-    replaced). ``graph=True`` replays the steps as a CUDA graph after the first. The runner's own cache and states
-    are left as they are."""
+    replaced). ``on_token(step)`` is called after each decode step. ``graph=True`` replays the steps as a CUDA graph
+    after the first. The runner's own cache and states are left as they are."""
     if prompt.dim() != 2 or prompt.numel() == 0:
         raise ValueError(f"expected prompts [groups, tokens], got {tuple(prompt.shape)}")
     if new_tokens < 1 or beams < 1:
         raise ValueError("beam search needs at least one beam and one new token")
+    if prompt.is_cuda and beams > MAX_BEAMS:
+        raise ValueError(f"beam search takes at most {MAX_BEAMS} beams on CUDA, got {beams}")
     every = 16  # steps between two looks at whether all beams have ended
     with isolated_state(runner):
         for start in range(0, prompt.shape[1], prefill_chunk):
@@ -236,6 +238,8 @@ def beam_search(runner, prompt, new_tokens, beams=4, end_token=-1, length_penalt
             if end_token >= 0 and step % every == 0 and bool(search.finished.all()):
                 break  # what follows would add end tokens alone
             stepper.step()
+            if on_token is not None:
+                on_token(step)
             if graph and stepper is search and step + 1 < new_tokens:
                 stepper = _StepGraph(search)
         search.record()

@@ -62,6 +62,14 @@ def _check_rows(name, part, pool, table, shape):
         raise TypeError(f"the CUDA paged cache takes bf16 {name}")
 
 
+def _check_out(given, to):
+    """What is written may be what is read, or lie apart from it."""
+    for part, out in zip(given, to):
+        start, other = part.data_ptr(), out.data_ptr()
+        if start != other and start < other + out.nbytes and other < start + part.nbytes:
+            raise ValueError("out must be the arguments themselves or apart from them")
+
+
 def check_parents(parents, rows, device):
     """[groups, beams] indices of each slot's parent within its group, ``rows`` slots in all."""
     if parents.dim() != 2 or parents.numel() != rows:
@@ -99,6 +107,7 @@ def advance_pages(pool, table, lengths, refs, tokens=1, parents=None, live=None,
         if out[0].shape != table.shape or out[3].shape != (1,) or out[3].dtype != torch.int32 or \
                 out[3].device != pool.device:
             raise ValueError("out must be (table, lengths, refs, status) like the arguments")
+        _check_out((table, lengths, refs), out)
     if pool.is_cuda:
         return tuple(native().advance_pages(pool, table, lengths, refs, tokens, parents, live, out))
     result = reference.advance_pages(pool, table, lengths, refs, tokens, parents, live)
@@ -119,6 +128,7 @@ def compact_pages(pool, table, refs, out=None):
         _check(pool, out[0], refs=out[1])
         if out[0].shape != table.shape:
             raise ValueError("out must be (table, refs) like the arguments")
+        _check_out((table, refs), out)
     if pool.is_cuda:
         return tuple(native().compact_pages(pool, table, refs, out))
     result = reference.compact_pages(pool, table, refs)

@@ -456,3 +456,120 @@ def test_greedy_is_one_beam_of_the_small_model():
     ids, scores, _ = beam_search(runner, prompt, 6, beams=1)
     # both take the largest of bf16 logits, which may differ where two are closest: compare while they agree
     assert ids[0, 0, 0] == greedy[0, 0] and scores.isfinite().all()
+
+
+def _search_state(G=2, K=4, seed=0):
+    """Tensors of a small search in the middle, and one step over them in place."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rows, V = G * K, 1501
+    cache = PagedCache(2, 2, 64, rows, 400, 150, 16, "cuda")
+    cache.pool.normal_(generator=g)
+    cache.advance_(33, live=torch.arange(K, device="cuda").expand(G, K) == 0)
+    cache.advance_(0, torch.zeros(G, K, dtype=torch.int64, device="cuda"))
+    x = torch.randn(rows, (2 * 6 + 4) * 64, device="cuda", generator=g).to(torch.bfloat16)
+    noise = torch.randn(rows, V, 384, device="cuda", generator=g) * 0.05
+    w = torch.randn(64, device="cuda", generator=g) * 0.1
+    freq = torch.rand(16, device="cuda", generator=g)
+    beams = [torch.arange(K, device="cuda").repeat(G, 1), torch.zeros(G, K, device="cuda"),
+             torch.ones(G, K, dtype=torch.int32, device="cuda"), torch.zeros(G, K, dtype=torch.bool, device="cuda")]
+    states = [torch.randn(rows, 3, 50, device="cuda", generator=g), torch.arange(rows * 7, device="cuda").view(rows, 7)]
+    seen = torch.zeros(rows, 384, device="cuda")
+
+    def step():
+        parents, scores, lengths, finished = beams
+        reorder_states_(states + [seen], parents)
+        cache.advance_(1, parents, ~finished)
+        q = cache.append_(1, x, w, w, freq, 6, 1e-6)
+        seen.mul_(0.5).add_(cache.attend(1, q, x[:, :768].view(rows, 6, 128)[..., 64:], K).reshape(rows, 384).float())
+        logits = torch.einsum("rc,rvc->rv", seen, noise).view(G, K, V)
+        tokens, *chosen = beam_select(logits, scores, lengths, finished, end_token=7, length_penalty=0.5)
+        for mine, new in zip(beams, chosen):
+            mine.copy_(new)
+        states[1].add_(tokens.view(rows, 1))
+        return [cache.pool, cache.table, cache.lengths, cache.refs, cache.status, seen, *states, *beams]
+
+    return step
+
+
+def test_a_captured_step_replays_like_an_eager_one():
+    eager, replayed = _search_state(), _search_state()
+    first = [x.clone() for x in replayed()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = replayed()
+    for got, want in zip(first, eager()):
+        assert torch.equal(got, want)
+    for _ in range(20):
+        graph.replay()
+        want = eager()
+        for got, value in zip(static, want):
+            assert torch.equal(got, value)
+    assert int(static[4]) == 0
+
+
+def test_calls_on_two_streams_at_once():
+    """Workspaces belong to a call: two searches on streams of their own do not meet."""
+    alone = _search_state(seed=1)
+    for _ in range(25):
+        want = alone()
+    steps = [_search_state(seed=1), _search_state(seed=1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(25):
+        results = []
+        for step, stream in zip(steps, streams):
+            with torch.cuda.stream(stream):
+                results.append(step())
+    torch.cuda.synchronize()
+    for result in results:
+        for got, value in zip(result, want):
+            assert torch.equal(got, value)
+
+
+def test_offsets_beyond_32_bits():
+    pages = 2 ** 31 // (2 * 2 * 4 * 64 * 256) + 40  # of 2 blocks and 4 heads of 256: more than 2^31 elements
+    pool = torch.empty(pages, 2, 2, 4, 64, 256, device="cuda", dtype=torch.bfloat16)
+    small = torch.randn(12, 2, 2, 4, 64, 256).to(torch.bfloat16)
+    pool[pages - 12:] = small.cuda()
+    table = torch.tensor([[0, 1, -1], [2, 3, 4]], dtype=torch.int32)
+    far = torch.where(table >= 0, table + pages - 12, table)
+    lengths = torch.tensor([100, 190], dtype=torch.int32)
+    q = torch.randn(2, 8, 256).to(torch.bfloat16)
+    out = paged_attention(q.cuda(), pool, 1, far.cuda(), lengths.cuda())
+    assert torch.equal(out, paged_attention(q.cuda(), small.cuda(), 1, table.cuda(), lengths.cuda()))
+    x = torch.randn(2, 24 * 256).to(torch.bfloat16).cuda()
+    w, freq = torch.zeros(256, device="cuda"), torch.ones(8, device="cuda")
+    near = small.cuda()
+    append_heads(x, pool, 1, far.cuda(), lengths.cuda(), w, w, freq, 8, 1e-6)
+    append_heads(x, near, 1, table.cuda(), lengths.cuda(), w, w, freq, 8, 1e-6)
+    k = torch.randn(2, 30, 4, 256).to(torch.bfloat16).cuda()
+    store_pages(pool, 0, far.cuda(), lengths.cuda(), k, k)
+    store_pages(near, 0, table.cuda(), lengths.cuda(), k, k)
+    assert torch.equal(pool[pages - 12:], near)
+    refs = torch.ones(pages, dtype=torch.int32)
+    refs[3] = refs[pages - 6] = refs[pages - 1] = 0
+    refs[pages - 12] = 2
+    shared = torch.tensor([[pages - 12, -1], [pages - 12, -1]], dtype=torch.int32, device="cuda")
+    held = torch.tensor([20, 20], dtype=torch.int32, device="cuda")
+    refs[4:6] = 0
+    new, _, count, status = advance_pages(pool, shared, held, refs.cuda(), 1)
+    assert new[0, 0] == 3 and new[1, 0] == pages - 12 and int(status) == 0
+    assert torch.equal(pool[3, ..., :20, :], near[0, ..., :20, :])
+    moved, _, used = compact_pages(pool, far.cuda(), count)
+    assert int(used) == int((count > 0).sum()) == pages - 4
+    # free were 4, 5, pages - 6 and pages - 1: of the last four pages the three in use move to the first three of those
+    assert torch.equal(pool[4], near[8]) and torch.equal(pool[5], near[9]) and torch.equal(pool[pages - 6], near[10])
+    assert torch.equal(moved.cpu(), far)
+    del pool
+    state = torch.arange(3, device="cuda", dtype=torch.uint8)[:, None].repeat(1, 3 << 30)
+    reorder_states_([state], torch.tensor([[2, 1, 1]], device="cuda"))
+    assert [int(state[r].min()) for r in range(3)] == [int(state[r].max()) for r in range(3)] == [2, 1, 1]
+    del state
+    wide = torch.empty(2 ** 31 + 5000, device="cuda", dtype=torch.bfloat16)
+    logits = wide.as_strided((2, 2, 2001), (2 ** 31 + 7, 2003, 1))
+    logits.normal_()
+    scores, ends = torch.zeros(2, 2, device="cuda"), torch.zeros(2, 2, dtype=torch.bool, device="cuda")
+    args = (scores, torch.ones(2, 2, dtype=torch.int32, device="cuda"), ends)
+    for a, b in zip(beam_select(logits, *args), beam_select(logits.clone(), *args)):
+        assert torch.equal(a, b)
