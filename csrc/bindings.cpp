@@ -4,10 +4,14 @@
 // stream of the tensors' device.
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <climits>
 #include <map>
 #include <string>
 #include <tuple>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <vector>
 
@@ -767,76 +771,149 @@ at::Tensor flash_attention(at::Tensor q, at::Tensor keys, at::Tensor values, at:
 }
 
 // ------------------------------------------------------------------ beam search
-// The Python layer (beams.py, paged.py) has checked shapes, types and devices.
+// These calls are short, so what the host does for them counts: arguments are checked here alone (with the errors that
+// the plain path raises), outputs come from the caching allocator without the dispatcher, workspaces without a tensor
+// (freed when the call returns: the allocator hands the memory out again on the same stream only).
+// Texts are put together without streams, whose number formatting crashes where the compiler's C++ library is not the
+// process's.
+std::string text(const char* s) { return s; }
+std::string text(int64_t v) { return std::to_string(v); }
+std::string text(int v) { return std::to_string(v); }
+std::string text(double v) { return std::to_string(v); }
+std::string text(at::ScalarType type) { return c10::toString(type); }
+std::string text(const at::Device& device) { return device.is_cuda() ? "cuda:" + std::to_string(device.index()) : "another device"; }
+std::string text(at::IntArrayRef sizes) {
+  std::string s = "(";
+  for (size_t i = 0; i < sizes.size(); ++i) s += (i ? ", " : "") + std::to_string(sizes[i]);
+  return s + ")";
+}
+template <typename E, typename... A>
+void want(bool ok, const A&... what) {
+  if (!ok) throw E((text(what) + ...));
+}
+using Value = py::value_error;
+using Type = py::type_error;
+
+at::Tensor new_like(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, t.device(), c10::nullopt));
+}
+c10::DataPtr workspace(long bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(bytes); }
+
 std::vector<at::Tensor> beam_select(at::Tensor logits, at::Tensor scores, at::Tensor lengths, at::Tensor finished,
                                     int64_t end_token, double penalty) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 3, "beam_select: logits must be CUDA [groups, beams, vocabulary]");
+  want<Value>(logits.is_cuda() && logits.dim() == 3 && logits.numel() > 0,
+              "expected logits [groups, beams, vocabulary], got ", logits.sizes());
   c10::cuda::CUDAGuard guard(logits.device());
   const int64_t G = logits.size(0), K = logits.size(1), V = logits.size(2);
-  TORCH_CHECK(K >= 1 && K <= 32 && V >= 1 && V <= (1 << 22), "beam_select: 1 to 32 beams and a vocabulary of 2^22 at most");
-  TORCH_CHECK(end_token >= -1 && end_token < V, "beam_select: end_token outside the vocabulary");
-  TORCH_CHECK(scores.scalar_type() == at::kFloat && lengths.scalar_type() == at::kInt &&
-                  finished.scalar_type() == at::kBool && scores.numel() == G * K && lengths.numel() == G * K &&
-                  finished.numel() == G * K && scores.device() == logits.device() &&
-                  lengths.device() == logits.device() && finished.device() == logits.device(),
-              "beam_select: scores fp32, lengths int32 and finished bool, one per beam");
+  auto beam_wise = [&](at::Tensor& t, at::ScalarType type, const char* name) {
+    want<Value>(t.dim() == 2 && t.size(0) == G && t.size(1) == K, name, " ", t.sizes(), " does not match logits ",
+                logits.sizes());
+    want<Type>(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+    want<Value>(t.device() == logits.device(), name, " and logits are on different devices");
+    if (!t.is_contiguous()) t = t.contiguous();
+  };
+  beam_wise(scores, at::kFloat, "scores");
+  beam_wise(lengths, at::kInt, "lengths");
+  beam_wise(finished, at::kBool, "finished");
+  want<Value>(end_token >= -1 && end_token < V, "end_token must be -1 or in 0..", V - 1, ", got ", end_token);
+  want<Value>(penalty >= -16.0 && penalty <= 16.0, "length_penalty must lie in -16..16, got ", penalty);
+  const bool half = logits.scalar_type() == at::kBFloat16;
+  want<Type>(half || logits.scalar_type() == at::kFloat, "beam_select takes bf16 or fp32 logits on CUDA");
+  want<Value>(K <= 32, "beam_select takes at most 32 beams on CUDA, got ", K);
+  want<Value>(V <= (1 << 22) - (1 << 15) && G <= (1 << 20), "beam_select: too many tokens or groups: ", logits.sizes());
   if (logits.stride(2) != 1 && V > 1) logits = logits.contiguous();
-  scores = scores.contiguous();
-  lengths = lengths.contiguous();
-  finished = finished.contiguous();
-  auto longs = scores.options().dtype(at::kLong);
-  auto tokens = at::empty({G, K}, longs), parents = at::empty({G, K}, longs);
-  auto out_scores = at::empty({G, K}, scores.options()), out_lengths = at::empty({G, K}, lengths.options());
-  auto out_finished = at::empty({G, K}, finished.options());
-  auto work = at::empty({rt_beam_select_workspace_bytes(G, K, V)}, scores.options().dtype(at::kByte));
-  check_cuda(rt_beam_select(dtype_code(logits), logits.data_ptr(), G, K, V, logits.stride(0), logits.stride(1),
+  auto tokens = new_like(logits, {G, K}, at::kLong), parents = new_like(logits, {G, K}, at::kLong);
+  auto out_scores = new_like(logits, {G, K}, at::kFloat), out_lengths = new_like(logits, {G, K}, at::kInt);
+  auto out_finished = new_like(logits, {G, K}, at::kBool);
+  const auto work = workspace(rt_beam_select_workspace_bytes(G, (int)K, V));
+  check_cuda(rt_beam_select(half, logits.data_ptr(), G, (int)K, V, logits.stride(0), logits.stride(1),
                             scores.data_ptr<float>(), lengths.data_ptr<int>(), finished.data_ptr<bool>(),
                             (int)end_token, penalty, reinterpret_cast<long*>(tokens.data_ptr<int64_t>()),
                             reinterpret_cast<long*>(parents.data_ptr<int64_t>()), out_scores.data_ptr<float>(),
-                            out_lengths.data_ptr<int>(), out_finished.data_ptr<bool>(), work.data_ptr(),
-                            stream_of(logits)),
+                            out_lengths.data_ptr<int>(), out_finished.data_ptr<bool>(), work.get(), stream_of(logits)),
              "beam_select");
   return {tokens, parents, out_scores, out_lengths, out_finished};
 }
 
+// [groups, beams] int64 of `rows` rows.
+void check_parents(const at::Tensor& parents, int64_t rows, const at::Device& device) {
+  want<Value>(parents.dim() == 2 && parents.numel() == rows, "expected parents [groups, beams] of ", rows,
+              " rows, got ", parents.sizes());
+  want<Type>(parents.scalar_type() == at::kLong && parents.device() == device, "parents must be int64 on ", device);
+}
+
 void reorder_rows_(std::vector<at::Tensor> states, at::Tensor parents) {
-  TORCH_CHECK(parents.is_cuda() && parents.scalar_type() == at::kLong && parents.dim() == 2 && parents.is_contiguous() &&
-                  parents.size(1) >= 1 && parents.size(1) <= 32,
-              "reorder_rows_: parents must be contiguous CUDA int64 [groups, 1 to 32 beams]");
+  const int64_t rows = parents.numel();
+  check_parents(parents, rows, parents.device());
+  TORCH_CHECK(parents.is_cuda(), "reorder_rows_: parents must be on a CUDA device");
   c10::cuda::CUDAGuard guard(parents.device());
   std::vector<void*> base;
   std::vector<long> bytes;
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
   for (const at::Tensor& t : states) {
-    TORCH_CHECK(t.device() == parents.device() && t.is_contiguous() && t.dim() >= 1 && t.size(0) == parents.numel() &&
-                    t.numel() > 0,
-                "reorder_rows_: states must be contiguous tensors of one row per beam");
+    want<Value>(t.dim() >= 1 && t.size(0) == rows, "expected states of ", rows, " rows, got ", t.sizes());
+    want<Value>(t.is_contiguous(), "states must be contiguous");
+    want<Value>(t.device() == parents.device(), "states and parents are on different devices");
+    const long size = t.numel() * (long)t.element_size();
+    if (size == 0) continue;
     base.push_back(t.data_ptr());
-    bytes.push_back(t.numel() / t.size(0) * (long)t.element_size());
+    bytes.push_back(size / rows);
+    const auto start = reinterpret_cast<uintptr_t>(base.back());
+    spans.emplace_back(start, start + size);
   }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    want<Value>(spans[i - 1].second <= spans[i].first, "states must not overlap");
+  if (base.empty() || parents.size(1) == 1) return;
+  want<Value>(parents.size(1) <= 32, "reorder_states_ takes at most 32 beams on CUDA, got ", parents.size(1));
+  if (!parents.is_contiguous()) parents = parents.contiguous();
   check_cuda(rt_reorder_rows(base.data(), bytes.data(), (int)base.size(),
                              reinterpret_cast<const long*>(parents.data_ptr<int64_t>()), parents.size(0),
                              (int)parents.size(1), stream_of(parents)),
              "reorder_rows_");
 }
 
-RtPool pool_of(const at::Tensor& pool, const at::Tensor& table) {
-  check_bf16(pool, "pool");
-  TORCH_CHECK(pool.dim() == 6 && pool.size(2) == 2 && pool.numel() > 0 && pool.size(0) < (1 << 30) &&
-                  pool.size(1) * pool.size(3) < (1 << 20),
-              "pool must be [pages, blocks, 2, heads, page, dim]");
-  TORCH_CHECK(pool.size(4) == 16 || pool.size(4) == 32 || pool.size(4) == 64, "a page holds 16, 32 or 64 tokens");
-  TORCH_CHECK(pool.size(5) == 64 || pool.size(5) == 128 || pool.size(5) == 256, "head size must be 64, 128 or 256");
-  TORCH_CHECK(table.device() == pool.device() && table.scalar_type() == at::kInt && table.is_contiguous() &&
-                  table.dim() == 2 && table.numel() > 0 && table.size(0) <= 1024 && table.size(1) < (1 << 24),
-              "table must be contiguous int32 [1 to 1024 rows, width] on the pool's device");
-  return {pool.data_ptr(), (int)pool.size(0), (int)pool.size(1), (int)pool.size(3), (int)pool.size(4),
-          (int)pool.size(5), (int)table.size(0), (int)table.size(1)};
+// int32 of a shape beside the pool.
+int* ints(const at::Tensor& t, const at::Tensor& pool, at::IntArrayRef shape, const char* name) {
+  want<Type>(t.scalar_type() == at::kInt && t.is_contiguous(), name, " must be contiguous int32");
+  want<Value>(t.sizes() == shape, name, " ", t.sizes(), " does not match ", shape);
+  want<Value>(t.device() == pool.device(), name, " is on ", t.device(), ", the pool on ", pool.device());
+  return t.data_ptr<int>();
 }
 
-int* ints(const at::Tensor& t, const at::Tensor& pool, int64_t numel, const char* name) {
-  TORCH_CHECK(t.device() == pool.device() && t.scalar_type() == at::kInt && t.is_contiguous() && t.numel() == numel,
-              name, " must be ", numel, " contiguous int32 on the pool's device");
-  return t.data_ptr<int>();
+// Checks a pool and its table. `block` -1: none is meant.
+RtPool pool_of(const at::Tensor& pool, const at::Tensor& table, int64_t block = -1) {
+  want<Value>(pool.dim() == 6 && pool.size(2) == 2 && pool.numel() > 0,
+              "expected a pool [pages, blocks, 2, heads, page, dim], got ", pool.sizes());
+  const int64_t page = pool.size(4), dim = pool.size(5);
+  want<Value>(page == 16 || page == 32 || page == 64, "a page holds (16, 32, 64) tokens, got ", page);
+  want<Value>(pool.is_contiguous(), "the pool must be contiguous");
+  want<Value>(table.dim() == 2 && table.numel() > 0, "expected a table [rows, width], got ", table.sizes());
+  ints(table, pool, table.sizes(), "table");
+  want<py::index_error>(block >= -1 && block < pool.size(1), "block ", block, " of ", pool.size(1));
+  want<Type>(pool.is_cuda() && pool.scalar_type() == at::kBFloat16 && (dim == 64 || dim == 128 || dim == 256),
+             "the CUDA paged cache takes bf16 and head sizes (64, 128, 256), got ", pool.scalar_type(), " and ", dim);
+  want<Value>(table.size(0) <= 1024, "the CUDA paged cache has at most 1024 rows, got ", table.size(0));
+  want<Value>(pool.size(0) < (1 << 30) && pool.size(1) * pool.size(3) < (1 << 20) && table.size(1) < (1 << 24) &&
+                  pool.numel() / dim <= INT_MAX,
+              "paged cache: size out of range");
+  return {pool.data_ptr(), (int)pool.size(0), (int)pool.size(1), (int)pool.size(3), (int)page,
+          (int)dim,        (int)table.size(0), (int)table.size(1)};
+}
+
+// bf16 of a shape on the pool's device, with unit inner stride.
+void bf16_rows(at::Tensor& t, const at::Tensor& pool, at::IntArrayRef shape, const char* name) {
+  want<Value>(t.sizes() == shape, name, " ", t.sizes(), " does not match ", shape);
+  want<Value>(t.device() == pool.device(), name, " is on ", t.device(), ", the pool on ", pool.device());
+  want<Type>(t.scalar_type() == at::kBFloat16, "the CUDA paged cache takes bf16 ", name);
+  if (t.stride(-1) != 1) t = t.contiguous();
+}
+
+// What is written may be what is read, or lie apart from it.
+void check_apart(const at::Tensor& in, const at::Tensor& out) {
+  const auto a = reinterpret_cast<uintptr_t>(in.data_ptr()), b = reinterpret_cast<uintptr_t>(out.data_ptr());
+  want<Value>(a == b || a >= b + out.nbytes() || b >= a + in.nbytes(),
+              "out must be the arguments themselves or apart from them");
 }
 
 std::vector<at::Tensor> advance_pages(at::Tensor pool, at::Tensor table, at::Tensor lengths, at::Tensor refs,
@@ -844,31 +921,40 @@ std::vector<at::Tensor> advance_pages(at::Tensor pool, at::Tensor table, at::Ten
                                       c10::optional<at::Tensor> live, c10::optional<std::vector<at::Tensor>> out) {
   const RtPool p = pool_of(pool, table);
   c10::cuda::CUDAGuard guard(pool.device());
-  TORCH_CHECK(tokens >= 0 && tokens <= (1 << 30), "advance_pages: tokens out of range");
+  const int* length = ints(lengths, pool, {p.rows}, "lengths");
+  const int* count = ints(refs, pool, {p.pages}, "refs");
+  want<Value>(tokens >= 0 && tokens <= (1 << 30), "tokens must lie in 0..2^30, got ", tokens);
   int K = 1;
   if (parents.has_value()) {
-    TORCH_CHECK(parents->device() == pool.device() && parents->scalar_type() == at::kLong && parents->dim() == 2 &&
-                    parents->is_contiguous() && parents->numel() == p.rows,
-                "advance_pages: parents must be contiguous int64 [groups, beams]");
+    check_parents(*parents, p.rows, pool.device());
+    if (!parents->is_contiguous()) parents = parents->contiguous();
     K = (int)parents->size(1);
   }
-  TORCH_CHECK(!live.has_value() || (live->device() == pool.device() && live->scalar_type() == at::kBool &&
-                                    live->is_contiguous() && live->numel() == p.rows),
-              "advance_pages: live must be one bool per row");
+  if (live.has_value()) {
+    want<Value>(live->scalar_type() == at::kBool && live->numel() == p.rows && live->device() == pool.device(),
+                "live must be ", p.rows, " bools on ", pool.device());
+    if (!live->is_contiguous()) live = live->contiguous();
+  }
   const bool given = out.has_value();
   if (!given)
-    out = std::vector<at::Tensor>{at::empty_like(table), at::empty_like(lengths), at::empty_like(refs),
-                                  at::empty({1}, lengths.options())};
-  TORCH_CHECK(out->size() == 4, "advance_pages: out is (table, lengths, refs, status)");
+    out = std::vector<at::Tensor>{new_like(pool, {p.rows, p.width}, at::kInt), new_like(pool, {p.rows}, at::kInt),
+                                  new_like(pool, {p.pages}, at::kInt), new_like(pool, {1}, at::kInt)};
+  want<Value>(out->size() == 4, "out must be (table, lengths, refs, status) like the arguments");
   const at::Tensor &t = (*out)[0], &l = (*out)[1], &r = (*out)[2], &st = (*out)[3];
-  auto work = at::empty({rt_advance_workspace_bytes(p.rows)}, table.options().dtype(at::kByte));
-  check_cuda(rt_advance_pages(&p, table.data_ptr<int>(), ints(lengths, pool, p.rows, "lengths"),
-                              ints(refs, pool, p.pages, "refs"), (int)tokens,
+  int* new_table = ints(t, pool, {p.rows, p.width}, "out table");
+  int* new_lengths = ints(l, pool, {p.rows}, "out lengths");
+  int* new_refs = ints(r, pool, {p.pages}, "out refs");
+  int* status = ints(st, pool, {1}, "out status");
+  if (given) {
+    check_apart(table, t);
+    check_apart(lengths, l);
+    check_apart(refs, r);
+  }
+  const auto work = workspace(rt_advance_workspace_bytes(p.rows));
+  check_cuda(rt_advance_pages(&p, table.data_ptr<int>(), length, count, (int)tokens,
                               parents.has_value() ? reinterpret_cast<const long*>(parents->data_ptr<int64_t>()) : nullptr,
-                              K, live.has_value() ? live->data_ptr<bool>() : nullptr,
-                              ints(t, pool, (int64_t)p.rows * p.width, "out table"), ints(l, pool, p.rows, "out lengths"),
-                              ints(r, pool, p.pages, "out refs"), ints(st, pool, 1, "out status"), given,
-                              work.data_ptr(), stream_of(pool)),
+                              K, live.has_value() ? live->data_ptr<bool>() : nullptr, new_table, new_lengths, new_refs,
+                              status, given, work.get(), stream_of(pool)),
              "advance_pages");
   return *out;
 }
@@ -877,13 +963,20 @@ std::vector<at::Tensor> compact_pages(at::Tensor pool, at::Tensor table, at::Ten
                                       c10::optional<std::vector<at::Tensor>> out) {
   const RtPool p = pool_of(pool, table);
   c10::cuda::CUDAGuard guard(pool.device());
-  if (!out.has_value()) out = std::vector<at::Tensor>{at::empty_like(table), at::empty_like(refs)};
-  TORCH_CHECK(out->size() == 2, "compact_pages: out is (table, refs)");
-  auto used = at::empty({1}, refs.options());
-  auto work = at::empty({rt_compact_workspace_bytes(p.pages)}, table.options().dtype(at::kByte));
-  check_cuda(rt_compact_pages(&p, table.data_ptr<int>(), ints(refs, pool, p.pages, "refs"),
-                              ints((*out)[0], pool, (int64_t)p.rows * p.width, "out table"),
-                              ints((*out)[1], pool, p.pages, "out refs"), used.data_ptr<int>(), work.data_ptr(),
+  const int* count = ints(refs, pool, {p.pages}, "refs");
+  const bool given = out.has_value();
+  if (!given)
+    out = std::vector<at::Tensor>{new_like(pool, {p.rows, p.width}, at::kInt), new_like(pool, {p.pages}, at::kInt)};
+  want<Value>(out->size() == 2, "out must be (table, refs) like the arguments");
+  int* new_table = ints((*out)[0], pool, {p.rows, p.width}, "out table");
+  int* new_refs = ints((*out)[1], pool, {p.pages}, "out refs");
+  if (given) {
+    check_apart(table, (*out)[0]);
+    check_apart(refs, (*out)[1]);
+  }
+  auto used = new_like(pool, {1}, at::kInt);
+  const auto work = workspace(rt_compact_workspace_bytes(p.pages));
+  check_cuda(rt_compact_pages(&p, table.data_ptr<int>(), count, new_table, new_refs, used.data_ptr<int>(), work.get(),
                               stream_of(pool)),
              "compact_pages");
   return {(*out)[0], (*out)[1], used};
@@ -891,69 +984,65 @@ std::vector<at::Tensor> compact_pages(at::Tensor pool, at::Tensor table, at::Ten
 
 void store_pages(at::Tensor pool, int64_t block, at::Tensor table, at::Tensor lengths, at::Tensor keys,
                  at::Tensor values) {
-  const RtPool p = pool_of(pool, table);
+  const RtPool p = pool_of(pool, table, block);
   c10::cuda::CUDAGuard guard(pool.device());
+  const int* length = ints(lengths, pool, {p.rows}, "lengths");
+  want<Value>(block >= 0 && keys.dim() == 4 && keys.size(0) >= 1 && p.rows % keys.size(0) == 0,
+              "expected keys [rows / beams, tokens, heads, dim], got ", keys.sizes());
+  const int64_t N = keys.size(0), T = keys.size(1);
+  want<Value>(T <= (1 << 30), "store_pages: too many tokens: ", T);
   long strides[2][3];
   for (int i = 0; i < 2; ++i) {
     at::Tensor& x = i ? values : keys;
-    TORCH_CHECK(x.device() == pool.device() && x.scalar_type() == at::kBFloat16 && x.dim() == 4 &&
-                    x.sizes() == keys.sizes() && x.size(0) >= 1 && p.rows % x.size(0) == 0 && x.size(2) == p.heads &&
-                    x.size(3) == p.dim && x.size(1) <= (1 << 30),
-                "store_pages: keys and values must be bf16 [rows / beams, tokens, heads, dim]");
-    if (x.stride(3) != 1) x = x.contiguous();
+    bf16_rows(x, pool, {N, T, p.heads, p.dim}, i ? "values" : "keys");
     for (int d = 0; d < 3; ++d) strides[i][d] = x.stride(d);
   }
-  check_cuda(rt_store_pages(&p, (int)block, table.data_ptr<int>(), ints(lengths, pool, p.rows, "lengths"),
-                            keys.data_ptr(), strides[0], values.data_ptr(), strides[1], (int)keys.size(1),
-                            p.rows / (int)keys.size(0), stream_of(pool)),
+  check_cuda(rt_store_pages(&p, (int)block, table.data_ptr<int>(), length, keys.data_ptr(), strides[0],
+                            values.data_ptr(), strides[1], (int)T, p.rows / (int)N, stream_of(pool)),
              "store_pages");
 }
 
 at::Tensor append_heads(at::Tensor x, at::Tensor pool, int64_t block, at::Tensor table, at::Tensor lengths,
                         at::Tensor q_weight, at::Tensor k_weight, at::Tensor inv_freq, int64_t heads, double eps) {
-  const RtPool p = pool_of(pool, table);
+  want<py::index_error>(block >= 0, "block ", block);
+  const RtPool p = pool_of(pool, table, block);
   c10::cuda::CUDAGuard guard(pool.device());
-  TORCH_CHECK(heads >= 1 && heads <= (1 << 16) && x.device() == pool.device() && x.scalar_type() == at::kBFloat16 &&
-                  x.dim() == 2 && x.size(0) == p.rows && x.size(1) == (2 * heads + 2 * p.heads) * p.dim,
-              "append_heads: x must be bf16 [rows, (2 heads + 2 kv heads) dim]");
-  for (const at::Tensor* w : {&q_weight, &k_weight, &inv_freq})
-    TORCH_CHECK(w->device() == pool.device() && w->scalar_type() == at::kFloat && w->is_contiguous() && w->dim() == 1,
-                "append_heads: weights and frequencies must be fp32 vectors");
-  TORCH_CHECK(q_weight.numel() == p.dim && k_weight.numel() == p.dim && 2 * inv_freq.numel() <= p.dim,
-              "append_heads: weights of one head and at most dim / 2 frequencies");
-  if (x.stride(1) != 1) x = x.contiguous();
-  auto q = at::empty({p.rows, heads, p.dim}, x.options());
-  check_cuda(rt_append_heads(&p, (int)block, table.data_ptr<int>(), ints(lengths, pool, p.rows, "lengths"), x.data_ptr(),
-                             x.stride(0), q_weight.data_ptr<float>(), k_weight.data_ptr<float>(),
-                             inv_freq.data_ptr<float>(), (int)inv_freq.numel(), (int)heads, (float)eps, q.data_ptr(),
-                             stream_of(pool)),
+  const int* length = ints(lengths, pool, {p.rows}, "lengths");
+  want<Value>(heads >= 1 && heads % p.heads == 0 && heads <= (1 << 16), heads, " query heads for ", p.heads, " key heads");
+  bf16_rows(x, pool, {p.rows, (2 * heads + 2 * p.heads) * p.dim}, "x");
+  want<Value>(q_weight.dim() == 1 && k_weight.dim() == 1 && inv_freq.dim() == 1 && q_weight.size(0) == p.dim &&
+                  k_weight.size(0) == p.dim && 2 * inv_freq.size(0) <= p.dim,
+              "expected weights of ", p.dim, " and at most ", p.dim / 2, " frequencies");
+  for (const at::Tensor* w : {&q_weight, &k_weight, &inv_freq}) {
+    want<Value>(w->device() == pool.device(), "weights and frequencies must be on ", pool.device());
+    want<Type>(w->scalar_type() == at::kFloat && w->is_contiguous(), "weights and frequencies must be contiguous fp32");
+  }
+  auto q = new_like(pool, {p.rows, heads, p.dim}, at::kBFloat16);
+  check_cuda(rt_append_heads(&p, (int)block, table.data_ptr<int>(), length, x.data_ptr(), x.stride(0),
+                             q_weight.data_ptr<float>(), k_weight.data_ptr<float>(), inv_freq.data_ptr<float>(),
+                             (int)inv_freq.numel(), (int)heads, (float)eps, q.data_ptr(), stream_of(pool)),
              "append_heads");
   return q;
 }
 
 at::Tensor paged_attention(at::Tensor q, at::Tensor pool, int64_t block, at::Tensor table, at::Tensor lengths,
                            c10::optional<at::Tensor> gate, int64_t group) {
-  const RtPool p = pool_of(pool, table);
+  want<py::index_error>(block >= 0, "block ", block);
+  const RtPool p = pool_of(pool, table, block);
   c10::cuda::CUDAGuard guard(pool.device());
-  TORCH_CHECK(q.device() == pool.device() && q.scalar_type() == at::kBFloat16 && q.dim() == 3 && q.size(0) == p.rows &&
-                  q.size(2) == p.dim && q.size(1) >= 1 && q.size(1) % p.heads == 0 && q.size(1) <= 64L * p.heads,
-              "paged_attention: q must be bf16 [rows, heads, dim], 1 to 64 heads per key head");
-  TORCH_CHECK(group >= 1 && group <= p.rows && p.rows % group == 0, "paged_attention: rows are no groups of ", group);
-  if (q.stride(2) != 1) q = q.contiguous();
-  at::Tensor g;
-  if (gate.has_value()) {
-    g = *gate;
-    TORCH_CHECK(g.device() == pool.device() && g.scalar_type() == at::kBFloat16 && g.sizes() == q.sizes(),
-                "paged_attention: gate must be like q");
-    if (g.stride(2) != 1) g = g.contiguous();
-  }
-  auto out = at::empty(q.sizes(), q.options());
+  const int* length = ints(lengths, pool, {p.rows}, "lengths");
+  want<Value>(q.dim() == 3 && q.size(1) >= 1 && q.size(1) % p.heads == 0 && q.size(1) <= 64L * p.heads,
+              "expected q [rows, heads, dim] with 1 to 64 query heads per key head, got ", q.sizes());
   const int heads = (int)q.size(1);
-  auto work = at::empty({rt_paged_attention_workspace_floats(&p, heads, (int)group)}, q.options().dtype(at::kFloat));
-  check_cuda(rt_paged_attention(&p, (int)block, table.data_ptr<int>(), ints(lengths, pool, p.rows, "lengths"),
-                                q.data_ptr(), q.stride(0), q.stride(1), heads, g.defined() ? g.data_ptr() : nullptr,
-                                g.defined() ? g.stride(0) : 0, g.defined() ? g.stride(1) : 0, (int)group, out.data_ptr(),
-                                work.data_ptr<float>(), stream_of(pool)),
+  bf16_rows(q, pool, {p.rows, heads, p.dim}, "q");
+  if (gate.has_value()) bf16_rows(*gate, pool, {p.rows, heads, p.dim}, "gate");
+  want<Value>(group >= 1 && group <= p.rows && p.rows % group == 0, p.rows, " rows are no groups of ", group);
+  auto out = new_like(pool, {p.rows, heads, p.dim}, at::kBFloat16);
+  const auto work = workspace(rt_paged_attention_workspace_floats(&p, heads, (int)group) * 4);
+  check_cuda(rt_paged_attention(&p, (int)block, table.data_ptr<int>(), length, q.data_ptr(), q.stride(0), q.stride(1),
+                                heads, gate.has_value() ? gate->data_ptr() : nullptr,
+                                gate.has_value() ? gate->stride(0) : 0, gate.has_value() ? gate->stride(1) : 0,
+                                (int)group, out.data_ptr(), static_cast<float*>(work.get()), stream_of(pool)),
              "paged_attention");
   return out;
 }

@@ -23,7 +23,7 @@ def beam_select(logits, scores, lengths, finished, end_token=-1, length_penalty=
     """(tokens int64, parents int64, scores fp32, lengths int32, finished bool), all [G, K]: one step of beam search
     for G groups of K beams.
 
-    ``logits`` [G, K, V] (bf16 or fp32 on CUDA) of the next token; ``scores`` [G, K] fp32, the sums of the beams'
+    ``logits`` [G, K, V] of the next token (on CUDA bf16 or fp32, at most 32 beams and 4161536 tokens); ``scores`` [G, K] fp32, the sums of the beams'
     log-probabilities; ``lengths`` [G, K] int32, their generated tokens; ``finished`` [G, K] bool. A running beam
     offers each token at score + log_softmax(logits), and is one token longer with it; a finished one offers itself
     alone, as one more ``end_token`` at its old score and length. A beam whose score is not finite, or whose logits
@@ -35,6 +35,8 @@ def beam_select(logits, scores, lengths, finished, end_token=-1, length_penalty=
     order of rank, so that what a surviving beam holds stays where it is. ``parents`` are slots of the same group;
     ``end_token`` -1: no token ends a beam. To start from one state per group, give its K beams the same logits and
     the scores 0, -inf, -inf, ..."""
+    if logits.is_cuda:
+        return tuple(native().beam_select(logits, scores, lengths, finished, end_token, length_penalty))
     if logits.dim() != 3 or logits.numel() == 0:
         raise ValueError(f"expected logits [groups, beams, vocabulary], got {tuple(logits.shape)}")
     G, K, V = logits.shape
@@ -52,12 +54,6 @@ def beam_select(logits, scores, lengths, finished, end_token=-1, length_penalty=
         raise ValueError(f"length_penalty must lie in -16..16, got {length_penalty}")
     if not logits.is_floating_point():
         raise TypeError("logits must be floating point")
-    if logits.is_cuda:
-        if logits.dtype not in (torch.bfloat16, torch.float32):
-            raise TypeError("beam_select takes bf16 or fp32 logits on CUDA")
-        if K > MAX_BEAMS:
-            raise ValueError(f"beam_select takes at most {MAX_BEAMS} beams on CUDA, got {K}")
-        return tuple(native().beam_select(logits, scores, lengths, finished, end_token, float(length_penalty)))
     return reference.beam_select(logits, scores, lengths, finished, end_token, length_penalty)
 
 
@@ -65,6 +61,8 @@ def reorder_states_(states, parents):
     """Rows of each tensor of ``states`` ([G * K, ...], contiguous, any type) replaced by their parents' rows, in
     place: slot k of group g takes what slot ``parents[g, k]`` held (int64 [G, K], any indices of the group; one
     outside it leaves its slot alone). Rows that stay are not touched. The tensors must not overlap."""
+    if parents.is_cuda:
+        return native().reorder_rows_(list(states), parents)
     states = list(states)
     rows, device = parents.numel(), parents.device
     check_parents(parents, rows, device)
@@ -83,14 +81,6 @@ def reorder_states_(states, parents):
     spans.sort()
     if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
         raise ValueError("states must not overlap")
-    if not spans or parents.shape[1] == 1:
-        return
-    if parents.is_cuda:
-        if parents.shape[1] > MAX_BEAMS:
-            raise ValueError(f"reorder_states_ takes at most {MAX_BEAMS} beams on CUDA, got {parents.shape[1]}")
-        native().reorder_rows_(states if len(spans) == len(states) else [state for state in states if state.numel()],
-                               parents.contiguous())
-        return
     source = reference.parent_rows(parents)
     with torch.no_grad():
         for state in states:

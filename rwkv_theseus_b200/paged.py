@@ -29,7 +29,7 @@ def _ints(name, part, shape, device):
 
 
 def _check(pool, table, lengths=None, refs=None, block=None):
-    """What all functions ask of a cache's tensors."""
+    """What all functions ask of a cache's tensors (the CUDA calls check theirs in the extension, which is faster)."""
     shape, held, device = pool.shape, table.shape, pool.device
     if len(shape) != 6 or shape[2] != 2 or 0 in shape:
         raise ValueError(f"expected a pool [pages, blocks, 2, heads, page, dim], got {tuple(shape)}")
@@ -58,8 +58,6 @@ def _check_rows(name, part, pool, table, shape):
         raise ValueError(f"{name} {tuple(part.shape)} does not match {tuple(shape)}")
     if part.device != pool.device:
         raise ValueError(f"{name} is on {part.device}, the pool on {pool.device}")
-    if pool.is_cuda and part.dtype != torch.bfloat16:
-        raise TypeError(f"the CUDA paged cache takes bf16 {name}")
 
 
 def _check_out(given, to):
@@ -91,25 +89,23 @@ def advance_pages(pool, table, lengths, refs, tokens=1, parents=None, live=None,
     status [1] int32 has bit 1 if the pool ran out (the entry is -1), 2 if a row would outgrow its table (it keeps its
     length), 4 if a parent lies outside its group (the row keeps its own history). ``out``: (table, lengths, refs,
     status) to write to, which may be the arguments themselves; its status keeps the bits that it has."""
+    if pool.is_cuda:
+        return tuple(native().advance_pages(pool, table, lengths, refs, tokens, parents, live, out))
     _check(pool, table, lengths, refs)
     rows = table.shape[0]
     if not 0 <= tokens <= 1 << 30:
         raise ValueError(f"tokens must lie in 0..2^30, got {tokens}")
     if parents is not None:
         check_parents(parents, rows, pool.device)
-        parents = parents.contiguous()
     if live is not None:
         if live.dtype != torch.bool or live.numel() != rows or live.device != pool.device:
             raise ValueError(f"live must be {rows} bools on {pool.device}")
-        live = live.contiguous()
     if out is not None:
         _check(pool, out[0], out[1], out[2])
         if out[0].shape != table.shape or out[3].shape != (1,) or out[3].dtype != torch.int32 or \
                 out[3].device != pool.device:
             raise ValueError("out must be (table, lengths, refs, status) like the arguments")
         _check_out((table, lengths, refs), out)
-    if pool.is_cuda:
-        return tuple(native().advance_pages(pool, table, lengths, refs, tokens, parents, live, out))
     result = reference.advance_pages(pool, table, lengths, refs, tokens, parents, live)
     if out is None:
         return result
@@ -123,14 +119,14 @@ def compact_pages(pool, table, refs, out=None):
     """(table, refs, used): the pages in use moved to the front of the pool, whose first ``used`` [1] pages they are
     then. The lowest page behind them goes to the lowest free page among them, and so on; pages that lie there
     already stay. ``out``: (table, refs) to write to, which may be the arguments themselves."""
+    if pool.is_cuda:
+        return tuple(native().compact_pages(pool, table, refs, out))
     _check(pool, table, refs=refs)
     if out is not None:
         _check(pool, out[0], refs=out[1])
         if out[0].shape != table.shape:
             raise ValueError("out must be (table, refs) like the arguments")
         _check_out((table, refs), out)
-    if pool.is_cuda:
-        return tuple(native().compact_pages(pool, table, refs, out))
     result = reference.compact_pages(pool, table, refs)
     if out is None:
         return result
@@ -142,16 +138,15 @@ def compact_pages(pool, table, refs, out=None):
 def store_pages(pool, block, table, lengths, keys, values):
     """Writes ``keys``, ``values`` [N, T, heads, dim] as the last T tokens of rows 0, R / N, 2 R / N, ... (the first of
     each group of beams); tokens before a row's first are dropped. For prompts, whose keys are rotated already."""
+    if pool.is_cuda:
+        return native().store_pages(pool, block, table, lengths, keys, values)
     _check(pool, table, lengths, block=block)
     if keys.dim() != 4 or keys.shape[0] < 1 or table.shape[0] % keys.shape[0]:
         raise ValueError(f"expected keys [rows / beams, tokens, heads, dim], got {tuple(keys.shape)}")
     shape = keys.shape[:2] + (pool.shape[3], pool.shape[5])
     _check_rows("keys", keys, pool, table, shape)
     _check_rows("values", values, pool, table, shape)
-    if pool.is_cuda:
-        native().store_pages(pool, block, table, lengths, keys, values)
-    else:
-        reference.store_pages(pool, block, table, lengths, keys, values)
+    reference.store_pages(pool, block, table, lengths, keys, values)
 
 
 def append_heads(x, pool, block, table, lengths, q_weight, k_weight, inv_freq, heads, eps):
@@ -161,6 +156,9 @@ def append_heads(x, pool, block, table, lengths, q_weight, k_weight, inv_freq, h
     keys, then the values. Queries and keys are normalised per head (times 1 + weight) and their first
     2 * len(inv_freq) components rotated to position lengths - 1, whose angle is formed in 64 bits. A row of length 0
     stores nothing."""
+    if pool.is_cuda:
+        return native().append_heads(x, pool, block, table, lengths, f32(q_weight), f32(k_weight), f32(inv_freq), heads,
+                                     eps)
     _check(pool, table, lengths, block=block)
     D = pool.shape[5]
     if heads < 1 or heads % pool.shape[3]:
@@ -170,9 +168,6 @@ def append_heads(x, pool, block, table, lengths, q_weight, k_weight, inv_freq, h
         raise ValueError(f"expected weights of {D} and at most {D // 2} frequencies")
     if any(part.device != pool.device for part in (q_weight, k_weight, inv_freq)):
         raise ValueError(f"weights and frequencies must be on {pool.device}")
-    if pool.is_cuda:
-        return native().append_heads(x, pool, block, table, lengths, f32(q_weight), f32(k_weight), f32(inv_freq),
-                                     heads, float(eps))
     return reference.append_heads(x, pool, block, table, lengths, q_weight, k_weight, inv_freq, heads, eps)
 
 
@@ -181,6 +176,8 @@ def paged_attention(q, pool, block, table, lengths, gate=None, group=1):
     dim^-0.5; query head h reads key head h // (Hq / heads). ``gate`` [R, Hq, dim]: the result is multiplied by its
     sigmoid. A row without tokens has zeros. ``group``: that many consecutive rows are beams of one prompt; a page
     that several of them hold is read once (a matter of speed, and of the order in which sums are formed)."""
+    if pool.is_cuda:
+        return native().paged_attention(q, pool, block, table, lengths, gate, group)
     _check(pool, table, lengths, block=block)
     R, H, D = table.shape[0], pool.shape[3], pool.shape[5]
     if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % H or q.shape[1] > 64 * H:
@@ -190,8 +187,6 @@ def paged_attention(q, pool, block, table, lengths, gate=None, group=1):
         _check_rows("gate", gate, pool, table, q.shape)
     if group < 1 or R % group:
         raise ValueError(f"{R} rows are no groups of {group}")
-    if pool.is_cuda:
-        return native().paged_attention(q, pool, block, table, lengths, gate, group)
     return reference.paged_attention(q, pool, block, table, lengths, gate)
 
 
