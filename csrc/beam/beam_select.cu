@@ -24,7 +24,6 @@ constexpr int LIST = 512;            // candidates of a segment
 constexpr int HELD = 8192;           // values of a block in registers
 constexpr int SEGMENT = HELD - 64;   // of a segment at most (its ends need not be aligned)
 constexpr int MAX_SEGMENTS = 512;
-constexpr int MERGE_THREADS = 1024, MERGE_WARPS = MERGE_THREADS / 32;
 constexpr int MERGE_LIST = 1024;     // candidates of a group
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -260,7 +259,9 @@ __global__ void __launch_bounds__(THREADS, 5) select_rows_kernel(const SelectArg
 // Block per group: the K best of its lists (one per beam and segment, sorted, K entries each). Their
 // heads give a bound that K candidates reach; the candidates that do are few, and each counts those before it. Where
 // equal heads make them too many, the best head is drawn K times instead.
+template <int MERGE_THREADS>
 __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const SelectArgs a) {
+  constexpr int MERGE_WARPS = MERGE_THREADS / 32;
   extern __shared__ unsigned char taken[];  // of each list
   __shared__ double base[32], norm[32];     // value = base + (z - top); rank = value / norm
   __shared__ float row_top[32];
@@ -443,14 +444,14 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
   __syncthreads();
   const int have = found;
   if (have <= MERGE_LIST) {
-    if (tid < have) {
-      const unsigned long long r = list_rank[tid];
-      const long f = list_flat[tid];
+    for (int i = tid; i < have; i += MERGE_THREADS) {
+      const unsigned long long r = list_rank[i];
+      const long f = list_flat[i];
       int place = 0;
       for (int j = 0; j < have; ++j) place += list_rank[j] > r || (list_rank[j] == r && list_flat[j] < f);
       if (place < K) {
         chosen[place] = f;
-        values[place] = list_value[tid];
+        values[place] = list_value[i];
       }
     }
   } else {
@@ -585,6 +586,8 @@ extern "C" cudaError_t rt_beam_select(int dtype, const void* logits, long groups
   if (dtype == 1) select_rows_kernel<__nv_bfloat16><<<blocks, THREADS, 0, s>>>(a);
   else select_rows_kernel<float><<<blocks, THREADS, 0, s>>>(a);
   RT_CUDA_CHECK(cudaGetLastError());
-  select_group_kernel<<<(unsigned)groups, MERGE_THREADS, K * a.segments, s>>>(a);
+  // (a warp per beam and a thread per list are enough: the barriers of a smaller block are cheaper)
+  if (K <= 8 && K * a.segments <= 256) select_group_kernel<256><<<(unsigned)groups, 256, K * a.segments, s>>>(a);
+  else select_group_kernel<1024><<<(unsigned)groups, 1024, K * a.segments, s>>>(a);
   return cudaGetLastError();
 }

@@ -12,9 +12,10 @@
 namespace {
 
 using bf16 = __nv_bfloat16;
-constexpr int THREADS = 1024, WARPS = THREADS / 32, MAX_ROWS = 1024, SMALL_POOL = 5120;
+constexpr int MAX_ROWS = 1024, SMALL_POOL = 5120;
 
 // Exclusive prefix sum over the block and its total. Two barriers.
+template <int WARPS>
 __device__ __forceinline__ int block_prefix(int v, int* warp_sums, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int x = v;
@@ -52,14 +53,15 @@ struct AdvanceArgs {
 };
 
 // SMALL: the counts fit shared memory, which takes three waits for memory out of the chain that this kernel is bound by.
-template <bool SMALL>
+template <bool SMALL, int THREADS>
 __global__ void __launch_bounds__(THREADS) advance_kernel(const AdvanceArgs a) {
-  __shared__ int source[MAX_ROWS];  // row whose history a row takes over, -1: none (not live)
-  __shared__ int before[MAX_ROWS];  // its last slot (of the partly filled page), -1: none
-  __shared__ int last[MAX_ROWS];    // partly filled page that a row appends to, -1: none
-  __shared__ int wants[MAX_ROWS];   // exclusive prefix of the pages that rows take
-  __shared__ int slot[MAX_ROWS];    // where a row's first taken page goes
-  __shared__ int target[MAX_ROWS];  // that page, -1: none found
+  constexpr int WARPS = THREADS / 32, ROWS = THREADS;
+  __shared__ int source[ROWS];  // row whose history a row takes over, -1: none (not live)
+  __shared__ int before[ROWS];  // its last slot (of the partly filled page), -1: none
+  __shared__ int last[ROWS];    // partly filled page that a row appends to, -1: none
+  __shared__ int wants[ROWS];   // exclusive prefix of the pages that rows take
+  __shared__ int slot[ROWS];    // where a row's first taken page goes
+  __shared__ int target[ROWS];  // that page, -1: none found
   __shared__ int counts[SMALL ? SMALL_POOL : 1];
   __shared__ int warp_sums[WARPS];
   __shared__ int bits;
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(THREADS) advance_kernel(const AdvanceArgs a) {
   }
   const int takes = grows ? (int)copy + (int)need - have : 0;
   int total = 0;
-  const int prefix = block_prefix(takes, warp_sums, total);
+  const int prefix = block_prefix<WARPS>(takes, warp_sums, total);
   if (tid < R) {
     wants[tid] = prefix;
     slot[tid] = have - (int)copy;
@@ -154,7 +156,7 @@ __global__ void __launch_bounds__(THREADS) advance_kernel(const AdvanceArgs a) {
     const int p = p0 + tid;
     const bool free = p < a.pages && count_of(p) <= 0;
     int here;
-    const int n = found + block_prefix(free, warp_sums, here);
+    const int n = found + block_prefix<WARPS>(free, warp_sums, here);
     if (free && n < total) {
       int lo = 0, hi = R - 1;  // the last row whose prefix is at most n: of equal ones only the last takes pages
       while (lo < hi) {
@@ -221,18 +223,19 @@ struct CompactArgs {
   int* count;
 };
 
-__global__ void __launch_bounds__(THREADS) compact_kernel(const CompactArgs a) {
+__global__ void __launch_bounds__(1024) compact_kernel(const CompactArgs a) {
+  constexpr int THREADS = 1024, WARPS = THREADS / 32;
   __shared__ int warp_sums[WARPS];
   const int tid = threadIdx.x;
   int mine = 0, used;
   for (int p = tid; p < a.pages; p += THREADS) mine += a.refs[p] > 0;
-  block_prefix(mine, warp_sums, used);
+  block_prefix<WARPS>(mine, warp_sums, used);
   int holes = 0, moves = 0;
   for (int p0 = 0; p0 < used; p0 += THREADS) {
     const int p = p0 + tid;
     const bool hole = p < used && a.refs[p] <= 0;
     int here;
-    const int n = holes + block_prefix(hole, warp_sums, here);
+    const int n = holes + block_prefix<WARPS>(hole, warp_sums, here);
     if (hole) a.holes[n] = p;
     if (p < used) a.place[p] = p;
     holes += here;
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(THREADS) compact_kernel(const CompactArgs a) {
     const int p = p0 + tid;
     const int count = p < a.pages ? a.refs[p] : 0;
     int here;
-    const int n = moves + block_prefix(count > 0, warp_sums, here);
+    const int n = moves + block_prefix<WARPS>(count > 0, warp_sums, here);
     if (count > 0) {
       const int to = a.holes[n];
       a.place[p] = to;
@@ -432,8 +435,10 @@ extern "C" cudaError_t rt_advance_pages(const RtPool* p, const int* table, const
   if (!pool_fits(p) || tokens < 0 || K < 1 || p->rows % K) return cudaErrorInvalidValue;
   AdvanceArgs a{table, lengths, refs, new_table, new_lengths, new_refs, status, keep_status, parents, live,
                 p->rows, K, p->width, p->pages, p->page, tokens, static_cast<int4*>(work)};
-  if (p->pages <= SMALL_POOL) advance_kernel<true><<<1, THREADS, 0, s>>>(a);
-  else advance_kernel<false><<<1, THREADS, 0, s>>>(a);
+  // (few rows: the barriers of a smaller block are cheaper)
+  if (p->rows <= 256 && p->pages <= SMALL_POOL) advance_kernel<true, 256><<<1, 256, 0, s>>>(a);
+  else if (p->pages <= SMALL_POOL) advance_kernel<true, 1024><<<1, 1024, 0, s>>>(a);
+  else advance_kernel<false, 1024><<<1, 1024, 0, s>>>(a);
   RT_CUDA_CHECK(cudaGetLastError());
   if (tokens == 0) return cudaSuccess;
   const int panels = p->blocks * 2 * p->heads;
@@ -459,7 +464,7 @@ extern "C" cudaError_t rt_compact_pages(const RtPool* p, const int* table, const
   a.place = reinterpret_cast<int*>(a.moves + p->pages);
   a.holes = a.place + p->pages;
   a.count = a.holes + p->pages;
-  compact_kernel<<<1, THREADS, 0, s>>>(a);
+  compact_kernel<<<1, 1024, 0, s>>>(a);
   RT_CUDA_CHECK(cudaGetLastError());
   const long vectors = (long)p->blocks * 2 * p->heads * p->page * p->dim / 8;
   const int parts = (int)std::min((vectors + 2047) / 2048, 4096L);  // 32 KB: eight vectors per thread
