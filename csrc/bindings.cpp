@@ -861,9 +861,12 @@ void reorder_rows_(std::vector<at::Tensor> states, at::Tensor parents) {
     const auto start = reinterpret_cast<uintptr_t>(base.back());
     spans.emplace_back(start, start + size);
   }
+  if (parents.is_contiguous())  // (a copy otherwise)
+    spans.emplace_back(reinterpret_cast<uintptr_t>(parents.data_ptr()),
+                       reinterpret_cast<uintptr_t>(parents.data_ptr()) + parents.nbytes());
   std::sort(spans.begin(), spans.end());
   for (size_t i = 1; i < spans.size(); ++i)
-    want<Value>(spans[i - 1].second <= spans[i].first, "states must not overlap");
+    want<Value>(spans[i - 1].second <= spans[i].first, "states and parents must not overlap");
   if (base.empty() || parents.size(1) == 1) return;
   want<Value>(parents.size(1) <= 32, "reorder_states_ takes at most 32 beams on CUDA, got ", parents.size(1));
   if (!parents.is_contiguous()) parents = parents.contiguous();
@@ -909,11 +912,18 @@ void bf16_rows(at::Tensor& t, const at::Tensor& pool, at::IntArrayRef shape, con
   if (t.stride(-1) != 1) t = t.contiguous();
 }
 
-// What is written may be what is read, or lie apart from it.
-void check_apart(const at::Tensor& in, const at::Tensor& out) {
-  const auto a = reinterpret_cast<uintptr_t>(in.data_ptr()), b = reinterpret_cast<uintptr_t>(out.data_ptr());
-  want<Value>(a == b || a >= b + out.nbytes() || b >= a + in.nbytes(),
-              "out must be the arguments themselves or apart from them");
+// What is written may be the argument of its place, or lie apart from all of them and from the rest that is written.
+void check_apart(const std::vector<at::Tensor>& in, const std::vector<at::Tensor>& out) {
+  auto apart = [](const at::Tensor& x, const at::Tensor& y) {
+    const auto a = reinterpret_cast<uintptr_t>(x.data_ptr()), b = reinterpret_cast<uintptr_t>(y.data_ptr());
+    return a >= b + y.nbytes() || b >= a + x.nbytes();
+  };
+  for (size_t i = 0; i < out.size(); ++i) {
+    bool ok = true;
+    for (size_t j = 0; j < in.size(); ++j) ok &= (i == j && in[j].data_ptr() == out[i].data_ptr()) || apart(in[j], out[i]);
+    for (size_t j = 0; j < i; ++j) ok &= apart(out[j], out[i]);
+    want<Value>(ok, "out must be the arguments themselves or apart from them");
+  }
 }
 
 std::vector<at::Tensor> advance_pages(at::Tensor pool, at::Tensor table, at::Tensor lengths, at::Tensor refs,
@@ -945,11 +955,7 @@ std::vector<at::Tensor> advance_pages(at::Tensor pool, at::Tensor table, at::Ten
   int* new_lengths = ints(l, pool, {p.rows}, "out lengths");
   int* new_refs = ints(r, pool, {p.pages}, "out refs");
   int* status = ints(st, pool, {1}, "out status");
-  if (given) {
-    check_apart(table, t);
-    check_apart(lengths, l);
-    check_apart(refs, r);
-  }
+  if (given) check_apart({table, lengths, refs}, *out);
   const auto work = workspace(rt_advance_workspace_bytes(p.rows));
   check_cuda(rt_advance_pages(&p, table.data_ptr<int>(), length, count, (int)tokens,
                               parents.has_value() ? reinterpret_cast<const long*>(parents->data_ptr<int64_t>()) : nullptr,
@@ -970,10 +976,7 @@ std::vector<at::Tensor> compact_pages(at::Tensor pool, at::Tensor table, at::Ten
   want<Value>(out->size() == 2, "out must be (table, refs) like the arguments");
   int* new_table = ints((*out)[0], pool, {p.rows, p.width}, "out table");
   int* new_refs = ints((*out)[1], pool, {p.pages}, "out refs");
-  if (given) {
-    check_apart(table, (*out)[0]);
-    check_apart(refs, (*out)[1]);
-  }
+  if (given) check_apart({table, refs}, *out);
   auto used = new_like(pool, {1}, at::kInt);
   const auto work = workspace(rt_compact_workspace_bytes(p.pages));
   check_cuda(rt_compact_pages(&p, table.data_ptr<int>(), count, new_table, new_refs, used.data_ptr<int>(), work.get(),

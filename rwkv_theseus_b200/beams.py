@@ -60,13 +60,14 @@ def beam_select(logits, scores, lengths, finished, end_token=-1, length_penalty=
 def reorder_states_(states, parents):
     """Rows of each tensor of ``states`` ([G * K, ...], contiguous, any type) replaced by their parents' rows, in
     place: slot k of group g takes what slot ``parents[g, k]`` held (int64 [G, K], any indices of the group; one
-    outside it leaves its slot alone). Rows that stay are not touched. The tensors must not overlap."""
+    outside it leaves its slot alone). Rows that stay are not touched. The tensors must not overlap; on CUDA a group has
+    at most 32 beams."""
     if parents.is_cuda:
         return native().reorder_rows_(list(states), parents)
     states = list(states)
     rows, device = parents.numel(), parents.device
     check_parents(parents, rows, device)
-    spans = []
+    spans = [(parents.data_ptr(), parents.data_ptr() + parents.nbytes)] if parents.is_contiguous() else []
     for state in states:
         if state.dim() < 1 or state.shape[0] != rows:
             raise ValueError(f"expected states of {rows} rows, got {tuple(state.shape)}")
@@ -80,7 +81,7 @@ def reorder_states_(states, parents):
             spans.append((start, start + size))
     spans.sort()
     if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
-        raise ValueError("states must not overlap")
+        raise ValueError("states and parents must not overlap")
     source = reference.parent_rows(parents)
     with torch.no_grad():
         for state in states:
@@ -209,8 +210,8 @@ def beam_search(runner, prompt, new_tokens, beams=4, end_token=-1, length_penalt
 
     A continuation ends with ``end_token`` (its ids are followed by more of them, and its length counts the first) or
     after ``new_tokens``. Scores are sums of log-probabilities; the order is that of score / length^length_penalty
-    (see ``beam_select``). ``page``: tokens in a page of the key/value cache (full-attention blocks that were not
-    replaced). ``on_token(step)`` is called after each decode step. ``graph=True`` replays the steps as a CUDA graph
+    (see ``beam_select``). ``page``: tokens in a page of the key/value cache (of full-attention blocks that were
+    not replaced, whose heads have 64, 128 or 256 components on CUDA). ``on_token(step)`` is called after each decode step. ``graph=True`` replays the steps as a CUDA graph
     after the first. The runner's own cache and states are left as they are."""
     if prompt.dim() != 2 or prompt.numel() == 0:
         raise ValueError(f"expected prompts [groups, tokens], got {tuple(prompt.shape)}")

@@ -61,10 +61,14 @@ def _check_rows(name, part, pool, table, shape):
 
 
 def _check_out(given, to):
-    """What is written may be what is read, or lie apart from it."""
-    for part, out in zip(given, to):
-        start, other = part.data_ptr(), out.data_ptr()
-        if start != other and start < other + out.nbytes and other < start + part.nbytes:
+    """What is written may be the argument of its place, or lie apart from all of them and from the rest."""
+    def apart(x, y):
+        a, b = x.data_ptr(), y.data_ptr()
+        return a >= b + y.nbytes or b >= a + x.nbytes
+
+    for i, out in enumerate(to):
+        if not all(apart(part, out) or i == j and part.data_ptr() == out.data_ptr() for j, part in enumerate(given)) or \
+                not all(apart(other, out) for other in to[:i]):
             raise ValueError("out must be the arguments themselves or apart from them")
 
 
@@ -118,7 +122,7 @@ def advance_pages(pool, table, lengths, refs, tokens=1, parents=None, live=None,
 def compact_pages(pool, table, refs, out=None):
     """(table, refs, used): the pages in use moved to the front of the pool, whose first ``used`` [1] pages they are
     then. The lowest page behind them goes to the lowest free page among them, and so on; pages that lie there
-    already stay. ``out``: (table, refs) to write to, which may be the arguments themselves."""
+    already stay. Pages that are held outside the table too move like the others. ``out``: (table, refs) to write to, which may be the arguments themselves."""
     if pool.is_cuda:
         return tuple(native().compact_pages(pool, table, refs, out))
     _check(pool, table, refs=refs)

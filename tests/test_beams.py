@@ -146,6 +146,8 @@ def test_states_refuse():
         reorder_states_([torch.randn(4, 6).t()], parents)
     with pytest.raises(ValueError, match="overlap"):
         reorder_states_([state, state], parents)
+    with pytest.raises(ValueError, match="overlap"):
+        reorder_states_([parents.view(-1)], parents)
     with pytest.raises(TypeError, match="int64"):
         reorder_states_([state], parents.int())
     with pytest.raises(ValueError, match="expected parents"):
@@ -316,6 +318,13 @@ def test_pages_refuse():
         advance_pages(pool, table, lengths, refs, parents=torch.zeros(1, 3, dtype=torch.int64))
     with pytest.raises(ValueError, match="live must be"):
         advance_pages(pool, table, lengths, refs, live=torch.ones(4))
+    status = torch.zeros(1, dtype=torch.int32)
+    both = torch.zeros(table.numel() + 1, dtype=torch.int32)
+    for out in ((both[1:].view(table.shape), lengths, refs, status), (table, lengths, refs, refs[:1])):
+        with pytest.raises(ValueError, match="apart"):
+            advance_pages(pool, both[:-1].view(table.shape), lengths, refs, out=out)
+    with pytest.raises(ValueError, match="apart"):
+        compact_pages(pool, both[:-1].view(table.shape), refs, out=(both[1:].view(table.shape), refs))
     q = torch.randn(4, 2, 4, dtype=torch.float64)
     with pytest.raises(IndexError, match="block 2"):
         paged_attention(q, pool, 2, table, lengths)

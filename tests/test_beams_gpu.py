@@ -95,6 +95,17 @@ def test_selection_refuses_on_cuda():
         beam_select(logits[:, :2].half(), scores[:, :2], lengths[:, :2], finished[:, :2])
     with pytest.raises(ValueError, match="different devices"):
         beam_select(logits[:, :2], scores[:, :2].cpu(), lengths[:, :2], finished[:, :2])
+    logits, scores, lengths, finished = _step(2, 3, 40, torch.float32)
+    for error, match, args, more in (
+            (ValueError, "expected logits", (logits[0], scores, lengths, finished), {}),
+            (ValueError, "expected logits", (logits[..., :0], scores, lengths, finished), {}),
+            (ValueError, "does not match", (logits, scores[:, :2], lengths, finished), {}),
+            (TypeError, "lengths must be", (logits, scores, lengths.long(), finished), {}),
+            (TypeError, "scores must be", (logits, scores.double(), lengths, finished), {}),
+            (ValueError, "end_token", (logits, scores, lengths, finished), dict(end_token=40)),
+            (ValueError, "length_penalty", (logits, scores, lengths, finished), dict(length_penalty=math.nan))):
+        with pytest.raises(error, match=match):
+            beam_select(*args, **more)
 
 
 # ---------------------------------------------------------------- states
@@ -129,6 +140,14 @@ def test_states_refuse_on_cuda():
         reorder_states_([torch.zeros(33, 2, device="cuda")], parents)
     with pytest.raises(ValueError, match="different devices"):
         reorder_states_([torch.zeros(33, 2)], parents)
+    two, state = parents[:, :2].contiguous(), torch.zeros(2, 4, device="cuda")
+    for error, match, states, by in ((ValueError, "2 rows", [state[:1]], two), (TypeError, "int64", [state], two.int()),
+                                     (ValueError, "contiguous", [torch.zeros(4, 2, device="cuda").t()], two),
+                                     (ValueError, "overlap", [state, state[1:].expand(2, 4).contiguous(), state], two),
+                                     (ValueError, "overlap", [two.view(-1)], two),
+                                     (ValueError, "expected parents", [state], two.view(-1))):
+        with pytest.raises(error, match=match):
+            reorder_states_(states, by)
 
 
 # ---------------------------------------------------------------- pages
@@ -386,6 +405,36 @@ def test_pages_refuse_on_cuda():
         cache.attend(0, q[:, :1].cpu())
     with pytest.raises(ValueError, match="lengths is on"):
         paged_attention(q[:, :1], cache.pool, 0, cache.table, cache.lengths.cpu())
+    pool, table, lengths, refs = cache.pool, cache.table, cache.lengths, cache.refs
+    status, both = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(9, dtype=torch.int32, device="cuda")
+    for out in ((both[1:].view(table.shape), lengths, refs, status), (table, lengths, refs, refs[:1])):
+        with pytest.raises(ValueError, match="apart"):
+            advance_pages(pool, both[:-1].view(table.shape), lengths, refs, out=out)
+    with pytest.raises(ValueError, match="apart"):
+        compact_pages(pool, both[:-1].view(table.shape), refs, out=(both[1:].view(table.shape), refs))
+    for error, match, call in (
+            (ValueError, "expected a pool", lambda: advance_pages(pool[0], table, lengths, refs)),
+            (ValueError, "contiguous", lambda: advance_pages(pool[..., ::2], table, lengths, refs)),
+            (TypeError, "table must be", lambda: advance_pages(pool, table.long(), lengths, refs)),
+            (ValueError, "lengths", lambda: advance_pages(pool, table, lengths[:1], refs)),
+            (ValueError, "refs", lambda: compact_pages(pool, table, refs[:3])),
+            (ValueError, "tokens must", lambda: advance_pages(pool, table, lengths, refs, tokens=-1)),
+            (ValueError, "expected parents", lambda: advance_pages(pool, table, lengths, refs, parents=refs.long()[None])),
+            (TypeError, "int64", lambda: advance_pages(pool, table, lengths, refs, parents=lengths[None])),
+            (ValueError, "live must be", lambda: advance_pages(pool, table, lengths, refs, live=lengths)),
+            (IndexError, "block 1", lambda: paged_attention(q[:, :1], pool, 1, table, lengths)),
+            (IndexError, "block -1", lambda: paged_attention(q[:, :1], pool, -1, table, lengths)),
+            (ValueError, "gate", lambda: paged_attention(q[:, :2], pool, 0, table, lengths, gate=q[:, :1])),
+            (ValueError, "groups of 3", lambda: paged_attention(q[:, :1], pool, 0, table, lengths, group=3)),
+            (ValueError, "query heads", lambda: append_heads(q[:, 0], pool, 0, table, lengths, q[0, 0], q[0, 0], q[0, 0], 0, 1.)),
+            (ValueError, "x .*does not match", lambda: append_heads(q[:, 0], pool, 0, table, lengths, q[0, 0], q[0, 0],
+                                                                   q[0, 0], 2, 1.)),
+            (ValueError, "frequencies", lambda: append_heads(q[:, :4].reshape(2, 256), pool, 0, table, lengths, q[0, 0],
+                                                            q[0, 0], q[0, 0], 1, 1.)),
+            (ValueError, "expected keys", lambda: store_pages(pool, 0, table, lengths, q[:, 0], q[:, 0])),
+            (ValueError, "values", lambda: store_pages(pool, 0, table, lengths, q[:, :1, None], q[:, :2, None]))):
+        with pytest.raises(error, match=match):
+            call()
 
 
 # ---------------------------------------------------------------- together
