@@ -49,7 +49,8 @@ struct AdvanceArgs {
   const long* parents;  // [rows / K, K] or null
   const bool* live;     // [rows] or null
   int rows, K, width, pages, page, tokens;
-  int4* copies;         // [rows]: (from, to, tokens, -); from = -1: none
+  int4* copies;         // [rows]: (from, to, tokens, -)
+  int* count;           // of them
 };
 
 // SMALL: the counts fit shared memory, which takes three waits for memory out of the chain that this kernel is bound by.
@@ -172,10 +173,12 @@ __global__ void __launch_bounds__(THREADS) advance_kernel(const AdvanceArgs a) {
     found += here;
   }
   __syncthreads();
-  if (tid < R) {
-    a.copies[tid] = make_int4(copy && target[tid] >= 0 ? mine : -1, target[tid], fill, 0);
-    a.new_lengths[tid] = length + (grows ? a.tokens : 0);
-  }
+  if (tid < R) a.new_lengths[tid] = length + (grows ? a.tokens : 0);
+  const bool copies = copy && target[tid] >= 0;
+  int listed;
+  const int at_copy = block_prefix<WARPS>(copies, warp_sums, listed);
+  if (copies) a.copies[at_copy] = make_int4(mine, target[tid], fill, 0);
+  if (tid == 0) *a.count = listed;
   if (SMALL)
     for (int p = tid; p < a.pages; p += THREADS) a.new_refs[p] = counts[p];
   if (tid == 0) {
@@ -198,15 +201,43 @@ __device__ __forceinline__ void copy_vectors(uint4* to, const uint4* from, long 
   for (; i < n; i += step) to[i] = from[i];
 }
 
-// The first `tokens` tokens of a page in every block and head, for each row's copy. Grid (parts, rows).
-__global__ void __launch_bounds__(256) copy_tokens_kernel(bf16* pool, const int4* copies, int panels, int page, int dim) {
-  const int4 c = copies[blockIdx.y];
-  if (c.x < 0) return;
-  const long size = (long)page * dim / 8;  // vectors of a panel: one block's keys or values of one head
-  const uint4* from = reinterpret_cast<const uint4*>(pool) + (long)c.x * panels * size;
-  uint4* to = reinterpret_cast<uint4*>(pool) + (long)c.y * panels * size;
-  for (int h = blockIdx.x; h < panels; h += gridDim.x)
-    copy_vectors<8>(to + h * size, from + h * size, c.z * dim / 8, threadIdx.x, blockDim.x);
+// The first tokens of a page in every block and head, for each listed copy. Blocks walk (copy, panel, half) and load the
+// next one's vectors before they store this one's.
+__global__ void __launch_bounds__(256) copy_tokens_kernel(bf16* pool, const int4* copies, const int* count, int panels,
+                                                          int page, int dim) {
+  constexpr int U = 4;  // 64 tokens of 256 components are 2 x 4 vectors per thread
+  const int size = page * dim / 8;  // vectors of a panel: one block's keys or values of one head
+  const int items = *count * panels * 2;
+  uint4* base = reinterpret_cast<uint4*>(pool);
+  uint4 v[U];
+  auto load = [&](int item, uint4*& to) {
+    int n = 0;
+    if (item < items) {
+      const int half = item & 1, pair = item >> 1, which = pair / panels, panel = pair - which * panels;
+      const int4 c = copies[which];
+      const int all = c.z * dim / 8, first = half ? (all + 1) / 2 : 0;
+      n = half ? all - first : (all + 1) / 2;
+      const uint4* from = base + ((long)c.x * panels + panel) * size + first;
+      to = base + ((long)c.y * panels + panel) * size + first;
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (k * 256 + (int)threadIdx.x < n) v[k] = from[k * 256 + threadIdx.x];
+    }
+    return n;
+  };
+  uint4* to = nullptr;
+  int n = load(blockIdx.x, to);
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    uint4 now[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) now[k] = v[k];
+    uint4* here = to;
+    const int m = n;
+    n = load(item + gridDim.x, to);
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (k * 256 + (int)threadIdx.x < m) here[k * 256 + threadIdx.x] = now[k];
+  }
 }
 
 struct CompactArgs {
@@ -425,7 +456,7 @@ Place place(const RtPool* p, const int* table, const int* lengths) {
 
 }  // namespace
 
-extern "C" long rt_advance_workspace_bytes(int rows) { return rows * (long)sizeof(int4); }
+extern "C" long rt_advance_workspace_bytes(int rows) { return (rows + 1) * (long)sizeof(int4); }
 
 // parents [rows / K, K] or null; live [rows] or null; the outputs may be the inputs. work: 16-byte aligned.
 extern "C" cudaError_t rt_advance_pages(const RtPool* p, const int* table, const int* lengths, const int* refs,
@@ -434,7 +465,7 @@ extern "C" cudaError_t rt_advance_pages(const RtPool* p, const int* table, const
                                         cudaStream_t s) {
   if (!pool_fits(p) || tokens < 0 || K < 1 || p->rows % K) return cudaErrorInvalidValue;
   AdvanceArgs a{table, lengths, refs, new_table, new_lengths, new_refs, status, keep_status, parents, live,
-                p->rows, K, p->width, p->pages, p->page, tokens, static_cast<int4*>(work)};
+                p->rows, K, p->width, p->pages, p->page, tokens, static_cast<int4*>(work) + 1, static_cast<int*>(work)};
   // (few rows: the barriers of a smaller block are cheaper)
   if (p->rows <= 256 && p->pages <= SMALL_POOL) advance_kernel<true, 256><<<1, 256, 0, s>>>(a);
   else if (p->pages <= SMALL_POOL) advance_kernel<true, 1024><<<1, 1024, 0, s>>>(a);
@@ -442,8 +473,10 @@ extern "C" cudaError_t rt_advance_pages(const RtPool* p, const int* table, const
   RT_CUDA_CHECK(cudaGetLastError());
   if (tokens == 0) return cudaSuccess;
   const int panels = p->blocks * 2 * p->heads;
-  copy_tokens_kernel<<<dim3((unsigned)std::min(panels, 1024), (unsigned)p->rows), 256, 0, s>>>(
-      static_cast<bf16*>(p->pool), a.copies, panels, p->page, p->dim);
+  const long items = (long)panels * 2 * p->rows;  // at most, and the blocks' next ones stay in range
+  if (items > INT_MAX - 65536) return cudaErrorInvalidValue;
+  copy_tokens_kernel<<<(unsigned)std::min(items, 148L * 6), 256, 0, s>>>(static_cast<bf16*>(p->pool), a.copies, a.count,
+                                                                       panels, p->page, p->dim);
   return cudaGetLastError();
 }
 
