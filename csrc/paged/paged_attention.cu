@@ -12,8 +12,11 @@
 //   warps 0, 1, 4, 5   softmax, two threads per query (32 keys each): scores against the query's reference, which is
 //               raised (O rescaled in TMEM) only where a score exceeds it by 2^8; P in bf16 (2^-8 of each weight at most,
 //               which the product needs; sums and outputs are fp32) as a swizzled tile.
-// The same with mma.sync (16 keys x 8 queries per instruction) took 76 us for eight beams of 32 k tokens at the 27B
-// heads: its operand loads alone are 2300 cycles of shared memory per tile, against 2700 that the tile's bytes leave.
+// Eight beams of 32 k shared tokens, 24 / 4 heads of 256 (135 MB): 37-39 us, of which 5 until the first tile, 25 for the
+// tiles (5.3 TB/s, or 2350 cycles each from L2) and 3 for the results, then 5 us to join them. The same with mma.sync (16
+// keys x 8 queries per instruction) took 76 us: its operand loads alone are 2300 cycles of shared memory per tile, against
+// 2700 that the tile's bytes leave. Queries of a row of 24 / 4 heads are 6 of a tile's 128 rows; a block's time does not
+// depend on how many there are, as the tile's bytes and the softmax's latency bound it.
 //
 // Keys that a row does not see (behind its last token, or in a missing page) get the weight 0 whatever they hold:
 // their scores are replaced, their values zeroed in shared memory.
@@ -60,6 +63,8 @@ struct Unit {
   uint64_t queries;  // of the members
 };
 
+static_assert(sizeof(Unit) == 24, "room for the units");
+
 template <int D> struct Shape {
   static constexpr int BOX = TILE * 128;                            // 64 components of a tile's keys or values
   static constexpr int HALF = TILE * D * 2;                         // all of them
@@ -102,6 +107,7 @@ __device__ __forceinline__ bool softmax_any(bool v) {
       : "memory");
   return r != 0;
 }
+
 // D += A B in the TMEM lanes whose bit is set among the first 64 (the others are not written, whatever the product is).
 __device__ __forceinline__ void mma_lanes(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t lo, uint32_t hi) {
   asm volatile(
@@ -220,7 +226,9 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
       int e[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        e[j] = lane >= rows ? -1 : i >= window ? sTail[(lane * 4 + j) * APART + i - window] : sTable[(lane * 4 + j) * AHEAD + t];
+        e[j] = lane >= rows  ? -1
+               : i >= window ? sTail[(lane * 4 + j) * APART + i - window]
+                             : sTable[(lane * 4 + j) * AHEAD + t];
       const int valid = min(max(length - i * TILE, 0), TILE);
       unsigned same = __match_any_sync(~0u, valid);
       bool any = false;
@@ -490,7 +498,8 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
       sm100::tmem_ld32(lanes + half * (D / 2) + c, o);
       sm100::tmem_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(line + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+      for (int i = 0; i < 32; i += 4)
+        *reinterpret_cast<float4*>(line + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
     }
     fence_proxy_async();
     if (used && !bad) {
@@ -509,7 +518,9 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
   }
 }
 
-__device__ __forceinline__ void finish(const AttendArgs& a, long rh, int D, int c, float4 o, float l, const float (&gate)[4]) {
+// Four components of a result: normalised, gated, rounded.
+__device__ __forceinline__ void finish(const AttendArgs& a, long rh, int D, int c, float4 o, float l,
+                                       const float (&gate)[4]) {
   const float scale = l == 0.f ? 0.f : 1.f / l;  // nothing seen: zeros
   float v[4] = {o.x * scale, o.y * scale, o.z * scale, o.w * scale};
   if (a.gate)

@@ -2,8 +2,9 @@
 //
 // A pool holds pages [pages, blocks, 2, heads, page, dim] bf16; table [rows, width], lengths [rows] and refs [pages]
 // (int32) say who holds them. Every decision is taken on the device by one block (a few thousand integers: bound by
-// its barriers), which leaves a list of copies for a second kernel (bound by memory). Nothing depends on the order of
-// an atomic: counts are sums, and free pages are numbered by their position.
+// its barriers and reads: 5-6 us for up to 256 rows), which leaves a list of copies for a second kernel (bound by memory:
+// 34 MB copied in 15 us from memory, 10 us from L2; 404 MB of whole pages in 134 us, 6.0 TB/s). Nothing depends on the
+// order of an atomic: counts are sums, and free pages are numbered by their position.
 #include <algorithm>
 #include <climits>
 #include "../api.h"
@@ -353,7 +354,8 @@ __global__ void __launch_bounds__(256) store_kernel(const StoreArgs a) {
     if (to < 0) continue;
     const bf16* x = a.x[kind] + n * a.batch[kind] + t * a.time[kind] + h * a.head[kind];
     if ((reinterpret_cast<uintptr_t>(x) & 15) == 0) {
-      if (lane * 8 < a.at.dim) *reinterpret_cast<uint4*>(a.pool + to + lane * 8) = *reinterpret_cast<const uint4*>(x + lane * 8);
+      const int c = lane * 8;
+      if (c < a.at.dim) *reinterpret_cast<uint4*>(a.pool + to + c) = *reinterpret_cast<const uint4*>(x + c);
     } else {
       for (int c = lane; c < a.at.dim; c += 32) a.pool[to + c] = x[c];
     }
@@ -375,7 +377,8 @@ struct AppendArgs {
   int vec;      // rows of x are 16-byte aligned
 };
 
-// One warp per (row, head): the query heads, then keys, then values. The angle position * frequency is reduced to a
+// One warp per (row, head): the query heads, then keys, then values (4 us for 64 rows of 24 + 4 heads of 256, of which the
+// 8 MB would take 1: two dependent reads and the launch). The angle position * frequency is reduced to a
 // turn in fp64 (in fp32 it is 0.01 off at position 2^17 already), its sine and cosine are fp32.
 __global__ void __launch_bounds__(128) append_kernel(const AppendArgs a) {
   __shared__ __align__(16) float buf[4][256];

@@ -23,9 +23,9 @@ def beam_select(logits, scores, lengths, finished, end_token=-1, length_penalty=
     """(tokens int64, parents int64, scores fp32, lengths int32, finished bool), all [G, K]: one step of beam search
     for G groups of K beams.
 
-    ``logits`` [G, K, V] of the next token (on CUDA bf16 or fp32, at most 32 beams and 4161536 tokens); ``scores`` [G, K] fp32, the sums of the beams'
-    log-probabilities; ``lengths`` [G, K] int32, their generated tokens; ``finished`` [G, K] bool. A running beam
-    offers each token at score + log_softmax(logits), and is one token longer with it; a finished one offers itself
+    ``logits`` [G, K, V] of the next token (on CUDA bf16 or fp32, at most 32 beams and 4161536 tokens); ``scores``
+    [G, K] fp32, the sums of the beams' log-probabilities; ``lengths`` [G, K] int32, their generated tokens;
+    ``finished`` [G, K] bool. A running beam offers each token at score + log_softmax(logits), and is one token longer with it; a finished one offers itself
     alone, as one more ``end_token`` at its old score and length. A beam whose score is not finite, or whose logits
     hold a NaN or +inf or are all -inf, offers nothing better than -inf. Of a group's K * V candidates the K with the
     largest score / max(length, 1)^length_penalty are kept, ranked in 64 bits, equal ones by the lowest beam, then
@@ -211,8 +211,8 @@ def beam_search(runner, prompt, new_tokens, beams=4, end_token=-1, length_penalt
     A continuation ends with ``end_token`` (its ids are followed by more of them, and its length counts the first) or
     after ``new_tokens``. Scores are sums of log-probabilities; the order is that of score / length^length_penalty
     (see ``beam_select``). ``page``: tokens in a page of the key/value cache (of full-attention blocks that were
-    not replaced, whose heads have 64, 128 or 256 components on CUDA). ``on_token(step)`` is called after each decode step. ``graph=True`` replays the steps as a CUDA graph
-    after the first. The runner's own cache and states are left as they are."""
+    not replaced, whose heads have 64, 128 or 256 components on CUDA). ``on_token(step)`` is called after each decode
+    step. ``graph=True`` replays the steps as a CUDA graph after the first. The runner's own cache and states are left as they are."""
     if prompt.dim() != 2 or prompt.numel() == 0:
         raise ValueError(f"expected prompts [groups, tokens], got {tuple(prompt.shape)}")
     if new_tokens < 1 or beams < 1:

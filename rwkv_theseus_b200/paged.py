@@ -122,7 +122,8 @@ def advance_pages(pool, table, lengths, refs, tokens=1, parents=None, live=None,
 def compact_pages(pool, table, refs, out=None):
     """(table, refs, used): the pages in use moved to the front of the pool, whose first ``used`` [1] pages they are
     then. The lowest page behind them goes to the lowest free page among them, and so on; pages that lie there
-    already stay. Pages that are held outside the table too move like the others. ``out``: (table, refs) to write to, which may be the arguments themselves."""
+    already stay. Pages that are held outside the table too move like the others. ``out``: (table, refs) to write to,
+    which may be the arguments themselves."""
     if pool.is_cuda:
         return tuple(native().compact_pages(pool, table, refs, out))
     _check(pool, table, refs=refs)

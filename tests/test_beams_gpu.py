@@ -284,7 +284,8 @@ def test_store(page):
     state = [x.cpu() for x in (cache.pool, cache.table, cache.lengths)]
     for N, T in ((6, 1), (6, page + 2), (3, 3 * page), (2, 0), (1, 4)):
         k = torch.randn(2, N, T + 3, 2, 64, generator=g).to(torch.bfloat16)[:, :, 1:T + 1]
-        store_pages(cache.pool, 1, cache.table, cache.lengths, k[0].cuda(), k[1].cuda().transpose(1, 2).contiguous().transpose(1, 2))
+        strided = k[1].cuda().transpose(1, 2).contiguous().transpose(1, 2)
+        store_pages(cache.pool, 1, cache.table, cache.lengths, k[0].cuda(), strided)
         reference.store_pages(state[0], 1, *state[1:], k[0], k[1])
         assert torch.equal(cache.pool.cpu(), state[0])
 
@@ -426,7 +427,8 @@ def test_pages_refuse_on_cuda():
             (IndexError, "block -1", lambda: paged_attention(q[:, :1], pool, -1, table, lengths)),
             (ValueError, "gate", lambda: paged_attention(q[:, :2], pool, 0, table, lengths, gate=q[:, :1])),
             (ValueError, "groups of 3", lambda: paged_attention(q[:, :1], pool, 0, table, lengths, group=3)),
-            (ValueError, "query heads", lambda: append_heads(q[:, 0], pool, 0, table, lengths, q[0, 0], q[0, 0], q[0, 0], 0, 1.)),
+            (ValueError, "query heads", lambda: append_heads(q[:, 0], pool, 0, table, lengths, q[0, 0], q[0, 0],
+                                                            q[0, 0], 0, 1.)),
             (ValueError, "x .*does not match", lambda: append_heads(q[:, 0], pool, 0, table, lengths, q[0, 0], q[0, 0],
                                                                    q[0, 0], 2, 1.)),
             (ValueError, "frequencies", lambda: append_heads(q[:, :4].reshape(2, 256), pool, 0, table, lengths, q[0, 0],
