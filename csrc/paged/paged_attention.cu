@@ -3,15 +3,16 @@
 // Bound by memory: every page that a row or its group's other beams hold has to be read once. So a block takes the
 // rows of a group together (one key head, every splits-th tile of 64 keys): of each tile it loads the pages that
 // differ between the rows, and each of them meets the queries of all rows that hold it (up to 64 queries; rows that do
-// not hold it get the weight 0). Roles (192 threads):
+// not hold it are left out). Roles (128 threads):
 //   warp 2      finds the tile's distinct pages (a lane per row) and brings their keys and values into a ring with TMA
 //               (128-byte swizzle, boxes of 64 components);
 //   warp 3      issues S = Q K^T (M = 128, N = 64) into one of two TMEM buffers and O += P V (N = dim), V read MN-major.
 //               The queries are rows 0-63 of the tile; what the products make of the rows behind them, which are whatever
 //               lies in shared memory there, stays in TMEM lanes that nobody reads;
-//   warps 0, 1, 4, 5   softmax, two threads per query (32 keys each): scores against the query's reference, which is
-//               raised (O rescaled in TMEM) only where a score exceeds it by 2^8; P in bf16 (2^-8 of each weight at most,
-//               which the product needs; sums and outputs are fp32) as a swizzled tile.
+//   warps 0, 1  softmax, a thread per query: scores against the query's reference, which is raised (O rescaled in TMEM)
+//               only where a score exceeds it by 2^8; P in bf16 (2^-8 of each weight at most, which the product needs; sums
+//               and outputs are fp32) as a swizzled tile. With two threads per query every unit needs their agreement.
+//
 // Eight beams of 32 k shared tokens, 24 / 4 heads of 256 (135 MB): 37-39 us, of which 5 until the first tile, 25 for the
 // tiles (5.3 TB/s, or 2350 cycles each from L2) and 3 for the results, then 5 us to join them. The same with mma.sync (16
 // keys x 8 queries per instruction) took 76 us: its operand loads alone are 2300 cycles of shared memory per tile, against
@@ -33,7 +34,7 @@
 namespace {
 
 using bf16 = __nv_bfloat16;
-constexpr int TILE = 64, QUERIES = 64, THREADS = 192;  // keys of a unit, queries of a block
+constexpr int TILE = 64, QUERIES = 64, THREADS = 128;  // keys of a unit, queries of a block
 constexpr int MAX_SPLITS = 296, UNITS = 8;
 constexpr int AHEAD = 8, APART = 16;  // tiles whose pages are looked up together; last tiles that may be dealt out by units
 constexpr float HEADROOM = 8.f;  // log2 that a score may exceed its reference by before that is raised
@@ -75,8 +76,7 @@ template <int D> struct Shape {
   static constexpr int KV = Q + QUERIES * D * 2;
   static constexpr int TABLE = KV + RING * HALF;                    // [32 rows][4][AHEAD tiles]
   static constexpr int TAIL = TABLE + 32 * 4 * AHEAD * 4;           // [32 rows][4][APART tiles]
-  static constexpr int MAX = TAIL + 32 * 4 * APART * 4;             // [64 queries][2]
-  static constexpr int UNIT = MAX + QUERIES * 2 * 4;
+  static constexpr int UNIT = TAIL + 32 * 4 * APART * 4;
   static constexpr int BARS = UNIT + UNITS * 24;
   static constexpr int BYTES = BARS + 8 * (2 * RING + UNITS + 8) + 16 + 1024;
   static constexpr uint32_t S = D, COLUMNS = D == 256 ? 512 : 256;  // TMEM: O, then two buffers of scores
@@ -93,21 +93,6 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-// Barrier of the 128 softmax threads, and whether any of them says so.
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-__device__ __forceinline__ bool softmax_any(bool v) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, 128, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"((uint32_t)v)
-      : "memory");
-  return r != 0;
-}
-
 // D += A B in the TMEM lanes whose bit is set among the first 64 (the others are not written, whatever the product is).
 __device__ __forceinline__ void mma_lanes(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t lo, uint32_t hi) {
   asm volatile(
@@ -128,7 +113,6 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
   uint8_t* smem = sm100::align_smem_1024(raw);
   uint8_t *sP = smem + Sh::P, *sQ = smem + Sh::Q, *sKV = smem + Sh::KV;
   int *sTable = reinterpret_cast<int*>(smem + Sh::TABLE), *sTail = reinterpret_cast<int*>(smem + Sh::TAIL);
-  float* sMax = reinterpret_cast<float*>(smem + Sh::MAX);
   Unit* units = reinterpret_cast<Unit*>(smem + Sh::UNIT);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sh::BARS);  // a tile of the ring has landed
   uint64_t* empty = full + RING;                                  // its products are done
@@ -156,10 +140,10 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
       sm100::mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < UNITS; ++i) sm100::mbar_init(&known[i], 1);
-    sm100::mbar_init(q_full, 128);
+    sm100::mbar_init(q_full, QUERIES);
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&s_full[i], 1);
-      sm100::mbar_init(&p_full[i], 128);
+      sm100::mbar_init(&p_full[i], QUERIES);
       sm100::mbar_init(&o_done[i], 1);
     }
     sm100::mbar_init(drain, 1);
@@ -348,18 +332,17 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
     __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax
-    const int half = warp >> 2, n = (warp & 1) * 32 + lane, st128 = (half * 2 + (warp & 1)) * 32 + lane;
-    const int row = n / a.per_kv, h = n % a.per_kv;
+    const int n = tid, row = n / a.per_kv, h = n % a.per_kv;
     const bool used = row < rows;  // a query, of row0 + row
     // queries into the product's layout; those that do not exist have weights 0
     {
-      constexpr int EACH = QUERIES * D / 8 / 128;  // 16-byte words of a thread
+      constexpr int EACH = QUERIES * D / 8 / 64;  // 16-byte words of a thread
 #pragma unroll
       for (int k0 = 0; k0 < EACH; k0 += 8) {
         uint4 v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int i = (k0 + k) * 128 + st128, m = i / (D / 8), c = i % (D / 8), r = m / a.per_kv;
+          const int i = (k0 + k) * 64 + tid, m = i / (D / 8), c = i % (D / 8), r = m / a.per_kv;
           v[k] = make_uint4(0, 0, 0, 0);
           if (k0 + k < EACH && r < rows) {
             const bf16* x = a.q + (row0 + r) * a.q_row + (long)(kv * a.per_kv + m % a.per_kv) * a.q_head + c * 8;
@@ -374,20 +357,20 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int i = (k0 + k) * 128 + st128, m = i / (D / 8), c = i % (D / 8);
+          const int i = (k0 + k) * 64 + tid, m = i / (D / 8), c = i % (D / 8);
           if (k0 + k < EACH) *reinterpret_cast<uint4*>(sQ + (c >> 3) * BOX + m * 128 + (((c & 7) ^ (m & 7)) << 4)) = v[k];
         }
       }
       fence_proxy_async();
       sm100::mbar_arrive(q_full);
     }
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 1) * 32) << 16);
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     {  // products add to O from the first on (the first product waits for these threads' first weights)
       float zero[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) zero[i] = 0.f;
 #pragma unroll 1
-      for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) sm100::tmem_st32(lanes + c, zero);
+      for (int c = 0; c < D; c += 32) sm100::tmem_st32(lanes + c, zero);
       sm100::tmem_wait_st();
     }
     float m = -INFINITY, l = 0.f;
@@ -395,43 +378,35 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
     bool bad = false;
     for (;; ++u) {
       const int st = u & 1;
-      // what ends the loop is agreed on at the first barrier, whichever thread's wait gives up
-      if (!bad) bad = !sm100::mbar_wait(&known[u % UNITS], (u / UNITS) & 1, abort);
-      bad = __any_sync(~0u, bad);
+      if (__any_sync(~0u, !sm100::mbar_wait(&known[u % UNITS], (u / UNITS) & 1, abort))) bad = true;
       const Unit unit = units[u % UNITS];
-      bool done = bad || unit.members == 0;
-      if (!done) done = bad = __any_sync(~0u, !sm100::mbar_wait(&s_full[st], (u >> 1) & 1, abort));
+      if (bad || unit.members == 0) break;
+      bad = __any_sync(~0u, !sm100::mbar_wait(&s_full[st], (u >> 1) & 1, abort));
+      if (bad) break;
       const bool member = used && (unit.members >> row & 1), partial = unit.valid < TILE || unit.there != 15u;
-      float s[32];
-      bool higher = false;  // a score far above the reference (or NaN, or the first): look at the maxima
-      if (!done) {
-        sm100::tc_fence_after();
-        sm100::tmem_ld32(lanes + Sh::S + st * TILE + half * 32, s);
-        sm100::tmem_wait_ld();
-        if (partial) {
+      float s[2][32];
+      sm100::tc_fence_after();
+      sm100::tmem_ld32(lanes + Sh::S + st * TILE, s[0]);
+      sm100::tmem_ld32(lanes + Sh::S + st * TILE + 32, s[1]);
+      sm100::tmem_wait_ld();
+      if (partial) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (half * 32 + i >= unit.valid || !(unit.there >> (half * 2 + i / 16) & 1)) s[i] = -INFINITY;
-        }
-        if (member) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            s[i] *= a.scale_log2;
-            higher |= !(s[i] - m <= HEADROOM);
-          }
-        }
+        for (int i = 0; i < TILE; ++i)
+          if (i >= unit.valid || !(unit.there >> (i / 16) & 1)) s[i / 32][i % 32] = -INFINITY;
       }
-      if (softmax_any(done || higher)) {
-        if (softmax_any(done)) break;
-        float top = -INFINITY;
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
-        sMax[n * 2 + half] = top;
-        softmax_sync();
-        top = fmaxf(m, fmaxf(sMax[n * 2], sMax[n * 2 + 1]));
-        const float keep = !member || top == m ? 1.f : ex2(m - top);  // (m of -inf: sums and outputs are 0 so far)
-        if (member) {
-          m = top;
+      for (int i = 0; i < TILE; ++i) {
+        s[i / 32][i % 32] *= a.scale_log2;
+        top[i & 3] = fmaxf(top[i & 3], s[i / 32][i % 32]);
+      }
+      const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      // a score far above the reference, or the first: the maximum is the reference from now on
+      const bool higher = member && !(most - m <= HEADROOM);
+      if (__any_sync(~0u, higher)) {
+        const float keep = higher && most > m ? ex2(m - most) : 1.f;  // (m of -inf: sums and outputs are 0 so far)
+        if (higher && most > m) {
+          m = most;
           l *= keep;
         }
         if (u > 0) {  // O must hold what came before it is rescaled
@@ -439,7 +414,7 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
           if (!bad && __any_sync(~0u, keep != 1.f)) {
             sm100::tc_fence_after();
 #pragma unroll 1
-            for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
+            for (int c = 0; c < D; c += 32) {
               float o[32];
               sm100::tmem_ld32(lanes + c, o);
               sm100::tmem_wait_ld();
@@ -456,46 +431,46 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
       if (partial) {  // values that nobody sees
         const int entry = 2 * u + 1, slot = entry % RING;
         bad |= __any_sync(~0u, !sm100::mbar_wait(&full[slot], (entry / RING) & 1, abort));
-        for (int i = st128; i < TILE * D / 8; i += 128) {  // boxes of 64 rows of 8 words
+        for (int i = tid; i < TILE * D / 8; i += QUERIES) {  // boxes of 64 rows of 8 words
           const int r = i / 8 % TILE;
           if (r >= unit.valid || !(unit.there >> (r / 16) & 1))
             *reinterpret_cast<uint4*>(sKV + slot * HALF + i * 16) = make_uint4(0, 0, 0, 0);
         }
       }
+      if (bad) break;
       const float base = m == -INFINITY ? 0.f : m;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
       uint8_t* weights = sP + st * Sh::P_BYTES + n * 128;
+      if (member) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
-        if (member) {
+        for (int c = 0; c < 8; ++c) {
+          uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float x = ex2(s[c * 8 + 2 * i] - base), y = ex2(s[c * 8 + 2 * i + 1] - base);
+            const int k = c * 8 + 2 * i;
+            const float x = ex2(s[k / 32][k % 32] - base), y = ex2(s[k / 32][k % 32 + 1] - base);
             sum[i] += x + y;
             w[i] = pack(x, y);
           }
+          *reinterpret_cast<uint4*>(weights + ((c ^ (n & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        *reinterpret_cast<uint4*>(weights + (((half * 4 + c) ^ (n & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       fence_proxy_async();
       sm100::tc_fence_before();
       sm100::mbar_arrive(&p_full[st]);
     }
     // ---- result: u units were seen (bad: it is none)
-    if (u > 0 && !bad) bad = !sm100::mbar_wait(&o_done[(u - 1) & 1], ((u - 1) >> 1) & 1, abort);
-    sMax[n * 2 + half] = l;
-    bad = softmax_any(bad || *abort);
+    if (u > 0 && !bad) bad = __any_sync(~0u, !sm100::mbar_wait(&o_done[(u - 1) & 1], ((u - 1) >> 1) & 1, abort));
     sm100::tc_fence_after();
     const long at = ((long)(row0 + row) * a.heads + kv * a.per_kv + h) * a.splits + split;
-    if (used && half == 0) a.stats[at] = make_float2(m, bad ? NAN : sMax[n * 2] + sMax[n * 2 + 1]);
-    // rows through shared memory (16 bytes apart beyond their size), half of a row with one copy; the ring has had its use
-    float* line = reinterpret_cast<float*>(sKV) + n * (D + 4) + half * (D / 2);
+    if (used) a.stats[at] = make_float2(m, bad ? NAN : l);
+    // rows through shared memory (16 bytes apart beyond their size), one copy each; the ring has had its use
+    float* line = reinterpret_cast<float*>(sKV) + n * (D + 4);
 #pragma unroll 1
-    for (int c = 0; c < D / 2; c += 32) {
+    for (int c = 0; c < D && !bad; c += 32) {
       float o[32];
-      sm100::tmem_ld32(lanes + half * (D / 2) + c, o);
+      sm100::tmem_ld32(lanes + c, o);
       sm100::tmem_wait_ld();
 #pragma unroll
       for (int i = 0; i < 32; i += 4)
@@ -503,8 +478,8 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
     }
     fence_proxy_async();
     if (used && !bad) {
-      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.sums + at * D + half * (D / 2)),
-                   "r"(sm100::smem_u32(line)), "r"(D * 2)
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.sums + at * D),
+                   "r"(sm100::smem_u32(line)), "r"(D * 4)
                    : "memory");
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
