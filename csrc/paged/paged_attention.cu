@@ -11,7 +11,7 @@
 //               lies in shared memory there, stays in TMEM lanes that nobody reads;
 //   warps 0, 1  softmax, a thread per query: scores against the query's reference, which is raised (O rescaled in TMEM)
 //               only where a score exceeds it by 2^8; P in bf16 (2^-8 of each weight at most, which the product needs; sums
-//               and outputs are fp32) as a swizzled tile. With two threads per query every unit needs their agreement.
+//               and outputs are fp32) in place of the scores. With two threads per query every unit needs their agreement.
 //
 // Eight beams of 32 k shared tokens, 24 / 4 heads of 256 (135 MB): 37-39 us, of which 5 until the first tile, 25 for the
 // tiles (5.3 TB/s, or 2350 cycles each from L2) and 3 for the results, then 5 us to join them. The same with mma.sync (16
@@ -67,19 +67,21 @@ struct Unit {
 static_assert(sizeof(Unit) == 24, "room for the units");
 
 template <int D> struct Shape {
+  // TMEM: O, two buffers of scores (whose weights replace them), and the queries where they fit beside them (D / 2 columns;
+  // products then read 4 KB less of shared memory each, which is what bounds them at N = 64). Two blocks per SM below 256.
+  static constexpr uint32_t COLUMNS = D == 256 ? 512 : 256, S = D, Q_COLUMN = S + 2 * TILE;
+  static constexpr bool Q_TMEM = Q_COLUMN + D / 2 <= COLUMNS;
   static constexpr int BOX = TILE * 128;                            // 64 components of a tile's keys or values
   static constexpr int HALF = TILE * D * 2;                         // all of them
-  static constexpr int RING = D == 256 ? 5 : D == 128 ? 4 : 8;      // tiles of keys or values (two blocks per SM below 256)
-  static constexpr int P = 0, P_BYTES = QUERIES * 128;              // two tiles of weights [64][64 keys]
-  // products read 64 rows more than a tile of weights or queries has: what follows has to be as long
-  static constexpr int Q = P + 2 * P_BYTES;                         // [D / 64][64][64]
-  static constexpr int KV = Q + QUERIES * D * 2;
+  static constexpr int RING = D == 256 ? 6 : D == 128 ? 5 : 8;      // tiles of keys or values
+  // products read 64 rows more than a tile of queries in shared memory has: what follows has to be as long
+  static constexpr int Q = 0;                                       // [D / 64][64][64]
+  static constexpr int KV = Q + (Q_TMEM ? 0 : QUERIES * D * 2);
   static constexpr int TABLE = KV + RING * HALF;                    // [32 rows][4][AHEAD tiles]
   static constexpr int TAIL = TABLE + 32 * 4 * AHEAD * 4;           // [32 rows][4][APART tiles]
   static constexpr int UNIT = TAIL + 32 * 4 * APART * 4;
   static constexpr int BARS = UNIT + UNITS * 24;
   static constexpr int BYTES = BARS + 8 * (2 * RING + UNITS + 8) + 16 + 1024;
-  static constexpr uint32_t S = D, COLUMNS = D == 256 ? 512 : 256;  // TMEM: O, then two buffers of scores
   static constexpr uint32_t IDESC_S = sm100::idesc_bf16(128, TILE, false, false);
   static constexpr uint32_t IDESC_O = sm100::idesc_bf16(128, D, false, true);
 };
@@ -93,13 +95,22 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// D = A B (+ D) with A in TMEM: two bf16 per column of its row's lane.
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // D += A B in the TMEM lanes whose bit is set among the first 64 (the others are not written, whatever the product is).
-__device__ __forceinline__ void mma_lanes(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t lo, uint32_t hi) {
+__device__ __forceinline__ void mma_lanes(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t lo, uint32_t hi) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %7, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %6}, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(~lo), "r"(~hi), "r"(~0u), "r"(1u)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%4, %5, %6, %6}, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(~lo), "r"(~hi), "r"(~0u), "r"(1u)
       : "memory");
 }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -111,7 +122,7 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
   constexpr int RING = Sh::RING, HALF = Sh::HALF, BOX = Sh::BOX, BOXES = D / 64;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = sm100::align_smem_1024(raw);
-  uint8_t *sP = smem + Sh::P, *sQ = smem + Sh::Q, *sKV = smem + Sh::KV;
+  uint8_t *sQ = smem + Sh::Q, *sKV = smem + Sh::KV;
   int *sTable = reinterpret_cast<int*>(smem + Sh::TABLE), *sTail = reinterpret_cast<int*>(smem + Sh::TAIL);
   Unit* units = reinterpret_cast<Unit*>(smem + Sh::UNIT);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Sh::BARS);  // a tile of the ring has landed
@@ -280,6 +291,7 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
     if (sm100::elect_one()) {
       const uint32_t qb = sm100::smem_u32(sQ);
       bool ok = sm100::mbar_wait(q_full, 0, abort), last = false;
+      sm100::tc_fence_after();
       auto scores = [&](int u) {  // of unit u, unless there is none
         if (!sm100::mbar_wait(&known[u % UNITS], (u / UNITS) & 1, abort)) return false;
         if (units[u % UNITS].members == 0) {
@@ -292,9 +304,12 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
         const uint32_t kb = sm100::smem_u32(sKV + slot * HALF);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint64_t ad = sm100::smem_desc(qb + (k >> 2) * BOX + (k & 3) * 32, 16, 1024);
+          const uint32_t d = tmem + Sh::S + (u & 1) * TILE;
           const uint64_t bd = sm100::smem_desc(kb + (k >> 2) * BOX + (k & 3) * 32, 16, 1024);
-          sm100::mma_bf16(tmem + Sh::S + (u & 1) * TILE, ad, bd, Sh::IDESC_S, k > 0);
+          if (Sh::Q_TMEM)
+            mma_tmem(d, tmem + Sh::Q_COLUMN + k * 8, bd, Sh::IDESC_S, k > 0);
+          else
+            sm100::mma_bf16(d, sm100::smem_desc(qb + (k >> 2) * BOX + (k & 3) * 32, 16, 1024), bd, Sh::IDESC_S, k > 0);
         }
         sm100::mma_commit(&s_full[u & 1]);
         sm100::mma_commit(&empty[slot]);
@@ -312,17 +327,17 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
         if (!sm100::mbar_wait(&full[slot], (entry / RING) & 1, abort)) break;
         sm100::tc_fence_after();
         const uint64_t queries = units[u % UNITS].queries;
-        const uint32_t pb = sm100::smem_u32(sP + (u & 1) * Sh::P_BYTES), vb = sm100::smem_u32(sKV + slot * HALF);
+        const uint32_t vb = sm100::smem_u32(sKV + slot * HALF);
 #pragma unroll
         for (int k = 0; k < TILE / 16; ++k) {
-          const uint64_t ad = sm100::smem_desc(pb + k * 32, 16, 1024);
           const uint64_t bd = sm100::smem_desc(vb + k * 2048, BOX, 1024);
-          mma_lanes(tmem, ad, bd, Sh::IDESC_O, (uint32_t)queries, (uint32_t)(queries >> 32));
+          mma_lanes(tmem, tmem + Sh::S + (u & 1) * TILE + k * 8, bd, Sh::IDESC_O, (uint32_t)queries, (uint32_t)(queries >> 32));
         }
         sm100::mma_commit(&o_done[u & 1]);
         sm100::mma_commit(&empty[slot]);
         if (!last) {
-          ok = scores(u + 2);
+          // the next scores take the weights' columns, which this product reads
+          ok = sm100::mbar_wait(&o_done[u & 1], (u >> 1) & 1, abort) && scores(u + 2);
           end += !last;
         }
       }
@@ -334,8 +349,36 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
     // ------------------------------------------------------------ softmax
     const int n = tid, row = n / a.per_kv, h = n % a.per_kv;
     const bool used = row < rows;  // a query, of row0 + row
-    // queries into the product's layout; those that do not exist have weights 0
-    {
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    // queries into the product's layout (zeros where there is none)
+    if (Sh::Q_TMEM) {
+      const bf16* x = a.q + (row0 + row) * a.q_row + (long)(kv * a.per_kv + h) * a.q_head;
+#pragma unroll 2
+      for (int c = 0; c < D; c += 64) {
+        uint4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (used && a.q_vec) {
+            v[k] = *reinterpret_cast<const uint4*>(x + c + k * 8);
+          } else if (used) {
+            bf16* e = reinterpret_cast<bf16*>(&v[k]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = x[c + k * 8 + j];
+          }
+        }
+        float w[32];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          w[4 * k] = __uint_as_float(v[k].x);
+          w[4 * k + 1] = __uint_as_float(v[k].y);
+          w[4 * k + 2] = __uint_as_float(v[k].z);
+          w[4 * k + 3] = __uint_as_float(v[k].w);
+        }
+        sm100::tmem_st32(lanes + Sh::Q_COLUMN + c / 2, w);
+      }
+      sm100::tmem_wait_st();
+    } else {
       constexpr int EACH = QUERIES * D / 8 / 64;  // 16-byte words of a thread
 #pragma unroll
       for (int k0 = 0; k0 < EACH; k0 += 8) {
@@ -362,9 +405,9 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
         }
       }
       fence_proxy_async();
-      sm100::mbar_arrive(q_full);
     }
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    sm100::tc_fence_before();
+    sm100::mbar_arrive(q_full);
     {  // products add to O from the first on (the first product waits for these threads' first weights)
       float zero[32];
 #pragma unroll
@@ -426,8 +469,6 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
           }
         }
       }
-      // the buffer of weights was last read by the product of unit u - 2
-      if (u >= 2) bad |= __any_sync(~0u, !sm100::mbar_wait(&o_done[st], ((u - 2) >> 1) & 1, abort));
       if (partial) {  // values that nobody sees
         const int entry = 2 * u + 1, slot = entry % RING;
         bad |= __any_sync(~0u, !sm100::mbar_wait(&full[slot], (entry / RING) & 1, abort));
@@ -440,23 +481,17 @@ __global__ void __launch_bounds__(THREADS) attend_kernel(const __grid_constant__
       if (bad) break;
       const float base = m == -INFINITY ? 0.f : m;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
-      uint8_t* weights = sP + st * Sh::P_BYTES + n * 128;
-      if (member) {
+      float w[32];  // two weights each (rows that do not hold the page: of no consequence)
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int k = c * 8 + 2 * i;
-            const float x = ex2(s[k / 32][k % 32] - base), y = ex2(s[k / 32][k % 32 + 1] - base);
-            sum[i] += x + y;
-            w[i] = pack(x, y);
-          }
-          *reinterpret_cast<uint4*>(weights + ((c ^ (n & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      for (int i = 0; i < 32; ++i) {
+        const float x = ex2(s[i / 16][i % 16 * 2] - base), y = ex2(s[i / 16][i % 16 * 2 + 1] - base);
+        sum[i & 3] += x + y;
+        w[i] = __uint_as_float(pack(x, y));
       }
-      fence_proxy_async();
+      if (member) l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      sm100::tmem_st32(lanes + Sh::S + st * TILE, w);
+      sm100::tmem_wait_st();
+      if (partial) fence_proxy_async();
       sm100::tc_fence_before();
       sm100::mbar_arrive(&p_full[st]);
     }
