@@ -213,6 +213,16 @@ __global__ void __launch_bounds__(THREADS, 5) select_rows_kernel(const SelectArg
         sum2 = add2(sum2, make_float2(ex2(y.x), ex2(y.y)));
       }
     }
+  } else {  // no number above -inf, but a NaN leaves the beam without a rank here too
+    bool none = single >= 0 && one != one;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float f[VEC];
+      unpack(u[i], f);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) none |= f[j] != f[j];
+    }
+    if (none) sum2.x = NAN;
   }
   double d = (double)sum2.x + (double)sum2.y;
 #pragma unroll

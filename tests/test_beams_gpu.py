@@ -77,6 +77,20 @@ def test_selection_corners(V, dtype):
     _check([logits, scores, lengths, finished], -1)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("at", [0, 20003, 29999, 40002])
+def test_a_nan_among_masked_logits_leaves_the_beam_nothing(at, dtype):
+    logits, scores, lengths, finished = _step(2, 3, 40003, dtype, seed=2)
+    logits[0, 1] = -INF  # but for a few, far from the NaN
+    logits[0, 1, 10000:10010] = 1.0
+    logits[0, 1, at] = math.nan
+    logits[1] = -INF
+    logits[1, 0, 10000:10010] = 1.0
+    logits[1, 2, at] = math.nan
+    finished.zero_()
+    _check([logits, scores, lengths, finished])
+
+
 def test_selection_takes_any_strides():
     logits, scores, lengths, finished = _step(3, 4, 1001, torch.float32)
     wide = torch.empty(4, 3, 2005, device="cuda")
