@@ -3,12 +3,12 @@
 //   value(b, v) = score_b + z_bv - log sum_w exp z_bw    (running beams)
 //   rank        = value / max(length_b + 1, 1)^penalty
 //
-// Within a beam the order is that of its logits, so a block per (beam, segment of the vocabulary) needs no softmax to
-// find the segment's K best: it holds the segment in registers, forms the segment's maximum and sum of exponentials
-// (terms in fp32, added up over threads in fp64), takes a bound from its threads' maxima that K values reach, and sorts
-// the few values that do. A second kernel, one block per group, joins the sums, ranks the segments' candidates in fp64
-// and keeps the K best. Ranks of different beams are off by the fp32 exponentials' error at worst (about 1e-7), those of
-// one beam differ by their logits alone.
+// Equal ranks go by the beam, then the logit, then the token. So within a beam the order is that of its logits, and a block
+// per (beam, segment of the vocabulary) needs no softmax to find the segment's K best: it holds the segment in registers,
+// forms the segment's maximum and sum of exponentials (terms in fp32, added up over threads in fp64), takes a bound from its
+// threads' maxima that K values reach, and sorts the few values that do. A second kernel, one block per group, joins the
+// sums, ranks the segments' candidates in fp64 and keeps the K best. Ranks of different beams are off by the fp32
+// exponentials' error at worst (about 1e-7), those of one beam differ by their logits alone.
 //
 // Eight groups of eight beams x 248077 fp32 logits (a sixth of them ended, 53 MB): 17 us for the segments, bound by half
 // of the issue slots and the phases of a block, 10 us for the groups, a chain of reads and barriers. Four beams x 4096:
@@ -29,6 +29,7 @@ constexpr int HELD = 8192;           // values of a block in registers
 constexpr int SEGMENT = HELD - 64;   // of a segment at most (its ends need not be aligned)
 constexpr int MAX_SEGMENTS = 512;
 constexpr int MERGE_LIST = 1024;     // candidates of a group
+static_assert((long)SEGMENT * MAX_SEGMENTS <= 1 << 22, "a token has 22 bits");
 constexpr float LOG2E = 1.4426950408889634f;
 
 // Order-preserving 32-bit key of a logit: -0 equals +0; 0 is below all of them. (Of a NaN any: its beam has no rank.)
@@ -292,6 +293,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.K, S = a.segments, lists = K * S;
   const long first = (long)blockIdx.x * K;
   if (tid == 0) found = 0;
+  if (tid < K) chosen[tid] = (long)tid << 54;
   const int whole = min((lists + 31) / 32, MERGE_WARPS), mine = lane * whole + warp;  // this thread's first list
   const unsigned long long first_head = warp < whole && mine < lists ? a.entries[(first * S + mine) * K] : 0ull;
   for (int b = warp; b < K; b += MERGE_WARPS) {
@@ -346,10 +348,12 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     value = -INFINITY;
     if (j >= K) return;
     int token;
+    unsigned below = 0;  // falls with the logit
     if (kind[b] == 0) {
       if (e == 0) return;
       token = (int)~(unsigned)e;
-      const float z = key_value((unsigned)(e >> 32));
+      below = ~(unsigned)(e >> 32);
+      const float z = key_value(~below);
       if (z > -INFINITY) value = base[b] + ((double)z - (double)row_top[b]);
     } else {
       if (seg > 0) return;
@@ -361,7 +365,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
       if (token >= a.V) return;
     }
     rank = rank_key(value / norm[b]);
-    flat = (long)b * a.V + token;
+    flat = (long)b << 54 | (long)below << 22 | token;  // equal ranks: beam, logit, token (of 22 bits)
   };
   // the upper half of a rank's key keeps its order. A warp's lists are spread over all beams, as they are not alike
   // (a thread may stand for several lists); each warp's k-th largest head, as in a segment
@@ -429,13 +433,16 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     }
   };
   // A row's candidates that can reach the bound have a logit of about (bound norm - base) + top; they are few, and only
-  // they are ranked. (The margin is far above the rounding of these steps; what it lets through is ranked in vain.)
+  // they are ranked. Rank, value and the terms here are rounded by 2^-53 of one of the three terms each (a score of -3e38,
+  // which a mask's lowest value leaves, swallows logits whole): the margin of 2^-48 of all, and of more than the logit's own
+  // rounding, is far above that, and what it lets through is ranked in vain.
   if (tid < K) {
     const unsigned long long key = (unsigned long long)least << 32;
     const double rank = __longlong_as_double((long long)(key >> 63 ? key & ~(1ull << 63) : ~key));
-    const double at_least = rank * norm[tid] - base[tid] + (double)row_top[tid];
+    const double reach = rank * norm[tid], at_least = reach - base[tid] + (double)row_top[tid];
+    const double margin = (fabs(reach) + fabs(base[tid]) + fabs((double)row_top[tid])) * 0x1p-48;
     // (NaN, of a bound below all numbers, lets everything through)
-    row_least[tid] = __double2float_rd(at_least - fabs(at_least) * 1e-6 - 1e-3);
+    row_least[tid] = __double2float_rd(at_least - margin - fabs(at_least) * 1e-6 - 1e-3);
   }
   __syncthreads();
   // a lane per entry, 32 / K lists per warp
@@ -532,7 +539,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
   // ---- slots: a parent's best child keeps the parent's, the others fill what is left in order
   const bool in = lane < K;
   const unsigned all = K == 32 ? ~0u : (1u << K) - 1;
-  const int parent = in ? (int)((unsigned)chosen[lane] / (unsigned)a.V) : 32 + lane;
+  const int parent = in ? (int)(chosen[lane] >> 54) : 32 + lane;
   const unsigned siblings = __match_any_sync(~0u, parent);
   const bool keeps = in && __ffs(siblings) - 1 == lane;
   unsigned left = all & ~__reduce_or_sync(~0u, in ? 1u << parent : 0u);
@@ -543,7 +550,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     for (int skip = __popc(others & ((1u << lane) - 1)); skip > 0; --skip) left &= left - 1;
     slot = __ffs(left) - 1;
   }
-  const long token = chosen[lane] - (long)parent * a.V, to = first + slot;
+  const long token = chosen[lane] & ((1 << 22) - 1), to = first + slot;
   a.tokens[to] = token;
   a.parents[to] = parent;
   a.out_scores[to] = (float)values[lane];

@@ -25,11 +25,11 @@ def beam_select(logits, scores, lengths, finished, end_token=-1, length_penalty=
 
     ``logits`` [G, K, V] of the next token (on CUDA bf16 or fp32, at most 32 beams and 4161536 tokens); ``scores``
     [G, K] fp32, the sums of the beams' log-probabilities; ``lengths`` [G, K] int32, their generated tokens;
-    ``finished`` [G, K] bool. A running beam offers each token at score + log_softmax(logits), and is one token longer with it; a finished one offers itself
-    alone, as one more ``end_token`` at its old score and length. A beam whose score is not finite, or whose logits
-    hold a NaN or +inf or are all -inf, offers nothing better than -inf. Of a group's K * V candidates the K with the
-    largest score / max(length, 1)^length_penalty are kept, ranked in 64 bits, equal ones by the lowest beam, then
-    token.
+    ``finished`` [G, K] bool. A running beam offers each token at score + log_softmax(logits), and is one token longer
+    with it; a finished one offers itself alone, as one more ``end_token`` at its old score and length. A beam whose
+    score is not finite, or whose logits hold a NaN or +inf or are all -inf, offers nothing better than -inf. Of a
+    group's K * V candidates the K with the largest score / max(length, 1)^length_penalty are kept, ranked in 64 bits,
+    equal ones by the lowest beam, then the largest logit, then the lowest token.
 
     They are not sorted: a parent's best child takes the parent's slot, and the others fill the slots that are left in
     order of rank, so that what a surviving beam holds stays where it is. ``parents`` are slots of the same group;

@@ -169,8 +169,13 @@ def beam_select(logits, scores, lengths, finished, end_token, length_penalty):
     if end_token >= 0:
         value[..., end_token] = torch.where(finished & fit, scores.double(), value[..., end_token])
     length = lengths + (~finished).to(lengths.dtype)
-    rank = (value / length.clamp_min(1).double().pow(length_penalty)[..., None]).flatten(1)
+    rank = value / length.clamp_min(1).double().pow(length_penalty)[..., None]
+    # of equal ranks the lowest beam, then the largest logit (a score of 1e16 swallows it), then the lowest token
+    order = logits.double().masked_fill(value == float("-inf"), float("-inf"))
+    order = order.sort(dim=-1, descending=True, stable=True)[1]
+    rank = rank.gather(-1, order).flatten(1)
     best = rank.sort(dim=1, descending=True, stable=True)[1][:, :K]
+    best = best // V * V + order.flatten(1).gather(1, best)
     best = best.gather(1, place_children(best // V))
     parents, tokens = best // V, best % V
     return (tokens, parents, value.flatten(1).gather(1, best).float(), length.gather(1, parents),

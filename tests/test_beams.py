@@ -106,6 +106,17 @@ def test_selection_against_all_candidates(case, penalty):
     _check_step(args, end, penalty)
 
 
+@pytest.mark.parametrize("score", [-1e14, -1e17, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("penalty", [0.0, 0.7])
+def test_scores_that_swallow_logits_leave_their_order(score, penalty):
+    logits, scores, lengths, finished = _step(V=40)
+    scores[:, 1:] = -math.inf
+    scores[:, 0] = score
+    tokens, parents, new_scores, _, _ = beam_select(logits, scores, lengths, finished, length_penalty=penalty)
+    assert (parents == 0).all() and torch.equal(new_scores, torch.full((2, 3), score))
+    assert torch.equal(tokens, logits[:, 0].sort(dim=1, descending=True)[1][:, :3])
+
+
 def test_selection_refuses():
     logits, scores, lengths, finished = _step()
     with pytest.raises(ValueError, match="expected logits"):

@@ -91,6 +91,18 @@ def test_a_nan_among_masked_logits_leaves_the_beam_nothing(at, dtype):
     _check([logits, scores, lengths, finished])
 
 
+@pytest.mark.parametrize("score", [-1e9, -1e14, -1e17, LOWEST])
+@pytest.mark.parametrize("G,K,V", [(2, 3, 40), (1, 4, 4096), (3, 32, 20011), (2, 5, 70001)])
+def test_scores_that_swallow_logits_leave_their_order(G, K, V, score):
+    logits, scores, lengths, finished = _step(G, K, V, torch.float32, seed=3)
+    finished.zero_()
+    scores[:] = -INF
+    scores[:, K // 2] = score
+    for penalty in (0.0, 0.7, -1.3):
+        _check([logits, scores, lengths, finished], 1, penalty)
+        _check([logits.bfloat16(), scores, lengths, finished], 1, penalty)  # (many equal logits)
+
+
 def test_selection_takes_any_strides():
     logits, scores, lengths, finished = _step(3, 4, 1001, torch.float32)
     wide = torch.empty(4, 3, 2005, device="cuda")
