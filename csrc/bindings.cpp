@@ -900,6 +900,7 @@ RtPool pool_of(const at::Tensor& pool, const at::Tensor& table, int64_t block = 
              "the CUDA paged cache takes bf16 and head sizes (64, 128, 256), got ", pool.scalar_type(), " and ", dim);
   want<Value>(table.size(0) <= 1024, "the CUDA paged cache has at most 1024 rows, got ", table.size(0));
   want<Value>(pool.size(0) < (1 << 30) && pool.size(1) * pool.size(3) < (1 << 20) && table.size(1) < (1 << 24) &&
+                  table.numel() <= INT_MAX && pool.size(1) * pool.size(3) * 4 * table.size(0) < (1 << 30) &&
                   pool.numel() / dim <= INT_MAX,
               "paged cache: size out of range");
   return {pool.data_ptr(), (int)pool.size(0), (int)pool.size(1), (int)pool.size(3), (int)page,

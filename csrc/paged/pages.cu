@@ -467,6 +467,9 @@ extern "C" cudaError_t rt_advance_pages(const RtPool* p, const int* table, const
                                         int* new_lengths, int* new_refs, int* status, int keep_status, void* work,
                                         cudaStream_t s) {
   if (!pool_fits(p) || tokens < 0 || K < 1 || p->rows % K) return cudaErrorInvalidValue;
+  const int panels = p->blocks * 2 * p->heads;
+  const long items = (long)panels * 2 * p->rows;  // of the copies at most, and the blocks' next ones stay in range
+  if (items > INT_MAX - 65536) return cudaErrorInvalidValue;
   AdvanceArgs a{table, lengths, refs, new_table, new_lengths, new_refs, status, keep_status, parents, live,
                 p->rows, K, p->width, p->pages, p->page, tokens, static_cast<int4*>(work) + 1, static_cast<int*>(work)};
   // (few rows: the barriers of a smaller block are cheaper)
@@ -475,9 +478,6 @@ extern "C" cudaError_t rt_advance_pages(const RtPool* p, const int* table, const
   else advance_kernel<false, 1024><<<1, 1024, 0, s>>>(a);
   RT_CUDA_CHECK(cudaGetLastError());
   if (tokens == 0) return cudaSuccess;
-  const int panels = p->blocks * 2 * p->heads;
-  const long items = (long)panels * 2 * p->rows;  // at most, and the blocks' next ones stay in range
-  if (items > INT_MAX - 65536) return cudaErrorInvalidValue;
   copy_tokens_kernel<<<(unsigned)std::min(items, 148L * 6), 256, 0, s>>>(static_cast<bf16*>(p->pool), a.copies, a.count,
                                                                        panels, p->page, p->dim);
   return cudaGetLastError();

@@ -212,11 +212,14 @@ def beam_search(runner, prompt, new_tokens, beams=4, end_token=-1, length_penalt
     after ``new_tokens``. Scores are sums of log-probabilities; the order is that of score / length^length_penalty
     (see ``beam_select``). ``page``: tokens in a page of the key/value cache (of full-attention blocks that were
     not replaced, whose heads have 64, 128 or 256 components on CUDA). ``on_token(step)`` is called after each decode
-    step. ``graph=True`` replays the steps as a CUDA graph after the first. The runner's own cache and states are left as they are."""
+    step. ``graph=True`` replays the steps as a CUDA graph after the first. The runner's own cache and states are left as
+    they are."""
     if prompt.dim() != 2 or prompt.numel() == 0:
         raise ValueError(f"expected prompts [groups, tokens], got {tuple(prompt.shape)}")
-    if new_tokens < 1 or beams < 1:
-        raise ValueError("beam search needs at least one beam and one new token")
+    if new_tokens < 1 or beams < 1 or prefill_chunk < 1:
+        raise ValueError("beam search needs at least one beam, one new token and one token per prefill chunk")
+    if graph and not prompt.is_cuda:
+        raise ValueError("graph steps need CUDA")
     if prompt.is_cuda and beams > MAX_BEAMS:
         raise ValueError(f"beam search takes at most {MAX_BEAMS} beams on CUDA, got {beams}")
     every = 16  # steps between two looks at whether all beams have ended

@@ -442,3 +442,11 @@ def test_search_refuses():
         beam_search(runner, torch.zeros(1, 3, dtype=torch.int64), 0)
     with pytest.raises(ValueError, match="page holds"):
         beam_search(runner, torch.zeros(1, 3, dtype=torch.int64), 4, page=5)
+
+
+def test_search_refuses_chunks_and_graphs_that_cannot_be():
+    runner = Runner(tiny_model())
+    with pytest.raises(ValueError, match="prefill chunk"):
+        beam_search(runner, torch.zeros(1, 3, dtype=torch.int64), 4, prefill_chunk=-1)
+    with pytest.raises(ValueError, match="graph steps need CUDA"):
+        beam_search(runner, torch.zeros(1, 3, dtype=torch.int64), 4, graph=True)

@@ -415,6 +415,15 @@ def test_scores_of_any_size():
     _check_attention(q, pool, table, lengths, None, group=2)
 
 
+def test_a_cache_with_too_many_rows_and_blocks_is_left_alone():
+    pool = torch.empty(1, 2 ** 18, 2, 1, 16, 64, device="cuda", dtype=torch.bfloat16)
+    table = torch.full((1024, 1), -1, device="cuda", dtype=torch.int32)
+    lengths, refs = torch.zeros(1024, device="cuda", dtype=torch.int32), torch.zeros(1, device="cuda", dtype=torch.int32)
+    with pytest.raises(ValueError, match="out of range"):
+        advance_pages(pool, table, lengths, refs, out=(table, lengths, refs, torch.zeros_like(refs)))
+    assert (table == -1).all() and (lengths == 0).all() and (refs == 0).all()
+
+
 def test_pages_refuse_on_cuda():
     cache = PagedCache(1, 1, 64, 2, 64, 4, 16, "cuda")
     with pytest.raises(TypeError, match="bf16 and head sizes"):
