@@ -13,11 +13,13 @@
 //               only where a score exceeds it by 2^8; P in bf16 (2^-8 of each weight at most, which the product needs; sums
 //               and outputs are fp32) in place of the scores. With two threads per query every unit needs their agreement.
 //
-// Eight beams of 32 k shared tokens, 24 / 4 heads of 256 (135 MB): 37-39 us, of which 5 until the first tile, 25 for the
-// tiles (5.3 TB/s, or 2350 cycles each from L2) and 3 for the results, then 5 us to join them. The same with mma.sync (16
-// keys x 8 queries per instruction) took 76 us: its operand loads alone are 2300 cycles of shared memory per tile, against
-// 2700 that the tile's bytes leave. Queries of a row of 24 / 4 heads are 6 of a tile's 128 rows; a block's time does not
-// depend on how many there are, as the tile's bytes and the softmax's latency bound it.
+// Eight beams of 32 k shared tokens, 24 / 4 heads of 256 (135 MB): 34 us, of which 4 until the first tile, 25 for the tiles
+// (5.3 TB/s; about 1900 cycles each from L2: scores 730, then weights and their product, which follow one another) and 2-3
+// for the results, then 5 us to join them. The same with mma.sync (16 keys x 8 queries per instruction) took 76 us: its
+// operand loads alone are 2300 cycles of shared memory per tile, against 2700 that the tile's bytes leave. Queries of a row
+// of 24 / 4 heads are 6 of a tile's 128 rows; a block's time does not depend on how many there are, as the tile's bytes and
+// the products' latency bound it. Tried without gain: one copy for a tile's keys instead of one per 64 components, a
+// shorter way to the classes of rows that are all alike (40 us in all against 39).
 //
 // Keys that a row does not see (behind its last token, or in a missing page) get the weight 0 whatever they hold:
 // their scores are replaced, their values zeroed in shared memory.
