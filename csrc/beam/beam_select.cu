@@ -11,8 +11,9 @@
 // exponentials' error at worst (about 1e-7), those of one beam differ by their logits alone.
 //
 // Eight groups of eight beams x 248077 fp32 logits (a sixth of them ended, 53 MB): 17 us for the segments, bound by half
-// of the issue slots and the phases of a block, 10 us for the groups, a chain of reads and barriers. Four beams x 4096:
-// 5 and 7 us.
+// of the issue slots and the phases of a block, 8 us for the groups, a chain of reads, barriers and code that each block
+// passes once (17 k cycles with a division and an exponential inlined at each use, 14 k with one copy of each; entries read
+// with the sums, or put down with one atomic per warp, were no faster). Four beams x 4096: 5 and 6 us.
 //
 // A finished beam is a list of its own: itself at the end token, then nothing (-inf) at the other tokens; a beam
 // without a finite score or sum is all -inf. So every group has K candidates whatever its logits hold.
@@ -271,6 +272,9 @@ __global__ void __launch_bounds__(THREADS, 5) select_rows_kernel(const SelectArg
   for (int i = have + tid; i < a.K; i += THREADS) out[i] = 0;
 }
 
+// (One copy of each: a block passes its code once, and the larger it is the longer it waits for instructions.)
+__device__ __noinline__ double exp_of(double x) { return exp(x); }
+
 // Block per group: the K best of its lists (one per beam and segment, sorted, K entries each). Their
 // heads give a bound that K candidates reach; the candidates that do are few, and each counts those before it. Where
 // equal heads make them too many, the best head is drawn K times instead.
@@ -295,6 +299,9 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
   if (tid == 0) found = 0;
   if (tid < K) chosen[tid] = (long)tid << 54;
   const int whole = min((lists + 31) / 32, MERGE_WARPS), mine = lane * whole + warp;  // this thread's first list
+  const float per_list = 1.f / S;
+  // (floor of i / S: i < 2^14 and S <= 512, so the half keeps the quotient 2^-10 off any whole number, 2^6 times its error)
+  auto row_of = [&](int i) { return __float2int_rd((i + 0.5f) * per_list); };
   const unsigned long long first_head = warp < whole && mine < lists ? a.entries[(first * S + mine) * K] : 0ull;
   for (int b = warp; b < K; b += MERGE_WARPS) {
     const long row = first + b;
@@ -319,12 +326,12 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) more = fmaxf(more, __shfl_xor_sync(~0u, more, o));
       if (more > top) {
-        sum *= top == -INFINITY ? 0.0 : exp((double)top - (double)more);
+        sum *= top == -INFINITY ? 0.0 : exp_of((double)top - (double)more);
         top = more;
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (s[j] != 0.0) sum += s[j] * (t[j] == top ? 1.0 : exp((double)t[j] - (double)top));  // NaN stays
+        if (s[j] != 0.0) sum += s[j] * (t[j] == top ? 1.0 : exp_of((double)t[j] - (double)top));  // NaN stays
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
@@ -339,10 +346,10 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     }
   }
   __syncthreads();
-  auto entry_of = [&](int i, int j) { return kind[i / S] == 0 && j < K ? a.entries[(first * S + i) * K + j] : 0ull; };
+  auto entry_of = [&](int i, int j) { return kind[row_of(i)] == 0 && j < K ? a.entries[(first * S + i) * K + j] : 0ull; };
   // j-th entry of list i, which is e where its row runs (rank key 0: there is none)
   auto item = [&](int i, int j, unsigned long long e, unsigned long long& rank, long& flat, double& value) {
-    const int b = i / S, seg = i - b * S;
+    const int b = row_of(i), seg = i - b * S;
     rank = 0;
     flat = LONG_MAX;
     value = -INFINITY;
@@ -419,17 +426,10 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
   }
   least = max(least, 1u);
   auto offer = [&](int i, int j, unsigned long long e) {
-    unsigned long long r;
-    long f;
-    double v;
-    item(i, j, e, r, f, v);
-    if ((unsigned)(r >> 32) >= least) {
-      const int to = atomicAdd(&found, 1);
-      if (to < MERGE_LIST) {
-        list_rank[to] = r;
-        list_flat[to] = f;
-        list_value[to] = v;
-      }
+    const int to = atomicAdd(&found, 1);
+    if (to < MERGE_LIST) {
+      list_rank[to] = e;
+      list_flat[to] = i << 5 | j;
     }
   };
   // A row's candidates that can reach the bound have a logit of about (bound norm - base) + top; they are few, and only
@@ -452,19 +452,33 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int i = i0 + k * MERGE_WARPS * per;
-      in[k] = sub < per && i < lists && kind[i / S] == 0 ? a.entries[(first * S + i) * K + j] : 0ull;
+      in[k] = sub < per && i < lists ? a.entries[(first * S + i) * K + j] : 0ull;
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int i = i0 + k * MERGE_WARPS * per;
-      if (in[k] && !(key_value((unsigned)(in[k] >> 32)) < row_least[i / S])) offer(i, j, in[k]);
+      const int i = i0 + k * MERGE_WARPS * per, b = row_of(min(i, lists - 1));
+      if (in[k] && kind[b] == 0 && !(key_value((unsigned)(in[k] >> 32)) < row_least[b])) offer(i, j, in[k]);
     }
   }
-  for (int e = tid; e < K * K; e += MERGE_THREADS)
-    if (kind[e / K] != 0) offer(e / K * S, e % K, 0ull);
+  const bool none_reach = least <= (unsigned)(rank_key(-INFINITY) >> 32);  // the bound is -inf
+  for (int e = tid; e < K * K; e += MERGE_THREADS) {
+    const int b = e / K;
+    if (kind[b] != 0 && (none_reach || (kind[b] == 1 && e == b * K))) offer(b * S, e - b * K, 0ull);
+  }
   __syncthreads();
   const int have = found;
   if (have <= MERGE_LIST) {
+    for (int i = tid; i < have; i += MERGE_THREADS) {
+      const int at = (int)list_flat[i];
+      unsigned long long r;
+      long f;
+      double v;
+      item(at >> 5, at & 31, list_rank[i], r, f, v);
+      list_rank[i] = r;
+      list_flat[i] = f;
+      list_value[i] = v;
+    }
+    __syncthreads();
     for (int i = tid; i < have; i += MERGE_THREADS) {
       const unsigned long long r = list_rank[i];
       const long f = list_flat[i];
