@@ -5,8 +5,10 @@
 // touches it, so any indices are safe without scratch memory, cycles and rows taken more than once included. Rows that
 // stay are neither read (unless a slot takes them over) nor written.
 //
-// Bound by memory: one read of each row that moves and one write of each that changes. 128 states of 172 MB per row, two of
-// four rows moving in two groups (1.4 GB): 225 us, 6.2 TB/s.
+// Bound by memory: one read of each row that moves and one write of each that changes. What is held in registers follows the
+// rows that are taken over, not the beams: few of many leave room for more columns of each. 128 states of 172 MB per row, two
+// of four rows moving in two groups (1.4 GB): 217 us, 6.5 TB/s; 20 of 27 rows of 7.5 MB: 42 us, 4.8 TB/s (80 us with registers
+// for every beam).
 #include <algorithm>
 #include <climits>
 #include "../api.h"
@@ -14,7 +16,7 @@
 
 namespace {
 
-constexpr int THREADS = 256, MAX_ITEMS = 128;
+constexpr int THREADS = 256, MAX_ITEMS = 128, ENOUGH = 592;  // blocks: four per SM
 
 struct Item {
   char* base;
@@ -25,54 +27,78 @@ struct ReorderArgs {
   Item item[MAX_ITEMS];
   const long* parents;
   int items, K, width;  // bytes that a thread moves at once
+  long columns;         // words of a row that a block moves
 };
 
 template <int N> struct Word;
 template <> struct Word<16> { using type = uint4; };
+template <> struct Word<8> { using type = uint2; };
 template <> struct Word<4> { using type = unsigned; };
 template <> struct Word<1> { using type = unsigned char; };
 
-// Columns of a thread: as many as fit some 32 words of 16 bytes in flight.
-constexpr int columns(int beams) { return beams >= 16 ? 1 : 16 / beams; }
-
-template <int B, int WIDTH>
-__device__ __forceinline__ void move(char* rows, long bytes, long chunk, const unsigned* children, int K) {
+// Columns [c0, end) of the rows that are taken over (N of them at most, held), U columns of each in a thread's registers.
+template <int N, int U, int WIDTH>
+__device__ __forceinline__ void move(char* rows, long bytes, long c0, long end, const int* from, const unsigned* children,
+                                     int held) {
   using W = typename Word<WIDTH>::type;
-  constexpr int U = columns(B);
-  const long words = bytes / WIDTH;
-  const long c0 = chunk * (THREADS * U) + threadIdx.x;
-  W v[B][U];
+#pragma unroll 1
+  for (; c0 < end; c0 += THREADS * U) {
+    W v[N][U];
 #pragma unroll
-  for (int j = 0; j < B; ++j)
-    if (j < K && children[j])
+    for (int j = 0; j < N; ++j)
+      if (j < held) {
+        const W* row = reinterpret_cast<const W*>(rows + from[j] * bytes);
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (c0 + i * THREADS < words) v[j][i] = *reinterpret_cast<const W*>(rows + j * bytes + (c0 + i * THREADS) * WIDTH);
+        for (int i = 0; i < U; ++i)
+          if (c0 + i * THREADS < end) v[j][i] = row[c0 + i * THREADS];
+      }
 #pragma unroll
-  for (int j = 0; j < B; ++j) {
-    if (j >= K) break;
-    for (unsigned to = children[j]; to; to &= to - 1) {
-      const int k = __ffs(to) - 1;
+    for (int j = 0; j < N; ++j) {
+      if (j >= held) break;
+      for (unsigned to = children[j]; to; to &= to - 1) {
+        W* row = reinterpret_cast<W*>(rows + (__ffs(to) - 1) * bytes);
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (c0 + i * THREADS < words) *reinterpret_cast<W*>(rows + k * bytes + (c0 + i * THREADS) * WIDTH) = v[j][i];
+        for (int i = 0; i < U; ++i)
+          if (c0 + i * THREADS < end) row[c0 + i * THREADS] = v[j][i];
+      }
     }
   }
 }
 
-// Grid (chunks of all tensors, groups).
-template <int B>
-__global__ void __launch_bounds__(THREADS) reorder_kernel(const __grid_constant__ ReorderArgs a) {
-  __shared__ unsigned children[B];  // slots other than itself that take a slot's row over
-  const int tid = threadIdx.x, K = a.K;
-  const long group = blockIdx.y;
-  if (tid < B) children[tid] = 0;
-  __syncthreads();
-  if (tid < K) {
-    const long p = a.parents[group * K + tid];
-    if (p >= 0 && p < K && p != tid) atomicOr(&children[p], 1u << tid);
+// As many columns of each row as keep 16 words in flight per thread (of half the size where 32 rows may be held: registers
+// for two blocks per SM).
+template <int B, int CAP, int WIDTH, int N = 1>
+__device__ __forceinline__ void move_held(char* rows, long bytes, long c0, long end, const int* from,
+                                          const unsigned* children, int held) {
+  if constexpr (N < B) {
+    if (held > N) return move_held<B, CAP, WIDTH, 2 * N>(rows, bytes, c0, end, from, children, held);
   }
-  __syncthreads();
+  if constexpr (N == 32 && WIDTH == 16)
+    move<N, 1, 8>(rows, bytes, 2 * (c0 - threadIdx.x) + threadIdx.x, 2 * end, from, children, held);
+  else
+    move<N, N >= 16 ? 1 : N * CAP >= 16 ? 16 / N : CAP, WIDTH>(rows, bytes, c0, end, from, children, held);
+}
+
+// Grid (chunks of all tensors, groups).
+template <int B, int CAP>
+__global__ void __launch_bounds__(THREADS) reorder_kernel(const __grid_constant__ ReorderArgs a) {
+  __shared__ int from[THREADS / 32][B];           // the rows that other slots take over (each warp finds them for itself,
+  __shared__ unsigned children[THREADS / 32][B];  // which takes no barrier), and those slots
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.K;
+  const long group = blockIdx.y;
+  const long p = lane < K ? a.parents[group * K + lane] : -1;
+  const bool moves = p >= 0 && p < K && p != lane;
+  const unsigned siblings = __match_any_sync(~0u, moves ? (int)p : 32 + lane);
+  const bool first = moves && __ffs(siblings) - 1 == lane;
+  const unsigned firsts = __ballot_sync(~0u, first);
+  const int held = __popc(firsts);
+  if (held == 0) return;
+  if (first) {
+    const int at = __popc(firsts & ((1u << lane) - 1));
+    from[warp][at] = (int)p;
+    children[warp][at] = siblings;
+  }
+  __syncwarp();
   int lo = 0, hi = a.items - 1;  // first tensor whose blocks end behind this one
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
@@ -82,22 +108,34 @@ __global__ void __launch_bounds__(THREADS) reorder_kernel(const __grid_constant_
   const Item it = a.item[lo];
   const long chunk = blockIdx.x - (lo ? a.item[lo - 1].chunks : 0);
   char* rows = it.base + group * K * it.bytes;
-  if (a.width == 16) move<B, 16>(rows, it.bytes, chunk, children, K);
-  else if (a.width == 4) move<B, 4>(rows, it.bytes, chunk, children, K);
-  else move<B, 1>(rows, it.bytes, chunk, children, K);
+  const long c0 = chunk * a.columns + tid, end = min((chunk + 1) * a.columns, it.bytes / a.width);
+  if (a.width == 16) move_held<B, CAP, 16>(rows, it.bytes, c0, end, from[warp], children[warp], held);
+  else if (a.width == 4) move_held<B, CAP, 4>(rows, it.bytes, c0, end, from[warp], children[warp], held);
+  else move_held<B, CAP, 1>(rows, it.bytes, c0, end, from[warp], children[warp], held);
 }
 
 template <int B>
 cudaError_t launch(ReorderArgs& a, long groups, cudaStream_t s) {
-  const long per = (long)THREADS * columns(B) * a.width;
+  // 16 words per thread, fewer where the blocks would be too few for the SMs; from four on a block's own start costs more
+  // (three rows of 1.9 MB: 9 us with blocks of four words and 13 with blocks of one). Its code takes no more than four at once
+  // then: a block waits for its code as well (four rows of 1.9 MB: 6 us).
+  int words = 16;
   long chunks = 0;
-  for (int i = 0; i < a.items; ++i) a.item[i].chunks = chunks += (a.item[i].bytes + per - 1) / per;
+  for (;; words /= 2) {
+    a.columns = (long)THREADS * words;
+    const long per = a.columns * a.width;
+    chunks = 0;
+    for (int i = 0; i < a.items; ++i) a.item[i].chunks = chunks += (a.item[i].bytes + per - 1) / per;
+    if (words == 4 || chunks * groups >= ENOUGH) break;
+  }
   if (chunks > INT_MAX) return cudaErrorInvalidValue;
   for (long g = 0; g < groups; g += 65535) {
     ReorderArgs b = a;
     b.parents += g * a.K;
     for (int i = 0; i < a.items; ++i) b.item[i].base += g * a.K * a.item[i].bytes;
-    reorder_kernel<B><<<dim3((unsigned)chunks, (unsigned)std::min(groups - g, 65535L)), THREADS, 0, s>>>(b);
+    const dim3 grid((unsigned)chunks, (unsigned)std::min(groups - g, 65535L));
+    if (words == 4) reorder_kernel<B, 4><<<grid, THREADS, 0, s>>>(b);
+    else reorder_kernel<B, 16><<<grid, THREADS, 0, s>>>(b);
   }
   return cudaGetLastError();
 }

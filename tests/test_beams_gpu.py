@@ -160,6 +160,26 @@ def test_states_follow_any_parents(G, K):
             assert torch.equal(state, value)
 
 
+@pytest.mark.parametrize("K", [2, 3, 6, 18, 32])
+@pytest.mark.parametrize("sources", [1, 2, 31])
+def test_long_rows_follow_few_and_many_parents(K, sources):
+    """Rows of several blocks, whose ends fall inside a thread's columns; words of 16, 4 and 1 bytes."""
+    G, g = 200, torch.Generator().manual_seed(K)
+    parents = torch.arange(K).repeat(G, 1)
+    for group in parents:
+        order = torch.randperm(K, generator=g)
+        kept = order[:min(sources, K - 1)]
+        moved = order[len(kept):]
+        group[moved] = kept[torch.randint(len(kept), (len(moved),), generator=g)]
+    parents[1] = parents[1].roll(1)  # one that takes over in a cycle
+    rows = (parents + torch.arange(G)[:, None] * K).view(-1).cuda()
+    for size in (131120, 70004, 20001):
+        state = torch.randint(256, (G * K, size), device="cuda", dtype=torch.uint8)
+        want = state[rows]
+        reorder_states_([state], parents.cuda())
+        assert torch.equal(state, want)
+
+
 def test_states_refuse_on_cuda():
     parents = torch.zeros(1, 33, dtype=torch.int64, device="cuda")
     with pytest.raises(ValueError, match="at most 32"):
