@@ -483,7 +483,12 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
       const unsigned long long r = list_rank[i];
       const long f = list_flat[i];
       int place = 0;
-      for (int j = 0; j < have; ++j) place += list_rank[j] > r || (list_rank[j] == r && list_flat[j] < f);
+#pragma unroll 8
+      for (int j = 0; j < have; ++j) {  // (both are read whatever they say, so that the reads do not wait for one another)
+        const unsigned long long other = list_rank[j];
+        const long at = list_flat[j];
+        place += (other > r) | ((other == r) & (at < f));
+      }
       if (place < K) {
         chosen[place] = f;
         values[place] = list_value[i];
