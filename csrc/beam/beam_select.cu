@@ -11,9 +11,9 @@
 // exponentials' error at worst (about 1e-7), those of one beam differ by their logits alone.
 //
 // Eight groups of eight beams x 248077 fp32 logits (a sixth of them ended, 53 MB): 17 us for the segments, bound by half
-// of the issue slots and the phases of a block, 8 us for the groups, a chain of reads, barriers and code that each block
-// passes once (17 k cycles with a division and an exponential inlined at each use, 14 k with one copy of each; entries read
-// with the sums, or put down with one atomic per warp, were no faster). Four beams x 4096: 5 and 6 us.
+// of the issue slots and the phases of a block, 6 us for the groups, a chain of reads, barriers and code that each block
+// passes once (17 k cycles with a division and an exponential inlined at each use and all lists' entries read, 11-12 k so).
+// Four beams x 4096: 5 and 6 us.
 //
 // A finished beam is a list of its own: itself at the end token, then nothing (-inf) at the other tokens; a beam
 // without a finite score or sum is all -inf. So every group has K candidates whatever its logits hold.
@@ -292,11 +292,11 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
   __shared__ double list_value[MERGE_LIST];
   __shared__ unsigned warp_bound[MERGE_WARPS], heads[MERGE_THREADS];
   __shared__ float row_least[32];
-  __shared__ int found;
+  __shared__ int found, reaching;
   __shared__ double values[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.K, S = a.segments, lists = K * S;
   const long first = (long)blockIdx.x * K;
-  if (tid == 0) found = 0;
+  if (tid == 0) found = reaching = 0;
   if (tid < K) chosen[tid] = (long)tid << 54;
   const int whole = min((lists + 31) / 32, MERGE_WARPS), mine = lane * whole + warp;  // this thread's first list
   const float per_list = 1.f / S;
@@ -376,6 +376,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
   };
   // the upper half of a rank's key keeps its order. A warp's lists are spread over all beams, as they are not alike
   // (a thread may stand for several lists); each warp's k-th largest head, as in a segment
+  unsigned best_head = 0;  // of this thread's lists
   if (warp < whole) {
     unsigned head = 0, t = 0;
     for (int i = mine; i < lists; i += 32 * whole) {
@@ -385,14 +386,14 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
       item(i, 0, i == mine ? first_head : entry_of(i, 0), r, f, v);
       head = max(head, (unsigned)(r >> 32));
     }
-    const unsigned best = head;
+    best_head = head;
     for (int k = (K + whole - 1) / whole; k > 0; --k) {
       t = __reduce_max_sync(~0u, head);
       const unsigned equal = __ballot_sync(~0u, head == t);
       if (lane == __ffs(equal) - 1) head = 0;
     }
     if (lane == 0) warp_bound[warp] = t;
-    heads[warp * 32 + lane] = best;
+    heads[warp * 32 + lane] = best_head;
   }
   __syncthreads();
   unsigned least = __reduce_min_sync(~0u, lane < whole ? warp_bound[lane] : ~0u);
@@ -444,22 +445,28 @@ __global__ void __launch_bounds__(MERGE_THREADS) select_group_kernel(const Selec
     // (NaN, of a bound below all numbers, lets everything through)
     row_least[tid] = __double2float_rd(at_least - margin - fabs(at_least) * 1e-6 - 1e-3);
   }
+  // only lists whose head reaches the bound are read on: of 608 lists of 32 beams some 40, and 10 KB of 156
+  unsigned* reached = heads;  // (which nobody reads any more)
+  if (warp < whole && best_head >= least) reached[atomicAdd(&reaching, 1)] = mine;
   __syncthreads();
   // a lane per entry, 32 / K lists per warp
-  const int per = 32 / K, sub = lane / K, j = lane - sub * K;
-  for (int i0 = warp * per + sub; i0 < lists; i0 += 8 * MERGE_WARPS * per) {
-    unsigned long long in[8];
+  const int per = 32 / K, sub = lane / K, j = lane - sub * K, slots = reaching;
+  for (int more = 0; more < lists; more += 32 * whole)
+    for (int w0 = warp * per + sub; w0 < slots; w0 += 2 * MERGE_WARPS * per) {
+      unsigned long long in[2];
+      int at[2];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = i0 + k * MERGE_WARPS * per;
-      in[k] = sub < per && i < lists ? a.entries[(first * S + i) * K + j] : 0ull;
-    }
+      for (int k = 0; k < 2; ++k) {
+        const int w = w0 + k * MERGE_WARPS * per;
+        at[k] = w < slots ? (int)reached[w] + more : lists;
+        in[k] = sub < per && at[k] < lists ? a.entries[(first * S + at[k]) * K + j] : 0ull;
+      }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = i0 + k * MERGE_WARPS * per, b = row_of(min(i, lists - 1));
-      if (in[k] && kind[b] == 0 && !(key_value((unsigned)(in[k] >> 32)) < row_least[b])) offer(i, j, in[k]);
+      for (int k = 0; k < 2; ++k) {
+        const int b = row_of(min(at[k], lists - 1));
+        if (in[k] && kind[b] == 0 && !(key_value((unsigned)(in[k] >> 32)) < row_least[b])) offer(at[k], j, in[k]);
+      }
     }
-  }
   const bool none_reach = least <= (unsigned)(rank_key(-INFINITY) >> 32);  // the bound is -inf
   for (int e = tid; e < K * K; e += MERGE_THREADS) {
     const int b = e / K;

@@ -103,6 +103,22 @@ def test_scores_that_swallow_logits_leave_their_order(G, K, V, score):
         _check([logits.bfloat16(), scores, lengths, finished], 1, penalty)  # (many equal logits)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_largest_vocabulary_and_most_beams(dtype):
+    V, g = 4161536, torch.Generator(device="cuda").manual_seed(4)
+    row = (torch.randperm(V, device="cuda", generator=g).float() * 2 ** -18).to(dtype)  # (bf16: many are equal)
+    scores = torch.full((1, 32), -INF, device="cuda")
+    scores[0, 5] = -1.0
+    tokens, parents, new, lengths, ended = beam_select(
+        row.expand(1, 32, V), scores, torch.ones(1, 32, device="cuda", dtype=torch.int32),
+        torch.zeros(1, 32, device="cuda", dtype=torch.bool))
+    want = row.sort(descending=True, stable=True)[1][:32]
+    order = [want[1:6], want[:1], want[6:]]  # slot 5 keeps its best child, the others fill the rest in order
+    assert torch.equal(tokens[0], torch.cat(order)) and (parents == 5).all() and (lengths == 2).all()
+    value = -1.0 + torch.log_softmax(row.double(), -1)[tokens[0]]
+    torch.testing.assert_close(new[0], value.float(), rtol=2 ** -23, atol=2 ** -21)
+
+
 def test_selection_takes_any_strides():
     logits, scores, lengths, finished = _step(3, 4, 1001, torch.float32)
     wide = torch.empty(4, 3, 2005, device="cuda")
